@@ -10,15 +10,18 @@ from .distconv import (  # noqa: F401
     LHS,
     RHS,
     Allreduce,
+    Attention,
     BackendDNNLib,
     BatchNormalization,
     Convolution,
     Distribution,
     HaloExchange,
+    LayerNormalization,
     LeakyReLU,
     Locale,
     Options,
     Pooling,
+    RotaryPositions,
     Tensor,
     TensorShuffler,
     create_convolution_d_output_tensor,

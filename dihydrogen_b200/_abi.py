@@ -25,6 +25,8 @@ HALO_SKIP_UNPACK = 0x2
 HALO_CLEAR_BOUNDARY = 0x4
 HALO_OPS = {"ID": 0 << 4, "SUM": 1 << 4, "MAX": 2 << 4, "MIN": 3 << 4}
 
+F32, BF16 = 0, 1
+
 MATH_FP32, MATH_TF32, MATH_FP32_SIMT, MATH_BF16 = 0, 1, 2, 3
 
 
@@ -87,6 +89,29 @@ class ConvDesc(ctypes.Structure):
     ]
 
 
+class RotaryDesc(ctypes.Structure):
+    _fields_ = [
+        ("nsd", c_int32),
+        ("head_dim", c_int32),
+        ("axis_channels", c_int32 * DCB_MAX_SPATIAL),
+        ("rotated_heads", c_int32),
+        ("interleaved", c_int32),
+        ("origin", c_int64 * DCB_MAX_SPATIAL),
+        ("base", c_double),
+        ("step", c_double * DCB_MAX_SPATIAL),
+    ]
+
+
+class AttentionDesc(ctypes.Structure):
+    _fields_ = [
+        ("q_heads", c_int32),
+        ("kv_heads", c_int32),
+        ("dtype", c_int32),
+        ("causal", c_int32),
+        ("scale", c_float),
+    ]
+
+
 class DcbError(RuntimeError):
     def __init__(self, status: int, where: str, detail: str):
         self.status = status
@@ -143,6 +168,20 @@ _SIGS = {
     "dcb_pool_bwd": (c_int32, [POINTER(PoolDesc), POINTER(NdDesc), POINTER(NdDesc), c_double, _P, _P, _P, c_double,
                                _P, _P, c_int64, _P]),
     "dcb_pool_bwd_workspace_bytes": (c_int64, [POINTER(PoolDesc), POINTER(NdDesc), POINTER(NdDesc)]),
+    "dcb_ln_fwd": (c_int32, [POINTER(NdDesc), c_int32, _P, _P, _P, c_float, POINTER(NdDesc), _P, _P, _P, _P]),
+    "dcb_ln_bwd": (c_int32, [POINTER(NdDesc), c_int32, _P, POINTER(NdDesc), _P, _P, _P, _P, POINTER(NdDesc), _P, _P, _P,
+                             _P, c_int64, _P]),
+    "dcb_ln_bwd_workspace_bytes": (c_int64, [POINTER(NdDesc), c_int32]),
+    "dcb_rotary_plan_create": (c_int32, [POINTER(RotaryDesc), POINTER(NdDesc), POINTER(_P)]),
+    "dcb_rotary_plan_destroy": (c_int32, [_P]),
+    "dcb_rotary_apply": (c_int32, [_P, POINTER(NdDesc), c_int32, _P, POINTER(NdDesc), c_int32, _P, c_int32, _P]),
+    "dcb_attention_fwd": (c_int32, [POINTER(AttentionDesc), POINTER(NdDesc), _P, POINTER(NdDesc), _P, POINTER(NdDesc),
+                                    _P, _P, _P, POINTER(NdDesc), _P, _P, _P, c_int64, _P]),
+    "dcb_attention_bwd": (c_int32, [POINTER(AttentionDesc), POINTER(NdDesc), _P, POINTER(NdDesc), _P, POINTER(NdDesc),
+                                    _P, _P, _P, POINTER(NdDesc), _P, _P, POINTER(NdDesc), _P, POINTER(NdDesc), _P,
+                                    POINTER(NdDesc), _P, POINTER(NdDesc), _P, _P, c_int64, _P]),
+    "dcb_attention_workspace_bytes": (c_int64, [POINTER(AttentionDesc), POINTER(NdDesc), POINTER(NdDesc), c_int32]),
+    "dcb_attention_status": (c_int32, [_P]),
     "dcb_shuffle_plan_create": (c_int32, [POINTER(TensorDesc), POINTER(TensorDesc), POINTER(Box), POINTER(Box),
                                           c_int32, c_int32, POINTER(_P)]),
     "dcb_shuffle_plan_destroy": (c_int32, [_P]),

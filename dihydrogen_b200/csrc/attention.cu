@@ -1,0 +1,378 @@
+// Attention between cells: argument checks, workspace, the kernels beside the products.
+#include "attention.cuh"
+
+namespace dcb
+{
+namespace
+{
+
+// Joins the parts of a split axis of keys: o = sum_s part_s 2^(m_s - m) / sum_s l_s 2^(m_s - m).
+template <class T>
+__global__ void __launch_bounds__(256) attn_join_fwd_kernel(AttnProblem p)
+{
+    wait_for_previous_kernel(p.part_o, p.part_ml);
+    const long long heads = (long long) p.n * p.q_heads, total = heads * p.d * p.sq;
+    for (long long at = (long long) blockIdx.x * 256 + threadIdx.x; at < total; at += (long long) gridDim.x * 256)
+    {
+        const long long row = at / p.sq, nh = row / p.d, n = nh / p.q_heads;
+        const int i = (int) (at - row * p.sq), c = (int) (row - nh * p.d);
+        const float* ml = p.part_ml + nh * p.sq + i;
+        const long long step = 2 * heads * p.sq;
+        float m = -INFINITY;
+        for (int s = 0; s < p.kv_splits; ++s)
+            m = fmaxf(m, ml[s * step]);
+        float l = 0.f, o = 0.f;
+        if (m != -INFINITY)
+            for (int s = 0; s < p.kv_splits; ++s)
+            {
+                const float f = exp2f(ml[s * step] - m);
+                l = fmaf(ml[s * step + heads * p.sq], f, l);
+                o = fmaf(p.part_o[s * total + at], f, o);
+            }
+        const bool none = l == 0.f || (p.q_mask && !p.q_mask[n * p.sq + i]);
+        const float v[1] = {none ? 0.f : o / l};
+        store_elems<1>(static_cast<T*>(p.o.p) + n * p.o.sn + ((nh - n * p.q_heads) * p.d + c) * p.o.sc + i, v);
+        if (c == 0)
+            p.lse[nh * p.sq + i] = none ? -INFINITY : (m + log2f(l)) / ATTN_LOG2E;
+    }
+}
+
+// Adds up the parts of a gradient in order.
+template <class T>
+__global__ void __launch_bounds__(256) attn_join_grad_kernel(const float* part, int splits, AttnTensor t, int n,
+                                                             int heads, int d, int cells)
+{
+    wait_for_previous_kernel(part);
+    const long long total = (long long) n * heads * d * cells;
+    for (long long at = (long long) blockIdx.x * 256 + threadIdx.x; at < total; at += (long long) gridDim.x * 256)
+    {
+        float v[1] = {0.f};
+        for (int s = 0; s < splits; ++s)
+            v[0] += part[s * total + at];
+        const long long row = at / cells, b = row / ((long long) heads * d);
+        store_elems<1>(static_cast<T*>(t.p) + b * t.sn + (row - b * heads * d) * t.sc + (at - row * cells), v);
+    }
+}
+
+// stats: lse in powers of two and delta = sum_c o d_o; a cell that takes no part has +infinity and 0, so that its
+// weights are exp2(s - infinity) = 0.
+template <class T>
+__global__ void __launch_bounds__(128) attn_stats_kernel(AttnProblem p)
+{
+    const long long heads = (long long) p.n * p.q_heads, total = heads * p.sq;
+    for (long long at = (long long) blockIdx.x * 128 + threadIdx.x; at < total; at += (long long) gridDim.x * 128)
+    {
+        const long long nh = at / p.sq, n = nh / p.q_heads;
+        const int i = (int) (at - nh * p.sq);
+        const float lse = p.lse[at];
+        float delta = 0.f;
+        const bool none = lse == -INFINITY || (p.q_mask && !p.q_mask[n * p.sq + i]);
+        if (!none)
+        {
+            const long long first = (nh - n * p.q_heads) * p.d;
+            const T* o = static_cast<const T*>(p.o.p) + n * p.o.sn + first * p.o.sc + i;
+            const T* g = static_cast<const T*>(p.d_o.p) + n * p.d_o.sn + first * p.d_o.sc + i;
+#pragma unroll 8
+            for (int c = 0; c < p.d; ++c)
+            {
+                float a[1], b[1];
+                load_elems<1>(o + c * p.o.sc, a);
+                load_elems<1>(g + c * p.d_o.sc, b);
+                delta = fmaf(a[0], b[0], delta);
+            }
+        }
+        p.stats[at] = none ? INFINITY : lse * ATTN_LOG2E;
+        p.stats[total + at] = delta;
+    }
+}
+
+// Zeros, and lse of a cell that sees nothing.
+template <class T>
+__global__ void __launch_bounds__(256) attn_fill_kernel(AttnTensor t, int n, long long channels, int cells, float* lse,
+                                                        long long lse_count)
+{
+    const long long total = n * channels * cells;
+    const long long at0 = (long long) blockIdx.x * 256 + threadIdx.x, step = (long long) gridDim.x * 256;
+    for (long long at = at0; at < total; at += step)
+    {
+        const long long row = at / cells, b = row / channels;
+        const float v[1] = {0.f};
+        store_elems<1>(static_cast<T*>(t.p) + b * t.sn + (row - b * channels) * t.sc + (at - row * cells), v);
+    }
+    if (lse)
+        for (long long at = at0; at < lse_count; at += step)
+            lse[at] = -INFINITY;
+}
+
+unsigned flat_blocks(long long total, int threads)
+{
+    return (unsigned) std::max<long long>(1, std::min<long long>((total + threads - 1) / threads, 16ll * num_sms()));
+}
+
+template <class F>
+int32_t with_type(int32_t dtype, F f)
+{
+    return dtype == DCB_BF16 ? f(bf16()) : f(float());
+}
+
+int32_t attn_fill(int32_t dtype, const AttnTensor& t, int n, long long channels, int cells, float* lse,
+                  long long lse_count, cudaStream_t s)
+{
+    return with_type(dtype, [&](auto e) -> int32_t {
+        const long long total = std::max(n * channels * cells, lse ? lse_count : 0);
+        if (total == 0)
+            return DCB_OK;
+        attn_fill_kernel<decltype(e)><<<flat_blocks(total, 256), 256, 0, s>>>(t, n, channels, cells, lse, lse_count);
+        DCB_LAUNCH_CHECK();
+        return DCB_OK;
+    });
+}
+
+int64_t cells_of(const dcb_nd_desc& d)
+{
+    return d.dims[0] * d.dims[1] * d.dims[2];
+}
+
+// What follows from the shapes alone.
+int32_t attn_shapes(const dcb_attention_desc* ad, const dcb_nd_desc* qd, const dcb_nd_desc* kd, AttnProblem* p)
+{
+    DCB_REQUIRE(ad, "null descriptor");
+    if (int32_t e = check_nd_desc(qd))
+        return e;
+    if (int32_t e = check_nd_desc(kd))
+        return e;
+    DCB_REQUIRE(known_dtype(ad->dtype), "dtype must be DCB_F32 or DCB_BF16");
+    DCB_REQUIRE(ad->q_heads >= 1 && ad->kv_heads >= 1 && ad->q_heads % ad->kv_heads == 0,
+                "q_heads must be a multiple of kv_heads");
+    DCB_REQUIRE(qd->c >= 1 && qd->c % ad->q_heads == 0, "channels of q must be q_heads heads");
+    const int64_t d = qd->c / ad->q_heads;
+    DCB_REQUIRE(kd->c == d * ad->kv_heads, "channels of k must be kv_heads heads of q's size");
+    DCB_REQUIRE(qd->n == kd->n, "q and k differ in samples");
+    DCB_REQUIRE(ad->scale > 0.f && ad->scale <= 3.0e38f, "scale must be positive and finite");
+    if (d > ATTN_MAX_HEAD)
+    {
+        set_last_error("unsupported: heads of more than 128 channels");
+        return DCB_UNSUPPORTED;
+    }
+    if (cells_of(*qd) >= (1ll << 30) || cells_of(*kd) >= (1ll << 30) || qd->n >= (1ll << 24) || ad->q_heads >= (1 << 16))
+    {
+        set_last_error("unsupported: 2^30 cells of a sample, 2^24 samples or 2^16 heads");
+        return DCB_UNSUPPORTED;
+    }
+    *p = AttnProblem();
+    p->n = (int) qd->n;
+    p->q_heads = ad->q_heads;
+    p->kv_heads = ad->kv_heads;
+    p->group = ad->q_heads / ad->kv_heads;
+    p->d = (int) d;
+    p->sq = (int) cells_of(*qd);
+    p->sk = (int) cells_of(*kd);
+    p->causal = ad->causal != 0;
+    p->offset = p->sk - p->sq;
+    p->scale = ad->scale * ATTN_LOG2E;
+    return DCB_OK;
+}
+
+int32_t attn_tensor(const dcb_nd_desc* d, const dcb_nd_desc* like, const void* ptr, const char* name, AttnTensor* t)
+{
+    if (int32_t e = check_nd_desc(d))
+        return e;
+    if (!same_extents(*d, *like))
+    {
+        set_last_error(std::string("bad argument: extents of ") + name);
+        return DCB_BAD_ARG;
+    }
+    if (run_level(*d) != 2)
+    {
+        set_last_error(std::string("unsupported: the cells of ") + name + " are not contiguous");
+        return DCB_UNSUPPORTED;
+    }
+    if (cells_of(*d) > 0 && d->n > 0)
+        DCB_REQUIRE(ptr, "null tensor");
+    *t = AttnTensor{const_cast<void*>(ptr), d->sn, d->sc};
+    return DCB_OK;
+}
+
+// The workspace, piece by piece; a null base only counts.
+struct Carve
+{
+    char* base;
+    int64_t used = 0;
+    float* floats(long long count)
+    {
+        float* p = base ? reinterpret_cast<float*>(base + used) : nullptr;
+        used += (count * 4 + 255) / 256 * 256;
+        return p;
+    }
+};
+
+int64_t attn_carve(AttnProblem* p, bool backward, void* workspace)
+{
+    Carve w{static_cast<char*>(workspace)};
+    attn_simt_splits(p, backward);
+    const long long qh = (long long) p->n * p->q_heads, kh = (long long) p->n * p->kv_heads;
+    if (!backward)
+    {
+        if (p->kv_splits > 1)
+        {
+            p->part_o = w.floats(p->kv_splits * qh * p->d * p->sq);
+            p->part_ml = w.floats(p->kv_splits * 2 * qh * p->sq);
+        }
+        return w.used;
+    }
+    p->stats = w.floats(2 * qh * p->sq);
+    if (p->kv_splits > 1)
+        p->part_dq = w.floats(p->kv_splits * qh * p->d * p->sq);
+    if (p->q_splits > 1)
+    {
+        p->part_dk = w.floats(p->q_splits * kh * p->d * p->sk);
+        p->part_dv = w.floats(p->q_splits * kh * p->d * p->sk);
+    }
+    return w.used;
+}
+
+int32_t attn_workspace(AttnProblem* p, bool backward, void* workspace, int64_t bytes)
+{
+    const int64_t need = attn_carve(p, backward, nullptr);
+    if (need > 0)
+    {
+        DCB_REQUIRE(workspace && bytes >= need, "workspace too small");
+        DCB_REQUIRE(reinterpret_cast<uintptr_t>(workspace) % 256 == 0, "workspace must be 256-byte aligned");
+        attn_carve(p, backward, workspace);
+    }
+    return DCB_OK;
+}
+
+int32_t attn_join_grad(int32_t dtype, const float* part, int splits, const AttnTensor& t, int n, int heads, int d,
+                       int cells, cudaStream_t s)
+{
+    return with_type(dtype, [&](auto e) -> int32_t {
+        DCB_CUDA_TRY(launch_overlapped(attn_join_grad_kernel<decltype(e)>,
+                                       dim3(flat_blocks((long long) n * heads * d * cells, 256)), 256, 0, s, part,
+                                       splits, t, n, heads, d, cells));
+        return DCB_OK;
+    });
+}
+
+} // namespace
+} // namespace dcb
+
+using namespace dcb;
+
+extern "C" {
+
+int64_t dcb_attention_workspace_bytes(const dcb_attention_desc* ad, const dcb_nd_desc* qd, const dcb_nd_desc* kd,
+                                      int32_t backward)
+{
+    AttnProblem p;
+    if (attn_shapes(ad, qd, kd, &p))
+        return -1;
+    return attn_carve(&p, backward != 0, nullptr);
+}
+
+int32_t dcb_attention_fwd(const dcb_attention_desc* ad, const dcb_nd_desc* qd, const void* q, const dcb_nd_desc* kd,
+                          const void* k, const dcb_nd_desc* vd, const void* v, const void* q_mask, const void* kv_mask,
+                          const dcb_nd_desc* od, void* o, void* lse, void* workspace, int64_t workspace_bytes,
+                          void* stream)
+{
+    AttnProblem p;
+    if (int32_t e = attn_shapes(ad, qd, kd, &p))
+        return e;
+    if (int32_t e = attn_tensor(qd, qd, q, "q", &p.q))
+        return e;
+    if (int32_t e = attn_tensor(kd, kd, k, "k", &p.k))
+        return e;
+    if (int32_t e = attn_tensor(vd, kd, v, "v", &p.v))
+        return e;
+    if (int32_t e = attn_tensor(od, qd, o, "o", &p.o))
+        return e;
+    if (p.n == 0 || p.sq == 0)
+        return DCB_OK;
+    DCB_REQUIRE(lse, "null lse");
+    cudaStream_t s = as_stream(stream);
+    p.lse = static_cast<float*>(lse);
+    p.q_mask = static_cast<const uint8_t*>(q_mask);
+    p.kv_mask = static_cast<const uint8_t*>(kv_mask);
+    if (p.sk == 0)
+        return attn_fill(ad->dtype, p.o, p.n, (long long) p.q_heads * p.d, p.sq, p.lse,
+                         (long long) p.n * p.q_heads * p.sq, s);
+    if (int32_t e = attn_workspace(&p, false, workspace, workspace_bytes))
+        return e;
+    if (int32_t e = attn_simt_fwd(p, ad->dtype, s))
+        return e;
+    if (p.kv_splits == 1)
+        return DCB_OK;
+    return with_type(ad->dtype, [&](auto e) -> int32_t {
+        DCB_CUDA_TRY(launch_overlapped(attn_join_fwd_kernel<decltype(e)>,
+                                       dim3(flat_blocks((long long) p.n * p.q_heads * p.d * p.sq, 256)), 256, 0, s, p));
+        return DCB_OK;
+    });
+}
+
+int32_t dcb_attention_bwd(const dcb_attention_desc* ad, const dcb_nd_desc* qd, const void* q, const dcb_nd_desc* kd,
+                          const void* k, const dcb_nd_desc* vd, const void* v, const void* q_mask, const void* kv_mask,
+                          const dcb_nd_desc* od, const void* o, const void* lse, const dcb_nd_desc* dod,
+                          const void* d_o, const dcb_nd_desc* dqd, void* dq, const dcb_nd_desc* dkd, void* dk,
+                          const dcb_nd_desc* dvd, void* dv, void* workspace, int64_t workspace_bytes, void* stream)
+{
+    AttnProblem p;
+    if (int32_t e = attn_shapes(ad, qd, kd, &p))
+        return e;
+    const struct
+    {
+        const dcb_nd_desc *d, *like;
+        const void* ptr;
+        const char* name;
+        AttnTensor* to;
+    } tensors[] = {{qd, qd, q, "q", &p.q},    {kd, kd, k, "k", &p.k},      {vd, kd, v, "v", &p.v},
+                   {od, qd, o, "o", &p.o},    {dod, qd, d_o, "d_o", &p.d_o}, {dqd, qd, dq, "dq", &p.dq},
+                   {dkd, kd, dk, "dk", &p.dk}, {dvd, kd, dv, "dv", &p.dv}};
+    for (const auto& t : tensors)
+        if (int32_t e = attn_tensor(t.d, t.like, t.ptr, t.name, t.to))
+            return e;
+    if (p.n == 0)
+        return DCB_OK;
+    cudaStream_t s = as_stream(stream);
+    if (p.sq == 0 || p.sk == 0) // one side is empty: the other's gradients are zero
+    {
+        if (int32_t e = attn_fill(ad->dtype, p.dq, p.n, (long long) p.q_heads * p.d, p.sq, nullptr, 0, s))
+            return e;
+        if (int32_t e = attn_fill(ad->dtype, p.dk, p.n, (long long) p.kv_heads * p.d, p.sk, nullptr, 0, s))
+            return e;
+        return attn_fill(ad->dtype, p.dv, p.n, (long long) p.kv_heads * p.d, p.sk, nullptr, 0, s);
+    }
+    DCB_REQUIRE(lse, "null lse");
+    p.lse = static_cast<float*>(const_cast<void*>(lse));
+    p.q_mask = static_cast<const uint8_t*>(q_mask);
+    p.kv_mask = static_cast<const uint8_t*>(kv_mask);
+    if (int32_t e = attn_workspace(&p, true, workspace, workspace_bytes))
+        return e;
+    const int32_t e = with_type(ad->dtype, [&](auto t) -> int32_t {
+        attn_stats_kernel<decltype(t)>
+            <<<flat_blocks((long long) p.n * p.q_heads * p.sq, 128), 128, 0, s>>>(p);
+        DCB_LAUNCH_CHECK();
+        return DCB_OK;
+    });
+    if (e)
+        return e;
+    if (int32_t err = attn_simt_bwd(p, ad->dtype, s))
+        return err;
+    if (p.q_splits > 1)
+    {
+        if (int32_t err = attn_join_grad(ad->dtype, p.part_dk, p.q_splits, p.dk, p.n, p.kv_heads, p.d, p.sk, s))
+            return err;
+        if (int32_t err = attn_join_grad(ad->dtype, p.part_dv, p.q_splits, p.dv, p.n, p.kv_heads, p.d, p.sk, s))
+            return err;
+    }
+    if (p.kv_splits > 1)
+        return attn_join_grad(ad->dtype, p.part_dq, p.kv_splits, p.dq, p.n, p.q_heads, p.d, p.sq, s);
+    return DCB_OK;
+}
+
+int32_t dcb_attention_status(void* stream)
+{
+    DCB_CUDA_TRY(cudaStreamSynchronize(as_stream(stream)));
+    return DCB_OK;
+}
+
+} // extern "C"

@@ -1,0 +1,60 @@
+// What the parts of attention share: the problem as the kernels see it, the split of a long axis
+// and the layout of the workspace.
+#pragma once
+
+#include "elem.cuh"
+
+#include <algorithm>
+
+namespace dcb
+{
+
+constexpr float ATTN_LOG2E = 1.4426950408889634f;
+constexpr int ATTN_MAX_HEAD = 128;
+
+// One tensor: [sample][head][channel of the head][cell], cells contiguous.
+struct AttnTensor
+{
+    void* p;
+    long long sn, sc; // element strides of samples and channels
+};
+
+struct AttnProblem
+{
+    int n, q_heads, kv_heads, group; // group = query heads of a key head
+    int d;                           // channels of a head
+    int sq, sk;                      // cells
+    int causal, offset;              // j <= i + offset
+    float scale;                     // of scores, times log2(e): kernels take powers of two
+    AttnTensor q, k, v, o, d_o, dq, dk, dv;
+    const uint8_t *q_mask, *kv_mask;
+    float* lse;                      // [n][q_heads][sq]
+    // Backward: lse in powers of two (+infinity where a cell sees nothing) and sum_d o d_o,
+    // [2][n * q_heads][sq].
+    float* stats;
+    // Parts of a split axis, joined by a kernel of their own:
+    //   forward  [splits][n * q_heads][d][sq] sums and [splits][2][n * q_heads][sq] maxima, sums of weights
+    //   backward [splits][n * heads][d][cells] sums
+    float *part_o, *part_ml, *part_dq, *part_dk, *part_dv;
+    int q_splits, kv_splits; // of the queries' axis (dk, dv), of the keys' axis (o, dq)
+};
+
+__host__ __device__ inline int attn_tiles(int cells, int tile)
+{
+    return (cells + tile - 1) / tile;
+}
+
+// Splits of a walk over `steps` tiles so that `work` walks fill `slots` blocks; a part walks `least` tiles at least.
+inline int attn_splits(long long work, int steps, long long slots, int least)
+{
+    if (work <= 0 || work >= slots)
+        return 1;
+    return (int) std::max<long long>(1, std::min<long long>(slots / work, steps / least));
+}
+
+// Kernels of attention_simt.cu (fp32).
+int32_t attn_simt_fwd(const AttnProblem& p, int32_t dtype, cudaStream_t stream);
+int32_t attn_simt_bwd(const AttnProblem& p, int32_t dtype, cudaStream_t stream);
+void attn_simt_splits(AttnProblem* p, bool backward);
+
+} // namespace dcb

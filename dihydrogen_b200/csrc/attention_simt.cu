@@ -1,0 +1,446 @@
+// Attention on the CUDA cores, forward and backward.
+//
+// Blocks of 256 threads hold tiles of 64 cells as [channel][cell], as memory has them.  A thread
+// has 4 x 4 scores of a 64 x 64 tile (outer products over the channels) and 4 cells x D / 16
+// channels of the result (products over the tile's other cells).  The forward pass keeps the
+// running maximum and sum of a row beside its result; the backward pass works the weights out
+// again from lse, once by tiles of keys (dk, dv) and once by tiles of queries (dq), so that every
+// result has one owner and its sums one order.
+#include "attention.cuh"
+
+namespace dcb
+{
+namespace
+{
+
+constexpr int AS_TILE = 64;
+constexpr int AS_PITCH = 68; // floats: rows 16-byte aligned, four rows on different banks
+constexpr int AS_THREADS = 256;
+constexpr int AS_LEAST = 4;  // tiles a part of a split axis walks at least
+
+// One head's cells [cell0, cell0 + 64) to shared memory as [channel][cell]; cells that are not there, and channels up to
+// D, as zeros.
+template <class T, int D>
+__device__ __forceinline__ void as_load(float* to, const AttnTensor& t, long long n, int head, int d, int cell0,
+                                        int cells, const uint8_t* mask)
+{
+    const T* p = static_cast<const T*>(t.p) + n * t.sn + (long long) head * d * t.sc + cell0;
+    const int j = threadIdx.x & 63;
+    const bool there = cell0 + j < cells && (!mask || mask[cell0 + j]);
+    for (int c = threadIdx.x >> 6; c < D; c += AS_THREADS / 64)
+    {
+        float v[1] = {0.f};
+        if (there && c < d)
+            load_elems<1>(p + c * t.sc + j, v);
+        to[c * AS_PITCH + j] = v[0];
+    }
+}
+
+// s[a][b] = sum_c A[c][4 ty + a] B[c][4 tx + b]
+template <int D>
+__device__ __forceinline__ void as_scores(const float* A, const float* B, int tx, int ty, float (&s)[4][4])
+{
+#pragma unroll
+    for (int a = 0; a < 4; ++a)
+#pragma unroll
+        for (int b = 0; b < 4; ++b)
+            s[a][b] = 0.f;
+#pragma unroll 4
+    for (int c = 0; c < D; ++c)
+    {
+        float x[4], y[4];
+        load_elems<4>(A + c * AS_PITCH + 4 * ty, x);
+        load_elems<4>(B + c * AS_PITCH + 4 * tx, y);
+#pragma unroll
+        for (int a = 0; a < 4; ++a)
+#pragma unroll
+            for (int b = 0; b < 4; ++b)
+                s[a][b] = fmaf(x[a], y[b], s[a][b]);
+    }
+}
+
+// acc[e][r] += sum_t W[t][4 ty + e] X[tx + 16 r][t]
+template <int D>
+__device__ __forceinline__ void as_accumulate(const float* W, const float* X, int tx, int ty, float (&acc)[4][D / 16])
+{
+#pragma unroll 2
+    for (int t = 0; t < AS_TILE; t += 4)
+    {
+        float w[4][4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+            load_elems<4>(W + (t + u) * AS_PITCH + 4 * ty, w[u]);
+#pragma unroll
+        for (int r = 0; r < D / 16; ++r)
+        {
+            float x[4];
+            load_elems<4>(X + (tx + 16 * r) * AS_PITCH + t, x);
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    acc[e][r] = fmaf(w[u][e], x[u], acc[e][r]);
+        }
+    }
+}
+
+// Results of 4 cells x D / 16 channels: to the tensor, or as a part to [head][channel][cell].
+template <class T, int D>
+__device__ __forceinline__ void as_store(const AttnTensor& t, float* part, long long nh, long long n, int head, int d,
+                                         int cell0, int cells, int tx, int ty, const float (&acc)[4][D / 16])
+{
+#pragma unroll
+    for (int r = 0; r < D / 16; ++r)
+    {
+        const int c = tx + 16 * r;
+        if (c >= d)
+            continue;
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+        {
+            const int i = cell0 + 4 * ty + e;
+            if (i >= cells)
+                continue;
+            const float v[1] = {acc[e][r]};
+            if (part)
+                part[(nh * d + c) * cells + i] = v[0];
+            else
+                store_elems<1>(static_cast<T*>(t.p) + n * t.sn + ((long long) head * d + c) * t.sc + i, v);
+        }
+    }
+}
+
+struct AsAt
+{
+    int tile, split;
+    long long nh, n;
+    int head;
+};
+
+__device__ __forceinline__ AsAt as_at(int tiles, int splits, int heads)
+{
+    AsAt a;
+    long long b = blockIdx.x;
+    a.tile = tiles - 1 - (int) (b % tiles); // causal: the longest walks first
+    b /= tiles;
+    a.split = (int) (b % splits);
+    a.nh = b / splits;
+    a.n = a.nh / heads;
+    a.head = (int) (a.nh - a.n * heads);
+    return a;
+}
+
+// Part `split` of `steps` tiles.
+__device__ __forceinline__ void as_range(int steps, int splits, int split, int* lo, int* hi)
+{
+    *lo = (int) ((long long) steps * split / splits);
+    *hi = (int) ((long long) steps * (split + 1) / splits);
+}
+
+template <class T, int D>
+__global__ void __launch_bounds__(AS_THREADS) attn_simt_fwd_kernel(AttnProblem p)
+{
+    extern __shared__ float smem[];
+    float *Q = smem, *K = Q + D * AS_PITCH, *V = K + D * AS_PITCH, *P = V + D * AS_PITCH;
+    __shared__ uint8_t see[AS_TILE];
+    const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+    const AsAt at = as_at(attn_tiles(p.sq, AS_TILE), p.kv_splits, p.q_heads);
+    const int i0 = at.tile * AS_TILE, kv_head = at.head / p.group;
+    const uint8_t* qm = p.q_mask ? p.q_mask + at.n * p.sq : nullptr;
+    const uint8_t* km = p.kv_mask ? p.kv_mask + at.n * p.sk : nullptr;
+    as_load<T, D>(Q, p.q, at.n, at.head, p.d, i0, p.sq, qm);
+    float m[4], l[4], acc[4][D / 16];
+#pragma unroll
+    for (int a = 0; a < 4; ++a)
+    {
+        m[a] = -INFINITY, l[a] = 0.f;
+#pragma unroll
+        for (int r = 0; r < D / 16; ++r)
+            acc[a][r] = 0.f;
+    }
+    int lo, hi;
+    as_range(attn_tiles(p.sk, AS_TILE), p.kv_splits, at.split, &lo, &hi);
+    if (p.causal)
+        hi = (int) min((long long) hi, max(0ll, (long long) i0 + AS_TILE - 1 + p.offset + AS_TILE) / AS_TILE);
+    for (int t = lo; t < hi; ++t)
+    {
+        const int j0 = t * AS_TILE;
+        __syncthreads();
+        as_load<T, D>(K, p.k, at.n, kv_head, p.d, j0, p.sk, km);
+        as_load<T, D>(V, p.v, at.n, kv_head, p.d, j0, p.sk, km);
+        if (threadIdx.x < AS_TILE)
+            see[threadIdx.x] = j0 + (int) threadIdx.x < p.sk && (!km || km[j0 + threadIdx.x]);
+        __syncthreads();
+        float s[4][4];
+        as_scores<D>(Q, K, tx, ty, s);
+#pragma unroll
+        for (int a = 0; a < 4; ++a)
+        {
+            float top = m[a];
+#pragma unroll
+            for (int b = 0; b < 4; ++b)
+            {
+                const int j = 4 * tx + b;
+                const bool ok = see[j] && (!p.causal || j0 + j <= i0 + 4 * ty + a + p.offset);
+                s[a][b] = ok ? s[a][b] * p.scale : -INFINITY;
+                top = fmaxf(top, s[a][b]);
+            }
+#pragma unroll
+            for (int h = 8; h >= 1; h /= 2)
+                top = fmaxf(top, __shfl_xor_sync(~0u, top, h));
+            const float base = top == -INFINITY ? 0.f : top, shrink = exp2f(m[a] - base);
+            m[a] = top;
+            float sum = 0.f;
+#pragma unroll
+            for (int b = 0; b < 4; ++b)
+            {
+                s[a][b] = exp2f(s[a][b] - base);
+                sum += s[a][b];
+            }
+#pragma unroll
+            for (int h = 8; h >= 1; h /= 2)
+                sum += __shfl_xor_sync(~0u, sum, h);
+            l[a] = fmaf(l[a], shrink, sum);
+#pragma unroll
+            for (int r = 0; r < D / 16; ++r)
+                acc[a][r] *= shrink;
+#pragma unroll
+            for (int b = 0; b < 4; ++b)
+                P[(4 * tx + b) * AS_PITCH + 4 * ty + a] = s[a][b];
+        }
+        __syncthreads();
+        as_accumulate<D>(P, V, tx, ty, acc);
+    }
+    const long long heads = (long long) p.n * p.q_heads;
+    if (p.kv_splits > 1)
+    {
+        if (tx == 0)
+#pragma unroll
+            for (int a = 0; a < 4; ++a)
+                if (i0 + 4 * ty + a < p.sq)
+                {
+                    float* ml = p.part_ml + (2 * heads * at.split + at.nh) * p.sq + i0 + 4 * ty + a;
+                    ml[0] = m[a];
+                    ml[heads * p.sq] = l[a];
+                }
+        as_store<T, D>(p.o, p.part_o + at.split * heads * p.d * p.sq, at.nh, at.n, at.head, p.d, i0, p.sq, tx, ty,
+                       acc);
+        return;
+    }
+#pragma unroll
+    for (int a = 0; a < 4; ++a)
+    {
+        const int i = i0 + 4 * ty + a;
+        const bool none = l[a] == 0.f || (qm && i < p.sq && !qm[i]);
+        const float f = none ? 0.f : 1.f / l[a];
+#pragma unroll
+        for (int r = 0; r < D / 16; ++r)
+            acc[a][r] = none ? 0.f : acc[a][r] * f;
+        if (tx == 0 && i < p.sq)
+            p.lse[at.nh * p.sq + i] = none ? -INFINITY : (m[a] + log2f(l[a])) / ATTN_LOG2E;
+    }
+    as_store<T, D>(p.o, nullptr, at.nh, at.n, at.head, p.d, i0, p.sq, tx, ty, acc);
+}
+
+// The weights and their gradients of a tile, P = exp2(s - lse), dS = P (dP - delta): [query][key] or [key][query].
+template <int D, bool BY_KEY>
+__device__ __forceinline__ void as_weights(const AttnProblem& p, const float* Q, const float* K, const float* V,
+                                           const float* dO, const float* lse, const float* delta, const uint8_t* see,
+                                           int i0, int j0, int tx, int ty, float* P, float* dS)
+{
+    float s[4][4], dp[4][4];
+    as_scores<D>(Q, K, tx, ty, s);
+    as_scores<D>(dO, V, tx, ty, dp);
+#pragma unroll
+    for (int a = 0; a < 4; ++a)
+    {
+        const int i = 4 * ty + a;
+        const float top = lse[i], del = delta[i];
+#pragma unroll
+        for (int b = 0; b < 4; ++b)
+        {
+            const int j = 4 * tx + b;
+            const bool ok = see[j] && (!p.causal || j0 + j <= i0 + i + p.offset);
+            const float w = ok ? exp2f(fmaf(s[a][b], p.scale, -top)) : 0.f;
+            const float g = w == 0.f ? 0.f : w * (dp[a][b] - del);
+            if (BY_KEY)
+            {
+                P[i * AS_PITCH + j] = w;
+                dS[i * AS_PITCH + j] = g;
+            }
+            else
+                dS[j * AS_PITCH + i] = g;
+        }
+    }
+}
+
+__device__ __forceinline__ void as_load_stats(const AttnProblem& p, long long nh, int i0, float* lse, float* delta)
+{
+    if (threadIdx.x < AS_TILE)
+    {
+        const int i = i0 + threadIdx.x;
+        lse[threadIdx.x] = i < p.sq ? p.stats[nh * p.sq + i] : INFINITY;
+        delta[threadIdx.x] = i < p.sq ? p.stats[((long long) p.n * p.q_heads + nh) * p.sq + i] : 0.f;
+    }
+}
+
+template <class T, int D>
+__global__ void __launch_bounds__(AS_THREADS) attn_simt_dkv_kernel(AttnProblem p)
+{
+    extern __shared__ float smem[];
+    float *K = smem, *V = K + D * AS_PITCH, *Q = V + D * AS_PITCH, *dO = Q + D * AS_PITCH, *P = dO + D * AS_PITCH,
+          *dS = P + AS_TILE * AS_PITCH;
+    __shared__ float lse[AS_TILE], delta[AS_TILE];
+    __shared__ uint8_t see[AS_TILE];
+    const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+    const AsAt at = as_at(attn_tiles(p.sk, AS_TILE), p.q_splits, p.kv_heads);
+    const int j0 = at.tile * AS_TILE;
+    const uint8_t* qm = p.q_mask ? p.q_mask + at.n * p.sq : nullptr;
+    const uint8_t* km = p.kv_mask ? p.kv_mask + at.n * p.sk : nullptr;
+    as_load<T, D>(K, p.k, at.n, at.head, p.d, j0, p.sk, km);
+    as_load<T, D>(V, p.v, at.n, at.head, p.d, j0, p.sk, km);
+    if (threadIdx.x < AS_TILE)
+        see[threadIdx.x] = j0 + (int) threadIdx.x < p.sk && (!km || km[j0 + threadIdx.x]);
+    float gk[4][D / 16], gv[4][D / 16];
+#pragma unroll
+    for (int a = 0; a < 4; ++a)
+#pragma unroll
+        for (int r = 0; r < D / 16; ++r)
+            gk[a][r] = gv[a][r] = 0.f;
+    const int tiles = attn_tiles(p.sq, AS_TILE);
+    int lo, hi;
+    as_range(tiles * p.group, p.q_splits, at.split, &lo, &hi);
+    for (int u = lo; u < hi; ++u)
+    {
+        const int g = u / tiles, i0 = (u - g * tiles) * AS_TILE, head = at.head * p.group + g;
+        if (p.causal && j0 > (long long) i0 + AS_TILE - 1 + p.offset)
+            continue;
+        __syncthreads();
+        as_load<T, D>(Q, p.q, at.n, head, p.d, i0, p.sq, qm);
+        as_load<T, D>(dO, p.d_o, at.n, head, p.d, i0, p.sq, qm);
+        as_load_stats(p, at.n * p.q_heads + head, i0, lse, delta);
+        __syncthreads();
+        as_weights<D, true>(p, Q, K, V, dO, lse, delta, see, i0, j0, tx, ty, P, dS);
+        __syncthreads();
+        as_accumulate<D>(P, dO, tx, ty, gv);
+        as_accumulate<D>(dS, Q, tx, ty, gk);
+    }
+#pragma unroll
+    for (int a = 0; a < 4; ++a)
+#pragma unroll
+        for (int r = 0; r < D / 16; ++r)
+            gk[a][r] *= p.scale / ATTN_LOG2E;
+    const long long size = (long long) p.n * p.kv_heads * p.d * p.sk * at.split;
+    as_store<T, D>(p.dk, p.q_splits > 1 ? p.part_dk + size : nullptr, at.nh, at.n, at.head, p.d, j0, p.sk, tx, ty, gk);
+    as_store<T, D>(p.dv, p.q_splits > 1 ? p.part_dv + size : nullptr, at.nh, at.n, at.head, p.d, j0, p.sk, tx, ty, gv);
+}
+
+template <class T, int D>
+__global__ void __launch_bounds__(AS_THREADS) attn_simt_dq_kernel(AttnProblem p)
+{
+    extern __shared__ float smem[];
+    float *Q = smem, *dO = Q + D * AS_PITCH, *K = dO + D * AS_PITCH, *V = K + D * AS_PITCH, *dS = V + D * AS_PITCH;
+    __shared__ float lse[AS_TILE], delta[AS_TILE];
+    __shared__ uint8_t see[AS_TILE];
+    const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+    const AsAt at = as_at(attn_tiles(p.sq, AS_TILE), p.kv_splits, p.q_heads);
+    const int i0 = at.tile * AS_TILE, kv_head = at.head / p.group;
+    const uint8_t* qm = p.q_mask ? p.q_mask + at.n * p.sq : nullptr;
+    const uint8_t* km = p.kv_mask ? p.kv_mask + at.n * p.sk : nullptr;
+    as_load<T, D>(Q, p.q, at.n, at.head, p.d, i0, p.sq, qm);
+    as_load<T, D>(dO, p.d_o, at.n, at.head, p.d, i0, p.sq, qm);
+    as_load_stats(p, at.nh, i0, lse, delta);
+    float gq[4][D / 16];
+#pragma unroll
+    for (int a = 0; a < 4; ++a)
+#pragma unroll
+        for (int r = 0; r < D / 16; ++r)
+            gq[a][r] = 0.f;
+    int lo, hi;
+    as_range(attn_tiles(p.sk, AS_TILE), p.kv_splits, at.split, &lo, &hi);
+    if (p.causal)
+        hi = (int) min((long long) hi, max(0ll, (long long) i0 + AS_TILE - 1 + p.offset + AS_TILE) / AS_TILE);
+    for (int t = lo; t < hi; ++t)
+    {
+        const int j0 = t * AS_TILE;
+        __syncthreads();
+        as_load<T, D>(K, p.k, at.n, kv_head, p.d, j0, p.sk, km);
+        as_load<T, D>(V, p.v, at.n, kv_head, p.d, j0, p.sk, km);
+        if (threadIdx.x < AS_TILE)
+            see[threadIdx.x] = j0 + (int) threadIdx.x < p.sk && (!km || km[j0 + threadIdx.x]);
+        __syncthreads();
+        as_weights<D, false>(p, Q, K, V, dO, lse, delta, see, i0, j0, tx, ty, nullptr, dS);
+        __syncthreads();
+        as_accumulate<D>(dS, K, tx, ty, gq);
+    }
+#pragma unroll
+    for (int a = 0; a < 4; ++a)
+#pragma unroll
+        for (int r = 0; r < D / 16; ++r)
+            gq[a][r] *= p.scale / ATTN_LOG2E;
+    float* part = p.kv_splits > 1 ? p.part_dq + (long long) at.split * p.n * p.q_heads * p.d * p.sq : nullptr;
+    as_store<T, D>(p.dq, part, at.nh, at.n, at.head, p.d, i0, p.sq, tx, ty, gq);
+}
+
+int32_t as_launch(void (*kernel)(AttnProblem), const AttnProblem& p, long long blocks, int smem, cudaStream_t stream)
+{
+    DCB_REQUIRE(blocks < (1ll << 31), "too many tiles");
+    if (blocks == 0)
+        return DCB_OK;
+    if (int32_t e = allow_dynamic_smem((const void*) kernel, smem))
+        return e;
+    kernel<<<(unsigned) blocks, AS_THREADS, smem, stream>>>(p);
+    DCB_LAUNCH_CHECK();
+    return DCB_OK;
+}
+
+template <class F>
+int32_t as_with(int32_t dtype, int d, F f)
+{
+    const auto sized = [&](auto t) -> int32_t {
+        if (d <= 32)
+            return f(t, std::integral_constant<int, 32>());
+        if (d <= 64)
+            return f(t, std::integral_constant<int, 64>());
+        return f(t, std::integral_constant<int, 128>());
+    };
+    return dtype == DCB_BF16 ? sized(bf16()) : sized(float());
+}
+
+} // namespace
+
+void attn_simt_splits(AttnProblem* p, bool backward)
+{
+    const long long slots = 2ll * num_sms(); // two blocks an SM, of tiles of 64 channels
+    p->kv_splits = attn_splits((long long) p->n * p->q_heads * attn_tiles(p->sq, AS_TILE), attn_tiles(p->sk, AS_TILE),
+                               slots, AS_LEAST);
+    p->q_splits = !backward ? 1
+                            : attn_splits((long long) p->n * p->kv_heads * attn_tiles(p->sk, AS_TILE),
+                                          attn_tiles(p->sq, AS_TILE) * p->group, slots, AS_LEAST);
+}
+
+int32_t attn_simt_fwd(const AttnProblem& p, int32_t dtype, cudaStream_t stream)
+{
+    return as_with(dtype, p.d, [&](auto t, auto d) {
+        constexpr int D = decltype(d)::value;
+        return as_launch(attn_simt_fwd_kernel<decltype(t), D>, p,
+                         (long long) p.n * p.q_heads * attn_tiles(p.sq, AS_TILE) * p.kv_splits,
+                         (3 * D + AS_TILE) * AS_PITCH * 4, stream);
+    });
+}
+
+int32_t attn_simt_bwd(const AttnProblem& p, int32_t dtype, cudaStream_t stream)
+{
+    return as_with(dtype, p.d, [&](auto t, auto d) {
+        constexpr int D = decltype(d)::value;
+        if (int32_t e = as_launch(attn_simt_dkv_kernel<decltype(t), D>, p,
+                                  (long long) p.n * p.kv_heads * attn_tiles(p.sk, AS_TILE) * p.q_splits,
+                                  (4 * D + 2 * AS_TILE) * AS_PITCH * 4, stream))
+            return e;
+        return as_launch(attn_simt_dq_kernel<decltype(t), D>, p,
+                         (long long) p.n * p.q_heads * attn_tiles(p.sq, AS_TILE) * p.kv_splits,
+                         (4 * D + AS_TILE) * AS_PITCH * 4, stream);
+    });
+}
+
+} // namespace dcb

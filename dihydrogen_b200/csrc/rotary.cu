@@ -1,0 +1,334 @@
+// Rotary positions on a grid: pairs of a head's channels turned by angles that grow along D, H
+// and W.
+//
+// One pass over the tensor, HBM bound.  The angles depend on a pair and on one coordinate of a
+// cell, not on the sample or the head: a thread owns a pair of channels at V neighbouring cells,
+// looks up V cosines and sines in the plan's tables (a few hundred kilobytes, in L2) and walks
+// over the heads with them, several heads' loads in flight.  A channel of no axis is a pair with
+// nothing to turn.
+#include "elem.cuh"
+
+#include <cmath>
+#include <new>
+
+struct dcb_rotary_plan
+{
+    dcb_rotary_desc rd;
+    int64_t n, c, dims[3];
+    float* tables;        // per axis: cosines [pair][position], then sines
+    long long table_at[3]; // in floats
+    int device;
+};
+
+namespace dcb
+{
+namespace
+{
+
+constexpr int ROT_UNROLL = 4; // heads in flight a thread
+
+struct RotArgs
+{
+    CellUnits units;   // of one sample
+    long long per_run, rows, rows_inner;
+    FastDiv w, h;      // a cell's coordinates
+    const float* tables;
+    long long table_at[3];
+    int dims[3];       // D, H, W
+    int first[3];      // an axis' first channel
+    int pairs[3];      // its pairs
+    int turned_pairs;  // of a head, all axes
+    int head_dim, heads, rotated, interleaved;
+    int head_chunks, chunk; // heads of a block: `chunk` from blockIdx.z % head_chunks on
+    int skip_copies;   // in place: what is not turned is there already
+    float sign;
+};
+
+// Slots of a head: its turned pairs, then the channels of no axis two at a time (the last may be alone).
+template <class TX, class TY, int V>
+__global__ void __launch_bounds__(256) rotary_kernel(const TX* x, RunStrides xs, TY* y, RunStrides ys, RotArgs a)
+{
+    wait_for_previous_kernel(x);
+    dependents_may_start();
+    const long long unit = (long long) blockIdx.x * 256 + threadIdx.x;
+    if (unit >= a.units.total)
+        return;
+    const int slot = blockIdx.y;
+    const long long n = blockIdx.z / a.head_chunks;
+    const int head0 = (int) (blockIdx.z - n * a.head_chunks) * a.chunk;
+    const int head1 = min(head0 + a.chunk, a.heads);
+    CellAt at = cell_at<V>(a.units, a.per_run, a.rows, a.rows_inner, unit);
+    at.n = n;
+
+    int c0, c1;
+    float co[V], si[V];
+    const bool turns = slot < a.turned_pairs;
+    if (turns)
+    {
+        int axis = 0, j = slot;
+        while (j >= a.pairs[axis])
+            j -= a.pairs[axis++];
+        c0 = a.first[axis] + (a.interleaved ? 2 * j : j);
+        c1 = c0 + (a.interleaved ? 1 : a.pairs[axis]);
+        const int len = a.dims[axis];
+        const float* cos_of = a.tables + a.table_at[axis] + (long long) j * len;
+        const float* sin_of = cos_of + (long long) a.pairs[axis] * len;
+#pragma unroll
+        for (int e = 0; e < V; ++e)
+        {
+            const uint32_t cell = (uint32_t) at.cell + e;
+            const uint32_t row = a.w.div(cell), plane = a.h.div(row);
+            const uint32_t p = axis == 2 ? cell - row * a.w.d : axis == 1 ? row - plane * a.h.d : plane;
+            co[e] = cos_of[p];
+            si[e] = a.sign * sin_of[p];
+        }
+    }
+    else
+    {
+        c0 = 2 * slot; // 2 turned_pairs channels lie before
+        c1 = c0 + 1 < a.head_dim ? c0 + 1 : -1;
+    }
+
+    const long long xo = offset_of(at, xs), yo = offset_of(at, ys);
+    for (int h = head0; h < head1; h += ROT_UNROLL)
+    {
+        float p[ROT_UNROLL][V], q[ROT_UNROLL][V];
+#pragma unroll
+        for (int i = 0; i < ROT_UNROLL; ++i)
+        {
+            const int head = h + i;
+            if (head >= head1 || (a.skip_copies && !(turns && head < a.rotated)))
+                continue;
+            const TX* px = x + xo + (long long) head * a.head_dim * xs.sc;
+            load_elems<V>(px + c0 * xs.sc, p[i]);
+            if (c1 >= 0)
+                load_elems<V>(px + c1 * xs.sc, q[i]);
+        }
+#pragma unroll
+        for (int i = 0; i < ROT_UNROLL; ++i)
+        {
+            const int head = h + i;
+            if (head >= head1 || (a.skip_copies && !(turns && head < a.rotated)))
+                continue;
+            if (turns && head < a.rotated)
+            {
+#pragma unroll
+                for (int e = 0; e < V; ++e)
+                {
+                    const float r = p[i][e] * co[e] - q[i][e] * si[e];
+                    q[i][e] = p[i][e] * si[e] + q[i][e] * co[e];
+                    p[i][e] = r;
+                }
+            }
+            TY* py = y + yo + (long long) head * a.head_dim * ys.sc;
+            store_elems<V>(py + c0 * ys.sc, p[i]);
+            if (c1 >= 0)
+                store_elems<V>(py + c1 * ys.sc, q[i]);
+        }
+    }
+}
+
+template <class TX, class TY>
+int32_t rotary_launch(int v, dim3 grid, const void* x, const RunStrides& xs, void* y, const RunStrides& ys,
+                      const RotArgs& a, cudaStream_t stream)
+{
+    const auto go = [&](auto kernel) -> int32_t {
+        DCB_CUDA_TRY(launch_overlapped(kernel, grid, 256, 0, stream, static_cast<const TX*>(x), xs,
+                                       static_cast<TY*>(y), ys, a));
+        return DCB_OK;
+    };
+    return v == 4   ? go(rotary_kernel<TX, TY, 4>)
+           : v == 2 ? go(rotary_kernel<TX, TY, 2>)
+                    : go(rotary_kernel<TX, TY, 1>);
+}
+
+bool same_strides(const dcb_nd_desc& a, const dcb_nd_desc& b)
+{
+    return a.sn == b.sn && a.sc == b.sc && a.strides[0] == b.strides[0] && a.strides[1] == b.strides[1]
+           && a.strides[2] == b.strides[2];
+}
+
+} // namespace
+} // namespace dcb
+
+using namespace dcb;
+
+extern "C" {
+
+int32_t dcb_rotary_plan_create(const dcb_rotary_desc* rd, const dcb_nd_desc* xd, dcb_rotary_plan** plan)
+{
+    DCB_REQUIRE(rd && plan, "null argument");
+    *plan = nullptr;
+    if (int32_t e = check_nd_desc(xd))
+        return e;
+    DCB_REQUIRE(rd->nsd == xd->nsd, "nsd differs from the tensor's");
+    DCB_REQUIRE(rd->head_dim >= 1 && xd->c >= 1 && xd->c % rd->head_dim == 0 && xd->c < (1 << 30),
+                "channels must be heads of head_dim");
+    const int64_t heads = xd->c / rd->head_dim;
+    DCB_REQUIRE(rd->rotated_heads >= 0 && rd->rotated_heads <= heads, "rotated_heads out of range");
+    int64_t turned = 0;
+    long long floats = 0;
+    for (int i = 0; i < 3; ++i)
+    {
+        DCB_REQUIRE(rd->axis_channels[i] >= 0 && rd->axis_channels[i] % 2 == 0, "axis_channels must be even");
+        DCB_REQUIRE(std::isfinite(rd->step[i]), "step must be finite");
+        turned += rd->axis_channels[i];
+        floats += (long long) rd->axis_channels[i] * xd->dims[i];
+    }
+    DCB_REQUIRE(rd->nsd == 3 || rd->axis_channels[0] == 0, "a 2-D tensor has no D");
+    DCB_REQUIRE(turned <= rd->head_dim, "axis_channels exceed head_dim");
+    DCB_REQUIRE(std::isfinite(rd->base) && rd->base > 0, "base must be positive");
+    if ((rd->head_dim + 1) / 2 > 65535 || xd->dims[0] * xd->dims[1] >= (1ll << 31) / (xd->dims[2] > 0 ? xd->dims[2] : 1))
+    {
+        set_last_error("unsupported: 2^31 cells of a sample, or heads of 2^17 channels");
+        return DCB_UNSUPPORTED;
+    }
+    dcb_rotary_plan* p = new (std::nothrow) dcb_rotary_plan();
+    std::vector<float> host;
+    try
+    {
+        if (!p)
+            throw std::bad_alloc();
+        host.resize((size_t) floats);
+    }
+    catch (const std::bad_alloc&)
+    {
+        delete p;
+        set_last_error("out of host memory");
+        return DCB_BAD_ARG;
+    }
+    p->rd = *rd;
+    p->n = xd->n;
+    p->c = xd->c;
+    p->tables = nullptr;
+    long long at = 0;
+    for (int i = 0; i < 3; ++i)
+    {
+        p->dims[i] = xd->dims[i];
+        p->table_at[i] = at;
+        const int pairs = rd->axis_channels[i] / 2;
+        for (int j = 0; j < pairs; ++j)
+        {
+            const double per = std::pow(rd->base, -2.0 * j / rd->axis_channels[i]);
+            for (int64_t k = 0; k < xd->dims[i]; ++k)
+            {
+                const double angle = rd->step[i] * (double) (rd->origin[i] + k) * per;
+                host[at + j * xd->dims[i] + k] = (float) std::cos(angle);
+                host[at + (pairs + j) * xd->dims[i] + k] = (float) std::sin(angle);
+            }
+        }
+        at += 2ll * pairs * xd->dims[i];
+    }
+    cudaError_t err = cudaGetDevice(&p->device);
+    if (err == cudaSuccess && floats > 0)
+    {
+        err = cudaMalloc(&p->tables, floats * sizeof(float));
+        if (err == cudaSuccess)
+            err = cudaMemcpy(p->tables, host.data(), floats * sizeof(float), cudaMemcpyHostToDevice);
+    }
+    if (err != cudaSuccess)
+    {
+        set_last_error(std::string("rotary plan: ") + cudaGetErrorString(err));
+        (void) cudaGetLastError();
+        if (p->tables)
+            cudaFree(p->tables);
+        delete p;
+        return DCB_CUDA_ERROR;
+    }
+    *plan = p;
+    return DCB_OK;
+}
+
+int32_t dcb_rotary_plan_destroy(dcb_rotary_plan* plan)
+{
+    if (plan)
+    {
+        if (plan->tables)
+            cudaFree(plan->tables);
+        delete plan;
+    }
+    return DCB_OK;
+}
+
+int32_t dcb_rotary_apply(const dcb_rotary_plan* plan, const dcb_nd_desc* xd, int32_t x_dtype, const void* x,
+                         const dcb_nd_desc* yd, int32_t y_dtype, void* y, int32_t inverse, void* stream)
+{
+    DCB_REQUIRE(plan, "null plan");
+    if (int32_t e = check_nd_desc(xd))
+        return e;
+    if (int32_t e = check_nd_desc(yd))
+        return e;
+    DCB_REQUIRE(same_extents(*xd, *yd), "x and y differ in extents");
+    DCB_REQUIRE(xd->nsd == plan->rd.nsd && xd->c == plan->c && xd->dims[0] == plan->dims[0]
+                    && xd->dims[1] == plan->dims[1] && xd->dims[2] == plan->dims[2],
+                "extents differ from the plan's");
+    DCB_REQUIRE(known_dtype(x_dtype) && known_dtype(y_dtype), "dtype must be DCB_F32 or DCB_BF16");
+    if (xd->n == 0 || xd->dims[0] == 0 || xd->dims[1] == 0 || xd->dims[2] == 0)
+        return DCB_OK;
+    DCB_REQUIRE(x && y, "null tensor");
+    DCB_REQUIRE(x != y || (x_dtype == y_dtype && same_strides(*xd, *yd)),
+                "in place the types and strides must be the same");
+    int device = 0;
+    DCB_CUDA_TRY(cudaGetDevice(&device));
+    DCB_REQUIRE(device == plan->device, "the plan lives on another device");
+    const int level = std::min(run_level(*xd), run_level(*yd));
+    DCB_REQUIRE(level >= 0, "W must have unit stride");
+    RunGeom rg;
+    RunStrides xs, ys;
+    make_runs(*xd, level, &rg, &xs);
+    make_runs(*yd, level, &rg, &ys);
+    drop_unused_strides(rg, &xs);
+    drop_unused_strides(rg, &ys);
+    const int v = std::min(run_vec_of(rg, xs, x, elem_bytes(x_dtype)), run_vec_of(rg, ys, y, elem_bytes(y_dtype)));
+    const dcb_rotary_desc& rd = plan->rd;
+    RotArgs a = {};
+    RunGeom one = rg;
+    one.n = 1;
+    a.units = cell_units(one, v);
+    a.per_run = rg.len / v;
+    a.rows = rg.rows;
+    a.rows_inner = rg.rows_inner;
+    a.w = FastDiv::of((uint32_t) xd->dims[2]);
+    a.h = FastDiv::of((uint32_t) xd->dims[1]);
+    a.tables = plan->tables;
+    int channel = 0;
+    for (int i = 0; i < 3; ++i)
+    {
+        a.table_at[i] = plan->table_at[i];
+        a.dims[i] = (int) xd->dims[i];
+        a.first[i] = channel;
+        a.pairs[i] = rd.axis_channels[i] / 2;
+        channel += rd.axis_channels[i];
+        a.turned_pairs += a.pairs[i];
+    }
+    a.head_dim = rd.head_dim;
+    a.heads = (int) (xd->c / rd.head_dim);
+    a.rotated = rd.rotated_heads;
+    a.interleaved = rd.interleaved != 0;
+    a.skip_copies = x == y;
+    a.sign = inverse ? -1.f : 1.f;
+    if (a.skip_copies && (a.rotated == 0 || a.turned_pairs == 0))
+        return DCB_OK;
+    const long long blocks_x = (a.units.total + 255) / 256;
+    const int slots = a.turned_pairs + (rd.head_dim - channel + 1) / 2;
+    // a thread keeps its angles for as many heads as leave four blocks for every SM's eight
+    a.chunk = a.heads;
+    while (a.chunk > ROT_UNROLL
+           && blocks_x * slots * xd->n * ((a.heads + a.chunk - 1) / a.chunk) < 16ll * num_sms())
+        a.chunk = std::max(ROT_UNROLL, a.chunk / 2);
+    a.head_chunks = (a.heads + a.chunk - 1) / a.chunk;
+    if (blocks_x >= (1ll << 31) || xd->n * a.head_chunks > 65535)
+    {
+        set_last_error("unsupported: more than 65535 samples times head groups");
+        return DCB_UNSUPPORTED;
+    }
+    const dim3 grid((unsigned) blocks_x, slots, (unsigned) (xd->n * a.head_chunks));
+    cudaStream_t s = as_stream(stream);
+    if (x_dtype == DCB_F32)
+        return y_dtype == DCB_F32 ? rotary_launch<float, float>(v, grid, x, xs, y, ys, a, s)
+                                  : rotary_launch<float, bf16>(v, grid, x, xs, y, ys, a, s);
+    return y_dtype == DCB_F32 ? rotary_launch<bf16, float>(v, grid, x, xs, y, ys, a, s)
+                              : rotary_launch<bf16, bf16>(v, grid, x, xs, y, ys, a, s);
+}
+
+} // extern "C"

@@ -14,6 +14,8 @@ Names, argument meaning and return conventions follow the reference:
 * ``Convolution``       convolution.hpp:19-3003
 * ``BatchNormalization`` batchnorm.hpp:100-581
 * ``LeakyReLU``         leaky_relu.hpp
+* ``LayerNormalization``, ``RotaryPositions``, ``Attention``   no counterpart there:
+                        attention blocks over the cells of an image or a volume
 
 Dimension order is the reference's everywhere in this module: index 0 is W,
 then H, [D], C, N; ``-2`` is C and ``-1`` is N.  Device buffers are torch CUDA
@@ -32,6 +34,8 @@ import torch
 
 from . import _abi
 from ._abi import ConvDesc, NdDesc, TensorDesc, call
+
+_DTYPES = {torch.float32: _abi.F32, torch.bfloat16: _abi.BF16}
 
 LHS, RHS = 0, 1
 SIDES = (LHS, RHS)
@@ -57,7 +61,7 @@ class _Geometry:
         self.local, self.overlap, self.pitch = list(t.local_shape), list(t.dist.overlap), t.pitch
         self.size = math.prod(self.local)
         self.strides = t.get_strides()
-        self.base = 4 * t.get_local_offset([0] * t.nd)
+        self.base = t.dtype.itemsize * t.get_local_offset([0] * t.nd)
         self.split_root = t.is_split_root()
         self.owned = tuple(slice(o, o + l) for o, l in reversed(list(zip(self.overlap, self.local))))
         self.descs = {}    # widths -> NdDesc
@@ -222,7 +226,12 @@ class Tensor:
 
     def __init__(self, shape, locale: Locale, dist: Distribution,
                  local_shape_of: Optional[Callable[[Sequence[int]], Sequence[int]]] = None,
-                 pitch_align: Optional[int] = None):
+                 pitch_align: Optional[int] = None, dtype: torch.dtype = torch.float32):
+        """``dtype``: torch.float32, which every operator takes, or torch.bfloat16, for the operators that
+        say so (``LayerNormalization``, ``RotaryPositions``, ``Attention``)."""
+        if dtype not in _DTYPES:
+            raise TypeError(f"a Tensor is of torch.float32 or torch.bfloat16, not {dtype}")
+        self.dtype = dtype
         self.shape = list(shape)
         self.locale = locale
         self.dist = dist.copy()
@@ -253,7 +262,7 @@ class Tensor:
         # that, while the kernels that read the window with its halo fetch from
         # the boundary below it.  Row: [lead pad][halo][owned][halo][tail pad].
         if pitch_align is None:
-            pitch_align = self.PITCH_ALIGN if self.dist.overlap[0] > 0 else 1
+            pitch_align = self.PITCH_ALIGN * 4 // dtype.itemsize if self.dist.overlap[0] > 0 else 1
         self.pitch_align = max(1, int(pitch_align))
         real_w = self.local_shape[0] + 2 * self.dist.overlap[0]
         self.lead = (-self.dist.overlap[0]) % self.pitch_align
@@ -262,7 +271,7 @@ class Tensor:
         self.buffer: Optional[torch.Tensor] = None
         self._storage: Optional[torch.Tensor] = None
 
-    PITCH_ALIGN = 4  # floats: 16 bytes
+    PITCH_ALIGN = 4  # floats: 16 bytes (8 elements of 16 bits)
 
     def _local_of(self, proc_idx):
         if self._local_shape_of is not None:
@@ -341,12 +350,21 @@ class Tensor:
         return g
 
     def _nd(self, lo=None, hi=None):
-        """nd_desc() by reference, made once per pair of widths."""
+        """nd_desc() by reference, made once per pair of widths; for the operators on single precision."""
+        self._single()
+        return self._nd_any(lo, hi)
+
+    def _single(self):
+        if self.dtype is not torch.float32:
+            raise TypeError(f"this operator takes tensors of torch.float32, not {self.dtype}")
+
+    def _nd_any(self, lo=None, hi=None):
+        """The same for the operators that take every type."""
         descs = self._geo().descs
         key = (tuple(lo), tuple(hi)) if lo is not None else None
         d = descs.get(key)
         if d is None:
-            d = descs[key] = self.nd_desc(lo, hi)
+            d = descs[key] = self._make_nd_desc(lo, hi)
         return ctypes.byref(d)
 
     # -- memory --
@@ -368,7 +386,7 @@ class Tensor:
         """A device array laid out like this shard's buffer (rows padded to the
         pitch); pass it to set_view."""
         shp = tuple(reversed(self.get_local_pitched_shape()))
-        return (torch.zeros if zero else torch.empty)(shp, dtype=torch.float32, device=device)
+        return (torch.zeros if zero else torch.empty)(shp, dtype=self.dtype, device=device)
 
     def allocate(self, device="cuda"):
         self.set_view(self.new_storage(device))
@@ -380,6 +398,8 @@ class Tensor:
         shard, of the halo-extended shape.  ``buffer`` is the halo-extended
         shard without the row padding, a strided view when rows are padded
         (it starts ``lead`` floats into the array)."""
+        if buf.dtype != self.dtype:
+            raise TypeError(f"set_view wants an array of {self.dtype}, not {buf.dtype}")
         real_w = self.local_shape[0] + 2 * self.dist.overlap[0]
         if tuple(buf.shape) == self.np_real_shape() and buf.stride(-1) == 1 and (
                 buf.dim() < 2 or buf.stride(-2) == self.pitch):
@@ -417,7 +437,13 @@ class Tensor:
     def zero(self, stream=None):
         _zero_on(stream, self._storage)
 
+    def channel_slice(self, first: int, count: int) -> "ChannelSlice":
+        """``count`` channels from ``first`` on of every sample, in place: a projection's queries, keys or
+        values as ``Attention`` takes them."""
+        return ChannelSlice(self, first, count)
+
     def desc(self) -> TensorDesc:
+        self._single()
         d = TensorDesc()
         d.ndims, d.dtype = self.nd, 0
         real = self.get_local_real_shape()
@@ -439,6 +465,10 @@ class Tensor:
         """cuDNN-style descriptor of the owned cells extended by widths_lo /
         widths_hi halo cells per spatial dimension
         (setup_tensor_descriptor, dnn_backend_impl.hpp:31-70)."""
+        self._single()
+        return self._make_nd_desc(widths_lo, widths_hi)
+
+    def _make_nd_desc(self, widths_lo=None, widths_hi=None) -> NdDesc:
         nsd = self.nd - 2
         lo = widths_lo or [0] * nsd
         hi = widths_hi or [0] * nsd
@@ -463,12 +493,36 @@ class Tensor:
         if off is None:
             lo = list(widths_lo or [0] * (self.nd - 2)) + [0, 0]
             idx = [self.dist.overlap[i] - lo[i] for i in range(self.nd)]
-            off = offsets[key] = 4 * self.get_local_offset(idx, True)
+            off = offsets[key] = self.dtype.itemsize * self.get_local_offset(idx, True)
         return self.buffer.data_ptr() + off
 
     def full_nd_desc(self) -> NdDesc:
         ov = self.dist.overlap[: self.nd - 2]
         return self.nd_desc(ov, ov)
+
+
+class ChannelSlice:
+    """A range of a Tensor's channels (``Tensor.channel_slice``)."""
+
+    def __init__(self, tensor: Tensor, first: int, count: int):
+        if not 0 <= first <= first + count <= tensor.local_shape[-2]:
+            raise ValueError(f"channels {first} to {first + count} of {tensor.local_shape[-2]}")
+        self.tensor, self.first, self.count = tensor, first, count
+        self.dtype, self.dist, self.nd = tensor.dtype, tensor.dist, tensor.nd
+        self.local_shape = tensor.local_shape[:-2] + [count, tensor.local_shape[-1]]
+        self._of = None
+
+    def _nd_any(self):
+        geo = self.tensor._geo()
+        if self._of is not geo:
+            self._of, self._desc = geo, self.tensor._make_nd_desc()
+            self._desc.c = self.count
+            self._base = self.dtype.itemsize * self.first * geo.strides[-2]
+        return ctypes.byref(self._desc)
+
+    def get_base_ptr(self) -> int:
+        self._nd_any()
+        return self.tensor.get_base_ptr() + self._base
 
 
 # ---------------------------------------------------------------------------
@@ -554,7 +608,7 @@ def create_input_tensor(shape, locale_shape, filter_dims, strides, dilations, lo
 
 
 def create_d_input_tensor(input: Tensor) -> Tensor:
-    return Tensor(input.shape, input.locale, input.dist, input._local_shape_of)
+    return Tensor(input.shape, input.locale, input.dist, input._local_shape_of, dtype=input.dtype)
 
 
 def create_convolution_output_tensor(input: Tensor, filter_shape, strides, pads, dilations) -> Tensor:
@@ -1437,6 +1491,281 @@ class BatchNormalization:
         self.backward_allreduce(scale_gradient, bias_gradient, mean_gradient, var_gradient)
         self.backward_stage2(input, d_output, mean, var, scale, mean_gradient, var_gradient, d_input)
         return 0
+
+
+# ---------------------------------------------------------------------------
+# Attention between cells, and what goes with it
+# ---------------------------------------------------------------------------
+def _workspace(nbytes: int, stream, device):
+    """Device memory for one call, from torch's allocator on the stream the call goes to: calls on other
+    streams and captured graphs never share it."""
+    if nbytes <= 0:
+        return None, 0
+    if stream is None:
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
+    else:
+        with torch.cuda.stream(stream):
+            ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
+    return ws, ws.data_ptr()
+
+
+def _check_vector(name, t, shape, dtypes=(torch.float32,), optional=False):
+    """A plain torch operand: the kernels take it as a dense array."""
+    if t is None:
+        if optional:
+            return 0
+        raise ValueError(f"{name} is missing")
+    if t.dtype not in dtypes or not t.is_contiguous() or t.numel() != math.prod(shape):
+        raise ValueError(f"{name} must be a contiguous array of {math.prod(shape)} {dtypes[0]}, not "
+                         f"{list(t.shape)} {t.dtype}")
+    return t.data_ptr()
+
+
+def _check_alike(what, first, *others):
+    for t in others:
+        if t.local_shape != first.local_shape or t.dtype != first.dtype:
+            raise ValueError(f"{what}: local shapes and types must agree: {first.local_shape} {first.dtype} and "
+                             f"{t.local_shape} {t.dtype}")
+
+
+class LayerNormalization:
+    """Layer normalisation over the channels of every cell.  No counterpart in
+    the reference; beside ``BatchNormalization``.  Takes tensors of
+    torch.float32 and torch.bfloat16, partitioned or not: a cell needs its own
+    channels only, and the gradients of scale and bias are all-reduced like
+    batch-norm's.  ``scale``, ``bias`` and their gradients are contiguous torch
+    tensors of C floats, ``mean`` and ``inv_std`` of one float per sample and
+    owned cell."""
+
+    def __init__(self, backend: BackendDNNLib, num_dims: int, epsilon: float):
+        if not epsilon >= 0:
+            raise ValueError("epsilon must not be negative")
+        self.be, self.num_dims, self.epsilon = backend, num_dims, float(epsilon)
+        self._last = (None, 0)
+
+    @staticmethod
+    def _cells(t):
+        return [t.local_shape[-1]] + t.local_shape[:-2]
+
+    def new_statistics(self, input: Tensor):
+        """Memory for ``mean`` and ``inv_std`` of a tensor like ``input``."""
+        both = torch.empty([2] + [self._cells(input)[0], math.prod(self._cells(input)[1:])], dtype=torch.float32,
+                           device=input.buffer.device)
+        return both[0], both[1]
+
+    def forward(self, input: Tensor, scale, bias, output: Tensor, mean=None, inv_std=None):
+        """``scale`` and ``bias`` may be None (1 and 0); so may ``mean`` and
+        ``inv_std`` where no backward pass follows.  ``output`` may be ``input``."""
+        _check_alike("layer normalisation", input, output)
+        C = input.local_shape[-2]
+        cells = self._cells(input)
+        pw, pb = _check_vector("scale", scale, [C], optional=True), _check_vector("bias", bias, [C], optional=True)
+        pm = _check_vector("mean", mean, cells, optional=True)
+        pi = _check_vector("inv_std", inv_std, cells, optional=True)
+        if input.get_local_size() == 0:
+            return 0
+        call("dcb_ln_fwd", input._nd_any(), _DTYPES[input.dtype], input.get_base_ptr(), pw, pb, self.epsilon,
+             output._nd_any(), output.get_base_ptr(), pm, pi, _stream_ptr(self.be.stream))
+        return 0
+
+    def backward_stage1(self, input: Tensor, d_output: Tensor, mean, inv_std, scale, scale_gradient, bias_gradient,
+                        d_input: Tensor):
+        """``d_input`` and this rank's sums of the gradients of scale and bias
+        (None: not wanted).  ``d_input`` may be ``d_output`` or ``input``."""
+        _check_alike("layer normalisation", input, d_output, d_input)
+        C, s = input.local_shape[-2], self.be.stream
+        cells = self._cells(input)
+        pm, pi = _check_vector("mean", mean, cells), _check_vector("inv_std", inv_std, cells)
+        pw = _check_vector("scale", scale, [C], optional=True)
+        if (scale_gradient is None) != (bias_gradient is None):
+            raise ValueError("the gradients of scale and bias are wanted together")
+        gw = _check_vector("scale_gradient", scale_gradient, [C], optional=True)
+        gb = _check_vector("bias_gradient", bias_gradient, [C], optional=True)
+        if input.get_local_size() == 0:
+            if gw:
+                _zero_on(s, scale_gradient, bias_gradient)
+            return 0
+        xd, dtype = input._nd_any(), _DTYPES[input.dtype]
+        nbytes = 0
+        if gw:
+            geo = input._geo()
+            if self._last[0] is not geo:
+                self._last = (geo, _abi.lib().dcb_ln_bwd_workspace_bytes(xd, dtype))
+            nbytes = self._last[1]
+        keep, ws = _workspace(nbytes, s, input.buffer.device)
+        call("dcb_ln_bwd", xd, dtype, input.get_base_ptr(), d_output._nd_any(), d_output.get_base_ptr(), pm, pi, pw,
+             d_input._nd_any(), d_input.get_base_ptr(), gw, gb, ws, nbytes, _stream_ptr(s))
+        if gw and not input._geo().split_root:  # a replica: its cells count once
+            _zero_on(s, scale_gradient, bias_gradient)
+        return 0
+
+    def backward_allreduce(self, scale_gradient, bias_gradient):
+        if scale_gradient is None:
+            return 0
+        ar, s = self.be.allreducer, self.be.stream
+        ar.allreduce(scale_gradient.data_ptr(), scale_gradient.numel(), s)
+        ar.allreduce(bias_gradient.data_ptr(), bias_gradient.numel(), s)
+        return 0
+
+    def backward(self, input: Tensor, d_output: Tensor, mean, inv_std, scale, scale_gradient, bias_gradient,
+                 d_input: Tensor):
+        self.backward_stage1(input, d_output, mean, inv_std, scale, scale_gradient, bias_gradient, d_input)
+        self.backward_allreduce(scale_gradient, bias_gradient)
+        return 0
+
+
+class RotaryPositions:
+    """Rotary positions on the grid of a tensor's cells.  No counterpart in the
+    reference.  Channels are heads of ``head_dim`` channels; of a head the first
+    channels are turned by the position along D (or time), the next ones by the
+    position along H, then W, the rest is copied, as are the heads from
+    ``rotated_heads`` on (the values of a packed projection).  Positions are
+    global: a shard of a partitioned tensor gets the angles of the whole one.
+    Input and output are of torch.float32 or torch.bfloat16 each; a
+    single-precision projection is rounded on its way to ``Attention``."""
+
+    def __init__(self, backend: BackendDNNLib, num_dims: int):
+        self.be, self.num_dims, self.nsd = backend, num_dims, num_dims - 2
+        self._plan = ctypes.c_void_p()
+
+    def __del__(self):
+        try:
+            if getattr(self, "_plan", None):
+                _abi.lib().dcb_rotary_plan_destroy(self._plan)
+        except Exception:
+            pass
+
+    def setup(self, input: Tensor, head_dim: int, axis_channels, rotated_heads: Optional[int] = None,
+              base: float = 10000.0, interleaved: bool = False, step=None):
+        """``axis_channels`` (even; how many of a head's channels belong to an
+        axis) and ``step`` (what a position counts, 1 by default) in reference
+        order (W first).  ``interleaved``: pairs are neighbours, not the two
+        halves of an axis' channels."""
+        nsd = self.nsd
+        if input.nd != self.num_dims or len(axis_channels) != nsd or (step is not None and len(step) != nsd):
+            raise ValueError(f"axis_channels and step have {nsd} entries, W first")
+        if self._plan:
+            _abi.lib().dcb_rotary_plan_destroy(self._plan)
+            self._plan = ctypes.c_void_p()
+        rd = _abi.RotaryDesc()
+        rd.nsd, rd.head_dim, rd.interleaved, rd.base = nsd, head_dim, bool(interleaved), float(base)
+        heads = input.local_shape[-2] // head_dim if head_dim > 0 else 0
+        rd.rotated_heads = heads if rotated_heads is None else rotated_heads
+        for i in range(nsd):
+            rd.axis_channels[2 - i], rd.origin[2 - i] = axis_channels[i], input.offset[i]
+            rd.step[2 - i] = 1.0 if step is None else float(step[i])
+        self._local = list(input.local_shape)
+        call("dcb_rotary_plan_create", ctypes.byref(rd), input._nd_any(), ctypes.byref(self._plan))
+
+    def _apply(self, x: Tensor, y: Tensor, inverse):
+        if x.local_shape[:-1] != self._local[:-1] or y.local_shape != x.local_shape:
+            raise ValueError(f"local shapes {x.local_shape} and {y.local_shape}, set up for {self._local}")
+        if math.prod(x.local_shape) == 0:
+            return 0
+        call("dcb_rotary_apply", self._plan, x._nd_any(), _DTYPES[x.dtype], x.get_base_ptr(), y._nd_any(),
+             _DTYPES[y.dtype], y.get_base_ptr(), inverse, _stream_ptr(self.be.stream))
+        return 0
+
+    def forward(self, input: Tensor, output: Tensor):
+        """``output`` may be ``input``."""
+        return self._apply(input, output, 0)
+
+    def backward(self, d_output: Tensor, d_input: Tensor):
+        """The gradient is turned back by the same angles.  In place, too."""
+        return self._apply(d_output, d_input, 1)
+
+
+class Attention:
+    """Scaled dot-product attention from the cells of one tensor to the cells of
+    another (or its own).  No counterpart in the reference.  ``q``, ``k``, ``v``
+    are Tensors or ``Tensor.channel_slice``s of a packed projection, of
+    torch.float32 (multiplied in fp32) or torch.bfloat16 (tensor cores); query
+    head h reads key head h // (q_heads // kv_heads).  Cells are in memory order
+    (D, H, W); ``causal`` lets cell i of the queries see the keys up to
+    i + (keys - queries).  A sample's cells have to be on one rank: re-distribute
+    a spatially partitioned tensor to sample-parallel first (``TensorShuffler``).
+
+    ``q_mask`` / ``kv_mask``: arrays of bool or uint8, one per sample and cell, 0
+    where a cell is not there; whatever such a cell holds is never read into a
+    result.  A cell that sees nothing gets 0 (``lse``: -infinity) and takes no
+    part in any gradient.  ``lse`` has one float per sample, query head and
+    cell."""
+
+    def __init__(self, backend: BackendDNNLib, num_dims: int, q_heads: int, kv_heads: Optional[int] = None,
+                 scale: Optional[float] = None, causal: bool = False):
+        self.be, self.num_dims = backend, num_dims
+        self.q_heads, self.kv_heads = q_heads, q_heads if kv_heads is None else kv_heads
+        if self.q_heads < 1 or self.kv_heads < 1 or self.q_heads % self.kv_heads:
+            raise ValueError("q_heads must be a multiple of kv_heads")
+        self.scale, self.causal = scale, bool(causal)
+        self._known = {}  # shapes -> (descriptor, workspace bytes forward, backward)
+
+    def _desc(self, q, k):
+        key = (tuple(q.local_shape), tuple(k.local_shape), q.dtype)
+        got = self._known.get(key)
+        if got is None:
+            if q.local_shape[-2] % self.q_heads or q.local_shape[-2] == 0:
+                raise ValueError(f"{q.local_shape[-2]} channels are not {self.q_heads} heads")
+            head_dim = q.local_shape[-2] // self.q_heads
+            ad = _abi.AttentionDesc(self.q_heads, self.kv_heads, _DTYPES[q.dtype], self.causal,
+                                    1.0 / math.sqrt(head_dim) if self.scale is None else self.scale)
+            size = []
+            for backward in (0, 1):
+                n = _abi.lib().dcb_attention_workspace_bytes(ctypes.byref(ad), q._nd_any(), k._nd_any(), backward)
+                if n < 0:
+                    raise ValueError("attention: " + _abi.lib().dcb_last_error().decode())
+                size.append(n)
+            got = self._known[key] = (ad, size)
+        return got
+
+    def _checked(self, q, k, v, q_like, kv_like, lse, q_mask, kv_mask):
+        for t in (q, k):
+            if t.nd != self.num_dims:
+                raise ValueError(f"a tensor of {t.nd} dimensions, set up for {self.num_dims}")
+        for t in (q, k, v) + q_like + kv_like:
+            for dim in range(t.nd - 1):
+                if t.dist.is_distributed(dim) and t.dist.locale_shape[dim] > 1:
+                    raise ValueError("attention needs all cells and channels of a sample on one rank: "
+                                     "re-distribute the tensor (TensorShuffler)")
+        _check_alike("attention", q, *q_like)
+        _check_alike("attention", k, v, *kv_like)
+        if q.dtype != k.dtype or q.local_shape[-1] != k.local_shape[-1]:
+            raise ValueError("attention: queries and keys differ in type or samples")
+        n, cells_q, cells_k = q.local_shape[-1], math.prod(q.local_shape[:-2]), math.prod(k.local_shape[:-2])
+        masks = (torch.bool, torch.uint8)
+        return (_check_vector("lse", lse, [n, self.q_heads, cells_q]),
+                _check_vector("q_mask", q_mask, [n, cells_q], masks, True),
+                _check_vector("kv_mask", kv_mask, [n, cells_k], masks, True))
+
+    def forward(self, q, k, v, output: Tensor, lse, q_mask=None, kv_mask=None):
+        pl, pq, pk = self._checked(q, k, v, (output,), (), lse, q_mask, kv_mask)
+        if math.prod(q.local_shape) == 0:
+            return 0
+        ad, size = self._desc(q, k)
+        s = self.be.stream
+        keep, ws = _workspace(size[0], s, lse.device)
+        call("dcb_attention_fwd", ctypes.byref(ad), q._nd_any(), q.get_base_ptr(), k._nd_any(), k.get_base_ptr(),
+             v._nd_any(), v.get_base_ptr(), pq, pk, output._nd_any(), output.get_base_ptr(), pl, ws, size[0],
+             _stream_ptr(s))
+        return 0
+
+    def backward(self, q, k, v, output: Tensor, lse, d_output: Tensor, d_q, d_k, d_v, q_mask=None, kv_mask=None):
+        """``output`` and ``lse`` as ``forward`` left them, with the same masks."""
+        pl, pq, pk = self._checked(q, k, v, (output, d_output, d_q), (d_k, d_v), lse, q_mask, kv_mask)
+        if q.local_shape[-1] == 0:
+            return 0
+        ad, size = self._desc(q, k)
+        s = self.be.stream
+        keep, ws = _workspace(size[1], s, lse.device)
+        call("dcb_attention_bwd", ctypes.byref(ad), q._nd_any(), q.get_base_ptr(), k._nd_any(), k.get_base_ptr(),
+             v._nd_any(), v.get_base_ptr(), pq, pk, output._nd_any(), output.get_base_ptr(), pl, d_output._nd_any(),
+             d_output.get_base_ptr(), d_q._nd_any(), d_q.get_base_ptr(), d_k._nd_any(), d_k.get_base_ptr(),
+             d_v._nd_any(), d_v.get_base_ptr(), ws, size[1], _stream_ptr(s))
+        return 0
+
+    def status(self) -> int:
+        """Whether a kernel gave up on one of its bounded waits since the last call (synchronises)."""
+        return _abi.lib().dcb_attention_status(_stream_ptr(self.be.stream))
 
 
 class Pooling:

@@ -82,7 +82,9 @@ typedef struct dcb_tensor_desc
     int64_t pitch; /* row pitch in elements; 0 = real_shape[0] */
 } dcb_tensor_desc;
 
+/* Element types.  Every entry point takes fp32 unless it has a dtype argument. */
 #define DCB_F32 0
+#define DCB_BF16 1
 
 /* ------------------------------------------------------------------------
  * Halo exchange.
@@ -401,6 +403,144 @@ int32_t dcb_pool_bwd(const dcb_pool_desc* pd, const dcb_nd_desc* xd,
 int64_t dcb_pool_bwd_workspace_bytes(const dcb_pool_desc* pd,
                                      const dcb_nd_desc* xd,
                                      const dcb_nd_desc* yd);
+
+/* ------------------------------------------------------------------------
+ * Layer normalisation over the channels of every cell (no counterpart in the
+ * reference, whose only normalisation is the batch-norm above; what attention
+ * over the cells of an image or a volume is built with).  Per sample and cell
+ *   mean = sum_c x / C,  inv_std = 1 / sqrt(sum_c (x - mean)^2 / C + eps),
+ *   y[c] = (x[c] - mean) * inv_std * scale[c] + bias[c].
+ * A cell needs its own channels only, so a partitioned tensor needs no
+ * communication but for the sums over cells of the gradients of scale and bias.
+ * x, y, dy, dx are of `dtype` (DCB_F32 or DCB_BF16; W has unit stride; no other
+ * stride is restricted and the descriptors may differ in strides); scale, bias and
+ * their gradients are C floats; mean and inv_std are one float per sample and
+ * cell, dense in the order N, D, H, W.  All sums are fp32 or wider.
+ * ------------------------------------------------------------------------ */
+/* scale and bias may be null (1 and 0), mean and inv_std too (not wanted).  y may
+ * be x. */
+int32_t dcb_ln_fwd(const dcb_nd_desc* xd, int32_t dtype, const void* x,
+                   const void* scale, const void* bias, float eps,
+                   const dcb_nd_desc* yd, void* y, void* mean, void* inv_std,
+                   void* stream);
+/* With g = dy * scale and u = (x - mean) * inv_std:
+ *   dx = inv_std * (g - sum_c g / C - u * sum_c (g * u) / C),
+ *   dscale[c] = sum dy * u,  dbias[c] = sum dy  over the cells xd describes
+ * (overwritten; a partitioned tensor's are then all-reduced).  mean and inv_std as
+ * dcb_ln_fwd left them; scale may be null; dscale and dbias may both be null (not
+ * wanted), and no workspace is needed then.  dx may be dy or x.  The sums over
+ * cells are taken in a fixed order: the same bits every run. */
+int32_t dcb_ln_bwd(const dcb_nd_desc* xd, int32_t dtype, const void* x,
+                   const dcb_nd_desc* dyd, const void* dy, const void* mean,
+                   const void* inv_std, const void* scale,
+                   const dcb_nd_desc* dxd, void* dx, void* dscale, void* dbias,
+                   void* workspace, int64_t workspace_bytes, void* stream);
+/* Device bytes dcb_ln_bwd needs on the current device (16-byte aligned; -1 for a
+ * bad descriptor).  Calls that may overlap need a workspace each. */
+int64_t dcb_ln_bwd_workspace_bytes(const dcb_nd_desc* xd, int32_t dtype);
+
+/* ------------------------------------------------------------------------
+ * Rotary positions on a grid (no counterpart in the reference).  A tensor's
+ * channels are heads of head_dim channels; the first axis_channels[0] channels of
+ * a head belong to D (or time), the next axis_channels[1] to H, the next
+ * axis_channels[2] to W, the rest to no axis.  Of an axis with a channels, pair j
+ * (channels j and j + a/2 of the axis, or 2j and 2j + 1 where `interleaved`) is
+ * turned by the angle
+ *   position * base^(-2j / a),  position = step * (origin + index along the axis):
+ *   (p, q) -> (p cos - q sin, p sin + q cos).
+ * Heads from rotated_heads on, and channels of no axis, are copied.  `origin` is
+ * the global index of the window's first cell, so that a shard of a partitioned
+ * tensor gets the angles of the whole one.
+ * ------------------------------------------------------------------------ */
+typedef struct dcb_rotary_desc
+{
+    int32_t nsd;
+    int32_t head_dim;
+    int32_t axis_channels[DCB_MAX_SPATIAL]; /* D,H,W; even; D: 0 if nsd == 2 */
+    int32_t rotated_heads;
+    int32_t interleaved;
+    int64_t origin[DCB_MAX_SPATIAL];
+    double base;
+    double step[DCB_MAX_SPATIAL];
+} dcb_rotary_desc;
+
+typedef struct dcb_rotary_plan dcb_rotary_plan;
+/* Checks the geometry and lays down the cosines and sines of the window's
+ * positions (worked out in fp64, held as fp32).  xd: extents only. */
+int32_t dcb_rotary_plan_create(const dcb_rotary_desc* rd,
+                               const dcb_nd_desc* xd, dcb_rotary_plan** plan);
+int32_t dcb_rotary_plan_destroy(dcb_rotary_plan* plan);
+/* y = turned x; inverse != 0 turns back, which is also the gradient.  The types
+ * may differ (x is rounded once, as it is written).  xd and yd have the plan's
+ * extents; W has unit stride; y may be x where type and strides are the same.
+ * Reads the plan only: calls may overlap.  The plan and the tensors live on the
+ * current device. */
+int32_t dcb_rotary_apply(const dcb_rotary_plan* plan, const dcb_nd_desc* xd,
+                         int32_t x_dtype, const void* x, const dcb_nd_desc* yd,
+                         int32_t y_dtype, void* y, int32_t inverse,
+                         void* stream);
+
+/* ------------------------------------------------------------------------
+ * Attention between the cells of a tensor, or from one tensor's cells to
+ * another's (no counterpart in the reference).  Channels are heads of
+ * head_dim = qd->c / q_heads channels; query head h reads key / value head
+ * h / (q_heads / kv_heads).  Per sample and head, over the cells i of q and j of
+ * k and v in the order D, H, W:
+ *   s_ij = scale * sum_d q_di k_dj   where i may see j,
+ *   o_di = sum_j v_dj exp(s_ij) / sum_j exp(s_ij),  lse_i = log sum_j exp(s_ij).
+ * i may see j if q_mask (n x cells of q bytes, may be null) is not 0 at i, kv_mask
+ * (n x cells of k) not at j, and, where `causal`, j <= i + (cells of k - cells of
+ * q).  A cell that sees nothing gets o = 0, lse = -infinity and takes no part in
+ * any gradient.  Cells that a mask takes out are never interpreted, whatever they
+ * hold; `causal` only sets the weight of a later cell to 0, its values have to be
+ * finite.  A sample's cells lie contiguous (a shard without halo; re-distribute a
+ * spatially partitioned tensor to sample-parallel first); sample and channel
+ * strides are free.  All tensors are of desc->dtype; lse is n x q_heads x cells of
+ * q floats.  fp32 tensors are multiplied in fp32; bf16 tensors on the tensor cores
+ * with fp32 accumulation, and their weights exp(s) are rounded to bf16.  The same
+ * bits every run.
+ * ------------------------------------------------------------------------ */
+typedef struct dcb_attention_desc
+{
+    int32_t q_heads, kv_heads; /* q_heads a multiple of kv_heads */
+    int32_t dtype;             /* DCB_F32, DCB_BF16 */
+    int32_t causal;
+    float scale;               /* positive */
+} dcb_attention_desc;
+
+/* head_dim of 129 and more: DCB_UNSUPPORTED.  vd has kd's extents, od qd's. */
+int32_t dcb_attention_fwd(const dcb_attention_desc* ad, const dcb_nd_desc* qd,
+                          const void* q, const dcb_nd_desc* kd, const void* k,
+                          const dcb_nd_desc* vd, const void* v,
+                          const void* q_mask, const void* kv_mask,
+                          const dcb_nd_desc* od, void* o, void* lse,
+                          void* workspace, int64_t workspace_bytes,
+                          void* stream);
+/* The gradients of q, k and v, the scores worked out again from q, k and lse.  o
+ * and lse as dcb_attention_fwd left them; dod, dqd have qd's extents, dkd, dvd
+ * kd's.  The gradients of a key head are sums over the query heads that read it. */
+int32_t dcb_attention_bwd(const dcb_attention_desc* ad, const dcb_nd_desc* qd,
+                          const void* q, const dcb_nd_desc* kd, const void* k,
+                          const dcb_nd_desc* vd, const void* v,
+                          const void* q_mask, const void* kv_mask,
+                          const dcb_nd_desc* od, const void* o,
+                          const void* lse, const dcb_nd_desc* dod,
+                          const void* d_o, const dcb_nd_desc* dqd, void* dq,
+                          const dcb_nd_desc* dkd, void* dk,
+                          const dcb_nd_desc* dvd, void* dv, void* workspace,
+                          int64_t workspace_bytes, void* stream);
+/* Device bytes that dcb_attention_fwd (backward == 0) or dcb_attention_bwd needs
+ * on the current device, whatever the tensors' strides and masks (256-byte
+ * aligned; -1 for a bad descriptor).  Calls that may overlap need a workspace
+ * each; nothing is kept in it between calls. */
+int64_t dcb_attention_workspace_bytes(const dcb_attention_desc* ad,
+                                      const dcb_nd_desc* qd,
+                                      const dcb_nd_desc* kd, int32_t backward);
+/* Synchronises `stream`, then reports whether a tensor-core kernel of an attention
+ * on the current device gave up on one of its bounded pipeline waits since the
+ * last call (DCB_CUDA_ERROR, record cleared) or not (DCB_OK).  Such a launch
+ * leaves its output incomplete. */
+int32_t dcb_attention_status(void* stream);
 
 /* ------------------------------------------------------------------------
  * Re-distribution between two block decompositions of one global tensor.

@@ -1,0 +1,306 @@
+"""Attention on the GPU, forward and backward, against its definition in 64 bits (attn_ref.attention)."""
+import math
+
+import pytest
+import torch
+
+import attn_ref as R
+import dihydrogen_b200 as dc
+from test_gpu_ln import backend, tensor
+
+pytestmark = pytest.mark.gpu
+TYPES = [torch.float32, torch.bfloat16]
+NAN = float("nan")
+
+
+def heads(t, h):
+    """[n, h d, dims] -> [n, h, cells, d]"""
+    n = t.shape[0]
+    return t.reshape(n, h, t.shape[1] // h, -1).transpose(-1, -2)
+
+
+def run(n, hq, hk, d, q_dims, kv_dims, dtype, causal=False, q_mask=None, kv_mask=None, seed=0, std=1.3, pad=0, mean=0.0,
+        poison=None, be=None, want_grad=True):
+    """One forward and backward pass; checks everything and returns what came out."""
+    g = torch.Generator().manual_seed(seed)
+    rnd = lambda h, dims: (torch.randn(n, h * d, *dims, generator=g) * std + mean).to(dtype)
+    q, k, v, do = rnd(hq, q_dims), rnd(hk, kv_dims), rnd(hk, kv_dims), rnd(hq, q_dims)
+    want = R.attention(heads(q, hq), heads(k, hk), heads(v, hk), 1 / math.sqrt(d), causal, q_mask, kv_mask,
+                       heads(do, hq) if want_grad else None, dtype)
+    dev = [t.cuda() for t in (q, k, v, do)]
+    if poison is not None:  # cells that are not there hold anything
+        for t, m in zip(dev, (q_mask, kv_mask, kv_mask, q_mask)):
+            if m is not None:
+                t.flatten(2).masked_fill_(~m.bool().cuda()[:, None, :], poison)
+    be = be or backend()
+    tq, tk, tv, tdo = (tensor(t, be, pad) for t in dev)
+    o, dq, dk, dv = (tensor(torch.full_like(t, NAN), be, pad) for t in (dev[0], dev[0], dev[1], dev[2]))
+    lse = torch.full((n, hq, math.prod(q_dims)), NAN, device="cuda")
+    at = dc.Attention(be, len(q_dims) + 2, hq, hk, causal=causal)
+    masks = dict(q_mask=None if q_mask is None else q_mask.cuda(), kv_mask=None if kv_mask is None else kv_mask.cuda())
+    at.forward(tq, tk, tv, o, lse, **masks)
+    if want_grad:
+        at.backward(tq, tk, tv, o, lse, tdo, dq, dk, dv, **masks)
+    assert at.status() == dc.distconv._abi.OK
+    assert torch.equal(torch.isneginf(lse.cpu()), torch.isneginf(want["lse"][0]))
+    R.close(lse, want["lse"], "lse")
+    R.close(heads(o.buffer, hq), want["o"], "o")
+    if want_grad:
+        R.close(heads(dq.buffer, hq), want["dq"], "dq")
+        R.close(heads(dk.buffer, hk), want["dk"], "dk")
+        R.close(heads(dv.buffer, hk), want["dv"], "dv")
+    return o.buffer, lse, dq.buffer, dk.buffer, dv.buffer
+
+
+SHAPES = [
+    # n, q heads, kv heads, channels of a head, cells of q, cells of k
+    (1, 1, 1, 16, (1, 1), (1, 1)),
+    (2, 2, 1, 8, (1, 1), (1, 7)),
+    (1, 2, 2, 32, (1, 63), (1, 65)),
+    (1, 1, 1, 64, (8, 16), (8, 16)),
+    (2, 4, 2, 64, (3, 5, 7), (3, 5, 7)),
+    (1, 2, 1, 128, (10, 13), (10, 13)),
+    (1, 3, 1, 40, (11, 12), (9, 31)),
+    (2, 2, 2, 80, (4, 4, 8), (5, 5, 13)),
+    (1, 8, 2, 96, (16, 20), (16, 20)),
+    (1, 1, 1, 1, (4, 9), (5, 8)),
+    (1, 2, 2, 7, (4, 9), (5, 8)),
+    (1, 2, 2, 64, (24, 24), (24, 24)),
+    (1, 2, 1, 128, (2, 150), (1, 520)),
+]
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=["f32", "bf16"])
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("shape", SHAPES, ids=str)
+def test_forward_and_backward(shape, causal, dtype):
+    run(*shape, dtype, causal=causal)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=["f32", "bf16"])
+@pytest.mark.parametrize("shape", [(1, 4, 4, 64, (1, 1), (30, 70)), (2, 8, 2, 128, (1, 2), (1, 5000)),
+                                   (1, 1, 1, 64, (60, 70), (1, 3)), (1, 2, 1, 32, (1, 130), (40, 101))], ids=str)
+def test_few_cells_against_many(shape, dtype):
+    """Long axes are split over blocks and joined."""
+    run(*shape, dtype)
+    run(*shape, dtype, causal=True)
+
+
+@pytest.mark.parametrize("poison", [0.0, NAN, float("inf"), -3.3e38])
+@pytest.mark.parametrize("dtype", TYPES, ids=["f32", "bf16"])
+@pytest.mark.parametrize("causal", [False, True])
+def test_masks(causal, dtype, poison):
+    """Random masks, a sample without keys, one without queries; what masked cells hold is never seen."""
+    g = torch.Generator().manual_seed(11)
+    for q_dims, kv_dims, d in (((9, 17), (9, 17), 64), ((1, 200), (13, 23), 32), ((3, 4), (1, 700), 128)):
+        qm = torch.rand(4, math.prod(q_dims), generator=g) < 0.7
+        km = torch.rand(4, math.prod(kv_dims), generator=g) < 0.6
+        km[1], qm[2] = False, False
+        km[3, : km.shape[1] // 2] = False
+        run(4, 2, 1, d, q_dims, kv_dims, dtype, causal=causal, q_mask=qm, kv_mask=km, poison=poison)
+        run(4, 2, 1, d, q_dims, kv_dims, dtype, causal=causal, kv_mask=km, poison=poison)
+        run(4, 2, 1, d, q_dims, kv_dims, dtype, causal=causal, q_mask=qm, poison=poison)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=["f32", "bf16"])
+def test_more_queries_than_keys_under_causal_order(dtype):
+    """The first cells see nothing."""
+    run(2, 2, 2, 64, (1, 300), (1, 140), dtype, causal=True)
+    run(1, 2, 1, 32, (1, 130), (1, 1), dtype, causal=True)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=["f32", "bf16"])
+@pytest.mark.parametrize("pad", [1, 3, 8])
+def test_unaligned_tensors(pad, dtype):
+    run(2, 4, 2, 64, (8, 16), (8, 24), dtype, pad=pad)
+    run(1, 2, 2, 72, (5, 27), (5, 27), dtype, pad=pad, causal=True)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=["f32", "bf16"])
+def test_large_and_equal_scores(dtype):
+    """Scores far from zero (the maximum is taken out), growing along the keys, and all the same."""
+    run(1, 2, 2, 64, (1, 140), (1, 300), dtype, std=4.0)
+    run(1, 1, 1, 16, (1, 140), (1, 300), dtype, std=0.0, mean=2.0)
+    g = torch.Generator().manual_seed(4)
+    q, k, v = (torch.randn(1, 64, 1, 400, generator=g) for _ in range(3))
+    k = k + torch.linspace(0, 3, 400) * q.mean(-1, keepdim=True).sign()
+    q = q + q.mean(-1, keepdim=True).sign()
+    be = backend()
+    q, k, v = (t.to(dtype) for t in (q, k, v))
+    want = R.attention(heads(q, 1), heads(k, 1), heads(v, 1), 0.125, dtype=dtype)
+    ts = [tensor(t.cuda(), be) for t in (q, k, v, q)]
+    lse = torch.empty(1, 1, 400, device="cuda")
+    dc.Attention(be, 4, 1).forward(*ts, lse)
+    R.close(heads(ts[3].buffer, 1), want["o"], "o")
+    R.close(lse, want["lse"], "lse")
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=["f32", "bf16"])
+def test_packed_projection_and_other_channels_untouched(dtype):
+    """q, k and v are channels of one tensor, their gradients of another; what lies between stays."""
+    g = torch.Generator().manual_seed(5)
+    n, hq, hk, d, dims = 2, 4, 2, 32, (6, 22)
+    qkv = torch.randn(n, (hq + 2 * hk) * d + 5, *dims, generator=g).to(dtype)
+    do = torch.randn(n, hq * d, *dims, generator=g).to(dtype)
+    be = backend()
+    t, dt = tensor(qkv.cuda(), be), tensor(torch.full_like(qkv, 3.0).cuda(), be)
+    o, tdo = tensor(torch.empty_like(do).cuda(), be), tensor(do.cuda(), be)
+    lse = torch.empty(n, hq, 132, device="cuda")
+    cut = lambda x: (x.channel_slice(5, hq * d), x.channel_slice(5 + hq * d, hk * d),
+                     x.channel_slice(5 + (hq + hk) * d, hk * d))
+    at = dc.Attention(be, 4, hq, hk)
+    at.forward(*cut(t), o, lse)
+    at.backward(*cut(t), o, lse, tdo, *cut(dt))
+    q, k, v = qkv[:, 5:].split([hq * d, hk * d, hk * d], 1)
+    want = R.attention(heads(q, hq), heads(k, hk), heads(v, hk), 1 / math.sqrt(d), d_o=heads(do, hq), dtype=dtype)
+    R.close(heads(o.buffer, hq), want["o"], "o")
+    assert bool((dt.buffer[:, :5] == 3.0).all())
+    dq, dk, dv = dt.buffer[:, 5:].split([hq * d, hk * d, hk * d], 1)
+    for name, x, h in (("dq", dq, hq), ("dk", dk, hk), ("dv", dv, hk)):
+        R.close(heads(x, h), want[name], name)
+
+
+def test_gradients_against_differences():
+    g = torch.Generator().manual_seed(6)
+    q, k, v, do = (torch.randn(1, 16, 3, 7, generator=g) for _ in range(4))
+    be = backend()
+    ts = [tensor(t.cuda(), be) for t in (q, k, v, do)]
+    o, dq, dk, dv = (tensor(torch.empty_like(q).cuda(), be) for _ in range(4))
+    lse = torch.empty(1, 2, 21, device="cuda")
+    at = dc.Attention(be, 4, 2)
+    at.forward(*ts[:3], o, lse)
+    at.backward(*ts[:3], o, lse, ts[3], dq, dk, dv)
+
+    def f(*x):
+        return (R.attention(*[heads(t, 2) for t in x], 8 ** -0.5)["o"][0] * heads(do, 2).double()).sum()
+
+    h, x = 1e-5, [t.double() for t in (q, k, v)]
+    for which, grad in enumerate((dq, dk, dv)):
+        for at_ in ((0, 0, 0, 0), (0, 9, 2, 3), (0, 15, 1, 6)):
+            step = torch.zeros_like(x[0])
+            step[at_] = h
+            up = [t + step if i == which else t for i, t in enumerate(x)]
+            down = [t - step if i == which else t for i, t in enumerate(x)]
+            slope = float(f(*up) - f(*down)) / (2 * h)
+            have = grad.buffer.cpu().double()
+            assert abs(slope - float(have[at_])) <= 1e-5 * float(have.abs().max())
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=["f32", "bf16"])
+def test_the_same_bits_every_run_on_streams_and_in_graphs(dtype):
+    shape = dict(n=2, hq=4, hk=2, d=64, q_dims=(9, 31), kv_dims=(9, 31))
+    first = [t.clone() for t in run(*shape.values(), dtype)]
+    s = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    again = run(*shape.values(), dtype, be=backend(s))
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(first, again))
+
+    g = torch.Generator().manual_seed(8)
+    be = backend()
+    sets = []
+    for k in range(2):
+        q, kk, v, do = (tensor((torch.randn(1, 128, 1, c, generator=g)).to(dtype).cuda(), be) for c in (40, 900, 900, 40))
+        o, dq, dk, dv = (tensor(torch.empty_like(t.buffer), be) for t in (q, q, kk, v))
+        lse = torch.empty(1, 2, 40, device="cuda")
+        at = dc.Attention(be, 4, 2)
+
+        def step():
+            at.forward(q, kk, v, o, lse)
+            at.backward(q, kk, v, o, lse, do, dq, dk, dv)
+
+        step()
+        torch.cuda.synchronize()
+        out = [t.buffer for t in (o, dq, dk, dv)] + [lse]
+        want = [t.clone() for t in out]
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            step()
+        sets.append((graph, out, want, (q, kk, v, do)))
+    streams = [torch.cuda.Stream() for _ in sets]
+    for _ in range(4):
+        for st, x in zip(streams, sets):
+            with torch.cuda.stream(st):
+                x[0].replay()
+    torch.cuda.synchronize()
+    for _g, out, want, _k in sets:
+        assert all(torch.equal(a, b) for a, b in zip(out, want))
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=["f32", "bf16"])
+def test_empty_sides(dtype):
+    be = backend()
+    at = dc.Attention(be, 4, 2)
+    e = lambda c: tensor(torch.full((2, 32, 1, c), 5.0, device="cuda").to(dtype), be)
+    q, k, o, dq, dk, dv = e(9), e(0), e(9), e(9), e(0), e(0)
+    lse = torch.zeros(2, 2, 9, device="cuda")
+    at.forward(q, k, k, o, lse)
+    assert not o.buffer.any() and bool(torch.isneginf(lse).all())
+    at.backward(q, k, k, o, lse, o, dq, dk, dv)
+    assert not dq.buffer.any()
+    q, k, dk, dv = e(0), e(9), e(9), e(9)
+    lse = torch.zeros(2, 2, 0, device="cuda")
+    at.forward(q, k, k, q, lse)
+    at.backward(q, k, k, q, lse, q, q, dk, dv)
+    assert not dk.buffer.any() and not dv.buffer.any()
+
+
+def test_a_block_of_a_network():
+    """Layer norm, projection by a 1 x 1 convolution, rotary positions, attention, and all their gradients."""
+    torch.manual_seed(0)
+    n, c, h, d, dims = 1, 16, 2, 16, (12, 20)
+    be = backend()
+    x, w = torch.randn(n, c, *dims), torch.randn(3 * h * d, c, 1, 1) / 4
+    dy = torch.randn(n, h * d, *dims)
+    gamma, beta = torch.rand(c) + 0.5, torch.randn(c)
+    new = lambda ch, dtype=torch.float32: tensor(torch.empty(n, ch, *dims, dtype=dtype, device="cuda"), be)
+    tx, u, du, dx = tensor(x.cuda(), be), new(c), new(c), new(c)
+    qkv, dqkv = new(3 * h * d), new(3 * h * d)
+    r, dr, o = new(3 * h * d, torch.bfloat16), new(3 * h * d, torch.bfloat16), new(h * d, torch.bfloat16)
+    tdo = tensor(dy.bfloat16().cuda(), be)
+    wt, dw = w.cuda(), torch.empty_like(w).cuda()
+    gc, bc, dg, db = gamma.cuda(), beta.cuda(), torch.empty(c, device="cuda"), torch.empty(c, device="cuda")
+    ln, rot, at = dc.LayerNormalization(be, 4, 1e-5), dc.RotaryPositions(be, 4), dc.Attention(be, 4, h)
+    conv = dc.Convolution(be, 4)
+    conv.setup(u, wt, qkv, du, dw, dqkv, [0, 0], [1, 1], [1, 1])
+    rot.setup(qkv, d, [8, 8], rotated_heads=2 * h)
+    mean, inv = ln.new_statistics(tx)
+    lse = torch.empty(n, h, 240, device="cuda")
+    cut = lambda t: [t.channel_slice(i * h * d, h * d) for i in range(3)]
+    ln.forward(tx, gc, bc, u, mean, inv)
+    conv.forward(1.0, u, wt, 0.0, qkv)
+    rot.forward(qkv, r)
+    at.forward(*cut(r), o, lse)
+    at.backward(*cut(r), o, lse, tdo, *cut(dr))
+    rot.backward(dr, dqkv)
+    conv.backward_data(1.0, wt, dqkv, 0.0, du)
+    conv.backward_filter(1.0, u, dqkv, 0.0, dw)
+    ln.backward(tx, du, mean, inv, gc, dg, db, dx)
+    assert at.status() == dc.distconv._abi.OK
+
+    leaves = [t.double().requires_grad_() for t in (x, gamma, beta, w)]
+    lx, lg, lb, lw = leaves
+    m = lx.mean(1, keepdim=True)
+    un = (lx - m) / torch.sqrt(((lx - m) ** 2).mean(1, keepdim=True) + 1e-5) * lg[None, :, None, None] + lb[None, :, None, None]
+    proj = torch.einsum("kc,ncyx->nkyx", lw[:, :, 0, 0], un).reshape(n, 3, h, d, *dims)
+    parts = []
+    for i in range(3):
+        t = proj[:, i]
+        if i < 2:
+            out = []
+            for axis, first in ((0, 0), (1, 8)):
+                pos = torch.arange(dims[axis], dtype=torch.float64).reshape((-1, 1) if axis == 0 else (1, -1))
+                ang = torch.stack([pos * 10000.0 ** (-2.0 * j / 8) for j in range(4)]).expand(4, *[s if k == axis else 1 for k, s in enumerate(dims)])
+                p, q = t[:, :, first:first + 4], t[:, :, first + 4:first + 8]
+                out += [p * ang.cos() - q * ang.sin(), p * ang.sin() + q * ang.cos()]
+            t = torch.cat(out, 2)
+        parts.append(t.reshape(n, h, d, -1).transpose(-1, -2))
+    q, k, v = parts
+    y = torch.softmax(q @ k.transpose(-1, -2) / 4.0, -1) @ v
+    y.backward(dy.bfloat16().double().reshape(n, h, d, -1).transpose(-1, -2))
+    # q, k, v (2^-8 each), weights, o, and the gradients' roundings: eight roundings of 2^-8 in the norm, each at most
+    # carried over once with a factor of about 1
+    rel = lambda a, b: float((a.double().cpu() - b).norm() / b.norm())
+    assert rel(heads(o.buffer, h), y.detach()) < 8 * 2 ** -8
+    for got, leaf in ((dx.buffer, lx), (dg, lg), (db, lb), (dw, lw)):
+        assert rel(got.reshape(leaf.shape), leaf.grad) < 8 * 2 ** -8
