@@ -59,12 +59,13 @@ __global__ void __launch_bounds__(256) attn_join_grad_kernel(const float* part, 
 template <class T>
 __global__ void __launch_bounds__(128) attn_stats_kernel(AttnProblem p)
 {
-    const long long heads = (long long) p.n * p.q_heads, total = heads * p.sq;
+    wait_for_previous_kernel(p.lse);
+    const long long heads = (long long) p.n * p.q_heads, total = heads * p.stats_pitch;
     for (long long at = (long long) blockIdx.x * 128 + threadIdx.x; at < total; at += (long long) gridDim.x * 128)
     {
-        const long long nh = at / p.sq, n = nh / p.q_heads;
-        const int i = (int) (at - nh * p.sq);
-        const float lse = p.lse[at];
+        const long long nh = at / p.stats_pitch, n = nh / p.q_heads;
+        const int i = (int) (at - nh * p.stats_pitch);
+        const float lse = i < p.sq ? p.lse[nh * p.sq + i] : -INFINITY;
         float delta = 0.f;
         const bool none = lse == -INFINITY || (p.q_mask && !p.q_mask[n * p.sq + i]);
         if (!none)
@@ -206,11 +207,24 @@ struct Carve
     }
 };
 
-int64_t attn_carve(AttnProblem* p, bool backward, void* workspace)
+int64_t attn_carve(AttnProblem* p, int32_t dtype, bool backward, void* workspace)
 {
     Carve w{static_cast<char*>(workspace)};
-    attn_simt_splits(p, backward);
+    const bool tc = dtype == DCB_BF16;
+    (tc ? attn_tc_splits : attn_simt_splits)(p, backward);
     const long long qh = (long long) p->n * p->q_heads, kh = (long long) p->n * p->kv_heads;
+    p->stats_pitch = tc ? (long long) attn_tiles(p->sq, 128) * 128 : p->sq;
+    if (tc)
+    {
+        const auto copy = [&](long long heads, int cells) {
+            return reinterpret_cast<bf16*>(w.floats(heads * p->d * ((cells + 7) / 8) * 4));
+        };
+        p->copy_q = copy(qh, p->sq);
+        p->copy_k = copy(kh, p->sk);
+        p->copy_v = copy(kh, p->sk);
+        p->copy_do = backward ? copy(qh, p->sq) : nullptr;
+        p->bits = reinterpret_cast<uint32_t*>(w.floats((long long) p->n * 4 * attn_tiles(p->sk, 128)));
+    }
     if (!backward)
     {
         if (p->kv_splits > 1)
@@ -220,7 +234,7 @@ int64_t attn_carve(AttnProblem* p, bool backward, void* workspace)
         }
         return w.used;
     }
-    p->stats = w.floats(2 * qh * p->sq);
+    p->stats = w.floats(2 * qh * p->stats_pitch);
     if (p->kv_splits > 1)
         p->part_dq = w.floats(p->kv_splits * qh * p->d * p->sq);
     if (p->q_splits > 1)
@@ -231,14 +245,14 @@ int64_t attn_carve(AttnProblem* p, bool backward, void* workspace)
     return w.used;
 }
 
-int32_t attn_workspace(AttnProblem* p, bool backward, void* workspace, int64_t bytes)
+int32_t attn_workspace(AttnProblem* p, int32_t dtype, bool backward, void* workspace, int64_t bytes)
 {
-    const int64_t need = attn_carve(p, backward, nullptr);
+    const int64_t need = attn_carve(p, dtype, backward, nullptr);
     if (need > 0)
     {
         DCB_REQUIRE(workspace && bytes >= need, "workspace too small");
         DCB_REQUIRE(reinterpret_cast<uintptr_t>(workspace) % 256 == 0, "workspace must be 256-byte aligned");
-        attn_carve(p, backward, workspace);
+        attn_carve(p, dtype, backward, workspace);
     }
     return DCB_OK;
 }
@@ -267,7 +281,7 @@ int64_t dcb_attention_workspace_bytes(const dcb_attention_desc* ad, const dcb_nd
     AttnProblem p;
     if (attn_shapes(ad, qd, kd, &p))
         return -1;
-    return attn_carve(&p, backward != 0, nullptr);
+    return attn_carve(&p, ad->dtype, backward != 0, nullptr);
 }
 
 int32_t dcb_attention_fwd(const dcb_attention_desc* ad, const dcb_nd_desc* qd, const void* q, const dcb_nd_desc* kd,
@@ -296,9 +310,9 @@ int32_t dcb_attention_fwd(const dcb_attention_desc* ad, const dcb_nd_desc* qd, c
     if (p.sk == 0)
         return attn_fill(ad->dtype, p.o, p.n, (long long) p.q_heads * p.d, p.sq, p.lse,
                          (long long) p.n * p.q_heads * p.sq, s);
-    if (int32_t e = attn_workspace(&p, false, workspace, workspace_bytes))
+    if (int32_t e = attn_workspace(&p, ad->dtype, false, workspace, workspace_bytes))
         return e;
-    if (int32_t e = attn_simt_fwd(p, ad->dtype, s))
+    if (int32_t e = ad->dtype == DCB_BF16 ? attn_tc_fwd(p, s) : attn_simt_fwd(p, s))
         return e;
     if (p.kv_splits == 1)
         return DCB_OK;
@@ -345,17 +359,17 @@ int32_t dcb_attention_bwd(const dcb_attention_desc* ad, const dcb_nd_desc* qd, c
     p.lse = static_cast<float*>(const_cast<void*>(lse));
     p.q_mask = static_cast<const uint8_t*>(q_mask);
     p.kv_mask = static_cast<const uint8_t*>(kv_mask);
-    if (int32_t e = attn_workspace(&p, true, workspace, workspace_bytes))
+    if (int32_t e = attn_workspace(&p, ad->dtype, true, workspace, workspace_bytes))
         return e;
     const int32_t e = with_type(ad->dtype, [&](auto t) -> int32_t {
-        attn_stats_kernel<decltype(t)>
-            <<<flat_blocks((long long) p.n * p.q_heads * p.sq, 128), 128, 0, s>>>(p);
-        DCB_LAUNCH_CHECK();
+        DCB_CUDA_TRY(launch_overlapped(attn_stats_kernel<decltype(t)>,
+                                       dim3(flat_blocks((long long) p.n * p.q_heads * p.stats_pitch, 128)), 128, 0, s,
+                                       p));
         return DCB_OK;
     });
     if (e)
         return e;
-    if (int32_t err = attn_simt_bwd(p, ad->dtype, s))
+    if (int32_t err = ad->dtype == DCB_BF16 ? attn_tc_bwd(p, s) : attn_simt_bwd(p, s))
         return err;
     if (p.q_splits > 1)
     {
@@ -372,7 +386,15 @@ int32_t dcb_attention_bwd(const dcb_attention_desc* ad, const dcb_nd_desc* qd, c
 int32_t dcb_attention_status(void* stream)
 {
     DCB_CUDA_TRY(cudaStreamSynchronize(as_stream(stream)));
-    return DCB_OK;
+    int* word = attn_tc_status();
+    int given_up = 0;
+    DCB_REQUIRE(word, "no status word on this device");
+    DCB_CUDA_TRY(cudaMemcpy(&given_up, word, sizeof(int), cudaMemcpyDeviceToHost));
+    if (!given_up)
+        return DCB_OK;
+    DCB_CUDA_TRY(cudaMemset(word, 0, sizeof(int)));
+    set_last_error("a tensor-core attention kernel gave up on a pipeline wait");
+    return DCB_CUDA_ERROR;
 }
 
 } // extern "C"

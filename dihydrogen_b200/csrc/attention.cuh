@@ -30,12 +30,17 @@ struct AttnProblem
     const uint8_t *q_mask, *kv_mask;
     float* lse;                      // [n][q_heads][sq]
     // Backward: lse in powers of two (+infinity where a cell sees nothing) and sum_d o d_o,
-    // [2][n * q_heads][sq].
+    // [2][n * q_heads][stats_pitch], +infinity and 0 behind the last cell.
     float* stats;
+    long long stats_pitch;
     // Parts of a split axis, joined by a kernel of their own:
     //   forward  [splits][n * q_heads][d][sq] sums and [splits][2][n * q_heads][sq] maxima, sums of weights
     //   backward [splits][n * heads][d][cells] sums
     float *part_o, *part_ml, *part_dq, *part_dk, *part_dv;
+    // Tensor cores: copies of tensors that bulk copies cannot address or whose masked cells have to be zeros, [n][heads *
+    // d][pitch] with rows of whole 16 bytes, and the keys' mask as bits.
+    bf16 *copy_q, *copy_k, *copy_v, *copy_do;
+    uint32_t* bits;
     int q_splits, kv_splits; // of the queries' axis (dk, dv), of the keys' axis (o, dq)
 };
 
@@ -52,9 +57,14 @@ inline int attn_splits(long long work, int steps, long long slots, int least)
     return (int) std::max<long long>(1, std::min<long long>(slots / work, steps / least));
 }
 
-// Kernels of attention_simt.cu (fp32).
-int32_t attn_simt_fwd(const AttnProblem& p, int32_t dtype, cudaStream_t stream);
-int32_t attn_simt_bwd(const AttnProblem& p, int32_t dtype, cudaStream_t stream);
+// Kernels of attention_tc.cu (bf16) and attention_simt.cu (fp32).
+int32_t attn_tc_fwd(const AttnProblem& p, cudaStream_t stream);
+int32_t attn_tc_bwd(const AttnProblem& p, cudaStream_t stream);
+void attn_tc_splits(AttnProblem* p, bool backward);
+int* attn_tc_status(); // device word of the current device
+
+int32_t attn_simt_fwd(const AttnProblem& p, cudaStream_t stream);
+int32_t attn_simt_bwd(const AttnProblem& p, cudaStream_t stream);
 void attn_simt_splits(AttnProblem* p, bool backward);
 
 } // namespace dcb

@@ -1,4 +1,4 @@
-// Attention on the CUDA cores, forward and backward.
+// Attention of fp32 tensors on the CUDA cores, forward and backward.
 //
 // Blocks of 256 threads hold tiles of 64 cells as [channel][cell], as memory has them.  A thread
 // has 4 x 4 scores of a 64 x 64 tile (outer products over the channels) and 4 cells x D / 16
@@ -20,11 +20,11 @@ constexpr int AS_LEAST = 4;  // tiles a part of a split axis walks at least
 
 // One head's cells [cell0, cell0 + 64) to shared memory as [channel][cell]; cells that are not there, and channels up to
 // D, as zeros.
-template <class T, int D>
+template <int D>
 __device__ __forceinline__ void as_load(float* to, const AttnTensor& t, long long n, int head, int d, int cell0,
                                         int cells, const uint8_t* mask)
 {
-    const T* p = static_cast<const T*>(t.p) + n * t.sn + (long long) head * d * t.sc + cell0;
+    const float* p = static_cast<const float*>(t.p) + n * t.sn + (long long) head * d * t.sc + cell0;
     const int j = threadIdx.x & 63;
     const bool there = cell0 + j < cells && (!mask || mask[cell0 + j]);
     for (int c = threadIdx.x >> 6; c < D; c += AS_THREADS / 64)
@@ -85,7 +85,7 @@ __device__ __forceinline__ void as_accumulate(const float* W, const float* X, in
 }
 
 // Results of 4 cells x D / 16 channels: to the tensor, or as a part to [head][channel][cell].
-template <class T, int D>
+template <int D>
 __device__ __forceinline__ void as_store(const AttnTensor& t, float* part, long long nh, long long n, int head, int d,
                                          int cell0, int cells, int tx, int ty, const float (&acc)[4][D / 16])
 {
@@ -105,7 +105,7 @@ __device__ __forceinline__ void as_store(const AttnTensor& t, float* part, long 
             if (part)
                 part[(nh * d + c) * cells + i] = v[0];
             else
-                store_elems<1>(static_cast<T*>(t.p) + n * t.sn + ((long long) head * d + c) * t.sc + i, v);
+                store_elems<1>(static_cast<float*>(t.p) + n * t.sn + ((long long) head * d + c) * t.sc + i, v);
         }
     }
 }
@@ -137,7 +137,7 @@ __device__ __forceinline__ void as_range(int steps, int splits, int split, int* 
     *hi = (int) ((long long) steps * (split + 1) / splits);
 }
 
-template <class T, int D>
+template <int D>
 __global__ void __launch_bounds__(AS_THREADS) attn_simt_fwd_kernel(AttnProblem p)
 {
     extern __shared__ float smem[];
@@ -148,7 +148,7 @@ __global__ void __launch_bounds__(AS_THREADS) attn_simt_fwd_kernel(AttnProblem p
     const int i0 = at.tile * AS_TILE, kv_head = at.head / p.group;
     const uint8_t* qm = p.q_mask ? p.q_mask + at.n * p.sq : nullptr;
     const uint8_t* km = p.kv_mask ? p.kv_mask + at.n * p.sk : nullptr;
-    as_load<T, D>(Q, p.q, at.n, at.head, p.d, i0, p.sq, qm);
+    as_load<D>(Q, p.q, at.n, at.head, p.d, i0, p.sq, qm);
     float m[4], l[4], acc[4][D / 16];
 #pragma unroll
     for (int a = 0; a < 4; ++a)
@@ -166,8 +166,8 @@ __global__ void __launch_bounds__(AS_THREADS) attn_simt_fwd_kernel(AttnProblem p
     {
         const int j0 = t * AS_TILE;
         __syncthreads();
-        as_load<T, D>(K, p.k, at.n, kv_head, p.d, j0, p.sk, km);
-        as_load<T, D>(V, p.v, at.n, kv_head, p.d, j0, p.sk, km);
+        as_load<D>(K, p.k, at.n, kv_head, p.d, j0, p.sk, km);
+        as_load<D>(V, p.v, at.n, kv_head, p.d, j0, p.sk, km);
         if (threadIdx.x < AS_TILE)
             see[threadIdx.x] = j0 + (int) threadIdx.x < p.sk && (!km || km[j0 + threadIdx.x]);
         __syncthreads();
@@ -223,7 +223,7 @@ __global__ void __launch_bounds__(AS_THREADS) attn_simt_fwd_kernel(AttnProblem p
                     ml[0] = m[a];
                     ml[heads * p.sq] = l[a];
                 }
-        as_store<T, D>(p.o, p.part_o + at.split * heads * p.d * p.sq, at.nh, at.n, at.head, p.d, i0, p.sq, tx, ty,
+        as_store<D>(p.o, p.part_o + at.split * heads * p.d * p.sq, at.nh, at.n, at.head, p.d, i0, p.sq, tx, ty,
                        acc);
         return;
     }
@@ -239,7 +239,7 @@ __global__ void __launch_bounds__(AS_THREADS) attn_simt_fwd_kernel(AttnProblem p
         if (tx == 0 && i < p.sq)
             p.lse[at.nh * p.sq + i] = none ? -INFINITY : (m[a] + log2f(l[a])) / ATTN_LOG2E;
     }
-    as_store<T, D>(p.o, nullptr, at.nh, at.n, at.head, p.d, i0, p.sq, tx, ty, acc);
+    as_store<D>(p.o, nullptr, at.nh, at.n, at.head, p.d, i0, p.sq, tx, ty, acc);
 }
 
 // The weights and their gradients of a tile, P = exp2(s - lse), dS = P (dP - delta): [query][key] or [key][query].
@@ -279,12 +279,12 @@ __device__ __forceinline__ void as_load_stats(const AttnProblem& p, long long nh
     if (threadIdx.x < AS_TILE)
     {
         const int i = i0 + threadIdx.x;
-        lse[threadIdx.x] = i < p.sq ? p.stats[nh * p.sq + i] : INFINITY;
-        delta[threadIdx.x] = i < p.sq ? p.stats[((long long) p.n * p.q_heads + nh) * p.sq + i] : 0.f;
+        lse[threadIdx.x] = i < p.sq ? p.stats[nh * p.stats_pitch + i] : INFINITY;
+        delta[threadIdx.x] = i < p.sq ? p.stats[((long long) p.n * p.q_heads + nh) * p.stats_pitch + i] : 0.f;
     }
 }
 
-template <class T, int D>
+template <int D>
 __global__ void __launch_bounds__(AS_THREADS) attn_simt_dkv_kernel(AttnProblem p)
 {
     extern __shared__ float smem[];
@@ -297,8 +297,8 @@ __global__ void __launch_bounds__(AS_THREADS) attn_simt_dkv_kernel(AttnProblem p
     const int j0 = at.tile * AS_TILE;
     const uint8_t* qm = p.q_mask ? p.q_mask + at.n * p.sq : nullptr;
     const uint8_t* km = p.kv_mask ? p.kv_mask + at.n * p.sk : nullptr;
-    as_load<T, D>(K, p.k, at.n, at.head, p.d, j0, p.sk, km);
-    as_load<T, D>(V, p.v, at.n, at.head, p.d, j0, p.sk, km);
+    as_load<D>(K, p.k, at.n, at.head, p.d, j0, p.sk, km);
+    as_load<D>(V, p.v, at.n, at.head, p.d, j0, p.sk, km);
     if (threadIdx.x < AS_TILE)
         see[threadIdx.x] = j0 + (int) threadIdx.x < p.sk && (!km || km[j0 + threadIdx.x]);
     float gk[4][D / 16], gv[4][D / 16];
@@ -316,8 +316,8 @@ __global__ void __launch_bounds__(AS_THREADS) attn_simt_dkv_kernel(AttnProblem p
         if (p.causal && j0 > (long long) i0 + AS_TILE - 1 + p.offset)
             continue;
         __syncthreads();
-        as_load<T, D>(Q, p.q, at.n, head, p.d, i0, p.sq, qm);
-        as_load<T, D>(dO, p.d_o, at.n, head, p.d, i0, p.sq, qm);
+        as_load<D>(Q, p.q, at.n, head, p.d, i0, p.sq, qm);
+        as_load<D>(dO, p.d_o, at.n, head, p.d, i0, p.sq, qm);
         as_load_stats(p, at.n * p.q_heads + head, i0, lse, delta);
         __syncthreads();
         as_weights<D, true>(p, Q, K, V, dO, lse, delta, see, i0, j0, tx, ty, P, dS);
@@ -331,11 +331,11 @@ __global__ void __launch_bounds__(AS_THREADS) attn_simt_dkv_kernel(AttnProblem p
         for (int r = 0; r < D / 16; ++r)
             gk[a][r] *= p.scale / ATTN_LOG2E;
     const long long size = (long long) p.n * p.kv_heads * p.d * p.sk * at.split;
-    as_store<T, D>(p.dk, p.q_splits > 1 ? p.part_dk + size : nullptr, at.nh, at.n, at.head, p.d, j0, p.sk, tx, ty, gk);
-    as_store<T, D>(p.dv, p.q_splits > 1 ? p.part_dv + size : nullptr, at.nh, at.n, at.head, p.d, j0, p.sk, tx, ty, gv);
+    as_store<D>(p.dk, p.q_splits > 1 ? p.part_dk + size : nullptr, at.nh, at.n, at.head, p.d, j0, p.sk, tx, ty, gk);
+    as_store<D>(p.dv, p.q_splits > 1 ? p.part_dv + size : nullptr, at.nh, at.n, at.head, p.d, j0, p.sk, tx, ty, gv);
 }
 
-template <class T, int D>
+template <int D>
 __global__ void __launch_bounds__(AS_THREADS) attn_simt_dq_kernel(AttnProblem p)
 {
     extern __shared__ float smem[];
@@ -347,8 +347,8 @@ __global__ void __launch_bounds__(AS_THREADS) attn_simt_dq_kernel(AttnProblem p)
     const int i0 = at.tile * AS_TILE, kv_head = at.head / p.group;
     const uint8_t* qm = p.q_mask ? p.q_mask + at.n * p.sq : nullptr;
     const uint8_t* km = p.kv_mask ? p.kv_mask + at.n * p.sk : nullptr;
-    as_load<T, D>(Q, p.q, at.n, at.head, p.d, i0, p.sq, qm);
-    as_load<T, D>(dO, p.d_o, at.n, at.head, p.d, i0, p.sq, qm);
+    as_load<D>(Q, p.q, at.n, at.head, p.d, i0, p.sq, qm);
+    as_load<D>(dO, p.d_o, at.n, at.head, p.d, i0, p.sq, qm);
     as_load_stats(p, at.nh, i0, lse, delta);
     float gq[4][D / 16];
 #pragma unroll
@@ -364,8 +364,8 @@ __global__ void __launch_bounds__(AS_THREADS) attn_simt_dq_kernel(AttnProblem p)
     {
         const int j0 = t * AS_TILE;
         __syncthreads();
-        as_load<T, D>(K, p.k, at.n, kv_head, p.d, j0, p.sk, km);
-        as_load<T, D>(V, p.v, at.n, kv_head, p.d, j0, p.sk, km);
+        as_load<D>(K, p.k, at.n, kv_head, p.d, j0, p.sk, km);
+        as_load<D>(V, p.v, at.n, kv_head, p.d, j0, p.sk, km);
         if (threadIdx.x < AS_TILE)
             see[threadIdx.x] = j0 + (int) threadIdx.x < p.sk && (!km || km[j0 + threadIdx.x]);
         __syncthreads();
@@ -379,7 +379,7 @@ __global__ void __launch_bounds__(AS_THREADS) attn_simt_dq_kernel(AttnProblem p)
         for (int r = 0; r < D / 16; ++r)
             gq[a][r] *= p.scale / ATTN_LOG2E;
     float* part = p.kv_splits > 1 ? p.part_dq + (long long) at.split * p.n * p.q_heads * p.d * p.sq : nullptr;
-    as_store<T, D>(p.dq, part, at.nh, at.n, at.head, p.d, i0, p.sq, tx, ty, gq);
+    as_store<D>(p.dq, part, at.nh, at.n, at.head, p.d, i0, p.sq, tx, ty, gq);
 }
 
 int32_t as_launch(void (*kernel)(AttnProblem), const AttnProblem& p, long long blocks, int smem, cudaStream_t stream)
@@ -395,16 +395,13 @@ int32_t as_launch(void (*kernel)(AttnProblem), const AttnProblem& p, long long b
 }
 
 template <class F>
-int32_t as_with(int32_t dtype, int d, F f)
+int32_t as_with(int d, F f)
 {
-    const auto sized = [&](auto t) -> int32_t {
-        if (d <= 32)
-            return f(t, std::integral_constant<int, 32>());
-        if (d <= 64)
-            return f(t, std::integral_constant<int, 64>());
-        return f(t, std::integral_constant<int, 128>());
-    };
-    return dtype == DCB_BF16 ? sized(bf16()) : sized(float());
+    if (d <= 32)
+        return f(std::integral_constant<int, 32>());
+    if (d <= 64)
+        return f(std::integral_constant<int, 64>());
+    return f(std::integral_constant<int, 128>());
 }
 
 } // namespace
@@ -419,25 +416,25 @@ void attn_simt_splits(AttnProblem* p, bool backward)
                                           attn_tiles(p->sq, AS_TILE) * p->group, slots, AS_LEAST);
 }
 
-int32_t attn_simt_fwd(const AttnProblem& p, int32_t dtype, cudaStream_t stream)
+int32_t attn_simt_fwd(const AttnProblem& p, cudaStream_t stream)
 {
-    return as_with(dtype, p.d, [&](auto t, auto d) {
+    return as_with(p.d, [&](auto d) {
         constexpr int D = decltype(d)::value;
-        return as_launch(attn_simt_fwd_kernel<decltype(t), D>, p,
+        return as_launch(attn_simt_fwd_kernel<D>, p,
                          (long long) p.n * p.q_heads * attn_tiles(p.sq, AS_TILE) * p.kv_splits,
                          (3 * D + AS_TILE) * AS_PITCH * 4, stream);
     });
 }
 
-int32_t attn_simt_bwd(const AttnProblem& p, int32_t dtype, cudaStream_t stream)
+int32_t attn_simt_bwd(const AttnProblem& p, cudaStream_t stream)
 {
-    return as_with(dtype, p.d, [&](auto t, auto d) {
+    return as_with(p.d, [&](auto d) {
         constexpr int D = decltype(d)::value;
-        if (int32_t e = as_launch(attn_simt_dkv_kernel<decltype(t), D>, p,
+        if (int32_t e = as_launch(attn_simt_dkv_kernel<D>, p,
                                   (long long) p.n * p.kv_heads * attn_tiles(p.sk, AS_TILE) * p.q_splits,
                                   (4 * D + 2 * AS_TILE) * AS_PITCH * 4, stream))
             return e;
-        return as_launch(attn_simt_dq_kernel<decltype(t), D>, p,
+        return as_launch(attn_simt_dq_kernel<D>, p,
                          (long long) p.n * p.q_heads * attn_tiles(p.sq, AS_TILE) * p.kv_splits,
                          (4 * D + AS_TILE) * AS_PITCH * 4, stream);
     });

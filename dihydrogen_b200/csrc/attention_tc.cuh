@@ -1,0 +1,317 @@
+// Attention on the tensor cores: what its three kernels share.
+//
+// A tile is 128 cells of one head, [channel][cell] as memory has it, in two halves of 64 cells: a
+// half is D rows of 128 bytes, fetched by one bulk tensor copy with the 128-byte swizzle.  The same
+// tile serves a product over the channels (cells are the rows or columns: the operand lies
+// "across", the reduction index strides over the 128-byte rows) and a product over the cells
+// (channels are the columns, the reduction index runs along the rows), so nothing is transposed.
+// Scores and their gradients never leave tensor memory but for the registers of the threads that
+// own a row; as operand of the second product they go back there, two bf16 to a column, over the
+// fp32 values that they were made from.
+#pragma once
+
+#include "attention.cuh"
+#include "conv_tc_common.cuh"
+
+namespace dcb
+{
+
+constexpr int AT_TILE = 128;
+// Two teams of 128 for the rows; a warp that issues products, one that issues copies, two that fill up the third
+// warpgroup.  384 threads are launched with 168 registers each; the teams take some of the third group's:
+// 2 x 216 + 72 = 3 x 168.
+constexpr int AT_THREADS = 384;
+constexpr int AT_TEAM_REGS = 216, AT_OTHER_REGS = 72;
+static_assert(2 * AT_TEAM_REGS + AT_OTHER_REGS <= 3 * 168, "more registers than the block was launched with");
+constexpr int AT_MMA_WARP = 8;
+constexpr int AT_TMA_WARP = 9;
+
+// A ring of shared-memory slots: use number i of a ring of n has slot i % n, lap i / n.
+struct AtRing
+{
+    uint32_t slot = 0, lap = 0;
+    __device__ __forceinline__ void next(uint32_t n)
+    {
+        if (++slot == n)
+        {
+            slot = 0;
+            ++lap;
+        }
+    }
+};
+
+// Both operands in shared memory.
+__device__ __forceinline__ void at_mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate)
+{
+    asm volatile("{\n\t"
+                 ".reg .pred p;\n\t"
+                 "setp.ne.b32 p, %4, 0;\n\t"
+                 "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t"
+                 "}" ::"r"(d),
+                 "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+                 : "memory");
+}
+
+// A in tensor memory.
+__device__ __forceinline__ void at_mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate)
+{
+    asm volatile("{\n\t"
+                 ".reg .pred p;\n\t"
+                 "setp.ne.b32 p, %4, 0;\n\t"
+                 "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t"
+                 "}" ::"r"(d),
+                 "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
+                 : "memory");
+}
+
+// bf16 x bf16 -> fp32, M = 128.  across: cells are that operand's rows, channels the reduction.
+__device__ __forceinline__ uint32_t at_idesc(uint32_t n, bool a_across, bool b_across)
+{
+    return (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t) a_across << 15) | ((uint32_t) b_across << 16)
+           | (n >> 3 << 17) | ((128u >> 4) << 24);
+}
+
+template <int D>
+struct AtTile
+{
+    static constexpr uint32_t HALF = D * 128;    // bytes of 64 cells
+    static constexpr uint32_t BYTES = 2 * HALF;
+    // The tile as operand across: cells in groups of 64, HALF apart; channels in groups of 8 rows, 1024 bytes apart.
+    static __device__ __forceinline__ uint64_t across(uint32_t saddr) { return make_desc(saddr, HALF, 1024, 2); }
+    // ... and along: channels in groups of 8 rows, 1024 bytes apart; 16 cells are 32 bytes of a row.
+    static __device__ __forceinline__ uint64_t along(uint32_t saddr) { return make_desc(saddr, 16, 1024, 2); }
+    // In units of 16 bytes, what 16 steps of the reduction index add to the start address.
+    static __device__ __forceinline__ uint32_t across_step(int k) { return (uint32_t) k * (2048 >> 4); }
+    static __device__ __forceinline__ uint32_t along_step(int k)
+    {
+        return ((uint32_t) (k >> 2) * HALF + (uint32_t) (k & 3) * 32) >> 4;
+    }
+};
+
+// d = A B' over the channels: both tiles across.
+template <int D>
+__device__ __forceinline__ void at_scores(uint32_t d, uint32_t a, uint32_t b, int ksteps)
+{
+    const uint64_t da = AtTile<D>::across(a), db = AtTile<D>::across(b);
+    const uint32_t idesc = at_idesc(AT_TILE, true, true);
+    for (int k = 0; k < ksteps; ++k)
+        at_mma_ss(d, da + AtTile<D>::across_step(k), db + AtTile<D>::across_step(k), idesc, k > 0);
+}
+
+// d += W B over 128 cells: W in tensor memory, 64 cells to 32 columns, the second half of them `gap` columns behind the
+// first's start.
+template <int D>
+__device__ __forceinline__ void at_weigh(uint32_t d, uint32_t w, uint32_t gap, uint32_t b, uint32_t n, bool first)
+{
+    const uint64_t db = AtTile<D>::along(b);
+    const uint32_t idesc = at_idesc(n, false, false);
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+        at_mma_ts(d, w + (k >> 2) * gap + (k & 3) * 8, db + AtTile<D>::along_step(k), idesc, !(first && k == 0));
+}
+
+__device__ __forceinline__ void at_tma_half(uint32_t dst, const CUtensorMap* map, int cell, int head, int n,
+                                            uint64_t* bar)
+{
+    asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes "
+                 "[%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(dst),
+                 "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(cell), "r"(0), "r"(head), "r"(n)
+                 : "memory");
+}
+
+// 128 cells of a head; cells and channels that are not there arrive as zeros (and count as bytes).
+template <int D>
+__device__ __forceinline__ void at_tma_tile(uint32_t dst, const CUtensorMap* map, int cell, int head, int n,
+                                            uint64_t* bar)
+{
+    at_tma_half(dst, map, cell, head, n, bar);
+    at_tma_half(dst + AtTile<D>::HALF, map, cell + 64, head, n, bar);
+}
+
+// `bytes` from a 16-byte aligned address.
+__device__ __forceinline__ void at_bulk(uint32_t dst, const void* src, uint32_t bytes, uint64_t* bar)
+{
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
+                 "l"(src), "r"(bytes), "r"(smem_u32(bar))
+                 : "memory");
+}
+
+__device__ __forceinline__ void at_tmem_ld32(uint32_t taddr, float* v)
+{
+    uint32_t r[32];
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+          "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+          "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(taddr));
+#pragma unroll
+    for (int i = 0; i < 32; ++i)
+        v[i] = __uint_as_float(r[i]);
+}
+
+__device__ __forceinline__ void at_tmem_wait_ld()
+{
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+}
+
+__device__ __forceinline__ void at_tmem_st32(uint32_t taddr, const uint32_t* r)
+{
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+        "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
+        "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(taddr),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
+        "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
+        "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+        : "memory");
+}
+
+__device__ __forceinline__ void at_tmem_wait_st()
+{
+    asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+}
+
+__device__ __forceinline__ float at_exp2(float x)
+{
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// A wait of a whole warp: it goes on, or gives up, as one.
+__device__ __forceinline__ bool at_warp_wait(uint64_t* bar, uint32_t parity, volatile int* give_up)
+{
+    return __all_sync(~0u, mbar_wait_t<0>(bar, parity, give_up));
+}
+
+// One arrival a warp, after all its lanes' work.
+__device__ __forceinline__ void at_warp_arrive(uint64_t* bar, int lane)
+{
+    tc_fence_before();
+    __syncwarp();
+    if (lane == 0)
+        mbar_arrive(bar);
+}
+
+// Which of 128 cells from j0 on are there: 32 to a word.
+__device__ __forceinline__ uint32_t at_there(const AttnProblem& p, const uint32_t* bits, int j0, int w)
+{
+    const int left = p.sk - (j0 + 32 * w);
+    if (bits)
+        return left > 0 ? bits[(j0 >> 5) + w] : 0u;
+    return left >= 32 ? ~0u : left <= 0 ? 0u : (1u << left) - 1u;
+}
+
+// ... and up to cell j0 + last.
+__device__ __forceinline__ uint32_t at_up_to(int last, int w)
+{
+    const int left = last - 32 * w + 1;
+    return left >= 32 ? ~0u : left <= 0 ? 0u : (1u << left) - 1u;
+}
+
+// Channels [c_lo, c_hi) of an accumulator's rows to a tensor ([channel][cell], this thread's cell is i), or as a part in
+// fp32.  nothing: no product was taken; zero: this row's result is 0 whatever it holds.
+__device__ __forceinline__ void at_store(const AttnTensor& t, float* part, long long nh, long long n, int head, int d,
+                                         int i, int cells, float factor, bool zero, bool nothing, uint32_t taddr,
+                                         int c_lo, int c_hi)
+{
+    bf16* out = static_cast<bf16*>(t.p) + n * t.sn + (long long) head * d * t.sc + i;
+    float* to = part + nh * d * (long long) cells + i;
+    for (int c0 = c_lo; c0 < min(c_hi, d); c0 += 32)
+    {
+        float v[32];
+        if (!nothing)
+        {
+            at_tmem_ld32(taddr + c0, v);
+            at_tmem_wait_ld();
+        }
+        if (i >= cells)
+            continue;
+#pragma unroll
+        for (int c = 0; c < 32; ++c)
+            if (c0 + c < d)
+            {
+                const float x = nothing || zero ? 0.f : v[c] * factor;
+                if (part)
+                    to[(long long) (c0 + c) * cells] = x;
+                else
+                    out[(c0 + c) * t.sc] = __float2bfloat16_rn(x);
+            }
+    }
+}
+
+struct AtMaps
+{
+    CUtensorMap q, k, v, d_o;
+};
+
+struct AtExtra
+{
+    const uint32_t* kv_bits; // mask of the keys, 32 to a word, [n][words]; null without a mask
+    long long words;
+    int* status;
+};
+
+// The end of every kernel: who gave up says so, waits for what he started, and the tensor memory goes back.
+__device__ __forceinline__ void at_finish(bool ok, int* status, int warp, int lane, uint32_t tmem)
+{
+    if (!ok && lane == 0)
+        atomicExch(status, 1);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    __syncwarp();
+    if (warp == AT_MMA_WARP)
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(TC_TMEM_COLS) : "memory");
+}
+
+// The 128-byte swizzle goes by address bits: tiles start on multiples of 1024 bytes.
+__device__ __forceinline__ bool at_misplaced(uint32_t base, int* status)
+{
+    if ((base & 1023u) == 0)
+        return false;
+    if (threadIdx.x == 0)
+        atomicExch(status, 1);
+    return true;
+}
+
+__device__ __forceinline__ void at_tmem_alloc(uint32_t* slot)
+{
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(slot)),
+                 "r"(TC_TMEM_COLS)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+}
+
+__device__ __forceinline__ void at_team_registers()
+{
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(AT_TEAM_REGS));
+}
+
+__device__ __forceinline__ void at_other_registers()
+{
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(AT_OTHER_REGS));
+}
+
+// Waits, bounded, for copies into slots that nobody waited for because the block gave up.
+__device__ __forceinline__ void at_drain(uint64_t* full, uint32_t slots, const AtRing& ring)
+{
+    int give_up = 0;
+    for (uint32_t s = 0; s < slots; ++s)
+    {
+        // the last lap that slot s was loaded in
+        const uint32_t uses = ring.lap + (s < ring.slot);
+        if (uses > 0)
+            mbar_wait_t<20>(&full[s], (uses - 1) & 1, &give_up);
+    }
+}
+
+int32_t attn_tc_fwd_launch(const AttnProblem& p, const AtMaps& maps, const AtExtra& ex, cudaStream_t stream);
+int32_t attn_tc_bwd_launch(const AttnProblem& p, const AtMaps& maps, const AtExtra& ex, cudaStream_t stream);
+
+} // namespace dcb

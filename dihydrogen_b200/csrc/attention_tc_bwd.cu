@@ -1,0 +1,535 @@
+// Attention backward on the tensor cores: two kernels, each result with one owner and one order of its sums.
+//
+// attn_tc_dkv_kernel: a block owns 128 keys of one key head and walks over the queries (of all query heads that read
+// it) in tiles of 128.  Everything is taken across, keys as rows: S' = K Q' and dP' = V dO' into tensor memory; the
+// weights P' = 2^(S' - lse) go back as bf16 over S' and dS' = P' (dP' - delta) over dP', operands of dV += P' dO and
+// dK += dS' Q.  lse and delta belong to columns and come out of shared memory.
+// attn_tc_dq_kernel: a block owns 128 queries and walks over the keys, queries as rows: S = Q K', dP = dO V',
+// dQ += dS K.  It works S and dP out a second time (7 products in all instead of 5), for which no sum over blocks is
+// needed: no atomics, no fp32 gradient in memory, the same bits every run.
+//
+// Two teams of 128 threads have 64 of the 128 columns each, all 128 rows.  The products of one step run under the
+// exponentials of another: P' and dS' are handed over apart, and the scores are taken a step (dkv) or two (dq) ahead.
+#include "attention_tc.cuh"
+
+namespace dcb
+{
+namespace
+{
+
+template <int D>
+struct AbShape
+{
+    static constexpr uint32_t A_SLOTS = D == 128 ? 3 : 4; // Q (dkv) or K (dq)
+    static constexpr uint32_t B_SLOTS = D == 128 ? 2 : 4; // dO (dkv) or V (dq)
+    static constexpr uint32_t OWN_AT = 0;                 // K, V (dkv) or Q, dO (dq)
+    static constexpr uint32_t A_AT = 2 * AtTile<D>::BYTES;
+    static constexpr uint32_t B_AT = A_AT + A_SLOTS * AtTile<D>::BYTES;
+    static constexpr uint32_t STATS_AT = B_AT + B_SLOTS * AtTile<D>::BYTES; // dkv: lse, delta of a dO slot
+    static constexpr uint32_t BARS_AT = STATS_AT + B_SLOTS * 1024;
+    static constexpr uint32_t SMEM = BARS_AT + 256;
+};
+static_assert(AbShape<128>::SMEM <= 227 * 1024, "shared memory of a block");
+
+struct AbBars
+{
+    uint64_t own_full, a_full[4], a_empty[4], b_full[4], b_empty[4], s_full[2], dp_full, p_ready, ds_ready, fin;
+    uint32_t tmem;
+    int give_up;
+};
+static_assert(sizeof(AbBars) <= 256, "the barriers' room");
+
+__device__ __forceinline__ void ab_init(AbBars& b, int warp)
+{
+    if (threadIdx.x == 0)
+    {
+        mbar_init(&b.own_full, 1);
+        for (int s = 0; s < 4; ++s)
+        {
+            mbar_init(&b.a_full[s], 1), mbar_init(&b.a_empty[s], 1);
+            mbar_init(&b.b_full[s], 1), mbar_init(&b.b_empty[s], 1);
+        }
+        mbar_init(&b.s_full[0], 1), mbar_init(&b.s_full[1], 1);
+        mbar_init(&b.dp_full, 1), mbar_init(&b.fin, 1);
+        mbar_init(&b.p_ready, 8), mbar_init(&b.ds_ready, 8);
+        b.give_up = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == AT_MMA_WARP)
+        at_tmem_alloc(&b.tmem);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+}
+
+// One thread of the block that gave up: the products that were issued end before the tensor memory goes back.
+__device__ __forceinline__ void ab_drain_products(AbBars& b)
+{
+    int none = 0;
+    mma_commit(&b.fin);
+    mbar_wait_t<20>(&b.fin, 0, &none);
+}
+
+template <int D>
+__global__ void __launch_bounds__(AT_THREADS, 1)
+    attn_tc_dkv_kernel(const __grid_constant__ AttnProblem p, const __grid_constant__ AtMaps maps,
+                       const __grid_constant__ AtExtra ex)
+{
+    using S = AbShape<D>;
+    extern __shared__ __align__(1024) uint8_t smem[];
+    const uint32_t base = smem_u32(smem);
+    AbBars& b = *reinterpret_cast<AbBars*>(smem + S::BARS_AT);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    volatile int* give_up = &b.give_up;
+    if (at_misplaced(base, ex.status))
+        return;
+
+    long long at = blockIdx.x;
+    const int tiles_k = attn_tiles(p.sk, AT_TILE), tiles_q = attn_tiles(p.sq, AT_TILE);
+    const int tile = (int) (at % tiles_k); // causal: the first keys have the longest walks
+    at /= tiles_k;
+    const int split = (int) (at % p.q_splits);
+    const long long nh = at / p.q_splits, n = nh / p.kv_heads;
+    const int head = (int) (nh - n * p.kv_heads);
+    const int j0 = tile * AT_TILE;
+    // the walk: tiles of queries from t0 on, of every query head of the group
+    int t0 = 0;
+    if (p.causal)
+        t0 = (int) min((long long) tiles_q, max(0ll, (long long) j0 - p.offset) / AT_TILE);
+    const int per_head = tiles_q - t0;
+    const long long all = (long long) per_head * p.group;
+    const int lo = (int) (all * split / p.q_splits), steps = (int) (all * (split + 1) / p.q_splits) - lo;
+
+    ab_init(b, warp);
+    const uint32_t tmem = b.tmem;
+    const float* stats = p.stats;
+    wait_for_previous_kernel(stats);
+    bool ok = true;
+    const uint32_t s_at = tmem, dp_at = tmem + 128, dv_at = tmem + 256, dk_at = tmem + 256 + D;
+
+    if (warp >= AT_MMA_WARP)
+    {
+        at_other_registers();
+        if (warp == AT_TMA_WARP)
+        {
+            if (lane == 0 && steps > 0)
+            {
+                mbar_expect_tx(&b.own_full, 2 * AtTile<D>::BYTES);
+                at_tma_tile<D>(base + S::OWN_AT, &maps.k, j0, head, (int) n, &b.own_full);
+                at_tma_tile<D>(base + S::OWN_AT + AtTile<D>::BYTES, &maps.v, j0, head, (int) n, &b.own_full);
+                AtRing ra, rb;
+                for (int u = 0; u < steps && ok; ++u)
+                {
+                    const int g = (lo + u) / per_head, i0 = (t0 + (lo + u) - g * per_head) * AT_TILE;
+                    const int q_head = head * p.group + g;
+                    if (ra.lap > 0)
+                        ok = mbar_wait_t<20>(&b.a_empty[ra.slot], (ra.lap - 1) & 1, give_up);
+                    if (!ok)
+                        break;
+                    mbar_expect_tx(&b.a_full[ra.slot], AtTile<D>::BYTES);
+                    at_tma_tile<D>(base + S::A_AT + ra.slot * AtTile<D>::BYTES, &maps.q, i0, q_head, (int) n,
+                                   &b.a_full[ra.slot]);
+                    ra.next(S::A_SLOTS);
+                    if (rb.lap > 0)
+                        ok = mbar_wait_t<20>(&b.b_empty[rb.slot], (rb.lap - 1) & 1, give_up);
+                    if (!ok)
+                        break;
+                    mbar_expect_tx(&b.b_full[rb.slot], AtTile<D>::BYTES + 1024);
+                    at_tma_tile<D>(base + S::B_AT + rb.slot * AtTile<D>::BYTES, &maps.d_o, i0, q_head, (int) n,
+                                   &b.b_full[rb.slot]);
+                    const float* row = stats + (n * p.q_heads + q_head) * p.stats_pitch + i0;
+                    at_bulk(base + S::STATS_AT + rb.slot * 1024, row, 512, &b.b_full[rb.slot]);
+                    at_bulk(base + S::STATS_AT + rb.slot * 1024 + 512,
+                            row + (long long) p.n * p.q_heads * p.stats_pitch, 512, &b.b_full[rb.slot]);
+                    rb.next(S::B_SLOTS);
+                }
+                if (!ok || *give_up)
+                {
+                    int none = 0;
+                    mbar_wait_t<20>(&b.own_full, 0, &none);
+                    at_drain(b.a_full, S::A_SLOTS, ra);
+                    at_drain(b.b_full, S::B_SLOTS, rb);
+                }
+            }
+        }
+        else if (warp == AT_MMA_WARP)
+        {
+            if (lane == 0 && steps > 0)
+            {
+                const int ksteps = (p.d + 15) / 16;
+                const uint32_t width = (uint32_t) ksteps * 16;
+                const uint32_t k_at = base + S::OWN_AT, v_at = k_at + AtTile<D>::BYTES;
+                AtRing ra, rb; // of the next tiles to wait for
+                uint32_t q_slot = 0, o_slot = 0;
+                const auto scores = [&] {
+                    ok = ok && mbar_wait_t<0>(&b.a_full[ra.slot], ra.lap & 1, give_up);
+                    if (!ok)
+                        return;
+                    tc_fence_after();
+                    at_scores<D>(s_at, k_at, base + S::A_AT + ra.slot * AtTile<D>::BYTES, ksteps);
+                    mma_commit(&b.s_full[0]);
+                    ra.next(S::A_SLOTS);
+                };
+                const auto weight_grads = [&] {
+                    ok = ok && mbar_wait_t<0>(&b.b_full[rb.slot], rb.lap & 1, give_up);
+                    if (!ok)
+                        return;
+                    tc_fence_after();
+                    at_scores<D>(dp_at, v_at, base + S::B_AT + rb.slot * AtTile<D>::BYTES, ksteps);
+                    mma_commit(&b.dp_full);
+                    rb.next(S::B_SLOTS);
+                };
+                ok = mbar_wait_t<0>(&b.own_full, 0, give_up);
+                scores();
+                weight_grads();
+                for (int u = 0; u < steps && ok; ++u)
+                {
+                    ok = mbar_wait_t<0>(&b.p_ready, u & 1, give_up);
+                    if (!ok)
+                        break;
+                    tc_fence_after();
+                    at_weigh<D>(dv_at, s_at, 64, base + S::B_AT + o_slot * AtTile<D>::BYTES, width, u == 0);
+                    if (u + 1 < steps)
+                        scores();
+                    ok = ok && mbar_wait_t<0>(&b.ds_ready, u & 1, give_up);
+                    if (!ok)
+                        break;
+                    tc_fence_after();
+                    at_weigh<D>(dk_at, dp_at, 64, base + S::A_AT + q_slot * AtTile<D>::BYTES, width, u == 0);
+                    mma_commit(&b.a_empty[q_slot]);
+                    mma_commit(&b.b_empty[o_slot]);
+                    q_slot = q_slot + 1 == S::A_SLOTS ? 0 : q_slot + 1;
+                    o_slot = o_slot + 1 == S::B_SLOTS ? 0 : o_slot + 1;
+                    if (u + 1 < steps)
+                        weight_grads();
+                }
+                if (ok)
+                    mma_commit(&b.fin);
+                else
+                    ab_drain_products(b);
+            }
+        }
+    }
+    else
+    {
+        at_team_registers();
+        const int team = warp >> 2;
+        const uint32_t lanes = (uint32_t) (warp & 3) << 21;
+        const int j = j0 + (threadIdx.x & 127);
+        const uint32_t s_mine = s_at + lanes + 64 * team, dp_mine = dp_at + lanes + 64 * team;
+        AtRing rb;
+        for (int u = 0; u < steps; ++u)
+        {
+            const int g = (lo + u) / per_head, i0 = (t0 + (lo + u) - g * per_head) * AT_TILE + 64 * team;
+            const float* lse = reinterpret_cast<const float*>(smem + S::STATS_AT + rb.slot * 1024) + 64 * team;
+            ok = at_warp_wait(&b.b_full[rb.slot], rb.lap & 1, give_up)
+                 && at_warp_wait(&b.s_full[0], u & 1, give_up);
+            if (!ok)
+                break;
+            rb.next(S::B_SLOTS);
+            tc_fence_after();
+            float w[64];
+            at_tmem_ld32(s_mine, w);
+            at_tmem_ld32(s_mine + 32, w + 32);
+            at_tmem_wait_ld();
+            // this key is seen by the cells from `first` on of this team's 64
+            const int first = p.causal ? j - p.offset - i0 : 0;
+            const bool cut = __any_sync(~0u, first > 0);
+#pragma unroll
+            for (int c = 0; c < 64; c += 4)
+            {
+                float l[4];
+                load_elems<4>(lse + c, l);
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    w[c + e] = at_exp2(fmaf(w[c + e], p.scale, -l[e]));
+            }
+            if (cut)
+            {
+#pragma unroll
+                for (int c = 0; c < 64; ++c)
+                    w[c] = c >= first ? w[c] : 0.f;
+            }
+            {
+                uint32_t packed[32];
+#pragma unroll
+                for (int c = 0; c < 32; ++c)
+                    packed[c] = pack_bf16(w[2 * c], w[2 * c + 1]);
+                at_tmem_st32(s_mine, packed);
+            }
+            at_tmem_wait_st();
+            at_warp_arrive(&b.p_ready, lane);
+
+            ok = at_warp_wait(&b.dp_full, u & 1, give_up);
+            if (!ok)
+                break;
+            tc_fence_after();
+            float d[64];
+            at_tmem_ld32(dp_mine, d);
+            at_tmem_ld32(dp_mine + 32, d + 32);
+            at_tmem_wait_ld();
+            const float* delta = lse + 128;
+            uint32_t packed[32];
+#pragma unroll
+            for (int c = 0; c < 64; c += 4)
+            {
+                float l[4];
+                load_elems<4>(delta + c, l);
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    d[c + e] = w[c + e] * (d[c + e] - l[e]);
+                packed[c / 2] = pack_bf16(d[c], d[c + 1]);
+                packed[c / 2 + 1] = pack_bf16(d[c + 2], d[c + 3]);
+            }
+            if (cut)
+            {
+#pragma unroll
+                for (int c = 0; c < 32; ++c)
+                    packed[c] = 2 * c >= first ? packed[c] : 2 * c + 1 >= first ? packed[c] & 0xffff0000u : 0u;
+            }
+            at_tmem_st32(dp_mine, packed);
+            at_tmem_wait_st();
+            at_warp_arrive(&b.ds_ready, lane);
+        }
+        if (ok && steps > 0)
+            ok = at_warp_wait(&b.fin, 0, give_up);
+        tc_fence_after();
+        if (ok)
+        {
+            const bool gone = p.kv_mask && j < p.sk && !p.kv_mask[n * p.sk + j];
+            const long long part = (long long) p.n * p.kv_heads * p.d * p.sk * split;
+            if (team == 0)
+                at_store(p.dv, p.q_splits > 1 ? p.part_dv + part : nullptr, nh, n, head, p.d, j, p.sk, 1.f, gone,
+                         steps == 0, dv_at + lanes, 0, D);
+            else
+                at_store(p.dk, p.q_splits > 1 ? p.part_dk + part : nullptr, nh, n, head, p.d, j, p.sk,
+                         p.scale / ATTN_LOG2E, gone, steps == 0, dk_at + lanes, 0, D);
+        }
+    }
+    at_finish(ok, ex.status, warp, lane, tmem);
+}
+
+template <int D>
+__global__ void __launch_bounds__(AT_THREADS, 1)
+    attn_tc_dq_kernel(const __grid_constant__ AttnProblem p, const __grid_constant__ AtMaps maps,
+                      const __grid_constant__ AtExtra ex)
+{
+    using S = AbShape<D>;
+    extern __shared__ __align__(1024) uint8_t smem[];
+    const uint32_t base = smem_u32(smem);
+    AbBars& b = *reinterpret_cast<AbBars*>(smem + S::BARS_AT);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    volatile int* give_up = &b.give_up;
+    if (at_misplaced(base, ex.status))
+        return;
+
+    long long at = blockIdx.x;
+    const int tiles_k = attn_tiles(p.sk, AT_TILE), tiles_q = attn_tiles(p.sq, AT_TILE);
+    const int tile = tiles_q - 1 - (int) (at % tiles_q); // causal: the longest walks first
+    at /= tiles_q;
+    const int split = (int) (at % p.kv_splits);
+    const long long nh = at / p.kv_splits, n = nh / p.q_heads;
+    const int head = (int) (nh - n * p.q_heads), kv_head = head / p.group;
+    const int i0 = tile * AT_TILE;
+    const int lo = (int) ((long long) tiles_k * split / p.kv_splits);
+    int hi = (int) ((long long) tiles_k * (split + 1) / p.kv_splits);
+    if (p.causal)
+        hi = (int) min((long long) hi, max(0ll, (long long) i0 + AT_TILE - 1 + p.offset + AT_TILE) / AT_TILE);
+    const int steps = max(0, hi - lo);
+
+    ab_init(b, warp);
+    const uint32_t tmem = b.tmem;
+    const uint32_t* bits = ex.kv_bits ? ex.kv_bits + n * ex.words : nullptr;
+    const float* stats = p.stats;
+    wait_for_previous_kernel(bits, stats);
+    bool ok = true;
+    const uint32_t s_at = tmem, dp_at = tmem + 256, dq_at = tmem + 384;
+
+    if (warp >= AT_MMA_WARP)
+    {
+        at_other_registers();
+        if (warp == AT_TMA_WARP)
+        {
+            if (lane == 0 && steps > 0)
+            {
+                mbar_expect_tx(&b.own_full, 2 * AtTile<D>::BYTES);
+                at_tma_tile<D>(base + S::OWN_AT, &maps.q, i0, head, (int) n, &b.own_full);
+                at_tma_tile<D>(base + S::OWN_AT + AtTile<D>::BYTES, &maps.d_o, i0, head, (int) n, &b.own_full);
+                AtRing ra, rb;
+                for (int u = 0; u < 2 * steps && ok; ++u) // K and V in turn
+                {
+                    AtRing& r = u & 1 ? rb : ra;
+                    const uint32_t slots = u & 1 ? S::B_SLOTS : S::A_SLOTS;
+                    uint64_t *full = u & 1 ? b.b_full : b.a_full, *empty = u & 1 ? b.b_empty : b.a_empty;
+                    if (r.lap > 0)
+                        ok = mbar_wait_t<20>(&empty[r.slot], (r.lap - 1) & 1, give_up);
+                    if (!ok)
+                        break;
+                    mbar_expect_tx(&full[r.slot], AtTile<D>::BYTES);
+                    at_tma_tile<D>(base + (u & 1 ? S::B_AT : S::A_AT) + r.slot * AtTile<D>::BYTES,
+                                   u & 1 ? &maps.v : &maps.k, (lo + (u >> 1)) * AT_TILE, kv_head, (int) n,
+                                   &full[r.slot]);
+                    r.next(slots);
+                }
+                if (!ok || *give_up)
+                {
+                    int none = 0;
+                    mbar_wait_t<20>(&b.own_full, 0, &none);
+                    at_drain(b.a_full, S::A_SLOTS, ra);
+                    at_drain(b.b_full, S::B_SLOTS, rb);
+                }
+            }
+        }
+        else if (warp == AT_MMA_WARP)
+        {
+            if (lane == 0 && steps > 0)
+            {
+                const int ksteps = (p.d + 15) / 16;
+                const uint32_t width = (uint32_t) ksteps * 16;
+                const uint32_t q_at = base + S::OWN_AT, do_at = q_at + AtTile<D>::BYTES;
+                AtRing ra, rb; // of the next tiles to wait for
+                uint32_t k_slot = 0;
+                int ahead = 0; // scores taken so far
+                const auto scores = [&] {
+                    ok = ok && mbar_wait_t<0>(&b.a_full[ra.slot], ra.lap & 1, give_up);
+                    if (!ok)
+                        return;
+                    tc_fence_after();
+                    at_scores<D>(s_at + 128 * (ahead & 1), q_at, base + S::A_AT + ra.slot * AtTile<D>::BYTES, ksteps);
+                    mma_commit(&b.s_full[ahead & 1]);
+                    ++ahead;
+                    ra.next(S::A_SLOTS);
+                };
+                const auto weight_grads = [&] {
+                    ok = ok && mbar_wait_t<0>(&b.b_full[rb.slot], rb.lap & 1, give_up);
+                    if (!ok)
+                        return;
+                    tc_fence_after();
+                    at_scores<D>(dp_at, do_at, base + S::B_AT + rb.slot * AtTile<D>::BYTES, ksteps);
+                    mma_commit(&b.dp_full);
+                    mma_commit(&b.b_empty[rb.slot]);
+                    rb.next(S::B_SLOTS);
+                };
+                ok = mbar_wait_t<0>(&b.own_full, 0, give_up);
+                scores();
+                weight_grads();
+                if (steps > 1)
+                    scores();
+                for (int u = 0; u < steps && ok; ++u)
+                {
+                    ok = mbar_wait_t<0>(&b.ds_ready, u & 1, give_up);
+                    if (!ok)
+                        break;
+                    tc_fence_after();
+                    at_weigh<D>(dq_at, dp_at, 64, base + S::A_AT + k_slot * AtTile<D>::BYTES, width, u == 0);
+                    mma_commit(&b.a_empty[k_slot]);
+                    k_slot = k_slot + 1 == S::A_SLOTS ? 0 : k_slot + 1;
+                    if (u + 1 < steps)
+                        weight_grads();
+                    if (u + 2 < steps)
+                        scores();
+                }
+                if (ok)
+                    mma_commit(&b.fin);
+                else
+                    ab_drain_products(b);
+            }
+        }
+    }
+    else
+    {
+        at_team_registers();
+        const int team = warp >> 2;
+        const uint32_t lanes = (uint32_t) (warp & 3) << 21;
+        const int i = i0 + (threadIdx.x & 127);
+        const uint32_t dp_mine = dp_at + lanes + 64 * team;
+        const float* row = stats + nh * p.stats_pitch + i; // up to a multiple of 128 cells
+        const float lse = row[0], delta = row[(long long) p.n * p.q_heads * p.stats_pitch];
+        for (int u = 0; u < steps; ++u)
+        {
+            const int j0 = (lo + u) * AT_TILE + 64 * team;
+            const uint32_t s_mine = s_at + lanes + 128 * (u & 1) + 64 * team;
+            ok = at_warp_wait(&b.s_full[u & 1], (u >> 1) & 1, give_up);
+            if (!ok)
+                break;
+            tc_fence_after();
+            float w[64];
+            at_tmem_ld32(s_mine, w);
+            at_tmem_ld32(s_mine + 32, w + 32);
+            at_tmem_wait_ld();
+#pragma unroll
+            for (int c = 0; c < 64; ++c)
+                w[c] = at_exp2(fmaf(w[c], p.scale, -lse));
+            ok = at_warp_wait(&b.dp_full, u & 1, give_up);
+            if (!ok)
+                break;
+            tc_fence_after();
+            float d[64];
+            at_tmem_ld32(dp_mine, d);
+            at_tmem_ld32(dp_mine + 32, d + 32);
+            at_tmem_wait_ld();
+            uint32_t see[2];
+            bool all = true;
+#pragma unroll
+            for (int k = 0; k < 2; ++k)
+            {
+                see[k] = at_there(p, bits, j0, k);
+                if (p.causal)
+                    see[k] &= at_up_to(i + p.offset - j0, k);
+                all = all && see[k] == ~0u;
+            }
+#pragma unroll
+            for (int c = 0; c < 64; ++c)
+                d[c] = w[c] * (d[c] - delta);
+            if (__any_sync(~0u, !all))
+            {
+#pragma unroll
+                for (int c = 0; c < 64; ++c)
+                    d[c] = see[c >> 5] >> (c & 31) & 1 ? d[c] : 0.f;
+            }
+            uint32_t packed[32];
+#pragma unroll
+            for (int c = 0; c < 32; ++c)
+                packed[c] = pack_bf16(d[2 * c], d[2 * c + 1]);
+            at_tmem_st32(dp_mine, packed);
+            at_tmem_wait_st();
+            at_warp_arrive(&b.ds_ready, lane);
+        }
+        if (ok && steps > 0)
+            ok = at_warp_wait(&b.fin, 0, give_up);
+        tc_fence_after();
+        if (ok)
+        {
+            float* part = p.kv_splits > 1 ? p.part_dq + (long long) split * p.n * p.q_heads * p.d * p.sq : nullptr;
+            at_store(p.dq, part, nh, n, head, p.d, i, p.sq, p.scale / ATTN_LOG2E, lse == INFINITY, steps == 0,
+                     dq_at + lanes, team * (D / 2), (team + 1) * (D / 2));
+        }
+    }
+    at_finish(ok, ex.status, warp, lane, tmem);
+}
+
+template <int D>
+int32_t ab_launch(const AttnProblem& p, const AtMaps& maps, const AtExtra& ex, cudaStream_t stream)
+{
+    const long long dkv = (long long) p.n * p.kv_heads * attn_tiles(p.sk, AT_TILE) * p.q_splits;
+    const long long dq = (long long) p.n * p.q_heads * attn_tiles(p.sq, AT_TILE) * p.kv_splits;
+    DCB_REQUIRE(dkv < (1ll << 31) && dq < (1ll << 31), "too many tiles");
+    if (int32_t e = allow_dynamic_smem((const void*) attn_tc_dkv_kernel<D>, AbShape<D>::SMEM))
+        return e;
+    if (int32_t e = allow_dynamic_smem((const void*) attn_tc_dq_kernel<D>, AbShape<D>::SMEM))
+        return e;
+    DCB_CUDA_TRY(launch_overlapped(attn_tc_dkv_kernel<D>, dim3((unsigned) dkv), AT_THREADS, AbShape<D>::SMEM, stream, p,
+                                   maps, ex));
+    DCB_CUDA_TRY(launch_overlapped(attn_tc_dq_kernel<D>, dim3((unsigned) dq), AT_THREADS, AbShape<D>::SMEM, stream, p,
+                                   maps, ex));
+    return DCB_OK;
+}
+
+} // namespace
+
+int32_t attn_tc_bwd_launch(const AttnProblem& p, const AtMaps& maps, const AtExtra& ex, cudaStream_t stream)
+{
+    return p.d <= 64 ? ab_launch<64>(p, maps, ex, stream) : ab_launch<128>(p, maps, ex, stream);
+}
+
+} // namespace dcb

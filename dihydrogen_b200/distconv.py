@@ -1684,6 +1684,7 @@ class Attention:
     (D, H, W); ``causal`` lets cell i of the queries see the keys up to
     i + (keys - queries).  A sample's cells have to be on one rank: re-distribute
     a spatially partitioned tensor to sample-parallel first (``TensorShuffler``).
+    ``num_dims`` is the queries'; an image's cells may read a volume's.
 
     ``q_mask`` / ``kv_mask``: arrays of bool or uint8, one per sample and cell, 0
     where a cell is not there; whatever such a cell holds is never read into a
@@ -1719,9 +1720,8 @@ class Attention:
         return got
 
     def _checked(self, q, k, v, q_like, kv_like, lse, q_mask, kv_mask):
-        for t in (q, k):
-            if t.nd != self.num_dims:
-                raise ValueError(f"a tensor of {t.nd} dimensions, set up for {self.num_dims}")
+        if q.nd != self.num_dims:
+            raise ValueError(f"queries of {q.nd} dimensions, set up for {self.num_dims}")
         for t in (q, k, v) + q_like + kv_like:
             for dim in range(t.nd - 1):
                 if t.dist.is_distributed(dim) and t.dist.locale_shape[dim] > 1:

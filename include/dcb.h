@@ -491,7 +491,7 @@ int32_t dcb_rotary_apply(const dcb_rotary_plan* plan, const dcb_nd_desc* xd,
  * i may see j if q_mask (n x cells of q bytes, may be null) is not 0 at i, kv_mask
  * (n x cells of k) not at j, and, where `causal`, j <= i + (cells of k - cells of
  * q).  A cell that sees nothing gets o = 0, lse = -infinity and takes no part in
- * any gradient.  Cells that a mask takes out are never interpreted, whatever they
+ * any gradient (its d_o has to be finite where no mask takes it out).  Cells that a mask takes out are never interpreted, whatever they
  * hold; `causal` only sets the weight of a later cell to 0, its values have to be
  * finite.  A sample's cells lie contiguous (a shard without halo; re-distribute a
  * spatially partitioned tensor to sample-parallel first); sample and channel
