@@ -85,6 +85,59 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi)
     return *reinterpret_cast<const uint32_t*>(&t);
 }
 
+// V neighbours as they are stored.  Loads that are taken ahead keep these and are converted where they are used: a
+// conversion right behind a load waits for it.
+template <class T, int V>
+struct RawElems;
+
+template <int V>
+struct RawElems<float, V>
+{
+    float v[V];
+    __device__ __forceinline__ void load(const float* p) { load_elems<V>(p, v); }
+    __device__ __forceinline__ float get(int e) const { return v[e]; }
+    __device__ __forceinline__ void clear()
+    {
+#pragma unroll
+        for (int e = 0; e < V; ++e)
+            v[e] = 0.f;
+    }
+};
+
+template <int V>
+struct RawElems<bf16, V>
+{
+    static constexpr int WORDS = (V + 1) / 2;
+    uint32_t w[WORDS];
+    __device__ __forceinline__ void load(const bf16* p)
+    {
+        if constexpr (V == 8)
+        {
+            const uint4 t = *reinterpret_cast<const uint4*>(p);
+            w[0] = t.x, w[1] = t.y, w[2] = t.z, w[3] = t.w;
+        }
+        else if constexpr (V == 4)
+        {
+            const uint2 t = *reinterpret_cast<const uint2*>(p);
+            w[0] = t.x, w[1] = t.y;
+        }
+        else if constexpr (V == 2)
+            w[0] = *reinterpret_cast<const uint32_t*>(p);
+        else
+            w[0] = *reinterpret_cast<const uint16_t*>(p);
+    }
+    __device__ __forceinline__ float get(int e) const
+    {
+        return __uint_as_float(e & 1 ? w[e / 2] & 0xffff0000u : w[e / 2] << 16);
+    }
+    __device__ __forceinline__ void clear()
+    {
+#pragma unroll
+        for (int i = 0; i < WORDS; ++i)
+            w[i] = 0;
+    }
+};
+
 template <int V>
 __device__ __forceinline__ void store_elems(float* p, const float (&v)[V])
 {
@@ -117,10 +170,10 @@ struct CellUnits
     int narrow;        // all numbers have 31 bits
 };
 
-inline CellUnits cell_units(const RunGeom& g, int v)
+// `per_run` units a run.
+inline CellUnits cell_units_of(const RunGeom& g, long long per_run)
 {
     CellUnits u;
-    const long long per_run = g.len / v;
     u.total = g.n * g.rows * per_run;
     u.cells = g.rows * g.len;
     u.len = g.len;
@@ -130,6 +183,11 @@ inline CellUnits cell_units(const RunGeom& g, int v)
     u.rows = safe(g.rows);
     u.rows_inner = safe(g.rows_inner);
     return u;
+}
+
+inline CellUnits cell_units(const RunGeom& g, int v)
+{
+    return cell_units_of(g, g.len / v);
 }
 
 struct CellAt

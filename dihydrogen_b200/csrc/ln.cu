@@ -1,11 +1,13 @@
 // Layer normalisation over the channels of every cell, forward and backward.
 //
 // In NC[D]HW a cell's channels lie a volume apart, its neighbours in W beside it.  A warp's
-// lanes therefore take neighbouring units of V cells, and a cell's C channels are dealt out to
-// the G warps of a group, K each: all accesses are coalesced, a tensor is read once and kept in
-// registers, and what the warps of a group exchange is two floats a cell (their sum and their
-// centred sum of squares forward, the two sums of the gradient backward).  HBM bound: 2 tensors
-// forward, 3 backward.
+// lanes therefore take neighbouring cells, V each, and a cell's C channels are dealt out to the G
+// warps of a group: all accesses are coalesced, and what the warps of a group exchange is two
+// floats a cell (their sum and their centred sum of squares forward, the two sums of the gradient
+// backward).  The channels are walked over twice, eight at a time, the second time out of L1 or L2,
+// where a tile of 32 V cells still is: HBM sees two tensors forward, three backward.  (With all of a
+// thread's channels in registers instead, addresses and predicates of the unrolled accesses took 50
+// instructions an element and 15 million bf16 values in rows of odd length 40 us.)
 #include "elem.cuh"
 
 namespace dcb
@@ -13,149 +15,313 @@ namespace dcb
 namespace
 {
 
-constexpr int LN_WIDE_WARPS = 16;  // warps of a block of the kernels for many channels
-constexpr int LN_CHUNK = 32;       // channels that a lane of those takes at a time
-constexpr int LN_MAX_GROUP = 16;   // warps of a group: 512 threads of up to 128 registers
-constexpr int LN_NARROW = LN_MAX_GROUP * 32;
-constexpr int LN_MAX_CHANNELS = 16384; // the wide backward kernel's sums fill 128 KB of shared memory
+constexpr int LN_STEP = 8;    // channels at a time
+constexpr int LN_WARPS = 8;   // of a block
+constexpr int LN_MAX_CHANNELS = 16384; // the backward kernel's sums of a channel fill 128 KB of shared memory
+
+// Blocks of the backward kernel that an SM's registers hold.
+__host__ __device__ constexpr int ln_bwd_blocks(int v)
+{
+    return v == 1 ? 4 : 2;
+}
 
 struct LnGeom
 {
-    CellUnits units;
+    CellUnits units;  // of V cells (FLAT) or of 32 V
     long long per_run, rows, rows_inner;
     int c, g;         // channels; warps of a group
-    long long tiles;  // of 32 units a group of warps
+    float inv_c;
+    long long tiles;  // of all groups of a block
 };
 
-__device__ __forceinline__ CellAt ln_cell(const LnGeom& g, long long unit, int v)
+// How a warp's cells lie.  FLAT: units of V neighbours packed over short runs.  ROWS: 32 V cells of one run, a lane has
+// V neighbours.  SPLIT: the same cells where a run starts off the alignment of such accesses, a lane's are 32 apart.
+// In the last two everything but the lane is the same for a warp, so that a channel's address costs no instruction
+// of the lanes.
+enum LnMode
 {
-    return v == 4   ? cell_at<4>(g.units, g.per_run, g.rows, g.rows_inner, unit)
-           : v == 2 ? cell_at<2>(g.units, g.per_run, g.rows, g.rows_inner, unit)
-                    : cell_at<1>(g.units, g.per_run, g.rows, g.rows_inner, unit);
-}
+    LN_FLAT,
+    LN_ROWS,
+    LN_SPLIT
+};
 
-// Sum and centred sum of squares of all channels from those of the groups' parts (Chan et al.): no cancellation
-// between large squares, whatever the mean.
-template <int V>
-__device__ __forceinline__ void ln_join(const float* part, int g, int c, int lane, float (&mean)[V], float (&m2)[V])
+template <int V, int MODE>
+struct LnAt
 {
-    float s[V], q[V], t[V];
-#pragma unroll
-    for (int e = 0; e < V; ++e)
-        s[e] = 0.f;
-    for (int i = 0; i < g; ++i)
+    using Lane = std::conditional_t<MODE == LN_FLAT, long long, uint32_t>;
+    CellAt cell; // the thread's first cell (FLAT), the warp's (else)
+    Lane lane;   // what a thread adds to the offset of that
+    int have;    // cells of the thread that are there
+    bool full;   // all cells of the warp are
+
+    __device__ __forceinline__ LnAt(const LnGeom& g, long long first, int l)
     {
-        load_elems<V>(part + (2 * i * 32 + lane) * V, t);
+        if (MODE == LN_FLAT)
+        {
+            const bool live = first + l < g.units.total;
+            cell = cell_at<V>(g.units, g.per_run, g.rows, g.rows_inner, live ? first + l : 0);
+            have = live ? V : 0;
+            full = first + 32 <= g.units.total;
+            lane = 0;
+            return;
+        }
+        const long long chunk = first >> 5;
+        const bool live = chunk < g.units.total;
+        cell = cell_at<32 * V>(g.units, g.per_run, g.rows, g.rows_inner, live ? chunk : 0);
+        const long long left = live ? g.units.len - cell.pos : 0;
+        full = left >= 32 * V;
+        lane = MODE == LN_ROWS ? l * V : l;
+        if (full)
+            have = V;
+        else if (MODE == LN_ROWS)
+            have = l * V < left ? V : 0; // runs are multiples of V
+        else
+            have = l < left ? (int) (left - l + 31) / 32 : 0;
+    }
+    __device__ __forceinline__ long long stat(const LnGeom& g) const { return cell.n * g.units.cells + cell.cell; }
+};
+
+// Values as they are stored; converted where they are used, since a conversion right behind a load waits for it.
+template <class T, int V, int MODE>
+struct LnRaw
+{
+    RawElems<T, V> r;
+    template <bool FULL>
+    __device__ __forceinline__ void load(const T* p, int have)
+    {
+        if (FULL || have > 0)
+            r.load(p);
+        else
+            r.clear();
+    }
+    __device__ __forceinline__ float get(int e) const { return r.get(e); }
+};
+
+template <class T, int V>
+struct LnRaw<T, V, LN_SPLIT>
+{
+    RawElems<T, 1> r[V];
+    template <bool FULL>
+    __device__ __forceinline__ void load(const T* p, int have)
+    {
 #pragma unroll
         for (int e = 0; e < V; ++e)
-            s[e] += t[e];
+            if (FULL || e < have)
+                r[e].load(p + 32 * e);
+            else
+                r[e].clear();
     }
-#pragma unroll
-    for (int e = 0; e < V; ++e)
-        mean[e] = s[e] / c, m2[e] = 0.f;
-    for (int i = 0; i < g; ++i)
+    __device__ __forceinline__ float get(int e) const { return r[e].get(0); }
+};
+
+template <int V, int MODE, bool FULL, class T>
+__device__ __forceinline__ void ln_store(T* p, const float (&v)[V], int have)
+{
+    if constexpr (MODE == LN_SPLIT)
     {
-        const int count = (c - i + g - 1) / g;
-        load_elems<V>(part + (2 * i * 32 + lane) * V, t);
-        load_elems<V>(part + ((2 * i + 1) * 32 + lane) * V, q);
 #pragma unroll
         for (int e = 0; e < V; ++e)
-        {
-            const float d = t[e] / count - mean[e];
-            m2[e] += q[e] + count * d * d;
-        }
-    }
-}
-
-template <class T, int V, int K>
-__global__ void __launch_bounds__(512)
-    ln_fwd_kernel(const T* x, RunStrides xs, T* y, RunStrides ys, const float* scale, const float* bias, float eps,
-                  float* mean_out, float* inv_std_out, LnGeom geo)
-{
-    extern __shared__ float part[];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int group = warp / geo.g, cg = warp - group * geo.g;
-    wait_for_previous_kernel(x, scale, bias);
-    dependents_may_start();
-    const long long unit = ((long long) blockIdx.x * (blockDim.x / 32 / geo.g) + group) * 32 + lane;
-    const bool live = unit < geo.units.total;
-    CellAt at = {};
-    float v[K][V];
-    if (live)
-    {
-        at = ln_cell(geo, unit, V);
-        const T* px = x + offset_of(at, xs);
-#pragma unroll
-        for (int k = 0; k < K; ++k)
-        {
-            const int c = cg + k * geo.g;
-            if (c < geo.c)
-                load_elems<V>(px + c * xs.sc, v[k]);
-        }
-    }
-    const int count = (geo.c - cg + geo.g - 1) / geo.g; // at least 1: g <= c
-    float sum[V], m2[V];
-#pragma unroll
-    for (int e = 0; e < V; ++e)
-    {
-        sum[e] = m2[e] = 0.f;
-#pragma unroll
-        for (int k = 0; k < K; ++k)
-            if (k < count)
-                sum[e] += live ? v[k][e] : 0.f;
-        const float m = sum[e] / count;
-#pragma unroll
-        for (int k = 0; k < K; ++k)
-            if (k < count)
+            if (FULL || e < have)
             {
-                const float d = (live ? v[k][e] : 0.f) - m;
-                m2[e] = fmaf(d, d, m2[e]);
+                const float t[1] = {v[e]};
+                store_elems<1>(p + 32 * e, t);
             }
     }
-    float mean[V];
-    if (geo.g > 1)
+    else if (FULL || have > 0)
+        store_elems<V>(p, v);
+}
+
+// Sum over the warps of a group of what each of them left for this thread's cells.
+template <int V>
+__device__ __forceinline__ void ln_gather(const float* part, int g, int lane, float (&sum)[V])
+{
+#pragma unroll
+    for (int e = 0; e < V; ++e)
+        sum[e] = 0.f;
+#pragma unroll 4
+    for (int i = 0; i < g; ++i)
     {
-        float* mine = part + group * geo.g * 2 * 32 * V;
-        store_elems<V>(mine + (2 * cg * 32 + lane) * V, sum);
-        store_elems<V>(mine + ((2 * cg + 1) * 32 + lane) * V, m2);
-        __syncthreads();
-        ln_join<V>(mine, geo.g, geo.c, lane, mean, m2);
+        float t[V];
+        load_elems<V>(part + (i * 32 + lane) * V, t);
+#pragma unroll
+        for (int e = 0; e < V; ++e)
+            sum[e] += t[e];
+    }
+}
+
+// What a thread is in its block.
+struct LnSelf
+{
+    int lane, groups, group, cg;
+    int count; // its channels: cg, cg + g, ...
+    __device__ __forceinline__ LnSelf(const LnGeom& g)
+    {
+        const int warp = __shfl_sync(~0u, (int) threadIdx.x >> 5, 0); // known to be uniform
+        lane = threadIdx.x & 31;
+        groups = LN_WARPS / g.g;
+        group = warp / g.g;
+        cg = warp - group * g.g;
+        count = (g.c - cg + g.g - 1) / g.g;
+    }
+};
+
+template <int M>
+struct LnSome
+{
+    static constexpr int value = M;
+};
+
+// f(first channel, how many), eight at a time and the rest in powers of two, so that how many there are is known when
+// compiled.  (Predicates on each of eight took twice the time for 50 channels.)
+template <bool FULL, class F>
+__device__ __forceinline__ void ln_steps(int count, F f)
+{
+    int i = 0;
+#pragma unroll 1
+    for (; i + LN_STEP <= count; i += LN_STEP)
+        f(i, LnSome<LN_STEP>());
+    if constexpr (FULL)
+    {
+        if (count & 4)
+            f(i, LnSome<4>()), i += 4;
+        if (count & 2)
+            f(i, LnSome<2>()), i += 2;
+        if (count & 1)
+            f(i, LnSome<1>());
     }
     else
     {
+#pragma unroll 1
+        for (; i < count; ++i)
+            f(i, LnSome<1>());
+    }
+}
+
+template <class T, int V, int MODE, bool FULL>
+__device__ __forceinline__ void ln_fwd_tile(const T* x, const RunStrides& xs, T* y, const RunStrides& ys,
+                                            const float* __restrict__ scale, const float* __restrict__ bias, float eps,
+                                            float* mean_out, float* inv_std_out, const LnGeom& geo, const LnSelf& me,
+                                            const LnAt<V, MODE>& at, float* sums, float* squares)
+{
+    const T* px = x + (offset_of(at.cell, xs) + me.cg * xs.sc) + at.lane;
+    const long long x_step = geo.g * xs.sc;
+    // mean and centred squares of eight channels at a time, joined with those before (Chan et al.): no cancellation,
+    // whatever the mean
+    float mean[V], m2[V];
+#pragma unroll
+    for (int e = 0; e < V; ++e)
+        mean[e] = m2[e] = 0.f;
+    const T* p = px;
+    ln_steps<FULL>(me.count, [&](int i, auto some) {
+        constexpr int m = decltype(some)::value;
+        LnRaw<T, V, MODE> v[m];
+#pragma unroll
+        for (int k = 0; k < m; ++k, p += x_step)
+                v[k].template load<FULL>(p, at.have);
+        const float inv_m = 1.f / m, f = m / (float) (i + m);
 #pragma unroll
         for (int e = 0; e < V; ++e)
-            mean[e] = sum[e] / count;
+        {
+            float s = 0.f, q = 0.f;
+#pragma unroll
+            for (int k = 0; k < m; ++k)
+                s += v[k].get(e);
+            s *= inv_m;
+#pragma unroll
+            for (int k = 0; k < m; ++k)
+                q = fmaf(v[k].get(e) - s, v[k].get(e) - s, q);
+            const float d = s - mean[e];
+            mean[e] = fmaf(d, f, mean[e]);
+            m2[e] += fmaf(d * d, f * i, q);
+        }
+    });
+    if (geo.g > 1)
+    {
+        float all[V];
+#pragma unroll
+        for (int e = 0; e < V; ++e)
+            all[e] = mean[e] * me.count;
+        store_elems<V>(sums + (me.cg * 32 + me.lane) * V, all);
+        __syncthreads();
+        ln_gather<V>(sums, geo.g, me.lane, all);
+#pragma unroll
+        for (int e = 0; e < V; ++e)
+        {
+            const float d = mean[e] - all[e] * geo.inv_c;
+            m2[e] = fmaf(d * d, (float) me.count, m2[e]);
+            mean[e] = all[e] * geo.inv_c;
+        }
+        store_elems<V>(squares + (me.cg * 32 + me.lane) * V, m2);
+        __syncthreads(); // behind it nobody reads `sums`, and behind the next tile's first nobody `squares`
+        ln_gather<V>(squares, geo.g, me.lane, m2);
     }
-    if (!live)
-        return;
     float inv[V];
 #pragma unroll
     for (int e = 0; e < V; ++e)
-        inv[e] = 1.f / sqrtf(m2[e] / geo.c + eps);
-    if (cg == 0)
+        inv[e] = 1.f / sqrtf(fmaf(m2[e], geo.inv_c, eps));
+    if (me.cg == 0)
     {
-        const long long i = at.n * geo.units.cells + at.cell;
+        const long long i = at.stat(geo);
         if (mean_out)
-            store_elems<V>(mean_out + i, mean);
+            ln_store<V, MODE, FULL>(mean_out + i + at.lane, mean, at.have);
         if (inv_std_out)
-            store_elems<V>(inv_std_out + i, inv);
+            ln_store<V, MODE, FULL>(inv_std_out + i + at.lane, inv, at.have);
     }
-    T* py = y + offset_of(at, ys);
+    p = px;
+    T* py = y + (offset_of(at.cell, ys) + me.cg * ys.sc) + at.lane;
+    const long long y_step = geo.g * ys.sc;
+    ln_steps<FULL>(me.count, [&](int i, auto some) {
+        constexpr int m = decltype(some)::value;
+        LnRaw<T, V, MODE> v[m];
+        float w[m], b[m];
 #pragma unroll
-    for (int k = 0; k < K; ++k)
+        for (int k = 0; k < m; ++k, p += x_step)
+            {
+                v[k].template load<FULL>(p, at.have);
+                const int c = me.cg + (i + k) * geo.g;
+                w[k] = scale ? __ldg(scale + c) : 1.f;
+                b[k] = bias ? __ldg(bias + c) : 0.f;
+            }
+#pragma unroll
+        for (int k = 0; k < m; ++k, py += y_step)
+            {
+                float out[V];
+#pragma unroll
+                for (int e = 0; e < V; ++e)
+                    out[e] = fmaf((v[k].get(e) - mean[e]) * inv[e], w[k], b[k]);
+                ln_store<V, MODE, FULL>(py, out, at.have);
+            }
+    });
+}
+
+// Shared memory: the groups' sums and their centred sums of squares.
+template <class T, int V, int MODE>
+__global__ void __launch_bounds__(32 * LN_WARPS, 4)
+    ln_fwd_kernel(const T* x, RunStrides xs, T* y, RunStrides ys, const float* scale, const float* bias, float eps,
+                  float* mean_out, float* inv_std_out, LnGeom geo)
+{
+    __shared__ float4 room[2 * LN_WARPS * 32 * V / 4];
+    const LnSelf me(geo);
+    float* sums = reinterpret_cast<float*>(room) + me.group * geo.g * 32 * V;
+    float* squares = sums + LN_WARPS * 32 * V;
+    wait_for_previous_kernel(x, scale, bias);
+    for (long long tile = blockIdx.x; tile < geo.tiles; tile += gridDim.x)
     {
-        const int c = cg + k * geo.g;
-        if (c < geo.c)
+        if (me.group == me.groups) // more warps than groups take
         {
-            const float w = scale ? scale[c] : 1.f, b = bias ? bias[c] : 0.f;
-            float out[V];
-#pragma unroll
-            for (int e = 0; e < V; ++e)
-                out[e] = fmaf((v[k][e] - mean[e]) * inv[e], w, b);
-            store_elems<V>(py + c * ys.sc, out);
+            if (geo.g > 1)
+                __syncthreads(), __syncthreads();
+            continue;
         }
+        const LnAt<V, MODE> at(geo, (tile * me.groups + me.group) * 32, me.lane);
+        if (at.full)
+            ln_fwd_tile<T, V, MODE, true>(x, xs, y, ys, scale, bias, eps, mean_out, inv_std_out, geo, me, at, sums,
+                                          squares);
+        else
+            ln_fwd_tile<T, V, MODE, false>(x, xs, y, ys, scale, bias, eps, mean_out, inv_std_out, geo, me, at, sums,
+                                           squares);
     }
+    dependents_may_start();
 }
 
 // Sums over a warp's lanes of K values a lane, by halves: lane l ends with the sum of value l mod K
@@ -182,321 +348,147 @@ __device__ __forceinline__ float ln_lane_sums(float (&v)[K], int lane)
     return r;
 }
 
-// Blocks walk over the tiles; the gradients of scale and bias stay in registers, K channels a
-// lane, and are added up over the lanes once, at the end: partial[which][channel][block].
-template <class T, int V, int K>
-__global__ void __launch_bounds__(512)
+template <class T, int V, int MODE, bool FULL>
+__device__ __forceinline__ void ln_bwd_tile(const T* x, const RunStrides& xs, const T* dy, const RunStrides& dys,
+                                            const float* mean_in, const float* inv_std_in,
+                                            const float* __restrict__ scale, T* dx, const RunStrides& dxs, bool grads,
+                                            const LnGeom& geo, const LnSelf& me, const LnAt<V, MODE>& at, float* mine,
+                                            float* acc)
+{
+    // what is not there is loaded as zeros and adds nothing
+    LnRaw<float, V, MODE> mean, inv;
+    const long long stat = at.stat(geo);
+    mean.template load<FULL>(mean_in + stat + at.lane, at.have);
+    inv.template load<FULL>(inv_std_in + stat + at.lane, at.have);
+    const T* px = x + (offset_of(at.cell, xs) + me.cg * xs.sc) + at.lane;
+    const T* pd = dy + (offset_of(at.cell, dys) + me.cg * dys.sc) + at.lane;
+    const long long x_step = geo.g * xs.sc, dy_step = geo.g * dys.sc;
+    float a[V], b[V];
+#pragma unroll
+    for (int e = 0; e < V; ++e)
+        a[e] = b[e] = 0.f;
+    const T *p = px, *d = pd;
+    ln_steps<FULL>(me.count, [&](int i, auto some) {
+        constexpr int m = decltype(some)::value;
+        LnRaw<T, V, MODE> x_of[m], dy_of[m];
+        float sw[m], sb[m];
+#pragma unroll
+        for (int k = 0; k < m; ++k, p += x_step, d += dy_step)
+        {
+            x_of[k].template load<FULL>(p, at.have);
+            dy_of[k].template load<FULL>(d, at.have);
+        }
+#pragma unroll
+        for (int k = 0; k < m; ++k)
+        {
+            sw[k] = sb[k] = 0.f;
+            const float w = scale ? __ldg(scale + me.cg + (i + k) * geo.g) : 1.f;
+#pragma unroll
+            for (int e = 0; e < V; ++e)
+            {
+                const float u = (x_of[k].get(e) - mean.get(e)) * inv.get(e), y = dy_of[k].get(e), g = y * w;
+                sw[k] = fmaf(y, u, sw[k]);
+                sb[k] += y;
+                a[e] += g;
+                b[e] = fmaf(g, u, b[e]);
+            }
+        }
+        if (grads) // a channel belongs to one warp of the group
+        {
+            const float tw = ln_lane_sums<m>(sw, me.lane), tb = ln_lane_sums<m>(sb, me.lane);
+            const int c = me.cg + (i + me.lane) * geo.g;
+            if (me.lane < m)
+            {
+                acc[c] += tw;
+                acc[geo.c + c] += tb;
+            }
+        }
+    });
+    if (geo.g > 1)
+    {
+        store_elems<V>(mine + (me.cg * 32 + me.lane) * V, a);
+        store_elems<V>(mine + (LN_WARPS * 32 + me.cg * 32 + me.lane) * V, b);
+        __syncthreads(); // the other half of the sums' room is free again behind the next tile's barrier
+        ln_gather<V>(mine, geo.g, me.lane, a);
+        ln_gather<V>(mine + LN_WARPS * 32 * V, geo.g, me.lane, b);
+    }
+#pragma unroll
+    for (int e = 0; e < V; ++e)
+        a[e] *= geo.inv_c, b[e] *= geo.inv_c;
+    p = px, d = pd;
+    T* po = dx + (offset_of(at.cell, dxs) + me.cg * dxs.sc) + at.lane;
+    const long long dx_step = geo.g * dxs.sc;
+    ln_steps<FULL>(me.count, [&](int i, auto some) {
+        constexpr int m = decltype(some)::value;
+        LnRaw<T, V, MODE> x_of[m], dy_of[m];
+        float w[m];
+#pragma unroll
+        for (int k = 0; k < m; ++k, p += x_step, d += dy_step)
+            {
+                x_of[k].template load<FULL>(p, at.have);
+                dy_of[k].template load<FULL>(d, at.have);
+                w[k] = scale ? __ldg(scale + me.cg + (i + k) * geo.g) : 1.f;
+            }
+#pragma unroll
+        for (int k = 0; k < m; ++k, po += dx_step)
+            {
+                float out[V];
+#pragma unroll
+                for (int e = 0; e < V; ++e)
+                {
+                    const float u = (x_of[k].get(e) - mean.get(e)) * inv.get(e);
+                    out[e] = inv.get(e) * (fmaf(dy_of[k].get(e), w[k], -a[e]) - u * b[e]);
+                }
+                ln_store<V, MODE, FULL>(po, out, at.have);
+            }
+    });
+}
+
+// Blocks walk over the tiles.  The gradients of scale and bias are added up over a tile's cells by exchanges between
+// the lanes, over the tiles in shared memory, [group][2][c], and leave as partial[which][channel][block].
+template <class T, int V, int MODE>
+__global__ void __launch_bounds__(32 * LN_WARPS, ln_bwd_blocks(V))
     ln_bwd_kernel(const T* x, RunStrides xs, const T* dy, RunStrides dys, const float* mean_in,
                   const float* inv_std_in, const float* scale, T* dx, RunStrides dxs, float* partial, LnGeom geo)
 {
-    extern __shared__ float part[];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int groups = blockDim.x / 32 / geo.g;
-    const int group = warp / geo.g, cg = warp - group * geo.g;
-    const int stage = groups * geo.g * 2 * 32 * V;
+    extern __shared__ float acc[];
+    __shared__ float4 room[2][2 * LN_WARPS * 32 * V / 4];
+    const LnSelf me(geo);
+    if (partial)
+        for (int i = threadIdx.x; i < 2 * geo.c * me.groups; i += 32 * LN_WARPS)
+            acc[i] = 0.f;
     wait_for_previous_kernel(x, dy, mean_in, inv_std_in, scale);
-    dependents_may_start();
-    float acc_w[K], acc_b[K], w[K];
-#pragma unroll
-    for (int k = 0; k < K; ++k)
-    {
-        acc_w[k] = acc_b[k] = 0.f;
-        const int c = cg + k * geo.g;
-        w[k] = scale && c < geo.c ? scale[c] : 1.f;
-    }
+    __syncthreads();
     int turn = 0;
     for (long long tile = blockIdx.x; tile < geo.tiles; tile += gridDim.x, turn ^= 1)
     {
-        const long long unit = (tile * groups + group) * 32 + lane;
-        const bool live = unit < geo.units.total;
-        CellAt at = {};
-        float u[K][V], d[K][V], mean[V], inv[V], a[V], b[V];
-        if (live)
+        if (me.group == me.groups) // more warps than groups take
         {
-            at = ln_cell(geo, unit, V);
-            const T* px = x + offset_of(at, xs);
-            const T* pd = dy + offset_of(at, dys);
-#pragma unroll
-            for (int k = 0; k < K; ++k)
-            {
-                const int c = cg + k * geo.g;
-                if (c < geo.c)
-                {
-                    load_elems<V>(px + c * xs.sc, u[k]);
-                    load_elems<V>(pd + c * dys.sc, d[k]);
-                }
-            }
-            load_elems<V>(mean_in + at.n * geo.units.cells + at.cell, mean);
-            load_elems<V>(inv_std_in + at.n * geo.units.cells + at.cell, inv);
+            if (geo.g > 1)
+                __syncthreads();
+            continue;
         }
-#pragma unroll
-        for (int e = 0; e < V; ++e)
-        {
-            a[e] = b[e] = 0.f;
-#pragma unroll
-            for (int k = 0; k < K; ++k)
-            {
-                const bool have = live && cg + k * geo.g < geo.c;
-                u[k][e] = have ? (u[k][e] - mean[e]) * inv[e] : 0.f;
-                d[k][e] = have ? d[k][e] : 0.f;
-                acc_w[k] = fmaf(d[k][e], u[k][e], acc_w[k]);
-                acc_b[k] += d[k][e];
-                const float g = d[k][e] * w[k];
-                a[e] += g;
-                b[e] = fmaf(g, u[k][e], b[e]);
-            }
-        }
-        if (geo.g > 1)
-        {
-            float* mine = part + turn * stage + group * geo.g * 2 * 32 * V;
-            store_elems<V>(mine + (2 * cg * 32 + lane) * V, a);
-            store_elems<V>(mine + ((2 * cg + 1) * 32 + lane) * V, b);
-            __syncthreads(); // the other half of `part` is free again behind the next tile's barrier
-#pragma unroll
-            for (int e = 0; e < V; ++e)
-                a[e] = b[e] = 0.f;
-            for (int i = 0; i < geo.g; ++i)
-            {
-                float s[V], t[V];
-                load_elems<V>(mine + (2 * i * 32 + lane) * V, s);
-                load_elems<V>(mine + ((2 * i + 1) * 32 + lane) * V, t);
-#pragma unroll
-                for (int e = 0; e < V; ++e)
-                    a[e] += s[e], b[e] += t[e];
-            }
-        }
-        if (live)
-        {
-#pragma unroll
-            for (int e = 0; e < V; ++e)
-                a[e] /= geo.c, b[e] /= geo.c;
-            T* po = dx + offset_of(at, dxs);
-#pragma unroll
-            for (int k = 0; k < K; ++k)
-            {
-                const int c = cg + k * geo.g;
-                if (c < geo.c)
-                {
-                    float out[V];
-#pragma unroll
-                    for (int e = 0; e < V; ++e)
-                        out[e] = inv[e] * (fmaf(d[k][e], w[k], -a[e]) - u[k][e] * b[e]);
-                    store_elems<V>(po + c * dxs.sc, out);
-                }
-            }
-        }
+        const LnAt<V, MODE> at(geo, (tile * me.groups + me.group) * 32, me.lane);
+        float* mine = reinterpret_cast<float*>(room[turn]) + me.group * geo.g * 32 * V;
+        float* sums = acc + me.group * 2 * geo.c;
+        if (at.full)
+            ln_bwd_tile<T, V, MODE, true>(x, xs, dy, dys, mean_in, inv_std_in, scale, dx, dxs, partial != nullptr, geo,
+                                          me, at, mine, sums);
+        else
+            ln_bwd_tile<T, V, MODE, false>(x, xs, dy, dys, mean_in, inv_std_in, scale, dx, dxs, partial != nullptr,
+                                           geo, me, at, mine, sums);
     }
+    dependents_may_start();
     if (!partial)
         return;
-    // groups of a block first, in order, then the lanes
-    const float sw = ln_lane_sums<K>(acc_w, lane), sb = ln_lane_sums<K>(acc_b, lane);
     __syncthreads();
-    const int slots = geo.g * K;
-    if (lane < K)
+    for (int i = threadIdx.x; i < 2 * geo.c; i += 32 * LN_WARPS)
     {
-        part[(group * 2) * slots + cg + lane * geo.g] = sw;
-        part[(group * 2 + 1) * slots + cg + lane * geo.g] = sb;
-    }
-    __syncthreads();
-    for (int i = threadIdx.x; i < 2 * geo.c; i += blockDim.x)
-    {
-        const int which = i >= geo.c, c = which ? i - geo.c : i;
         float s = 0.f;
-        for (int p = 0; p < groups; ++p)
-            s += part[(p * 2 + which) * slots + c];
+        for (int p = 0; p < me.groups; ++p)
+            s += acc[p * 2 * geo.c + i];
         partial[(long long) i * gridDim.x + blockIdx.x] = s;
     }
-}
-
-// More channels than a block's registers hold: the cell's channels are read twice, the second time from L2 (a
-// block's tile of 32 cells is 128 bytes a channel).
-template <class T>
-__global__ void __launch_bounds__(32 * LN_WIDE_WARPS)
-    ln_fwd_wide_kernel(const T* x, RunStrides xs, T* y, RunStrides ys, const float* scale, const float* bias,
-                       float eps, float* mean_out, float* inv_std_out, LnGeom geo)
-{
-    __shared__ float part[2][LN_WIDE_WARPS][2][32];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int chunks = (geo.c + LN_CHUNK - 1) / LN_CHUNK;
-    wait_for_previous_kernel(x, scale, bias);
-    dependents_may_start();
-    int turn = 0;
-    for (long long tile = blockIdx.x; tile < geo.tiles; tile += gridDim.x, turn ^= 1)
-    {
-        const long long unit = tile * 32 + lane;
-        const bool live = unit < geo.units.total;
-        const CellAt at = ln_cell(geo, live ? unit : 0, 1);
-        const T* px = x + offset_of(at, xs);
-        float mean = 0.f, m2 = 0.f;
-        int have = 0;
-        for (int q = warp; q < chunks; q += LN_WIDE_WARPS)
-        {
-            const int c0 = q * LN_CHUNK, count = min(LN_CHUNK, geo.c - c0);
-            float v[LN_CHUNK][1], s = 0.f, t = 0.f;
-#pragma unroll
-            for (int k = 0; k < LN_CHUNK; ++k)
-                if (k < count)
-                    load_elems<1>(px + (c0 + k) * xs.sc, v[k]);
-#pragma unroll
-            for (int k = 0; k < LN_CHUNK; ++k)
-                if (k < count)
-                    s += v[k][0];
-            s /= count;
-#pragma unroll
-            for (int k = 0; k < LN_CHUNK; ++k)
-                if (k < count)
-                    t = fmaf(v[k][0] - s, v[k][0] - s, t);
-            const float d = s - mean;
-            m2 += t + d * d * ((float) have * count / (have + count));
-            mean += d * count / (have + count);
-            have += count;
-        }
-        part[turn][warp][0][lane] = mean;
-        part[turn][warp][1][lane] = m2;
-        __syncthreads();
-        mean = m2 = 0.f;
-        have = 0;
-        for (int i = 0; i < LN_WIDE_WARPS; ++i)
-        {
-            int count = 0; // channels of warp i
-            for (int q = i; q < chunks; q += LN_WIDE_WARPS)
-                count += min(LN_CHUNK, geo.c - q * LN_CHUNK);
-            if (count == 0)
-                break;
-            const float d = part[turn][i][0][lane] - mean;
-            m2 += part[turn][i][1][lane] + d * d * ((float) have * count / (have + count));
-            mean += d * count / (have + count);
-            have += count;
-        }
-        if (!live)
-            continue;
-        const float inv = 1.f / sqrtf(m2 / geo.c + eps);
-        if (warp == 0)
-        {
-            const long long i = at.n * geo.units.cells + at.cell;
-            if (mean_out)
-                mean_out[i] = mean;
-            if (inv_std_out)
-                inv_std_out[i] = inv;
-        }
-        T* py = y + offset_of(at, ys);
-        for (int q = warp; q < chunks; q += LN_WIDE_WARPS)
-        {
-            const int c0 = q * LN_CHUNK, count = min(LN_CHUNK, geo.c - c0);
-            float v[LN_CHUNK][1];
-#pragma unroll
-            for (int k = 0; k < LN_CHUNK; ++k)
-                if (k < count)
-                    load_elems<1>(px + (c0 + k) * xs.sc, v[k]);
-#pragma unroll
-            for (int k = 0; k < LN_CHUNK; ++k)
-                if (k < count)
-                {
-                    const int c = c0 + k;
-                    float out[1] = {fmaf((v[k][0] - mean) * inv, scale ? scale[c] : 1.f, bias ? bias[c] : 0.f)};
-                    store_elems<1>(py + c * ys.sc, out);
-                }
-        }
-    }
-}
-
-template <class T>
-__global__ void __launch_bounds__(32 * LN_WIDE_WARPS)
-    ln_bwd_wide_kernel(const T* x, RunStrides xs, const T* dy, RunStrides dys, const float* mean_in,
-                       const float* inv_std_in, const float* scale, T* dx, RunStrides dxs, float* partial, LnGeom geo)
-{
-    extern __shared__ float acc[]; // [2][c]: a channel belongs to one warp
-    __shared__ float part[2][LN_WIDE_WARPS][2][32];
-    constexpr int HALF = LN_CHUNK / 2; // channels at a time: x and dy are both held
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int chunks = (geo.c + HALF - 1) / HALF;
-    for (int i = threadIdx.x; i < 2 * geo.c; i += blockDim.x)
-        acc[i] = 0.f;
-    wait_for_previous_kernel(x, dy, mean_in, inv_std_in, scale);
-    dependents_may_start();
-    __syncthreads();
-    int turn = 0;
-    for (long long tile = blockIdx.x; tile < geo.tiles; tile += gridDim.x, turn ^= 1)
-    {
-        const long long unit = tile * 32 + lane;
-        const bool live = unit < geo.units.total;
-        const CellAt at = ln_cell(geo, live ? unit : 0, 1);
-        const T* px = x + offset_of(at, xs);
-        const T* pd = dy + offset_of(at, dys);
-        const float mean = mean_in[at.n * geo.units.cells + at.cell];
-        const float inv = inv_std_in[at.n * geo.units.cells + at.cell];
-        float a = 0.f, b = 0.f;
-        for (int q = warp; q < chunks; q += LN_WIDE_WARPS)
-        {
-            const int c0 = q * HALF, count = min(HALF, geo.c - c0);
-            float u[HALF][1], d[HALF][1], wu[HALF], wb[HALF];
-#pragma unroll
-            for (int k = 0; k < HALF; ++k)
-                if (k < count)
-                {
-                    load_elems<1>(px + (c0 + k) * xs.sc, u[k]);
-                    load_elems<1>(pd + (c0 + k) * dys.sc, d[k]);
-                }
-#pragma unroll
-            for (int k = 0; k < HALF; ++k)
-            {
-                const bool use = live && k < count;
-                const float uu = use ? (u[k][0] - mean) * inv : 0.f;
-                const float dd = use ? d[k][0] : 0.f;
-                const float g = dd * (scale && k < count ? scale[c0 + k] : 1.f);
-                a += g;
-                b = fmaf(g, uu, b);
-                wu[k] = dd * uu;
-                wb[k] = dd;
-            }
-            if (partial)
-            {
-                const float sw = ln_lane_sums<HALF>(wu, lane), sb = ln_lane_sums<HALF>(wb, lane);
-                if (lane < count)
-                {
-                    acc[c0 + lane] += sw;
-                    acc[geo.c + c0 + lane] += sb;
-                }
-            }
-        }
-        part[turn][warp][0][lane] = a;
-        part[turn][warp][1][lane] = b;
-        __syncthreads();
-        a = b = 0.f;
-#pragma unroll
-        for (int i = 0; i < LN_WIDE_WARPS; ++i)
-            a += part[turn][i][0][lane], b += part[turn][i][1][lane];
-        if (!live)
-            continue;
-        a /= geo.c;
-        b /= geo.c;
-        T* po = dx + offset_of(at, dxs);
-        for (int q = warp; q < chunks; q += LN_WIDE_WARPS)
-        {
-            const int c0 = q * HALF, count = min(HALF, geo.c - c0);
-            float u[HALF][1], d[HALF][1];
-#pragma unroll
-            for (int k = 0; k < HALF; ++k)
-                if (k < count)
-                {
-                    load_elems<1>(px + (c0 + k) * xs.sc, u[k]);
-                    load_elems<1>(pd + (c0 + k) * dys.sc, d[k]);
-                }
-#pragma unroll
-            for (int k = 0; k < HALF; ++k)
-                if (k < count)
-                {
-                    const float uu = (u[k][0] - mean) * inv;
-                    float out[1] = {inv * (fmaf(d[k][0], scale ? scale[c0 + k] : 1.f, -a) - uu * b)};
-                    store_elems<1>(po + (c0 + k) * dxs.sc, out);
-                }
-        }
-    }
-    if (!partial)
-        return;
-    __syncthreads();
-    for (int i = threadIdx.x; i < 2 * geo.c; i += blockDim.x)
-        partial[(long long) i * gridDim.x + blockIdx.x] = acc[i];
 }
 
 // A warp a channel and gradient: the blocks' sums in order, in fp64.
@@ -526,43 +518,29 @@ __global__ void __launch_bounds__(256) ln_zero_kernel(float* dscale, float* dbia
         dscale[i] = dbias[i] = 0.f;
 }
 
-// What a launch is made of: cells of an access, channels of a thread, warps of a group, groups of a block.
+// What a launch is made of: cells of a thread, warps of a group, how the cells lie.
 struct LnChoice
 {
-    int v, k, g, groups;
-    bool wide;
+    int v, g, mode;
 };
 
-LnChoice ln_choose(int c, int vmax, long long cells_of_all)
+// vmax: neighbours that one access may fetch.  len: cells of a run.
+LnChoice ln_choose(int c, int vmax, long long len, long long cells)
 {
-    LnChoice h = {1, 32, 1, 1, c > LN_NARROW};
-    if (h.wide)
-        return h;
-    // V K = 32 values a thread.  Wide accesses first; fewer cells a thread where the tiles would not give every
-    // SM two blocks, or where so many channels need more warps than a group has.
-    for (int v = vmax; v >= 1; v /= 2)
-    {
-        h.v = v;
-        h.k = v == 4 ? 8 : v == 2 ? 16 : 32;
-        while (h.k > 4 && h.k / 2 >= c)
-            h.k /= 2;
-        h.g = (c + h.k - 1) / h.k;
-        if (v == 1 || (h.g <= LN_MAX_GROUP && cells_of_all >= 2ll * num_sms() * 32 * v))
-            break;
-    }
-    while (h.k > 4 && (c + h.k / 2 - 1) / (h.k / 2) <= 8) // small K, more warps: up to 8 to a group
-    {
-        h.k /= 2;
-        h.g = (c + h.k - 1) / h.k;
-    }
-    h.groups = h.g >= 8 ? 1 : 8 / h.g;
+    LnChoice h;
+    // Four cells a thread where that leaves every SM a block of tiles; else one.  A run's last tile wastes up to a
+    // quarter of the lanes; shorter runs are packed.
+    const bool four = cells >= 4ll * 32 * num_sms();
+    h.mode = four && len >= 512 ? (vmax == 4 ? LN_ROWS : LN_SPLIT) : LN_FLAT;
+    h.v = h.mode != LN_FLAT || (four && vmax == 4) ? 4 : 1;
+    // as many warps a group as have eight channels each, more where there are few tiles
+    const long long tiles = (cells + 32 * h.v - 1) / (32 * h.v);
+    h.g = 1;
+    while (h.g < LN_WARPS && (c > LN_STEP * h.g || (c >= 2 * h.g && tiles * h.g < 8ll * num_sms())))
+        h.g *= 2;
     return h;
 }
 
-long long ln_blocks_max()
-{
-    return 8ll * num_sms();
-}
 
 int32_t ln_check(const dcb_nd_desc* xd, int32_t dtype)
 {
@@ -601,68 +579,57 @@ int32_t ln_with_types(int32_t dtype, F f)
 LnGeom ln_geometry(const RunGeom& rg, const LnChoice& h)
 {
     LnGeom g;
-    g.units = cell_units(rg, h.v);
-    g.per_run = rg.len / h.v;
+    g.per_run = h.mode == LN_FLAT ? rg.len / h.v : (rg.len + 32 * h.v - 1) / (32 * h.v);
+    g.units = cell_units_of(rg, g.per_run);
     g.rows = rg.rows;
     g.rows_inner = rg.rows_inner;
     g.c = (int) rg.c;
     g.g = h.g;
-    g.tiles = (g.units.total + 32ll * h.groups - 1) / (32ll * h.groups);
+    g.inv_c = 1.f / g.c;
+    const long long a_tile = LN_WARPS / h.g * (h.mode == LN_FLAT ? 32 : 1); // units
+    g.tiles = (g.units.total + a_tile - 1) / a_tile;
     return g;
 }
 
-template <class T, int V, int K>
-int32_t ln_launch_fwd(const LnChoice& h, const LnGeom& g, const void* x, const RunStrides& xs, void* y,
-                      const RunStrides& ys, const void* scale, const void* bias, float eps, void* mean, void* inv_std,
-                      cudaStream_t stream)
+template <class T, int V, int MODE>
+int32_t ln_launch_fwd(const LnGeom& g, const void* x, const RunStrides& xs, void* y, const RunStrides& ys,
+                      const void* scale, const void* bias, float eps, void* mean, void* inv_std, cudaStream_t stream)
 {
-    DCB_REQUIRE(g.tiles < (1ll << 31), "too many cells");
-    const size_t smem = h.g > 1 ? sizeof(float) * h.groups * h.g * 2 * 32 * V : 0;
-    DCB_CUDA_TRY(launch_overlapped(ln_fwd_kernel<T, V, K>, dim3((unsigned) g.tiles), 32 * h.g * h.groups, smem, stream,
+    const unsigned blocks = (unsigned) std::min<long long>(g.tiles, 4ll * num_sms());
+    DCB_CUDA_TRY(launch_overlapped(ln_fwd_kernel<T, V, MODE>, dim3(blocks), 32 * LN_WARPS, 0, stream,
                                    static_cast<const T*>(x), xs, static_cast<T*>(y), ys,
                                    static_cast<const float*>(scale), static_cast<const float*>(bias), eps,
                                    static_cast<float*>(mean), static_cast<float*>(inv_std), g));
     return DCB_OK;
 }
 
-template <class T, int V, int K>
-int32_t ln_launch_bwd(const LnChoice& h, const LnGeom& g, unsigned blocks, const void* x, const RunStrides& xs,
-                      const void* dy, const RunStrides& dys, const void* mean, const void* inv_std, const void* scale,
-                      void* dx, const RunStrides& dxs, float* partial, cudaStream_t stream)
+template <class T, int V, int MODE>
+int32_t ln_launch_bwd(const LnGeom& g, unsigned blocks, const void* x, const RunStrides& xs, const void* dy,
+                      const RunStrides& dys, const void* mean, const void* inv_std, const void* scale, void* dx,
+                      const RunStrides& dxs, float* partial, cudaStream_t stream)
 {
-    const int warps = h.g * h.groups;
-    const size_t smem = sizeof(float)
-                        * std::max(h.g > 1 ? 2 * warps * 2 * 32 * V : 0, partial ? 2 * warps * K : 0);
-    if (smem > 48 * 1024)
-        if (int32_t e = allow_dynamic_smem((const void*) ln_bwd_kernel<T, V, K>, 160 * 1024))
+    const int smem = partial ? 8 * g.c * (LN_WARPS / g.g) : 0;
+    if (smem > 32 * 1024)
+        if (int32_t e = allow_dynamic_smem((const void*) ln_bwd_kernel<T, V, MODE>, 8 * LN_MAX_CHANNELS))
             return e;
-    DCB_CUDA_TRY(launch_overlapped(ln_bwd_kernel<T, V, K>, dim3(blocks), 32 * warps, smem, stream,
+    DCB_CUDA_TRY(launch_overlapped(ln_bwd_kernel<T, V, MODE>, dim3(blocks), 32 * LN_WARPS, smem, stream,
                                    static_cast<const T*>(x), xs, static_cast<const T*>(dy), dys,
                                    static_cast<const float*>(mean), static_cast<const float*>(inv_std),
                                    static_cast<const float*>(scale), static_cast<T*>(dx), dxs, partial, g));
     return DCB_OK;
 }
 
-// f<V, K>() for the choice.
+// f(V, MODE) for the choice.
 template <class F>
 int32_t ln_with_shape(const LnChoice& h, F f)
 {
     using std::integral_constant;
-#define DCB_LN_CASE(VV, KK)                                                                                            \
-    if (h.v == VV && h.k == KK)                                                                                        \
-        return f(integral_constant<int, VV>(), integral_constant<int, KK>());
-    DCB_LN_CASE(4, 4)
-    DCB_LN_CASE(4, 8)
-    DCB_LN_CASE(2, 4)
-    DCB_LN_CASE(2, 8)
-    DCB_LN_CASE(2, 16)
-    DCB_LN_CASE(1, 4)
-    DCB_LN_CASE(1, 8)
-    DCB_LN_CASE(1, 16)
-    DCB_LN_CASE(1, 32)
-#undef DCB_LN_CASE
-    set_last_error("layer norm: no kernel for this shape");
-    return DCB_UNSUPPORTED;
+    if (h.mode == LN_ROWS)
+        return f(integral_constant<int, 4>(), integral_constant<int, LN_ROWS>());
+    if (h.mode == LN_SPLIT)
+        return f(integral_constant<int, 4>(), integral_constant<int, LN_SPLIT>());
+    return h.v == 4 ? f(integral_constant<int, 4>(), integral_constant<int, LN_FLAT>())
+                    : f(integral_constant<int, 1>(), integral_constant<int, LN_FLAT>());
 }
 
 } // namespace
@@ -696,22 +663,13 @@ int32_t dcb_ln_fwd(const dcb_nd_desc* xd, int32_t dtype, const void* x, const vo
     const int es = elem_bytes(dtype);
     const int vmax = std::min(std::min(run_vec_of(rg, xs, x, es), run_vec_of(rg, ys, y, es)),
                               std::min(run_vec_of(rg, none, mean, 4), run_vec_of(rg, none, inv_std, 4)));
-    const LnChoice h = ln_choose((int) rg.c, vmax, rg.n * rg.rows * rg.len);
+    const LnChoice h = ln_choose((int) rg.c, vmax, rg.len, rg.n * rg.rows * rg.len);
     const LnGeom g = ln_geometry(rg, h);
     return ln_with_types(dtype, [&](auto t) -> int32_t {
         using T = decltype(t);
-        if (h.wide)
-        {
-            const unsigned blocks = (unsigned) std::min<long long>(g.tiles, 4ll * num_sms());
-            DCB_CUDA_TRY(launch_overlapped(ln_fwd_wide_kernel<T>, dim3(blocks), 32 * LN_WIDE_WARPS, 0,
-                                           as_stream(stream), static_cast<const T*>(x), xs, static_cast<T*>(y), ys,
-                                           static_cast<const float*>(scale), static_cast<const float*>(bias), eps,
-                                           static_cast<float*>(mean), static_cast<float*>(inv_std), g));
-            return DCB_OK;
-        }
-        return ln_with_shape(h, [&](auto v, auto k) {
-            return ln_launch_fwd<T, decltype(v)::value, decltype(k)::value>(h, g, x, xs, y, ys, scale, bias, eps, mean,
-                                                                            inv_std, as_stream(stream));
+        return ln_with_shape(h, [&](auto v, auto mode) {
+            return ln_launch_fwd<T, decltype(v)::value, decltype(mode)::value>(g, x, xs, y, ys, scale, bias, eps, mean,
+                                                                               inv_std, as_stream(stream));
         });
     });
 }
@@ -720,7 +678,7 @@ int64_t dcb_ln_bwd_workspace_bytes(const dcb_nd_desc* xd, int32_t dtype)
 {
     if (ln_check(xd, dtype))
         return -1;
-    return 4 * 2 * xd->c * ln_blocks_max();
+    return 4 * 2 * xd->c * ln_bwd_blocks(1) * (int64_t) num_sms();
 }
 
 int32_t dcb_ln_bwd(const dcb_nd_desc* xd, int32_t dtype, const void* x, const dcb_nd_desc* dyd, const void* dy,
@@ -766,30 +724,15 @@ int32_t dcb_ln_bwd(const dcb_nd_desc* xd, int32_t dtype, const void* x, const dc
     const int es = elem_bytes(dtype);
     int vmax = std::min(run_vec_of(rg, xs, x, es), std::min(run_vec_of(rg, dys, dy, es), run_vec_of(rg, dxs, dx, es)));
     vmax = std::min(vmax, std::min(run_vec_of(rg, none, mean, 4), run_vec_of(rg, none, inv_std, 4)));
-    const LnChoice h = ln_choose(c, vmax, rg.n * rg.rows * rg.len);
+    const LnChoice h = ln_choose(c, vmax, rg.len, rg.n * rg.rows * rg.len);
     const LnGeom g = ln_geometry(rg, h);
     float* partial = dscale ? static_cast<float*>(workspace) : nullptr;
-    unsigned blocks = 0;
+    const unsigned blocks = (unsigned) std::min<long long>(g.tiles, (long long) ln_bwd_blocks(h.v) * num_sms());
     const int32_t e = ln_with_types(dtype, [&](auto t) -> int32_t {
         using T = decltype(t);
-        if (h.wide)
-        {
-            blocks = (unsigned) std::min<long long>(g.tiles, num_sms());
-            const int smem = 8 * c;
-            if (int32_t err = allow_dynamic_smem((const void*) ln_bwd_wide_kernel<T>, 8 * LN_MAX_CHANNELS))
-                return err;
-            DCB_CUDA_TRY(launch_overlapped(ln_bwd_wide_kernel<T>, dim3(blocks), 32 * LN_WIDE_WARPS, smem, s,
-                                           static_cast<const T*>(x), xs, static_cast<const T*>(dy), dys,
-                                           static_cast<const float*>(mean), static_cast<const float*>(inv_std),
-                                           static_cast<const float*>(scale), static_cast<T*>(dx), dxs, partial, g));
-            return DCB_OK;
-        }
-        // about 16 warps an SM: what 128 registers a thread leave room for
-        blocks = (unsigned) std::min<long long>(
-            g.tiles, std::min<long long>(ln_blocks_max(), (long long) num_sms() * std::max(1, 16 / (h.g * h.groups))));
-        return ln_with_shape(h, [&](auto v, auto k) {
-            return ln_launch_bwd<T, decltype(v)::value, decltype(k)::value>(h, g, blocks, x, xs, dy, dys, mean,
-                                                                            inv_std, scale, dx, dxs, partial, s);
+        return ln_with_shape(h, [&](auto v, auto mode) {
+            return ln_launch_bwd<T, decltype(v)::value, decltype(mode)::value>(g, blocks, x, xs, dy, dys, mean,
+                                                                               inv_std, scale, dx, dxs, partial, s);
         });
     });
     if (e != DCB_OK || !dscale)
