@@ -40,28 +40,46 @@ struct AtRing
     }
 };
 
+// The warp that issues products runs converged, and only the instructions themselves are one lane's: their operands are
+// then uniform registers, as they want them.  (With one lane running the whole loop an instruction took 140 clocks to
+// issue: 12 of them 1700.)
+__device__ __forceinline__ uint32_t at_elect()
+{
+    uint32_t e;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.b32 %0, 1, 0, p;\n\t}" : "=r"(e));
+    return e;
+}
+
+__device__ __forceinline__ void at_commit(uint64_t* bar, uint32_t elected)
+{
+    if (elected)
+        mma_commit(bar);
+}
+
 // Both operands in shared memory.
-__device__ __forceinline__ void at_mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate)
+__device__ __forceinline__ void at_mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate,
+                                          uint32_t elected)
 {
     asm volatile("{\n\t"
-                 ".reg .pred p;\n\t"
+                 ".reg .pred p, e;\n\t"
                  "setp.ne.b32 p, %4, 0;\n\t"
-                 "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t"
+                 "setp.ne.b32 e, %5, 0;\n\t"
+                 "@e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t"
                  "}" ::"r"(d),
-                 "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
-                 : "memory");
+                 "l"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(elected));
 }
 
 // A in tensor memory.
-__device__ __forceinline__ void at_mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate)
+__device__ __forceinline__ void at_mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate,
+                                          uint32_t elected)
 {
     asm volatile("{\n\t"
-                 ".reg .pred p;\n\t"
+                 ".reg .pred p, e;\n\t"
                  "setp.ne.b32 p, %4, 0;\n\t"
-                 "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t"
+                 "setp.ne.b32 e, %5, 0;\n\t"
+                 "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t"
                  "}" ::"r"(d),
-                 "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
-                 : "memory");
+                 "r"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(elected));
 }
 
 // bf16 x bf16 -> fp32, M = 128.  across: cells are that operand's rows, channels the reduction.
@@ -88,26 +106,30 @@ struct AtTile
     }
 };
 
-// d = A B' over the channels: both tiles across.
+// d = A B' over the channels, 16 a step: both tiles across.
 template <int D>
-__device__ __forceinline__ void at_scores(uint32_t d, uint32_t a, uint32_t b, int ksteps)
+__device__ __forceinline__ void at_scores(uint32_t d, uint32_t a, uint32_t b, int ksteps, uint32_t elected)
 {
     const uint64_t da = AtTile<D>::across(a), db = AtTile<D>::across(b);
     const uint32_t idesc = at_idesc(AT_TILE, true, true);
-    for (int k = 0; k < ksteps; ++k)
-        at_mma_ss(d, da + AtTile<D>::across_step(k), db + AtTile<D>::across_step(k), idesc, k > 0);
+#pragma unroll
+    for (int k = 0; k < D / 16; ++k)
+        if (k < ksteps)
+            at_mma_ss(d, da + AtTile<D>::across_step(k), db + AtTile<D>::across_step(k), idesc, k > 0, elected);
 }
 
 // d += W B over 128 cells: W in tensor memory, 64 cells to 32 columns, the second half of them `gap` columns behind the
 // first's start.
 template <int D>
-__device__ __forceinline__ void at_weigh(uint32_t d, uint32_t w, uint32_t gap, uint32_t b, uint32_t n, bool first)
+__device__ __forceinline__ void at_weigh(uint32_t d, uint32_t w, uint32_t gap, uint32_t b, uint32_t n, bool first,
+                                         uint32_t elected)
 {
     const uint64_t db = AtTile<D>::along(b);
     const uint32_t idesc = at_idesc(n, false, false);
 #pragma unroll
     for (int k = 0; k < 8; ++k)
-        at_mma_ts(d, w + (k >> 2) * gap + (k & 3) * 8, db + AtTile<D>::along_step(k), idesc, !(first && k == 0));
+        at_mma_ts(d, w + (k >> 2) * gap + (k & 3) * 8, db + AtTile<D>::along_step(k), idesc, !(first && k == 0),
+                  elected);
 }
 
 __device__ __forceinline__ void at_tma_half(uint32_t dst, const CUtensorMap* map, int cell, int head, int n,
@@ -174,6 +196,13 @@ __device__ __forceinline__ void at_tmem_st32(uint32_t taddr, const uint32_t* r)
 __device__ __forceinline__ void at_tmem_wait_st()
 {
     asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+}
+
+__device__ __forceinline__ float at_max3(float a, float b, float c)
+{
+    float y;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
+    return y;
 }
 
 __device__ __forceinline__ float at_exp2(float x)

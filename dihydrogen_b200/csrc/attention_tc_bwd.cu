@@ -62,11 +62,11 @@ __device__ __forceinline__ void ab_init(AbBars& b, int warp)
     tc_fence_after();
 }
 
-// One thread of the block that gave up: the products that were issued end before the tensor memory goes back.
-__device__ __forceinline__ void ab_drain_products(AbBars& b)
+// The block gave up: the products that were issued end before the tensor memory goes back.
+__device__ __forceinline__ void ab_drain_products(AbBars& b, uint32_t elected)
 {
     int none = 0;
-    mma_commit(&b.fin);
+    at_commit(&b.fin, elected);
     mbar_wait_t<20>(&b.fin, 0, &none);
 }
 
@@ -79,7 +79,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
     extern __shared__ __align__(1024) uint8_t smem[];
     const uint32_t base = smem_u32(smem);
     AbBars& b = *reinterpret_cast<AbBars*>(smem + S::BARS_AT);
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = __shfl_sync(~0u, (int) threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     volatile int* give_up = &b.give_up;
     if (at_misplaced(base, ex.status))
         return;
@@ -101,7 +101,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
     const int lo = (int) (all * split / p.q_splits), steps = (int) (all * (split + 1) / p.q_splits) - lo;
 
     ab_init(b, warp);
-    const uint32_t tmem = b.tmem;
+    const uint32_t tmem = __shfl_sync(~0u, b.tmem, 0); // known to be uniform
     const float* stats = p.stats;
     wait_for_previous_kernel(stats);
     bool ok = true;
@@ -154,59 +154,60 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
         }
         else if (warp == AT_MMA_WARP)
         {
-            if (lane == 0 && steps > 0)
+            if (steps > 0)
             {
+                const uint32_t elected = at_elect();
                 const int ksteps = (p.d + 15) / 16;
                 const uint32_t width = (uint32_t) ksteps * 16;
                 const uint32_t k_at = base + S::OWN_AT, v_at = k_at + AtTile<D>::BYTES;
                 AtRing ra, rb; // of the next tiles to wait for
                 uint32_t q_slot = 0, o_slot = 0;
                 const auto scores = [&] {
-                    ok = ok && mbar_wait_t<0>(&b.a_full[ra.slot], ra.lap & 1, give_up);
+                    ok = ok && at_warp_wait(&b.a_full[ra.slot], ra.lap & 1, give_up);
                     if (!ok)
                         return;
                     tc_fence_after();
-                    at_scores<D>(s_at, k_at, base + S::A_AT + ra.slot * AtTile<D>::BYTES, ksteps);
-                    mma_commit(&b.s_full[0]);
+                    at_scores<D>(s_at, k_at, base + S::A_AT + ra.slot * AtTile<D>::BYTES, ksteps, elected);
+                    at_commit(&b.s_full[0], elected);
                     ra.next(S::A_SLOTS);
                 };
                 const auto weight_grads = [&] {
-                    ok = ok && mbar_wait_t<0>(&b.b_full[rb.slot], rb.lap & 1, give_up);
+                    ok = ok && at_warp_wait(&b.b_full[rb.slot], rb.lap & 1, give_up);
                     if (!ok)
                         return;
                     tc_fence_after();
-                    at_scores<D>(dp_at, v_at, base + S::B_AT + rb.slot * AtTile<D>::BYTES, ksteps);
-                    mma_commit(&b.dp_full);
+                    at_scores<D>(dp_at, v_at, base + S::B_AT + rb.slot * AtTile<D>::BYTES, ksteps, elected);
+                    at_commit(&b.dp_full, elected);
                     rb.next(S::B_SLOTS);
                 };
-                ok = mbar_wait_t<0>(&b.own_full, 0, give_up);
+                ok = at_warp_wait(&b.own_full, 0, give_up);
                 scores();
                 weight_grads();
                 for (int u = 0; u < steps && ok; ++u)
                 {
-                    ok = mbar_wait_t<0>(&b.p_ready, u & 1, give_up);
+                    ok = at_warp_wait(&b.p_ready, u & 1, give_up);
                     if (!ok)
                         break;
                     tc_fence_after();
-                    at_weigh<D>(dv_at, s_at, 64, base + S::B_AT + o_slot * AtTile<D>::BYTES, width, u == 0);
+                    at_weigh<D>(dv_at, s_at, 64, base + S::B_AT + o_slot * AtTile<D>::BYTES, width, u == 0, elected);
                     if (u + 1 < steps)
                         scores();
-                    ok = ok && mbar_wait_t<0>(&b.ds_ready, u & 1, give_up);
+                    ok = ok && at_warp_wait(&b.ds_ready, u & 1, give_up);
                     if (!ok)
                         break;
                     tc_fence_after();
-                    at_weigh<D>(dk_at, dp_at, 64, base + S::A_AT + q_slot * AtTile<D>::BYTES, width, u == 0);
-                    mma_commit(&b.a_empty[q_slot]);
-                    mma_commit(&b.b_empty[o_slot]);
+                    at_weigh<D>(dk_at, dp_at, 64, base + S::A_AT + q_slot * AtTile<D>::BYTES, width, u == 0, elected);
+                    at_commit(&b.a_empty[q_slot], elected);
+                    at_commit(&b.b_empty[o_slot], elected);
                     q_slot = q_slot + 1 == S::A_SLOTS ? 0 : q_slot + 1;
                     o_slot = o_slot + 1 == S::B_SLOTS ? 0 : o_slot + 1;
                     if (u + 1 < steps)
                         weight_grads();
                 }
                 if (ok)
-                    mma_commit(&b.fin);
+                    at_commit(&b.fin, elected);
                 else
-                    ab_drain_products(b);
+                    ab_drain_products(b, elected);
             }
         }
     }
@@ -318,7 +319,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
     extern __shared__ __align__(1024) uint8_t smem[];
     const uint32_t base = smem_u32(smem);
     AbBars& b = *reinterpret_cast<AbBars*>(smem + S::BARS_AT);
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = __shfl_sync(~0u, (int) threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     volatile int* give_up = &b.give_up;
     if (at_misplaced(base, ex.status))
         return;
@@ -338,7 +339,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
     const int steps = max(0, hi - lo);
 
     ab_init(b, warp);
-    const uint32_t tmem = b.tmem;
+    const uint32_t tmem = __shfl_sync(~0u, b.tmem, 0); // known to be uniform
     const uint32_t* bits = ex.kv_bits ? ex.kv_bits + n * ex.words : nullptr;
     const float* stats = p.stats;
     wait_for_previous_kernel(bits, stats);
@@ -382,8 +383,9 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
         }
         else if (warp == AT_MMA_WARP)
         {
-            if (lane == 0 && steps > 0)
+            if (steps > 0)
             {
+                const uint32_t elected = at_elect();
                 const int ksteps = (p.d + 15) / 16;
                 const uint32_t width = (uint32_t) ksteps * 16;
                 const uint32_t q_at = base + S::OWN_AT, do_at = q_at + AtTile<D>::BYTES;
@@ -391,38 +393,38 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
                 uint32_t k_slot = 0;
                 int ahead = 0; // scores taken so far
                 const auto scores = [&] {
-                    ok = ok && mbar_wait_t<0>(&b.a_full[ra.slot], ra.lap & 1, give_up);
+                    ok = ok && at_warp_wait(&b.a_full[ra.slot], ra.lap & 1, give_up);
                     if (!ok)
                         return;
                     tc_fence_after();
-                    at_scores<D>(s_at + 128 * (ahead & 1), q_at, base + S::A_AT + ra.slot * AtTile<D>::BYTES, ksteps);
-                    mma_commit(&b.s_full[ahead & 1]);
+                    at_scores<D>(s_at + 128 * (ahead & 1), q_at, base + S::A_AT + ra.slot * AtTile<D>::BYTES, ksteps, elected);
+                    at_commit(&b.s_full[ahead & 1], elected);
                     ++ahead;
                     ra.next(S::A_SLOTS);
                 };
                 const auto weight_grads = [&] {
-                    ok = ok && mbar_wait_t<0>(&b.b_full[rb.slot], rb.lap & 1, give_up);
+                    ok = ok && at_warp_wait(&b.b_full[rb.slot], rb.lap & 1, give_up);
                     if (!ok)
                         return;
                     tc_fence_after();
-                    at_scores<D>(dp_at, do_at, base + S::B_AT + rb.slot * AtTile<D>::BYTES, ksteps);
-                    mma_commit(&b.dp_full);
-                    mma_commit(&b.b_empty[rb.slot]);
+                    at_scores<D>(dp_at, do_at, base + S::B_AT + rb.slot * AtTile<D>::BYTES, ksteps, elected);
+                    at_commit(&b.dp_full, elected);
+                    at_commit(&b.b_empty[rb.slot], elected);
                     rb.next(S::B_SLOTS);
                 };
-                ok = mbar_wait_t<0>(&b.own_full, 0, give_up);
+                ok = at_warp_wait(&b.own_full, 0, give_up);
                 scores();
                 weight_grads();
                 if (steps > 1)
                     scores();
                 for (int u = 0; u < steps && ok; ++u)
                 {
-                    ok = mbar_wait_t<0>(&b.ds_ready, u & 1, give_up);
+                    ok = at_warp_wait(&b.ds_ready, u & 1, give_up);
                     if (!ok)
                         break;
                     tc_fence_after();
-                    at_weigh<D>(dq_at, dp_at, 64, base + S::A_AT + k_slot * AtTile<D>::BYTES, width, u == 0);
-                    mma_commit(&b.a_empty[k_slot]);
+                    at_weigh<D>(dq_at, dp_at, 64, base + S::A_AT + k_slot * AtTile<D>::BYTES, width, u == 0, elected);
+                    at_commit(&b.a_empty[k_slot], elected);
                     k_slot = k_slot + 1 == S::A_SLOTS ? 0 : k_slot + 1;
                     if (u + 1 < steps)
                         weight_grads();
@@ -430,9 +432,9 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
                         scores();
                 }
                 if (ok)
-                    mma_commit(&b.fin);
+                    at_commit(&b.fin, elected);
                 else
-                    ab_drain_products(b);
+                    ab_drain_products(b, elected);
             }
         }
     }

@@ -43,7 +43,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
     extern __shared__ __align__(1024) uint8_t smem[];
     const uint32_t base = smem_u32(smem);
     AfBars& b = *reinterpret_cast<AfBars*>(smem + S::BARS_AT);
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = __shfl_sync(~0u, (int) threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     volatile int* give_up = &b.give_up;
     if (at_misplaced(base, ex.status))
         return;
@@ -85,7 +85,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem = b.tmem;
+    const uint32_t tmem = __shfl_sync(~0u, b.tmem, 0); // known to be uniform
     const uint32_t* bits = ex.kv_bits ? ex.kv_bits + n * ex.words : nullptr;
     wait_for_previous_kernel(bits);
     bool ok = true;
@@ -123,62 +123,64 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
         }
         else if (warp == AT_MMA_WARP)
         {
-            if (lane == 0 && most > 0)
+            if (most > 0)
             {
+                const uint32_t elected = at_elect();
                 const int ksteps = (p.d + 15) / 16;
                 const uint32_t width = (uint32_t) ksteps * 16;
                 const auto tile_of = [&](uint32_t slot) { return base + S::RING_AT + slot * AtTile<D>::BYTES; };
                 AtRing r; // the tile after the last one that was waited for
-                ok = mbar_wait_t<0>(&b.q_full, 0, give_up) && mbar_wait_t<0>(&b.full[r.slot], r.lap & 1, give_up);
+                ok = at_warp_wait(&b.q_full, 0, give_up) && at_warp_wait(&b.full[r.slot], r.lap & 1, give_up);
                 tc_fence_after();
                 uint32_t k_slot = r.slot;
                 r.next(S::SLOTS);
                 for (int t = 0; t < 2 && ok; ++t)
                     if (steps[t] > 0)
                     {
-                        at_scores<D>(tmem + t * AT_TILE, base + S::Q_AT + t * AtTile<D>::BYTES, tile_of(k_slot), ksteps);
-                        mma_commit(&b.s_full[t]);
+                        at_scores<D>(tmem + t * AT_TILE, base + S::Q_AT + t * AtTile<D>::BYTES, tile_of(k_slot), ksteps,
+                                     elected);
+                        at_commit(&b.s_full[t], elected);
                     }
                 if (ok)
-                    mma_commit(&b.empty[k_slot]);
+                    at_commit(&b.empty[k_slot], elected);
                 for (int j = 0; j < most && ok; ++j)
                 {
                     const uint32_t v_slot = r.slot;
-                    ok = mbar_wait_t<0>(&b.full[r.slot], r.lap & 1, give_up);
+                    ok = at_warp_wait(&b.full[r.slot], r.lap & 1, give_up);
                     r.next(S::SLOTS);
                     bool have_k = false;
                     for (int t = 0; t < 2 && ok; ++t)
                     {
                         if (j < steps[t])
                         {
-                            ok = mbar_wait_t<0>(&b.p_ready[t], j & 1, give_up);
+                            ok = at_warp_wait(&b.p_ready[t], j & 1, give_up);
                             if (!ok)
                                 break;
                             tc_fence_after();
-                            at_weigh<D>(tmem + 2 * AT_TILE + t * D, tmem + t * AT_TILE, 32, tile_of(v_slot), width, j == 0);
+                            at_weigh<D>(tmem + 2 * AT_TILE + t * D, tmem + t * AT_TILE, 32, tile_of(v_slot), width, j == 0,
+                                    elected);
                             if (j + 1 == steps[t])
-                                mma_commit(&b.o_full[t]);
+                                at_commit(&b.o_full[t], elected);
                         }
                         if (t == 1)
-                            mma_commit(&b.empty[v_slot]);
+                            at_commit(&b.empty[v_slot], elected);
                         if (j + 1 < steps[t])
                         {
                             if (!have_k)
                             {
-                                ok = mbar_wait_t<0>(&b.full[r.slot], r.lap & 1, give_up);
+                                ok = at_warp_wait(&b.full[r.slot], r.lap & 1, give_up);
                                 if (!ok)
                                     break;
                                 tc_fence_after();
                                 have_k = true;
                             }
-                            at_scores<D>(tmem + t * AT_TILE, base + S::Q_AT + t * AtTile<D>::BYTES, tile_of(r.slot),
-                                         ksteps);
-                            mma_commit(&b.s_full[t]);
+                            at_scores<D>(tmem + t * AT_TILE, base + S::Q_AT + t * AtTile<D>::BYTES, tile_of(r.slot), ksteps, elected);
+                            at_commit(&b.s_full[t], elected);
                         }
                     }
                     if (ok && j + 1 < most)
                     {
-                        mma_commit(&b.empty[r.slot]);
+                        at_commit(&b.empty[r.slot], elected);
                         r.next(S::SLOTS);
                     }
                 }
@@ -186,7 +188,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
                 {
                     // what was issued ends before the tensor memory is given back
                     int none = 0;
-                    mma_commit(&b.q_full);
+                    at_commit(&b.q_full, elected);
                     mbar_wait_t<20>(&b.q_full, 1, &none);
                 }
             }
@@ -228,11 +230,15 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
                 for (int c = 0; c < 128; ++c)
                     s[c] = see[c >> 5] >> (c & 31) & 1 ? s[c] : -INFINITY;
             }
-            float m0 = -INFINITY, m1 = -INFINITY, m2 = -INFINITY, m3 = -INFINITY;
+            float m0 = s[0], m1 = s[1], m2 = s[2], m3 = s[3];
 #pragma unroll
-            for (int c = 0; c < 128; c += 4)
-                m0 = fmaxf(m0, s[c]), m1 = fmaxf(m1, s[c + 1]), m2 = fmaxf(m2, s[c + 2]), m3 = fmaxf(m3, s[c + 3]);
-            const float mine = fmaxf(fmaxf(m0, m1), fmaxf(m2, m3)) * p.scale;
+            for (int c = 4; c < 124; c += 8)
+            {
+                m0 = at_max3(m0, s[c], s[c + 1]), m1 = at_max3(m1, s[c + 2], s[c + 3]);
+                m2 = at_max3(m2, s[c + 4], s[c + 5]), m3 = at_max3(m3, s[c + 6], s[c + 7]);
+            }
+            m0 = at_max3(m0, s[124], s[125]), m1 = at_max3(m1, s[126], s[127]);
+            const float mine = at_max3(fmaxf(m0, m1), m2, m3) * p.scale;
             const bool grown = mine > top + AF_GROWTH;
             if (__any_sync(~0u, grown))
             {
