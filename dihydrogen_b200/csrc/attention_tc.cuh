@@ -98,38 +98,31 @@ struct AtTile
     static __device__ __forceinline__ uint64_t across(uint32_t saddr) { return make_desc(saddr, HALF, 1024, 2); }
     // ... and along: channels in groups of 8 rows, 1024 bytes apart; 16 cells are 32 bytes of a row.
     static __device__ __forceinline__ uint64_t along(uint32_t saddr) { return make_desc(saddr, 16, 1024, 2); }
-    // In units of 16 bytes, what 16 steps of the reduction index add to the start address.
+    // In units of 16 bytes, what 16 channels add to the start address (16 cells, along: 2).
     static __device__ __forceinline__ uint32_t across_step(int k) { return (uint32_t) k * (2048 >> 4); }
-    static __device__ __forceinline__ uint32_t along_step(int k)
-    {
-        return ((uint32_t) (k >> 2) * HALF + (uint32_t) (k & 3) * 32) >> 4;
-    }
 };
 
-// d = A B' over the channels, 16 a step: both tiles across.
-template <int D>
+// d = A B' over the channels, 16 a step: both tiles across, 128 cells of A, N of B.
+template <int D, int N>
 __device__ __forceinline__ void at_scores(uint32_t d, uint32_t a, uint32_t b, int ksteps, uint32_t elected)
 {
     const uint64_t da = AtTile<D>::across(a), db = AtTile<D>::across(b);
-    const uint32_t idesc = at_idesc(AT_TILE, true, true);
+    const uint32_t idesc = at_idesc(N, true, true);
 #pragma unroll
     for (int k = 0; k < D / 16; ++k)
         if (k < ksteps)
             at_mma_ss(d, da + AtTile<D>::across_step(k), db + AtTile<D>::across_step(k), idesc, k > 0, elected);
 }
 
-// d += W B over 128 cells: W in tensor memory, 64 cells to 32 columns, the second half of them `gap` columns behind the
-// first's start.
+// d += W B over 64 cells: W in tensor memory, two to a column; B is half a tile.
 template <int D>
-__device__ __forceinline__ void at_weigh(uint32_t d, uint32_t w, uint32_t gap, uint32_t b, uint32_t n, bool first,
-                                         uint32_t elected)
+__device__ __forceinline__ void at_weigh(uint32_t d, uint32_t w, uint32_t b, uint32_t n, bool first, uint32_t elected)
 {
     const uint64_t db = AtTile<D>::along(b);
     const uint32_t idesc = at_idesc(n, false, false);
 #pragma unroll
-    for (int k = 0; k < 8; ++k)
-        at_mma_ts(d, w + (k >> 2) * gap + (k & 3) * 8, db + AtTile<D>::along_step(k), idesc, !(first && k == 0),
-                  elected);
+    for (int k = 0; k < 4; ++k)
+        at_mma_ts(d, w + k * 8, db + k * 2, idesc, !(first && k == 0), elected);
 }
 
 __device__ __forceinline__ void at_tma_half(uint32_t dst, const CUtensorMap* map, int cell, int head, int n,
@@ -193,6 +186,16 @@ __device__ __forceinline__ void at_tmem_st32(uint32_t taddr, const uint32_t* r)
         : "memory");
 }
 
+__device__ __forceinline__ void at_tmem_st16(uint32_t taddr, const uint32_t* r)
+{
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+        "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(taddr),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+        : "memory");
+}
+
 __device__ __forceinline__ void at_tmem_wait_st()
 {
     asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
@@ -203,6 +206,40 @@ __device__ __forceinline__ float at_max3(float a, float b, float c)
     float y;
     asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
     return y;
+}
+
+// Two floats to an instruction.
+__device__ __forceinline__ uint64_t at_pair(float lo, float hi)
+{
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+    return r;
+}
+
+__device__ __forceinline__ void at_unpair(uint64_t v, float& lo, float& hi)
+{
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
+}
+
+__device__ __forceinline__ uint64_t at_fma2(uint64_t a, uint64_t b, uint64_t c)
+{
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+
+__device__ __forceinline__ uint64_t at_add2(uint64_t a, uint64_t b)
+{
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+
+__device__ __forceinline__ uint64_t at_mul2(uint64_t a, uint64_t b)
+{
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
 }
 
 __device__ __forceinline__ float at_exp2(float x)
@@ -216,6 +253,39 @@ __device__ __forceinline__ float at_exp2(float x)
 __device__ __forceinline__ bool at_warp_wait(uint64_t* bar, uint32_t parity, volatile int* give_up)
 {
     return __all_sync(~0u, mbar_wait_t<0>(bar, parity, give_up));
+}
+
+// Which of two barriers (of those that `left` names) completes its phase first; -1: gave up.  Bounded like every wait.
+__device__ __forceinline__ int at_first_ready(uint64_t* b0, uint64_t* b1, uint32_t left, uint32_t parity,
+                                              volatile int* give_up)
+{
+    const auto done = [&](uint64_t* bar) {
+        uint32_t d;
+        asm volatile("{\n\t"
+                     ".reg .pred p;\n\t"
+                     "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+                     "selp.b32 %0, 1, 0, p;\n\t"
+                     "}"
+                     : "=r"(d)
+                     : "r"(smem_u32(bar)), "r"(parity)
+                     : "memory");
+        return d;
+    };
+    if (left != 3) // one of them only: the ordinary wait
+        return at_warp_wait(left == 1 ? b0 : b1, parity, give_up) ? (int) (left >> 1) : -1;
+    const long long begin = clock64();
+#pragma unroll 1
+    for (uint32_t it = 0; it < (1u << 24); ++it)
+    {
+        if (__all_sync(~0u, done(b0)))
+            return 0;
+        if (__all_sync(~0u, done(b1)))
+            return 1;
+        if ((it & 255) == 255 && __any_sync(~0u, *give_up || clock64() - begin > 500000000ll))
+            break;
+    }
+    *give_up = 1;
+    return -1;
 }
 
 // One arrival a warp, after all its lanes' work.
@@ -287,6 +357,7 @@ struct AtExtra
 };
 
 // The end of every kernel: who gave up says so, waits for what he started, and the tensor memory goes back.
+template <uint32_t COLUMNS = TC_TMEM_COLS>
 __device__ __forceinline__ void at_finish(bool ok, int* status, int warp, int lane, uint32_t tmem)
 {
     if (!ok && lane == 0)
@@ -296,7 +367,7 @@ __device__ __forceinline__ void at_finish(bool ok, int* status, int warp, int la
     tc_fence_after();
     __syncwarp();
     if (warp == AT_MMA_WARP)
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(TC_TMEM_COLS) : "memory");
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(COLUMNS) : "memory");
 }
 
 // The 128-byte swizzle goes by address bits: tiles start on multiples of 1024 bytes.
@@ -309,22 +380,25 @@ __device__ __forceinline__ bool at_misplaced(uint32_t base, int* status)
     return true;
 }
 
+template <uint32_t COLUMNS = TC_TMEM_COLS>
 __device__ __forceinline__ void at_tmem_alloc(uint32_t* slot)
 {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(slot)),
-                 "r"(TC_TMEM_COLS)
+                 "r"(COLUMNS)
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
 }
 
-__device__ __forceinline__ void at_team_registers()
+template <int N>
+__device__ __forceinline__ void at_more_registers()
 {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(AT_TEAM_REGS));
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
 }
 
-__device__ __forceinline__ void at_other_registers()
+template <int N>
+__device__ __forceinline__ void at_fewer_registers()
 {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(AT_OTHER_REGS));
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
 }
 
 // Waits, bounded, for copies into slots that nobody waited for because the block gave up.
@@ -340,6 +414,8 @@ __device__ __forceinline__ void at_drain(uint64_t* full, uint32_t slots, const A
     }
 }
 
+// Few queries against many keys: both teams of a block have the same queries.
+bool attn_tc_apart(const AttnProblem& p);
 int32_t attn_tc_fwd_launch(const AttnProblem& p, const AtMaps& maps, const AtExtra& ex, cudaStream_t stream);
 int32_t attn_tc_bwd_launch(const AttnProblem& p, const AtMaps& maps, const AtExtra& ex, cudaStream_t stream);
 

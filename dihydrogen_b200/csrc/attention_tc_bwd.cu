@@ -109,7 +109,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
 
     if (warp >= AT_MMA_WARP)
     {
-        at_other_registers();
+        at_fewer_registers<AT_OTHER_REGS>();
         if (warp == AT_TMA_WARP)
         {
             if (lane == 0 && steps > 0)
@@ -167,7 +167,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
                     if (!ok)
                         return;
                     tc_fence_after();
-                    at_scores<D>(s_at, k_at, base + S::A_AT + ra.slot * AtTile<D>::BYTES, ksteps, elected);
+                    at_scores<D, 128>(s_at, k_at, base + S::A_AT + ra.slot * AtTile<D>::BYTES, ksteps, elected);
                     at_commit(&b.s_full[0], elected);
                     ra.next(S::A_SLOTS);
                 };
@@ -176,7 +176,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
                     if (!ok)
                         return;
                     tc_fence_after();
-                    at_scores<D>(dp_at, v_at, base + S::B_AT + rb.slot * AtTile<D>::BYTES, ksteps, elected);
+                    at_scores<D, 128>(dp_at, v_at, base + S::B_AT + rb.slot * AtTile<D>::BYTES, ksteps, elected);
                     at_commit(&b.dp_full, elected);
                     rb.next(S::B_SLOTS);
                 };
@@ -189,14 +189,18 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
                     if (!ok)
                         break;
                     tc_fence_after();
-                    at_weigh<D>(dv_at, s_at, 64, base + S::B_AT + o_slot * AtTile<D>::BYTES, width, u == 0, elected);
+                    for (int h = 0; h < 2; ++h)
+                        at_weigh<D>(dv_at, s_at + 64 * h, base + S::B_AT + o_slot * AtTile<D>::BYTES + h * AtTile<D>::HALF, width,
+                                    u == 0 && h == 0, elected);
                     if (u + 1 < steps)
                         scores();
                     ok = ok && at_warp_wait(&b.ds_ready, u & 1, give_up);
                     if (!ok)
                         break;
                     tc_fence_after();
-                    at_weigh<D>(dk_at, dp_at, 64, base + S::A_AT + q_slot * AtTile<D>::BYTES, width, u == 0, elected);
+                    for (int h = 0; h < 2; ++h)
+                        at_weigh<D>(dk_at, dp_at + 64 * h, base + S::A_AT + q_slot * AtTile<D>::BYTES + h * AtTile<D>::HALF, width,
+                                    u == 0 && h == 0, elected);
                     at_commit(&b.a_empty[q_slot], elected);
                     at_commit(&b.b_empty[o_slot], elected);
                     q_slot = q_slot + 1 == S::A_SLOTS ? 0 : q_slot + 1;
@@ -213,7 +217,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
     }
     else
     {
-        at_team_registers();
+        at_more_registers<AT_TEAM_REGS>();
         const int team = warp >> 2;
         const uint32_t lanes = (uint32_t) (warp & 3) << 21;
         const int j = j0 + (threadIdx.x & 127);
@@ -348,7 +352,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
 
     if (warp >= AT_MMA_WARP)
     {
-        at_other_registers();
+        at_fewer_registers<AT_OTHER_REGS>();
         if (warp == AT_TMA_WARP)
         {
             if (lane == 0 && steps > 0)
@@ -397,7 +401,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
                     if (!ok)
                         return;
                     tc_fence_after();
-                    at_scores<D>(s_at + 128 * (ahead & 1), q_at, base + S::A_AT + ra.slot * AtTile<D>::BYTES, ksteps, elected);
+                    at_scores<D, 128>(s_at + 128 * (ahead & 1), q_at, base + S::A_AT + ra.slot * AtTile<D>::BYTES, ksteps, elected);
                     at_commit(&b.s_full[ahead & 1], elected);
                     ++ahead;
                     ra.next(S::A_SLOTS);
@@ -407,7 +411,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
                     if (!ok)
                         return;
                     tc_fence_after();
-                    at_scores<D>(dp_at, do_at, base + S::B_AT + rb.slot * AtTile<D>::BYTES, ksteps, elected);
+                    at_scores<D, 128>(dp_at, do_at, base + S::B_AT + rb.slot * AtTile<D>::BYTES, ksteps, elected);
                     at_commit(&b.dp_full, elected);
                     at_commit(&b.b_empty[rb.slot], elected);
                     rb.next(S::B_SLOTS);
@@ -423,7 +427,9 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
                     if (!ok)
                         break;
                     tc_fence_after();
-                    at_weigh<D>(dq_at, dp_at, 64, base + S::A_AT + k_slot * AtTile<D>::BYTES, width, u == 0, elected);
+                    for (int h = 0; h < 2; ++h)
+                        at_weigh<D>(dq_at, dp_at + 64 * h, base + S::A_AT + k_slot * AtTile<D>::BYTES + h * AtTile<D>::HALF, width,
+                                    u == 0 && h == 0, elected);
                     at_commit(&b.a_empty[k_slot], elected);
                     k_slot = k_slot + 1 == S::A_SLOTS ? 0 : k_slot + 1;
                     if (u + 1 < steps)
@@ -440,7 +446,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
     }
     else
     {
-        at_team_registers();
+        at_more_registers<AT_TEAM_REGS>();
         const int team = warp >> 2;
         const uint32_t lanes = (uint32_t) (warp & 3) << 21;
         const int i = i0 + (threadIdx.x & 127);

@@ -1,11 +1,15 @@
 // Attention forward on the tensor cores.
 //
 // A block has two tiles of 128 query cells of one head, each with a team of 128 threads, one row a
-// thread, and walks over tiles of 128 keys.  While one team turns its scores into weights the tensor
-// cores work for the other: S = Q K' into 128 columns of tensor memory, then, the weights written
-// back as bf16 over the scores, O += P V.  A row's weights are powers of two about a maximum that
-// is renewed only when it has grown by more than 2^8 since; then the thread scales its row of O.
-// (The sums are exact about any base that keeps them in range.)
+// thread, and walks over the keys, 64 at a step.  A team's scores have two places of 64 columns in
+// tensor memory: while its threads turn one step's scores into weights, the tensor cores take the
+// next step's, S = Q K', and, the weights written back as bf16 over their scores, O += P V of the
+// step before.  A team so never waits for a product (with one place of 128 columns it did for a
+// third of the time: 4 x 4096 cells, 8 heads of 64 channels, 257 us).  A row's weights are powers of two
+// about a maximum that is renewed only when it has grown by more than 2^8 since; then the thread
+// scales its row of O.  (The sums are exact about any base that keeps them in range.)
+//
+// Few queries (APART): both teams have the same 128 of them and a part of the keys each.
 #include "attention_tc.cuh"
 
 namespace dcb
@@ -16,30 +20,45 @@ namespace
 
 constexpr float AF_GROWTH = 8.f;
 
-template <int D>
+// Heads of 64 channels: two blocks an SM, of half its tensor memory each, so that an SM sub-core has four rows' warps
+// and its exponentials never pause; a team has one place for scores then.  128 channels: one block.
+template <int D, bool APART>
 struct AfShape
 {
-    static constexpr uint32_t SLOTS = D == 128 ? 5 : 8; // of K and V tiles in turn
+    static constexpr int BLOCKS = D == 64 && !APART ? 2 : 1; // an SM
+    static constexpr int PLACES = BLOCKS == 2 ? 1 : 2;  // for 64 columns of a team's scores
+    static constexpr uint32_t O_AT = 2 * PLACES * 64;   // column of O, D a team
+    static constexpr uint32_t SLOTS = D == 128 ? 5 : BLOCKS == 2 ? 4 : 8; // of K and V tiles in turn
+    static constexpr uint32_t COLUMNS = 512 / BLOCKS;
+    // registers: 3 x 80 (two blocks) or 3 x 168 at launch
+    static constexpr int TEAM_REGS = BLOCKS == 2 ? 104 : AT_TEAM_REGS;
+    static constexpr int OTHER_REGS = BLOCKS == 2 ? 32 : AT_OTHER_REGS;
     static constexpr uint32_t Q_AT = 0;
     static constexpr uint32_t RING_AT = 2 * AtTile<D>::BYTES;
     static constexpr uint32_t BARS_AT = RING_AT + SLOTS * AtTile<D>::BYTES;
     static constexpr uint32_t SMEM = BARS_AT + 256;
 };
+template <int D, bool APART>
+constexpr bool af_fits = AfShape<D, APART>::O_AT + 2 * D <= AfShape<D, APART>::COLUMNS
+                         && AfShape<D, APART>::BLOCKS * (AfShape<D, APART>::SMEM + 1024) <= 228 * 1024;
+static_assert(af_fits<64, false> && af_fits<64, true> && af_fits<128, false> && af_fits<128, true>,
+              "tensor memory of a block, shared memory of an SM's blocks");
+static_assert(2 * AfShape<64, false>::TEAM_REGS + AfShape<64, false>::OTHER_REGS <= 3 * 80, "registers of two blocks");
 
 struct AfBars
 {
-    uint64_t q_full, full[8], empty[8], s_full[2], p_ready[2], o_full[2];
+    uint64_t q_full, full[8], empty[8], s_full[2][2], p_ready[2][2], o_done[2], fin[2];
     uint32_t tmem;
     int give_up;
 };
 static_assert(sizeof(AfBars) <= 256, "the barriers' room");
 
-template <int D>
-__global__ void __launch_bounds__(AT_THREADS, 1)
+template <int D, bool APART>
+__global__ void __launch_bounds__(AT_THREADS, AfShape<D, APART>::BLOCKS)
     attn_tc_fwd_kernel(const __grid_constant__ AttnProblem p, const __grid_constant__ AtMaps maps,
                        const __grid_constant__ AtExtra ex)
 {
-    using S = AfShape<D>;
+    using S = AfShape<D, APART>;
     extern __shared__ __align__(1024) uint8_t smem[];
     const uint32_t base = smem_u32(smem);
     AfBars& b = *reinterpret_cast<AfBars*>(smem + S::BARS_AT);
@@ -49,26 +68,31 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
         return;
 
     long long at = blockIdx.x;
-    const int blocks_q = attn_tiles(p.sq, 2 * AT_TILE);
+    const int blocks_q = APART ? 1 : attn_tiles(p.sq, 2 * AT_TILE);
     const int block_q = blocks_q - 1 - (int) (at % blocks_q); // causal: the longest walks first
     at /= blocks_q;
-    const int split = (int) (at % p.kv_splits);
-    const long long nh = at / p.kv_splits, n = nh / p.q_heads;
+    const int splits = APART ? p.kv_splits / 2 : p.kv_splits;
+    const int split = (int) (at % splits);
+    const long long nh = at / splits, n = nh / p.q_heads;
     const int head = (int) (nh - n * p.q_heads), kv_head = head / p.group;
     const int i0 = block_q * 2 * AT_TILE;
     const int tiles = attn_tiles(p.sk, AT_TILE);
-    const int lo = (int) ((long long) tiles * split / p.kv_splits);
-    const int hi = (int) ((long long) tiles * (split + 1) / p.kv_splits);
-    int steps[2]; // of either team
+    int lo[2], steps[2]; // of either team: first tile of keys, steps of 64 keys
     for (int t = 0; t < 2; ++t)
     {
-        const int first = i0 + t * AT_TILE;
-        int end = hi;
+        const int part = APART ? 2 * split + t : split, first = APART ? 0 : i0 + t * AT_TILE;
+        lo[t] = (int) ((long long) tiles * part / p.kv_splits);
+        const int hi = (int) ((long long) tiles * (part + 1) / p.kv_splits);
+        int end = min(p.sk, hi * AT_TILE); // cells
         if (p.causal)
-            end = (int) min((long long) hi, max(0ll, (long long) first + AT_TILE - 1 + p.offset + AT_TILE) / AT_TILE);
-        steps[t] = first < p.sq ? max(0, end - lo) : 0;
+            end = (int) min((long long) end, max(0ll, (long long) first + AT_TILE + p.offset));
+        steps[t] = first < p.sq ? max(0, end - lo[t] * AT_TILE + 63) / 64 : 0;
     }
     const int most = max(steps[0], steps[1]);
+    // K and V tiles in the order that they are needed in: number of team t's, of the j-th tile
+    const auto k_number = [&](int t, int j) { return (uint32_t) (APART ? 4 * j + t : 2 * j); };
+    const auto v_number = [&](int t, int j) { return (uint32_t) (APART ? 4 * j + 2 + t : 2 * j + 1); };
+    constexpr int SHARED = APART ? 2 : 1; // tiles of K a step of two
 
     if (threadIdx.x == 0)
     {
@@ -76,12 +100,16 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
         for (uint32_t s = 0; s < S::SLOTS; ++s)
             mbar_init(&b.full[s], 1), mbar_init(&b.empty[s], 1);
         for (int t = 0; t < 2; ++t)
-            mbar_init(&b.s_full[t], 1), mbar_init(&b.p_ready[t], 4), mbar_init(&b.o_full[t], 1);
+        {
+            for (int h = 0; h < 2; ++h)
+                mbar_init(&b.s_full[t][h], 1), mbar_init(&b.p_ready[t][h], 4);
+            mbar_init(&b.o_done[t], 1), mbar_init(&b.fin[t], 1);
+        }
         b.give_up = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == AT_MMA_WARP)
-        at_tmem_alloc(&b.tmem);
+        at_tmem_alloc<S::COLUMNS>(&b.tmem);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -92,25 +120,29 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
 
     if (warp >= AT_MMA_WARP)
     {
-        at_other_registers();
+        at_fewer_registers<S::OTHER_REGS>();
         if (warp == AT_TMA_WARP)
         {
             if (lane == 0 && most > 0)
             {
-                mbar_expect_tx(&b.q_full, 2 * AtTile<D>::BYTES);
-                for (int t = 0; t < 2; ++t)
+                const int own = APART ? 1 : 2; // query tiles
+                mbar_expect_tx(&b.q_full, own * AtTile<D>::BYTES);
+                for (int t = 0; t < own; ++t)
                     at_tma_tile<D>(base + S::Q_AT + t * AtTile<D>::BYTES, &maps.q, i0 + t * AT_TILE, head, (int) n,
                                    &b.q_full);
                 AtRing r;
-                for (int u = 0; u < 2 * most && ok; ++u)
+                const int loads = 2 * SHARED * ((most + 1) / 2);
+                for (int u = 0; u < loads && ok; ++u)
                 {
+                    const int j = u / (2 * SHARED), t = u % SHARED;
+                    const bool value = u % (2 * SHARED) >= SHARED;
                     if (r.lap > 0)
                         ok = mbar_wait_t<20>(&b.empty[r.slot], (r.lap - 1) & 1, give_up);
                     if (!ok)
                         break;
                     mbar_expect_tx(&b.full[r.slot], AtTile<D>::BYTES);
-                    at_tma_tile<D>(base + S::RING_AT + r.slot * AtTile<D>::BYTES, u & 1 ? &maps.v : &maps.k,
-                                   (lo + (u >> 1)) * AT_TILE, kv_head, (int) n, &b.full[r.slot]);
+                    at_tma_tile<D>(base + S::RING_AT + r.slot * AtTile<D>::BYTES, value ? &maps.v : &maps.k,
+                                   (lo[t] + j) * AT_TILE, kv_head, (int) n, &b.full[r.slot]);
                     r.next(S::SLOTS);
                 }
                 if (!ok || *give_up)
@@ -128,61 +160,79 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
                 const uint32_t elected = at_elect();
                 const int ksteps = (p.d + 15) / 16;
                 const uint32_t width = (uint32_t) ksteps * 16;
-                const auto tile_of = [&](uint32_t slot) { return base + S::RING_AT + slot * AtTile<D>::BYTES; };
-                AtRing r; // the tile after the last one that was waited for
-                ok = at_warp_wait(&b.q_full, 0, give_up) && at_warp_wait(&b.full[r.slot], r.lap & 1, give_up);
-                tc_fence_after();
-                uint32_t k_slot = r.slot;
-                r.next(S::SLOTS);
-                for (int t = 0; t < 2 && ok; ++t)
-                    if (steps[t] > 0)
-                    {
-                        at_scores<D>(tmem + t * AT_TILE, base + S::Q_AT + t * AtTile<D>::BYTES, tile_of(k_slot), ksteps,
-                                     elected);
-                        at_commit(&b.s_full[t], elected);
-                    }
-                if (ok)
-                    at_commit(&b.empty[k_slot], elected);
-                for (int j = 0; j < most && ok; ++j)
+                const auto tile_of = [&](uint32_t number) {
+                    return base + S::RING_AT + number % S::SLOTS * AtTile<D>::BYTES;
+                };
+                const auto arrived = [&](uint32_t number) {
+                    ok = ok && at_warp_wait(&b.full[number % S::SLOTS], number / S::SLOTS & 1, give_up);
+                };
+                const auto release = [&](uint32_t number) { at_commit(&b.empty[number % S::SLOTS], elected); };
+                // every tile that was asked for is waited for, also by a team without work on it
+                const auto keys_arrived = [&](int j) {
+                    for (int t = 0; t < SHARED; ++t)
+                        arrived(k_number(t, j));
+                    tc_fence_after();
+                };
+                const auto scores = [&](int t, int u) {
+                    at_scores<D, 64>(tmem + (t * S::PLACES + u % S::PLACES) * 64,
+                                     base + S::Q_AT + (APART ? 0 : t * AtTile<D>::BYTES),
+                                     tile_of(k_number(t, u >> 1)) + (u & 1) * AtTile<D>::HALF, ksteps, elected);
+                    at_commit(&b.s_full[t][u % S::PLACES], elected);
+                };
+                ok = at_warp_wait(&b.q_full, 0, give_up);
+                keys_arrived(0);
+                // behind the last team's second half of a tile the slot is free
+                const auto keys_done = [&](int u) {
+                    if (ok && (u & 1) && u < most)
+                        for (int t = 0; t < SHARED; ++t)
+                            release(k_number(t, u >> 1));
+                };
+                for (int u = 0; u < S::PLACES; ++u)
                 {
-                    const uint32_t v_slot = r.slot;
-                    ok = at_warp_wait(&b.full[r.slot], r.lap & 1, give_up);
-                    r.next(S::SLOTS);
-                    bool have_k = false;
-                    for (int t = 0; t < 2 && ok; ++t)
+                    for (int t = 0; t < 2; ++t)
+                        if (ok && u < steps[t])
+                            scores(t, u);
+                    keys_done(u);
+                }
+                for (int u = 0; u < most && ok; ++u)
+                {
+                    const int j = u >> 1, ahead = u + S::PLACES;
+                    if ((u & 1) == 0)
                     {
-                        if (j < steps[t])
-                        {
-                            ok = at_warp_wait(&b.p_ready[t], j & 1, give_up);
-                            if (!ok)
-                                break;
-                            tc_fence_after();
-                            at_weigh<D>(tmem + 2 * AT_TILE + t * D, tmem + t * AT_TILE, 32, tile_of(v_slot), width, j == 0,
-                                    elected);
-                            if (j + 1 == steps[t])
-                                at_commit(&b.o_full[t], elected);
-                        }
-                        if (t == 1)
-                            at_commit(&b.empty[v_slot], elected);
-                        if (j + 1 < steps[t])
+                        for (int t = 0; t < SHARED; ++t)
+                            arrived(v_number(t, j));
+                        tc_fence_after();
+                    }
+                    bool have_k = ahead & 1;
+                    // the teams in the order that they are ready in
+                    uint32_t left = (u < steps[0] ? 1u : 0u) | (u < steps[1] ? 2u : 0u);
+                    while (left && ok)
+                    {
+                        const int t = at_first_ready(&b.p_ready[0][u % S::PLACES], &b.p_ready[1][u % S::PLACES], left,
+                                                     u / S::PLACES & 1, give_up);
+                        ok = t >= 0;
+                        if (!ok)
+                            break;
+                        left &= ~(1u << t);
+                        tc_fence_after();
+                        at_weigh<D>(tmem + S::O_AT + t * D, tmem + (t * S::PLACES + u % S::PLACES) * 64,
+                                    tile_of(v_number(t, j)) + (u & 1) * AtTile<D>::HALF, width, u == 0, elected);
+                        at_commit(&b.o_done[t], elected);
+                        if (u + 1 == steps[t])
+                            at_commit(&b.fin[t], elected);
+                        if (ahead < steps[t])
                         {
                             if (!have_k)
-                            {
-                                ok = at_warp_wait(&b.full[r.slot], r.lap & 1, give_up);
-                                if (!ok)
-                                    break;
-                                tc_fence_after();
-                                have_k = true;
-                            }
-                            at_scores<D>(tmem + t * AT_TILE, base + S::Q_AT + t * AtTile<D>::BYTES, tile_of(r.slot), ksteps, elected);
-                            at_commit(&b.s_full[t], elected);
+                                keys_arrived(ahead >> 1);
+                            have_k = true;
+                            if (ok)
+                                scores(t, ahead);
                         }
                     }
-                    if (ok && j + 1 < most)
-                    {
-                        at_commit(&b.empty[r.slot], elected);
-                        r.next(S::SLOTS);
-                    }
+                    if (ok && (u & 1))
+                        for (int t = 0; t < SHARED; ++t)
+                            release(v_number(t, j));
+                    keys_done(ahead);
                 }
                 if (!ok)
                 {
@@ -196,133 +246,243 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
     }
     else
     {
-        at_team_registers();
+        at_more_registers<S::TEAM_REGS>();
         const int t = warp >> 2;
         const uint32_t lanes = (uint32_t) (warp & 3) << 21; // 32 lanes of tensor memory a warp
-        const uint32_t s_at = tmem + lanes + t * AT_TILE, o_at = tmem + lanes + 2 * AT_TILE + t * D;
-        const int i = i0 + t * AT_TILE + (threadIdx.x & 127);
+        const uint32_t o_at = tmem + lanes + S::O_AT + t * D;
+        const int row0 = (APART ? 0 : i0 + t * AT_TILE) + (warp & 3) * 32, i = row0 + lane;
+        const int part = APART ? 2 * split + t : split;
+        const bool rows = row0 < p.sq; // else no row of this warp is a cell: what its weights are reaches nobody
         float top = -INFINITY, sum = 0.f; // the base of the weights so far and their sum
-        for (int j = 0; j < steps[t]; ++j)
-        {
-            const int j0 = (lo + j) * AT_TILE;
-            ok = at_warp_wait(&b.s_full[t], j & 1, give_up);
-            if (!ok)
-                break;
+        float mine = -INFINITY;           // the largest score of the step that comes next
+        const auto score_at = [&](int u) { return tmem + lanes + (t * S::PLACES + u % S::PLACES) * 64; };
+        const auto wait_scores = [&](int u) {
+            ok = ok && at_warp_wait(&b.s_full[t][u % S::PLACES], u / S::PLACES & 1, give_up);
             tc_fence_after();
-            float s[128];
-#pragma unroll
-            for (int c = 0; c < 4; ++c)
-                at_tmem_ld32(s_at + 32 * c, s + 32 * c);
-            at_tmem_wait_ld();
-            uint32_t see[4];
-            bool all = true;
-#pragma unroll
-            for (int w = 0; w < 4; ++w)
+            return ok;
+        };
+        uint32_t see[2];  // which keys of the coming step this row may see
+        bool cut = false; // whether some row of the warp may not see all of them
+        // steps whose keys are there and, where the order is causal, not behind the warp's first row
+        int open = 0;
+        if (!bits)
+            open = (int) min((long long) p.sk, p.causal ? (long long) row0 + p.offset + 1 : (long long) p.sk) - lo[t] * AT_TILE;
+        open = open > 0 ? open / 64 : 0;
+        const auto mask = [&](int c, float x) { return see[c >> 5] >> (c & 31) & 1 ? x : -INFINITY; };
+        // masks and maximum of a step's scores, which have arrived
+        const auto look = [&](int u, float (&s)[64]) {
+            cut = u >= open;
+            if (cut)
             {
-                see[w] = at_there(p, bits, j0, w);
-                if (p.causal)
-                    see[w] &= at_up_to(i + p.offset - j0, w);
-                all = all && see[w] == ~0u;
-            }
-            if (__any_sync(~0u, !all))
-            {
+                const int j0 = lo[t] * AT_TILE + u * 64;
 #pragma unroll
-                for (int c = 0; c < 128; ++c)
-                    s[c] = see[c >> 5] >> (c & 31) & 1 ? s[c] : -INFINITY;
+                for (int w = 0; w < 2; ++w)
+                {
+                    see[w] = at_there(p, bits, j0, w);
+                    if (p.causal)
+                        see[w] &= at_up_to(i + p.offset - j0, w);
+                }
+#pragma unroll
+                for (int c = 0; c < 64; ++c)
+                    s[c] = mask(c, s[c]);
             }
             float m0 = s[0], m1 = s[1], m2 = s[2], m3 = s[3];
 #pragma unroll
-            for (int c = 4; c < 124; c += 8)
+            for (int c = 4; c < 60; c += 8)
             {
                 m0 = at_max3(m0, s[c], s[c + 1]), m1 = at_max3(m1, s[c + 2], s[c + 3]);
                 m2 = at_max3(m2, s[c + 4], s[c + 5]), m3 = at_max3(m3, s[c + 6], s[c + 7]);
             }
-            m0 = at_max3(m0, s[124], s[125]), m1 = at_max3(m1, s[126], s[127]);
-            const float mine = at_max3(fmaxf(m0, m1), m2, m3) * p.scale;
+            m0 = at_max3(m0, s[60], s[61]), m1 = at_max3(m1, s[62], s[63]);
+            mine = at_max3(fmaxf(m0, m1), m2, m3) * p.scale;
+        };
+        // The base of step u's weights; O follows where it grows.
+        const auto renew = [&](int u) {
             const bool grown = mine > top + AF_GROWTH;
-            if (__any_sync(~0u, grown))
+            if (!__any_sync(~0u, grown))
+                return;
+            const float shrink = grown ? at_exp2(top - mine) : 1.f;
+            top = grown ? mine : top;
+            sum *= shrink;
+            if (u == 0)
+                return;
+            // O of the step before: with these scores' arrival all but that step have been added, and the next one waits
+            // for this one's weights
+            ok = at_warp_wait(&b.o_done[t], (u - 1) & 1, give_up);
+            if (!ok)
+                return;
+            tc_fence_after();
+            for (int c0 = 0; c0 < p.d; c0 += 32)
             {
-                const float shrink = grown ? at_exp2(top - mine) : 1.f;
-                top = grown ? mine : top;
-                sum *= shrink;
-                if (j > 0)
-                {
-                    for (int c0 = 0; c0 < p.d; c0 += 32)
+                float o[32];
+                at_tmem_ld32(o_at + c0, o);
+                at_tmem_wait_ld();
+#pragma unroll
+                for (int c = 0; c < 32; ++c)
+                    o[c] *= shrink;
+                at_tmem_st32(o_at + c0, reinterpret_cast<const uint32_t*>(o));
+            }
+        };
+        uint64_t scale2, base2, l0, l1;
+        const auto begin = [&] {
+            const float base_of = top == -INFINITY ? 0.f : top;
+            scale2 = at_pair(p.scale, p.scale), base2 = at_pair(-base_of, -base_of);
+            l0 = l1 = 0;
+        };
+        // weights of 16 scores, to the h-th eight columns
+        const auto weigh = [&](int u, int h, const float* s) {
+            uint32_t w[8];
+#pragma unroll
+            for (int c = 0; c < 16; c += 4)
+            {
+                float e[4];
+#pragma unroll
+                for (int k = 0; k < 4; k += 2)
+                    at_unpair(at_fma2(at_pair(s[c + k], s[c + k + 1]), scale2, base2), e[k], e[k + 1]);
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                    e[k] = at_exp2(e[k]);
+                l0 = at_add2(l0, at_pair(e[0], e[1]));
+                l1 = at_add2(l1, at_pair(e[2], e[3]));
+                w[c / 2] = pack_bf16(e[0], e[1]);
+                w[c / 2 + 1] = pack_bf16(e[2], e[3]);
+            }
+            tmem_st8(score_at(u) + 8 * h, w);
+        };
+        const auto hand_over = [&](int u) {
+            float a, c;
+            at_unpair(at_add2(l0, l1), a, c);
+            sum += a + c;
+            at_tmem_wait_st();
+            at_warp_arrive(&b.p_ready[t][u % S::PLACES], lane);
+        };
+        const auto fetch = [&](int u, float (&s)[64]) {
+            if (!wait_scores(u))
+                return;
+            at_tmem_ld32(score_at(u), s);
+            at_tmem_ld32(score_at(u) + 32, s + 32);
+            at_tmem_wait_ld();
+            look(u, s);
+        };
+        if (steps[t] > 0 && rows)
+        {
+            if constexpr (S::BLOCKS == 1)
+            {
+                // Half way through step u the scores of the next one are fetched, which have been taken meanwhile.
+                const auto step = [&](int u, float (&s)[64], float (&next)[64]) {
+                    renew(u);
+                    if (!ok)
+                        return;
+                    begin();
+                    weigh(u, 0, s);
+                    weigh(u, 1, s + 16);
+                    if (u + 1 < steps[t])
                     {
-                        float o[32];
-                        at_tmem_ld32(o_at + c0, o);
+                        if (!wait_scores(u + 1))
+                            return;
+                        at_tmem_ld32(score_at(u + 1), next);
+                        at_tmem_ld32(score_at(u + 1) + 32, next + 32);
+                    }
+                    weigh(u, 2, s + 32);
+                    weigh(u, 3, s + 48);
+                    hand_over(u);
+                    if (u + 1 < steps[t])
+                    {
+                        at_tmem_wait_ld();
+                        look(u + 1, next);
+                    }
+                };
+                float even[64], odd[64];
+                fetch(0, even);
+                for (int u = 0; u < steps[t] && ok; u += 2)
+                {
+                    step(u, even, odd);
+                    if (u + 1 < steps[t] && ok)
+                        step(u + 1, odd, even);
+                }
+            }
+            else
+            {
+                // Half the registers: the scores are fetched once for their maximum and again, 16 at a time, for their
+                // weights, which go over scores that have been fetched.
+                for (int u = 0; u < steps[t] && ok; ++u)
+                {
+                    {
+                        float s[64];
+                        fetch(u, s);
+                    }
+                    if (ok)
+                        renew(u);
+                    if (!ok)
+                        break;
+                    begin();
+#pragma unroll
+                    for (int h = 0; h < 4; ++h)
+                    {
+                        uint32_t raw[16];
+                        float s[16];
+                        tmem_ld16(score_at(u) + 16 * h, raw);
                         at_tmem_wait_ld();
 #pragma unroll
-                        for (int c = 0; c < 32; ++c)
-                            o[c] *= shrink;
-                        at_tmem_st32(o_at + c0, reinterpret_cast<const uint32_t*>(o));
+                        for (int c = 0; c < 16; ++c)
+                            s[c] = __uint_as_float(raw[c]);
+                        if (cut)
+                        {
+#pragma unroll
+                            for (int c = 0; c < 16; ++c)
+                                s[c] = mask(16 * h + c, s[c]);
+                        }
+                        weigh(u, h, s);
                     }
+                    hand_over(u);
                 }
             }
-            const float base_of = top == -INFINITY ? 0.f : top;
-            float l0 = 0.f, l1 = 0.f, l2 = 0.f, l3 = 0.f;
-#pragma unroll
-            for (int half = 0; half < 2; ++half)
-            {
-                uint32_t w[32];
-#pragma unroll
-                for (int c = 0; c < 64; c += 4)
-                {
-                    const float* x = s + 64 * half + c;
-                    const float e0 = at_exp2(fmaf(x[0], p.scale, -base_of)), e1 = at_exp2(fmaf(x[1], p.scale, -base_of));
-                    const float e2 = at_exp2(fmaf(x[2], p.scale, -base_of)), e3 = at_exp2(fmaf(x[3], p.scale, -base_of));
-                    l0 += e0, l1 += e1, l2 += e2, l3 += e3;
-                    w[c / 2] = pack_bf16(e0, e1);
-                    w[c / 2 + 1] = pack_bf16(e2, e3);
-                }
-                at_tmem_st32(s_at + 32 * half, w);
-            }
-            sum += (l0 + l1) + (l2 + l3);
-            at_tmem_wait_st();
-            at_warp_arrive(&b.p_ready[t], lane);
+        }
+        else
+        {
+            for (int u = 0; u < steps[t] && wait_scores(u); ++u)
+                at_warp_arrive(&b.p_ready[t][u % S::PLACES], lane);
         }
         if (ok && steps[t] > 0)
-            ok = at_warp_wait(&b.o_full[t], 0, give_up);
+            ok = at_warp_wait(&b.fin[t], 0, give_up); // o_done may be two steps away
         tc_fence_after();
-        if (ok)
+        if (ok && rows)
         {
             const bool nothing = steps[t] == 0;
-            if (i0 + t * AT_TILE < p.sq)
+            const long long heads = (long long) p.n * p.q_heads;
+            if (p.kv_splits > 1)
             {
-                const long long heads = (long long) p.n * p.q_heads;
-                if (p.kv_splits > 1)
+                if (i < p.sq)
                 {
-                    if (i < p.sq)
-                    {
-                        float* ml = p.part_ml + (2 * heads * split + nh) * p.sq + i;
-                        ml[0] = top;
-                        ml[heads * p.sq] = sum;
-                    }
-                    at_store(p.o, p.part_o + split * heads * p.d * p.sq, nh, n, head, p.d, i, p.sq, 1.f, false, nothing,
-                             o_at, 0, D);
+                    float* ml = p.part_ml + (2 * heads * part + nh) * p.sq + i;
+                    ml[0] = top;
+                    ml[heads * p.sq] = sum;
                 }
-                else
-                {
-                    const bool none = sum == 0.f || (p.q_mask && i < p.sq && !p.q_mask[n * p.sq + i]);
-                    at_store(p.o, nullptr, nh, n, head, p.d, i, p.sq, 1.f / sum, none, nothing, o_at, 0, D);
-                    if (i < p.sq)
-                        p.lse[nh * p.sq + i] = none ? -INFINITY : (top + log2f(sum)) / ATTN_LOG2E;
-                }
+                at_store(p.o, p.part_o + part * heads * p.d * p.sq, nh, n, head, p.d, i, p.sq, 1.f, false, nothing, o_at,
+                         0, D);
+            }
+            else
+            {
+                const bool none = sum == 0.f || (p.q_mask && i < p.sq && !p.q_mask[n * p.sq + i]);
+                at_store(p.o, nullptr, nh, n, head, p.d, i, p.sq, 1.f / sum, none, nothing, o_at, 0, D);
+                if (i < p.sq)
+                    p.lse[nh * p.sq + i] = none ? -INFINITY : (top + log2f(sum)) / ATTN_LOG2E;
             }
         }
     }
-    at_finish(ok, ex.status, warp, lane, tmem);
+    at_finish<S::COLUMNS>(ok, ex.status, warp, lane, tmem);
 }
 
-template <int D>
+template <int D, bool APART>
 int32_t af_launch(const AttnProblem& p, const AtMaps& maps, const AtExtra& ex, cudaStream_t stream)
 {
-    const long long blocks = (long long) p.n * p.q_heads * attn_tiles(p.sq, 2 * AT_TILE) * p.kv_splits;
+    const long long blocks = (long long) p.n * p.q_heads
+                             * (APART ? p.kv_splits / 2 : (long long) attn_tiles(p.sq, 2 * AT_TILE) * p.kv_splits);
     DCB_REQUIRE(blocks < (1ll << 31), "too many tiles");
-    if (int32_t e = allow_dynamic_smem((const void*) attn_tc_fwd_kernel<D>, AfShape<D>::SMEM))
+    if (int32_t e = allow_dynamic_smem((const void*) attn_tc_fwd_kernel<D, APART>, AfShape<D, APART>::SMEM))
         return e;
-    DCB_CUDA_TRY(launch_overlapped(attn_tc_fwd_kernel<D>, dim3((unsigned) blocks), AT_THREADS, AfShape<D>::SMEM, stream,
-                                   p, maps, ex));
+    DCB_CUDA_TRY(launch_overlapped(attn_tc_fwd_kernel<D, APART>, dim3((unsigned) blocks), AT_THREADS, AfShape<D, APART>::SMEM,
+                                   stream, p, maps, ex));
     return DCB_OK;
 }
 
@@ -330,7 +490,9 @@ int32_t af_launch(const AttnProblem& p, const AtMaps& maps, const AtExtra& ex, c
 
 int32_t attn_tc_fwd_launch(const AttnProblem& p, const AtMaps& maps, const AtExtra& ex, cudaStream_t stream)
 {
-    return p.d <= 64 ? af_launch<64>(p, maps, ex, stream) : af_launch<128>(p, maps, ex, stream);
+    if (attn_tc_apart(p))
+        return p.d <= 64 ? af_launch<64, true>(p, maps, ex, stream) : af_launch<128, true>(p, maps, ex, stream);
+    return p.d <= 64 ? af_launch<64, false>(p, maps, ex, stream) : af_launch<128, false>(p, maps, ex, stream);
 }
 
 } // namespace dcb
