@@ -171,13 +171,13 @@ bool attn_tc_apart(const AttnProblem& p)
 
 void attn_tc_splits(AttnProblem* p, bool backward)
 {
-    const long long slots = num_sms();
+    const long long slots = (p->d <= 64 ? 2 : 1) * num_sms(); // blocks at a time
     const long long q_tiles = attn_tiles(p->sq, AT_TILE), k_tiles = attn_tiles(p->sk, AT_TILE);
     const long long qh = (long long) p->n * p->q_heads, kh = (long long) p->n * p->kv_heads;
     p->q_splits = backward ? attn_splits(kh * k_tiles, (int) std::min<long long>(q_tiles * p->group, 1 << 30), slots, 2)
                            : 1;
     if (!backward && attn_tc_apart(*p))
-        p->kv_splits = 2 * attn_splits(qh, (int) k_tiles / 2, slots, 2);
+        p->kv_splits = 2 * attn_splits(qh, (int) k_tiles / 2, num_sms(), 2);
     else
         p->kv_splits = attn_splits(qh * (backward ? q_tiles : (q_tiles + 1) / 2), (int) k_tiles, slots, 2);
 }

@@ -143,6 +143,16 @@ __device__ __forceinline__ void at_tma_tile(uint32_t dst, const CUtensorMap* map
     at_tma_half(dst + AtTile<D>::HALF, map, cell + 64, head, n, bar);
 }
 
+template <int D, int CELLS>
+__device__ __forceinline__ void at_tma_cells(uint32_t dst, const CUtensorMap* map, int cell, int head, int n,
+                                             uint64_t* bar)
+{
+    if constexpr (CELLS == 64)
+        at_tma_half(dst, map, cell, head, n, bar);
+    else
+        at_tma_tile<D>(dst, map, cell, head, n, bar);
+}
+
 // `bytes` from a 16-byte aligned address.
 __device__ __forceinline__ void at_bulk(uint32_t dst, const void* src, uint32_t bytes, uint64_t* bar)
 {

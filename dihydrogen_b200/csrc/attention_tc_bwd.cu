@@ -8,8 +8,10 @@
 // dQ += dS K.  It works S and dP out a second time (7 products in all instead of 5), for which no sum over blocks is
 // needed: no atomics, no fp32 gradient in memory, the same bits every run.
 //
-// Two teams of 128 threads have 64 of the 128 columns each, all 128 rows.  The products of one step run under the
-// exponentials of another: P' and dS' are handed over apart, and the scores are taken a step (dkv) or two (dq) ahead.
+// Two teams of 128 threads have half of a step's columns each, all 128 rows.  The products of one part of a step run
+// under the exponentials of another: P' and dS' are handed over apart, and the scores are taken a step (dkv) or two
+// (dq) ahead.  Heads of 128 channels: steps of 128 columns, one block an SM, whose tensor memory they fill.  Heads of 64:
+// steps of 64 columns and two blocks an SM, whose steps fall under one another's.
 #include "attention_tc.cuh"
 
 namespace dcb
@@ -20,16 +22,30 @@ namespace
 template <int D>
 struct AbShape
 {
+    static constexpr int BLOCKS = D == 64 ? 2 : 1;        // an SM
+    static constexpr int STEP = D == 64 ? 64 : 128;       // columns
+    static constexpr int MINE = STEP / 2;                 // of a team
+    static constexpr uint32_t COLUMNS = 512 / BLOCKS;     // of tensor memory
+    static constexpr int TEAM_REGS = BLOCKS == 2 ? 104 : AT_TEAM_REGS;
+    static constexpr int OTHER_REGS = BLOCKS == 2 ? 32 : AT_OTHER_REGS;
+    static constexpr uint32_t BYTES = AtTile<D>::HALF * (STEP / 64); // of a step's operand
     static constexpr uint32_t A_SLOTS = D == 128 ? 3 : 4; // Q (dkv) or K (dq)
-    static constexpr uint32_t B_SLOTS = D == 128 ? 2 : 4; // dO (dkv) or V (dq)
-    static constexpr uint32_t OWN_AT = 0;                 // K, V (dkv) or Q, dO (dq)
+    static constexpr uint32_t B_SLOTS = D == 128 ? 2 : 3; // dO (dkv) or V (dq)
+    static constexpr uint32_t OWN_AT = 0;                 // K, V (dkv) or Q, dO (dq): 128 cells each
     static constexpr uint32_t A_AT = 2 * AtTile<D>::BYTES;
-    static constexpr uint32_t B_AT = A_AT + A_SLOTS * AtTile<D>::BYTES;
-    static constexpr uint32_t STATS_AT = B_AT + B_SLOTS * AtTile<D>::BYTES; // dkv: lse, delta of a dO slot
-    static constexpr uint32_t BARS_AT = STATS_AT + B_SLOTS * 1024;
+    static constexpr uint32_t B_AT = A_AT + A_SLOTS * BYTES;
+    static constexpr uint32_t STATS_AT = B_AT + B_SLOTS * BYTES; // dkv: lse, delta of a dO slot
+    static constexpr uint32_t BARS_AT = STATS_AT + B_SLOTS * 8 * STEP;
     static constexpr uint32_t SMEM = BARS_AT + 256;
+    // columns: dkv S, dP, dV, dK; dq S twice, dP, dQ
+    static constexpr uint32_t DKV_DP = STEP, DKV_DV = 2 * STEP, DKV_DK = 2 * STEP + D;
+    static constexpr uint32_t DQ_DP = 2 * STEP, DQ_DQ = 3 * STEP;
 };
-static_assert(AbShape<128>::SMEM <= 227 * 1024, "shared memory of a block");
+template <int D>
+constexpr bool ab_fits = AbShape<D>::DKV_DK + D <= AbShape<D>::COLUMNS && AbShape<D>::DQ_DQ + D <= AbShape<D>::COLUMNS
+                         && AbShape<D>::BLOCKS * (AbShape<D>::SMEM + 1024) <= 228 * 1024;
+static_assert(ab_fits<64> && ab_fits<128>, "tensor memory of a block, shared memory of an SM's blocks");
+static_assert(2 * AbShape<64>::TEAM_REGS + AbShape<64>::OTHER_REGS <= 3 * 80, "registers of two blocks");
 
 struct AbBars
 {
@@ -39,6 +55,7 @@ struct AbBars
 };
 static_assert(sizeof(AbBars) <= 256, "the barriers' room");
 
+template <uint32_t COLUMNS>
 __device__ __forceinline__ void ab_init(AbBars& b, int warp)
 {
     if (threadIdx.x == 0)
@@ -56,7 +73,7 @@ __device__ __forceinline__ void ab_init(AbBars& b, int warp)
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == AT_MMA_WARP)
-        at_tmem_alloc(&b.tmem);
+        at_tmem_alloc<COLUMNS>(&b.tmem);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -70,8 +87,40 @@ __device__ __forceinline__ void ab_drain_products(AbBars& b, uint32_t elected)
     mbar_wait_t<20>(&b.fin, 0, &none);
 }
 
+// d += W B over a step's cells: a team's half of W lies at the start of its scores' columns, two cells to a column.
 template <int D>
-__global__ void __launch_bounds__(AT_THREADS, 1)
+__device__ __forceinline__ void ab_weigh(uint32_t d, uint32_t w, uint32_t b, uint32_t n, bool first, uint32_t elected)
+{
+    constexpr int MINE = AbShape<D>::MINE;
+    const uint32_t idesc = at_idesc(n, false, false);
+#pragma unroll
+    for (int k = 0; k < 2 * MINE / 16; ++k)
+    {
+        const int team = k / (MINE / 16), in_team = k % (MINE / 16);
+        const uint64_t db = AtTile<D>::along(b + k / 4 * AtTile<D>::HALF) + k % 4 * 2;
+        at_mma_ts(d, w + team * MINE + in_team * 8, db, idesc, !(first && k == 0), elected);
+    }
+}
+
+template <int N>
+__device__ __forceinline__ void ab_fetch(uint32_t taddr, float (&v)[N])
+{
+#pragma unroll
+    for (int c = 0; c < N; c += 32)
+        at_tmem_ld32(taddr + c, v + c);
+}
+
+template <int N>
+__device__ __forceinline__ void ab_put(uint32_t taddr, const uint32_t (&v)[N])
+{
+    if constexpr (N == 32)
+        at_tmem_st32(taddr, v);
+    else
+        at_tmem_st16(taddr, v);
+}
+
+template <int D>
+__global__ void __launch_bounds__(AT_THREADS, AbShape<D>::BLOCKS)
     attn_tc_dkv_kernel(const __grid_constant__ AttnProblem p, const __grid_constant__ AtMaps maps,
                        const __grid_constant__ AtExtra ex)
 {
@@ -85,31 +134,31 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
         return;
 
     long long at = blockIdx.x;
-    const int tiles_k = attn_tiles(p.sk, AT_TILE), tiles_q = attn_tiles(p.sq, AT_TILE);
+    const int tiles_k = attn_tiles(p.sk, AT_TILE), steps_q = attn_tiles(p.sq, S::STEP);
     const int tile = (int) (at % tiles_k); // causal: the first keys have the longest walks
     at /= tiles_k;
     const int split = (int) (at % p.q_splits);
     const long long nh = at / p.q_splits, n = nh / p.kv_heads;
     const int head = (int) (nh - n * p.kv_heads);
     const int j0 = tile * AT_TILE;
-    // the walk: tiles of queries from t0 on, of every query head of the group
+    // the walk: steps of queries from t0 on, of every query head of the group
     int t0 = 0;
     if (p.causal)
-        t0 = (int) min((long long) tiles_q, max(0ll, (long long) j0 - p.offset) / AT_TILE);
-    const int per_head = tiles_q - t0;
+        t0 = (int) min((long long) steps_q, max(0ll, (long long) j0 - p.offset) / S::STEP);
+    const int per_head = steps_q - t0;
     const long long all = (long long) per_head * p.group;
     const int lo = (int) (all * split / p.q_splits), steps = (int) (all * (split + 1) / p.q_splits) - lo;
 
-    ab_init(b, warp);
+    ab_init<S::COLUMNS>(b, warp);
     const uint32_t tmem = __shfl_sync(~0u, b.tmem, 0); // known to be uniform
     const float* stats = p.stats;
     wait_for_previous_kernel(stats);
     bool ok = true;
-    const uint32_t s_at = tmem, dp_at = tmem + 128, dv_at = tmem + 256, dk_at = tmem + 256 + D;
+    const uint32_t s_at = tmem, dp_at = tmem + S::DKV_DP, dv_at = tmem + S::DKV_DV, dk_at = tmem + S::DKV_DK;
 
     if (warp >= AT_MMA_WARP)
     {
-        at_fewer_registers<AT_OTHER_REGS>();
+        at_fewer_registers<S::OTHER_REGS>();
         if (warp == AT_TMA_WARP)
         {
             if (lane == 0 && steps > 0)
@@ -120,27 +169,27 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
                 AtRing ra, rb;
                 for (int u = 0; u < steps && ok; ++u)
                 {
-                    const int g = (lo + u) / per_head, i0 = (t0 + (lo + u) - g * per_head) * AT_TILE;
+                    const int g = (lo + u) / per_head, i0 = (t0 + (lo + u) - g * per_head) * S::STEP;
                     const int q_head = head * p.group + g;
                     if (ra.lap > 0)
                         ok = mbar_wait_t<20>(&b.a_empty[ra.slot], (ra.lap - 1) & 1, give_up);
                     if (!ok)
                         break;
-                    mbar_expect_tx(&b.a_full[ra.slot], AtTile<D>::BYTES);
-                    at_tma_tile<D>(base + S::A_AT + ra.slot * AtTile<D>::BYTES, &maps.q, i0, q_head, (int) n,
-                                   &b.a_full[ra.slot]);
+                    mbar_expect_tx(&b.a_full[ra.slot], S::BYTES);
+                    at_tma_cells<D, S::STEP>(base + S::A_AT + ra.slot * S::BYTES, &maps.q, i0, q_head, (int) n,
+                                             &b.a_full[ra.slot]);
                     ra.next(S::A_SLOTS);
                     if (rb.lap > 0)
                         ok = mbar_wait_t<20>(&b.b_empty[rb.slot], (rb.lap - 1) & 1, give_up);
                     if (!ok)
                         break;
-                    mbar_expect_tx(&b.b_full[rb.slot], AtTile<D>::BYTES + 1024);
-                    at_tma_tile<D>(base + S::B_AT + rb.slot * AtTile<D>::BYTES, &maps.d_o, i0, q_head, (int) n,
-                                   &b.b_full[rb.slot]);
+                    mbar_expect_tx(&b.b_full[rb.slot], S::BYTES + 8 * S::STEP);
+                    at_tma_cells<D, S::STEP>(base + S::B_AT + rb.slot * S::BYTES, &maps.d_o, i0, q_head, (int) n,
+                                             &b.b_full[rb.slot]);
                     const float* row = stats + (n * p.q_heads + q_head) * p.stats_pitch + i0;
-                    at_bulk(base + S::STATS_AT + rb.slot * 1024, row, 512, &b.b_full[rb.slot]);
-                    at_bulk(base + S::STATS_AT + rb.slot * 1024 + 512,
-                            row + (long long) p.n * p.q_heads * p.stats_pitch, 512, &b.b_full[rb.slot]);
+                    at_bulk(base + S::STATS_AT + rb.slot * 8 * S::STEP, row, 4 * S::STEP, &b.b_full[rb.slot]);
+                    at_bulk(base + S::STATS_AT + rb.slot * 8 * S::STEP + 4 * S::STEP,
+                            row + (long long) p.n * p.q_heads * p.stats_pitch, 4 * S::STEP, &b.b_full[rb.slot]);
                     rb.next(S::B_SLOTS);
                 }
                 if (!ok || *give_up)
@@ -167,7 +216,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
                     if (!ok)
                         return;
                     tc_fence_after();
-                    at_scores<D, 128>(s_at, k_at, base + S::A_AT + ra.slot * AtTile<D>::BYTES, ksteps, elected);
+                    at_scores<D, S::STEP>(s_at, k_at, base + S::A_AT + ra.slot * S::BYTES, ksteps, elected);
                     at_commit(&b.s_full[0], elected);
                     ra.next(S::A_SLOTS);
                 };
@@ -176,7 +225,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
                     if (!ok)
                         return;
                     tc_fence_after();
-                    at_scores<D, 128>(dp_at, v_at, base + S::B_AT + rb.slot * AtTile<D>::BYTES, ksteps, elected);
+                    at_scores<D, S::STEP>(dp_at, v_at, base + S::B_AT + rb.slot * S::BYTES, ksteps, elected);
                     at_commit(&b.dp_full, elected);
                     rb.next(S::B_SLOTS);
                 };
@@ -189,18 +238,14 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
                     if (!ok)
                         break;
                     tc_fence_after();
-                    for (int h = 0; h < 2; ++h)
-                        at_weigh<D>(dv_at, s_at + 64 * h, base + S::B_AT + o_slot * AtTile<D>::BYTES + h * AtTile<D>::HALF, width,
-                                    u == 0 && h == 0, elected);
+                    ab_weigh<D>(dv_at, s_at, base + S::B_AT + o_slot * S::BYTES, width, u == 0, elected);
                     if (u + 1 < steps)
                         scores();
                     ok = ok && at_warp_wait(&b.ds_ready, u & 1, give_up);
                     if (!ok)
                         break;
                     tc_fence_after();
-                    for (int h = 0; h < 2; ++h)
-                        at_weigh<D>(dk_at, dp_at + 64 * h, base + S::A_AT + q_slot * AtTile<D>::BYTES + h * AtTile<D>::HALF, width,
-                                    u == 0 && h == 0, elected);
+                    ab_weigh<D>(dk_at, dp_at, base + S::A_AT + q_slot * S::BYTES, width, u == 0, elected);
                     at_commit(&b.a_empty[q_slot], elected);
                     at_commit(&b.b_empty[o_slot], elected);
                     q_slot = q_slot + 1 == S::A_SLOTS ? 0 : q_slot + 1;
@@ -217,31 +262,30 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
     }
     else
     {
-        at_more_registers<AT_TEAM_REGS>();
+        at_more_registers<S::TEAM_REGS>();
         const int team = warp >> 2;
         const uint32_t lanes = (uint32_t) (warp & 3) << 21;
         const int j = j0 + (threadIdx.x & 127);
-        const uint32_t s_mine = s_at + lanes + 64 * team, dp_mine = dp_at + lanes + 64 * team;
+        const uint32_t s_mine = s_at + lanes + S::MINE * team, dp_mine = dp_at + lanes + S::MINE * team;
         AtRing rb;
         for (int u = 0; u < steps; ++u)
         {
-            const int g = (lo + u) / per_head, i0 = (t0 + (lo + u) - g * per_head) * AT_TILE + 64 * team;
-            const float* lse = reinterpret_cast<const float*>(smem + S::STATS_AT + rb.slot * 1024) + 64 * team;
+            const int g = (lo + u) / per_head, i0 = (t0 + (lo + u) - g * per_head) * S::STEP + S::MINE * team;
+            const float* lse = reinterpret_cast<const float*>(smem + S::STATS_AT + rb.slot * 8 * S::STEP) + S::MINE * team;
             ok = at_warp_wait(&b.b_full[rb.slot], rb.lap & 1, give_up)
                  && at_warp_wait(&b.s_full[0], u & 1, give_up);
             if (!ok)
                 break;
             rb.next(S::B_SLOTS);
             tc_fence_after();
-            float w[64];
-            at_tmem_ld32(s_mine, w);
-            at_tmem_ld32(s_mine + 32, w + 32);
+            float w[S::MINE];
+            ab_fetch<S::MINE>(s_mine, w);
             at_tmem_wait_ld();
-            // this key is seen by the cells from `first` on of this team's 64
+            // this key is seen by the cells from `first` on of this team's
             const int first = p.causal ? j - p.offset - i0 : 0;
             const bool cut = __any_sync(~0u, first > 0);
 #pragma unroll
-            for (int c = 0; c < 64; c += 4)
+            for (int c = 0; c < S::MINE; c += 4)
             {
                 float l[4];
                 load_elems<4>(lse + c, l);
@@ -252,15 +296,15 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
             if (cut)
             {
 #pragma unroll
-                for (int c = 0; c < 64; ++c)
+                for (int c = 0; c < S::MINE; ++c)
                     w[c] = c >= first ? w[c] : 0.f;
             }
             {
-                uint32_t packed[32];
+                uint32_t packed[S::MINE / 2];
 #pragma unroll
-                for (int c = 0; c < 32; ++c)
+                for (int c = 0; c < S::MINE / 2; ++c)
                     packed[c] = pack_bf16(w[2 * c], w[2 * c + 1]);
-                at_tmem_st32(s_mine, packed);
+                ab_put<S::MINE / 2>(s_mine, packed);
             }
             at_tmem_wait_st();
             at_warp_arrive(&b.p_ready, lane);
@@ -269,14 +313,13 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
             if (!ok)
                 break;
             tc_fence_after();
-            float d[64];
-            at_tmem_ld32(dp_mine, d);
-            at_tmem_ld32(dp_mine + 32, d + 32);
+            float d[S::MINE];
+            ab_fetch<S::MINE>(dp_mine, d);
             at_tmem_wait_ld();
-            const float* delta = lse + 128;
-            uint32_t packed[32];
+            const float* delta = lse + S::STEP;
+            uint32_t packed[S::MINE / 2];
 #pragma unroll
-            for (int c = 0; c < 64; c += 4)
+            for (int c = 0; c < S::MINE; c += 4)
             {
                 float l[4];
                 load_elems<4>(delta + c, l);
@@ -289,10 +332,10 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
             if (cut)
             {
 #pragma unroll
-                for (int c = 0; c < 32; ++c)
+                for (int c = 0; c < S::MINE / 2; ++c)
                     packed[c] = 2 * c >= first ? packed[c] : 2 * c + 1 >= first ? packed[c] & 0xffff0000u : 0u;
             }
-            at_tmem_st32(dp_mine, packed);
+            ab_put<S::MINE / 2>(dp_mine, packed);
             at_tmem_wait_st();
             at_warp_arrive(&b.ds_ready, lane);
         }
@@ -311,11 +354,11 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
                          p.scale / ATTN_LOG2E, gone, steps == 0, dk_at + lanes, 0, D);
         }
     }
-    at_finish(ok, ex.status, warp, lane, tmem);
+    at_finish<S::COLUMNS>(ok, ex.status, warp, lane, tmem);
 }
 
 template <int D>
-__global__ void __launch_bounds__(AT_THREADS, 1)
+__global__ void __launch_bounds__(AT_THREADS, AbShape<D>::BLOCKS)
     attn_tc_dq_kernel(const __grid_constant__ AttnProblem p, const __grid_constant__ AtMaps maps,
                       const __grid_constant__ AtExtra ex)
 {
@@ -329,30 +372,30 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
         return;
 
     long long at = blockIdx.x;
-    const int tiles_k = attn_tiles(p.sk, AT_TILE), tiles_q = attn_tiles(p.sq, AT_TILE);
+    const int steps_k = attn_tiles(p.sk, S::STEP), tiles_q = attn_tiles(p.sq, AT_TILE);
     const int tile = tiles_q - 1 - (int) (at % tiles_q); // causal: the longest walks first
     at /= tiles_q;
     const int split = (int) (at % p.kv_splits);
     const long long nh = at / p.kv_splits, n = nh / p.q_heads;
     const int head = (int) (nh - n * p.q_heads), kv_head = head / p.group;
     const int i0 = tile * AT_TILE;
-    const int lo = (int) ((long long) tiles_k * split / p.kv_splits);
-    int hi = (int) ((long long) tiles_k * (split + 1) / p.kv_splits);
+    const int lo = (int) ((long long) steps_k * split / p.kv_splits);
+    int hi = (int) ((long long) steps_k * (split + 1) / p.kv_splits);
     if (p.causal)
-        hi = (int) min((long long) hi, max(0ll, (long long) i0 + AT_TILE - 1 + p.offset + AT_TILE) / AT_TILE);
+        hi = (int) min((long long) hi, max(0ll, (long long) i0 + AT_TILE - 1 + p.offset + S::STEP) / S::STEP);
     const int steps = max(0, hi - lo);
 
-    ab_init(b, warp);
+    ab_init<S::COLUMNS>(b, warp);
     const uint32_t tmem = __shfl_sync(~0u, b.tmem, 0); // known to be uniform
     const uint32_t* bits = ex.kv_bits ? ex.kv_bits + n * ex.words : nullptr;
     const float* stats = p.stats;
     wait_for_previous_kernel(bits, stats);
     bool ok = true;
-    const uint32_t s_at = tmem, dp_at = tmem + 256, dq_at = tmem + 384;
+    const uint32_t s_at = tmem, dp_at = tmem + S::DQ_DP, dq_at = tmem + S::DQ_DQ;
 
     if (warp >= AT_MMA_WARP)
     {
-        at_fewer_registers<AT_OTHER_REGS>();
+        at_fewer_registers<S::OTHER_REGS>();
         if (warp == AT_TMA_WARP)
         {
             if (lane == 0 && steps > 0)
@@ -370,10 +413,10 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
                         ok = mbar_wait_t<20>(&empty[r.slot], (r.lap - 1) & 1, give_up);
                     if (!ok)
                         break;
-                    mbar_expect_tx(&full[r.slot], AtTile<D>::BYTES);
-                    at_tma_tile<D>(base + (u & 1 ? S::B_AT : S::A_AT) + r.slot * AtTile<D>::BYTES,
-                                   u & 1 ? &maps.v : &maps.k, (lo + (u >> 1)) * AT_TILE, kv_head, (int) n,
-                                   &full[r.slot]);
+                    mbar_expect_tx(&full[r.slot], S::BYTES);
+                    at_tma_cells<D, S::STEP>(base + (u & 1 ? S::B_AT : S::A_AT) + r.slot * S::BYTES,
+                                             u & 1 ? &maps.v : &maps.k, (lo + (u >> 1)) * S::STEP, kv_head, (int) n,
+                                             &full[r.slot]);
                     r.next(slots);
                 }
                 if (!ok || *give_up)
@@ -401,7 +444,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
                     if (!ok)
                         return;
                     tc_fence_after();
-                    at_scores<D, 128>(s_at + 128 * (ahead & 1), q_at, base + S::A_AT + ra.slot * AtTile<D>::BYTES, ksteps, elected);
+                    at_scores<D, S::STEP>(s_at + S::STEP * (ahead & 1), q_at, base + S::A_AT + ra.slot * S::BYTES, ksteps, elected);
                     at_commit(&b.s_full[ahead & 1], elected);
                     ++ahead;
                     ra.next(S::A_SLOTS);
@@ -411,7 +454,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
                     if (!ok)
                         return;
                     tc_fence_after();
-                    at_scores<D, 128>(dp_at, do_at, base + S::B_AT + rb.slot * AtTile<D>::BYTES, ksteps, elected);
+                    at_scores<D, S::STEP>(dp_at, do_at, base + S::B_AT + rb.slot * S::BYTES, ksteps, elected);
                     at_commit(&b.dp_full, elected);
                     at_commit(&b.b_empty[rb.slot], elected);
                     rb.next(S::B_SLOTS);
@@ -427,9 +470,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
                     if (!ok)
                         break;
                     tc_fence_after();
-                    for (int h = 0; h < 2; ++h)
-                        at_weigh<D>(dq_at, dp_at + 64 * h, base + S::A_AT + k_slot * AtTile<D>::BYTES + h * AtTile<D>::HALF, width,
-                                    u == 0 && h == 0, elected);
+                    ab_weigh<D>(dq_at, dp_at, base + S::A_AT + k_slot * S::BYTES, width, u == 0, elected);
                     at_commit(&b.a_empty[k_slot], elected);
                     k_slot = k_slot + 1 == S::A_SLOTS ? 0 : k_slot + 1;
                     if (u + 1 < steps)
@@ -446,40 +487,38 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
     }
     else
     {
-        at_more_registers<AT_TEAM_REGS>();
+        at_more_registers<S::TEAM_REGS>();
         const int team = warp >> 2;
         const uint32_t lanes = (uint32_t) (warp & 3) << 21;
         const int i = i0 + (threadIdx.x & 127);
-        const uint32_t dp_mine = dp_at + lanes + 64 * team;
+        const uint32_t dp_mine = dp_at + lanes + S::MINE * team;
         const float* row = stats + nh * p.stats_pitch + i; // up to a multiple of 128 cells
         const float lse = row[0], delta = row[(long long) p.n * p.q_heads * p.stats_pitch];
         for (int u = 0; u < steps; ++u)
         {
-            const int j0 = (lo + u) * AT_TILE + 64 * team;
-            const uint32_t s_mine = s_at + lanes + 128 * (u & 1) + 64 * team;
+            const int j0 = (lo + u) * S::STEP + S::MINE * team;
+            const uint32_t s_mine = s_at + lanes + S::STEP * (u & 1) + S::MINE * team;
             ok = at_warp_wait(&b.s_full[u & 1], (u >> 1) & 1, give_up);
             if (!ok)
                 break;
             tc_fence_after();
-            float w[64];
-            at_tmem_ld32(s_mine, w);
-            at_tmem_ld32(s_mine + 32, w + 32);
+            float w[S::MINE];
+            ab_fetch<S::MINE>(s_mine, w);
             at_tmem_wait_ld();
 #pragma unroll
-            for (int c = 0; c < 64; ++c)
+            for (int c = 0; c < S::MINE; ++c)
                 w[c] = at_exp2(fmaf(w[c], p.scale, -lse));
             ok = at_warp_wait(&b.dp_full, u & 1, give_up);
             if (!ok)
                 break;
             tc_fence_after();
-            float d[64];
-            at_tmem_ld32(dp_mine, d);
-            at_tmem_ld32(dp_mine + 32, d + 32);
+            float d[S::MINE];
+            ab_fetch<S::MINE>(dp_mine, d);
             at_tmem_wait_ld();
-            uint32_t see[2];
+            uint32_t see[S::MINE / 32];
             bool all = true;
 #pragma unroll
-            for (int k = 0; k < 2; ++k)
+            for (int k = 0; k < S::MINE / 32; ++k)
             {
                 see[k] = at_there(p, bits, j0, k);
                 if (p.causal)
@@ -487,19 +526,19 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
                 all = all && see[k] == ~0u;
             }
 #pragma unroll
-            for (int c = 0; c < 64; ++c)
+            for (int c = 0; c < S::MINE; ++c)
                 d[c] = w[c] * (d[c] - delta);
             if (__any_sync(~0u, !all))
             {
 #pragma unroll
-                for (int c = 0; c < 64; ++c)
+                for (int c = 0; c < S::MINE; ++c)
                     d[c] = see[c >> 5] >> (c & 31) & 1 ? d[c] : 0.f;
             }
-            uint32_t packed[32];
+            uint32_t packed[S::MINE / 2];
 #pragma unroll
-            for (int c = 0; c < 32; ++c)
+            for (int c = 0; c < S::MINE / 2; ++c)
                 packed[c] = pack_bf16(d[2 * c], d[2 * c + 1]);
-            at_tmem_st32(dp_mine, packed);
+            ab_put<S::MINE / 2>(dp_mine, packed);
             at_tmem_wait_st();
             at_warp_arrive(&b.ds_ready, lane);
         }
@@ -513,7 +552,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
                      dq_at + lanes, team * (D / 2), (team + 1) * (D / 2));
         }
     }
-    at_finish(ok, ex.status, warp, lane, tmem);
+    at_finish<S::COLUMNS>(ok, ex.status, warp, lane, tmem);
 }
 
 template <int D>
