@@ -18,8 +18,9 @@ __global__ void __launch_bounds__(256) attn_join_fwd_kernel(AttnProblem p)
         const int i = (int) (at - row * p.sq), c = (int) (row - nh * p.d);
         const float* ml = p.part_ml + nh * p.sq + i;
         const long long step = 2 * heads * p.sq;
+        const bool gone = p.q_mask && !p.q_mask[n * p.sq + i]; // its parts were not written
         float m = -INFINITY;
-        for (int s = 0; s < p.kv_splits; ++s)
+        for (int s = 0; s < p.kv_splits && !gone; ++s)
             m = fmaxf(m, ml[s * step]);
         float l = 0.f, o = 0.f;
         if (m != -INFINITY)
@@ -29,7 +30,7 @@ __global__ void __launch_bounds__(256) attn_join_fwd_kernel(AttnProblem p)
                 l = fmaf(ml[s * step + heads * p.sq], f, l);
                 o = fmaf(p.part_o[s * total + at], f, o);
             }
-        const bool none = l == 0.f || (p.q_mask && !p.q_mask[n * p.sq + i]);
+        const bool none = l == 0.f;
         const float v[1] = {none ? 0.f : o / l};
         store_elems<1>(static_cast<T*>(p.o.p) + n * p.o.sn + ((nh - n * p.q_heads) * p.d + c) * p.o.sc + i, v);
         if (c == 0)
@@ -40,50 +41,80 @@ __global__ void __launch_bounds__(256) attn_join_fwd_kernel(AttnProblem p)
 // Adds up the parts of a gradient in order.
 template <class T>
 __global__ void __launch_bounds__(256) attn_join_grad_kernel(const float* part, int splits, AttnTensor t, int n,
-                                                             int heads, int d, int cells)
+                                                             int heads, int d, int cells, const uint8_t* mask)
 {
-    wait_for_previous_kernel(part);
+    wait_for_previous_kernel(part, mask);
     const long long total = (long long) n * heads * d * cells;
     for (long long at = (long long) blockIdx.x * 256 + threadIdx.x; at < total; at += (long long) gridDim.x * 256)
     {
         float v[1] = {0.f};
-        for (int s = 0; s < splits; ++s)
-            v[0] += part[s * total + at];
         const long long row = at / cells, b = row / ((long long) heads * d);
+        if (!mask || mask[b * cells + (at - row * cells)])
+            for (int s = 0; s < splits; ++s)
+                v[0] += part[s * total + at];
         store_elems<1>(static_cast<T*>(t.p) + b * t.sn + (row - b * heads * d) * t.sc + (at - row * cells), v);
     }
 }
 
+constexpr int ATTN_STATS_CELLS = 64, ATTN_STATS_WARPS = 8; // of a block: two cells a lane, an eighth of the channels a warp
+
 // stats: lse in powers of two and delta = sum_c o d_o; a cell that takes no part has +infinity and 0, so that its
-// weights are exp2(s - infinity) = 0.
+// weights are exp2(s - infinity) = 0.  (With a thread a cell, a load after the other, 2 x 4096 cells, 8 heads of 64
+// channels took 19 us.)
 template <class T>
-__global__ void __launch_bounds__(128) attn_stats_kernel(AttnProblem p)
+__global__ void __launch_bounds__(32 * ATTN_STATS_WARPS) attn_stats_kernel(AttnProblem p)
 {
+    __shared__ float part[ATTN_STATS_WARPS][ATTN_STATS_CELLS];
     wait_for_previous_kernel(p.lse);
-    const long long heads = (long long) p.n * p.q_heads, total = heads * p.stats_pitch;
-    for (long long at = (long long) blockIdx.x * 128 + threadIdx.x; at < total; at += (long long) gridDim.x * 128)
+    dependents_may_start();
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const long long heads = (long long) p.n * p.q_heads;
+    const int chunks = (int) ((p.stats_pitch + ATTN_STATS_CELLS - 1) / ATTN_STATS_CELLS);
+    for (long long at = blockIdx.x; at < heads * chunks; at += gridDim.x)
     {
-        const long long nh = at / p.stats_pitch, n = nh / p.q_heads;
-        const int i = (int) (at - nh * p.stats_pitch);
-        const float lse = i < p.sq ? p.lse[nh * p.sq + i] : -INFINITY;
-        float delta = 0.f;
-        const bool none = lse == -INFINITY || (p.q_mask && !p.q_mask[n * p.sq + i]);
-        if (!none)
+        const long long nh = at / chunks, n = nh / p.q_heads, first = (nh - n * p.q_heads) * p.d;
+        const int i0 = (int) (at - nh * chunks) * ATTN_STATS_CELLS;
+        const int* index = p.q_side.index ? p.q_side.index + n * p.sq : nullptr;
+        const int count = index ? p.q_side.count[n] : p.sq;
+        const T* o = static_cast<const T*>(p.o.p) + n * p.o.sn + first * p.o.sc;
+        const T* g = static_cast<const T*>(p.d_o.p) + n * p.d_o.sn + first * p.d_o.sc;
+        bool there[2];
+        int cell[2];
+        float sum[2] = {0.f, 0.f};
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
         {
-            const long long first = (nh - n * p.q_heads) * p.d;
-            const T* o = static_cast<const T*>(p.o.p) + n * p.o.sn + first * p.o.sc + i;
-            const T* g = static_cast<const T*>(p.d_o.p) + n * p.d_o.sn + first * p.d_o.sc + i;
-#pragma unroll 8
-            for (int c = 0; c < p.d; ++c)
-            {
-                float a[1], b[1];
-                load_elems<1>(o + c * p.o.sc, a);
-                load_elems<1>(g + c * p.d_o.sc, b);
-                delta = fmaf(a[0], b[0], delta);
-            }
+            const int r = i0 + lane + 32 * e;
+            there[e] = r < count;
+            cell[e] = there[e] && index ? index[r] : r;
         }
-        p.stats[at] = none ? INFINITY : lse * ATTN_LOG2E;
-        p.stats[total + at] = delta;
+#pragma unroll 4
+        for (int c = warp; c < p.d; c += ATTN_STATS_WARPS)
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+                if (there[e])
+                {
+                    float a[1], b[1];
+                    load_elems<1>(o + c * p.o.sc + cell[e], a);
+                    load_elems<1>(g + c * p.d_o.sc + cell[e], b);
+                    sum[e] = fmaf(a[0], b[0], sum[e]);
+                }
+        part[warp][lane] = sum[0];
+        part[warp][lane + 32] = sum[1];
+        __syncthreads();
+        const int i = i0 + (int) threadIdx.x;
+        if (threadIdx.x < ATTN_STATS_CELLS && i < p.stats_pitch)
+        {
+            float delta = 0.f;
+            for (int w = 0; w < ATTN_STATS_WARPS; ++w)
+                delta += part[w][threadIdx.x];
+            const int at_cell = i < count && index ? index[i] : i;
+            const float lse = i < count ? p.lse[nh * p.sq + at_cell] : -INFINITY;
+            const bool none = lse == -INFINITY || (p.q_mask && !p.q_mask[n * p.sq + at_cell]);
+            p.stats[nh * p.stats_pitch + i] = none ? INFINITY : lse * ATTN_LOG2E;
+            p.stats[heads * p.stats_pitch + nh * p.stats_pitch + i] = none ? 0.f : delta;
+        }
+        __syncthreads();
     }
 }
 
@@ -223,7 +254,15 @@ int64_t attn_carve(AttnProblem* p, int32_t dtype, bool backward, void* workspace
         p->copy_k = copy(kh, p->sk);
         p->copy_v = copy(kh, p->sk);
         p->copy_do = backward ? copy(qh, p->sq) : nullptr;
-        p->bits = reinterpret_cast<uint32_t*>(w.floats((long long) p->n * 4 * attn_tiles(p->sk, 128)));
+        const auto side = [&](int cells, bool masked) {
+            AttnSide t;
+            t.index = reinterpret_cast<int*>(w.floats((long long) p->n * cells));
+            t.before = reinterpret_cast<int*>(w.floats((long long) p->n * (cells + 1)));
+            t.count = reinterpret_cast<int*>(w.floats(p->n));
+            return masked ? t : AttnSide{};
+        };
+        p->q_side = side(p->sq, p->q_mask != nullptr);
+        p->kv_side = side(p->sk, p->kv_mask != nullptr);
     }
     if (!backward)
     {
@@ -258,12 +297,12 @@ int32_t attn_workspace(AttnProblem* p, int32_t dtype, bool backward, void* works
 }
 
 int32_t attn_join_grad(int32_t dtype, const float* part, int splits, const AttnTensor& t, int n, int heads, int d,
-                       int cells, cudaStream_t s)
+                       int cells, const uint8_t* mask, cudaStream_t s)
 {
     return with_type(dtype, [&](auto e) -> int32_t {
         DCB_CUDA_TRY(launch_overlapped(attn_join_grad_kernel<decltype(e)>,
                                        dim3(flat_blocks((long long) n * heads * d * cells, 256)), 256, 0, s, part,
-                                       splits, t, n, heads, d, cells));
+                                       splits, t, n, heads, d, cells, mask));
         return DCB_OK;
     });
 }
@@ -312,6 +351,9 @@ int32_t dcb_attention_fwd(const dcb_attention_desc* ad, const dcb_nd_desc* qd, c
                          (long long) p.n * p.q_heads * p.sq, s);
     if (int32_t e = attn_workspace(&p, ad->dtype, false, workspace, workspace_bytes))
         return e;
+    if (ad->dtype == DCB_BF16)
+        if (int32_t e = attn_tc_index(p, s))
+            return e;
     if (int32_t e = ad->dtype == DCB_BF16 ? attn_tc_fwd(p, s) : attn_simt_fwd(p, s))
         return e;
     if (p.kv_splits == 1)
@@ -361,10 +403,16 @@ int32_t dcb_attention_bwd(const dcb_attention_desc* ad, const dcb_nd_desc* qd, c
     p.kv_mask = static_cast<const uint8_t*>(kv_mask);
     if (int32_t e = attn_workspace(&p, ad->dtype, true, workspace, workspace_bytes))
         return e;
+    if (ad->dtype == DCB_BF16)
+        if (int32_t err = attn_tc_index(p, s))
+            return err;
     const int32_t e = with_type(ad->dtype, [&](auto t) -> int32_t {
         DCB_CUDA_TRY(launch_overlapped(attn_stats_kernel<decltype(t)>,
-                                       dim3(flat_blocks((long long) p.n * p.q_heads * p.stats_pitch, 128)), 128, 0, s,
-                                       p));
+                                       dim3((unsigned) std::min<long long>(
+                                           (long long) p.n * p.q_heads
+                                               * ((p.stats_pitch + ATTN_STATS_CELLS - 1) / ATTN_STATS_CELLS),
+                                           8ll * num_sms())),
+                                       32 * ATTN_STATS_WARPS, 0, s, p));
         return DCB_OK;
     });
     if (e)
@@ -373,13 +421,13 @@ int32_t dcb_attention_bwd(const dcb_attention_desc* ad, const dcb_nd_desc* qd, c
         return err;
     if (p.q_splits > 1)
     {
-        if (int32_t err = attn_join_grad(ad->dtype, p.part_dk, p.q_splits, p.dk, p.n, p.kv_heads, p.d, p.sk, s))
+        if (int32_t err = attn_join_grad(ad->dtype, p.part_dk, p.q_splits, p.dk, p.n, p.kv_heads, p.d, p.sk, p.kv_mask, s))
             return err;
-        if (int32_t err = attn_join_grad(ad->dtype, p.part_dv, p.q_splits, p.dv, p.n, p.kv_heads, p.d, p.sk, s))
+        if (int32_t err = attn_join_grad(ad->dtype, p.part_dv, p.q_splits, p.dv, p.n, p.kv_heads, p.d, p.sk, p.kv_mask, s))
             return err;
     }
     if (p.kv_splits > 1)
-        return attn_join_grad(ad->dtype, p.part_dq, p.kv_splits, p.dq, p.n, p.q_heads, p.d, p.sq, s);
+        return attn_join_grad(ad->dtype, p.part_dq, p.kv_splits, p.dq, p.n, p.q_heads, p.d, p.sq, p.q_mask, s);
     return DCB_OK;
 }
 

@@ -19,6 +19,13 @@ struct AttnTensor
     long long sn, sc; // element strides of samples and channels
 };
 
+// The cells of a side that a mask leaves, for the tensor-core kernels: they see those cells only, one after the other.
+// Per sample the cells' indices, how many lie before a cell, how many there are.  Null without a mask.
+struct AttnSide
+{
+    int *index, *before, *count; // [n][cells], [n][cells + 1], [n]
+};
+
 struct AttnProblem
 {
     int n, q_heads, kv_heads, group; // group = query heads of a key head
@@ -30,17 +37,17 @@ struct AttnProblem
     const uint8_t *q_mask, *kv_mask;
     float* lse;                      // [n][q_heads][sq]
     // Backward: lse in powers of two (+infinity where a cell sees nothing) and sum_d o d_o,
-    // [2][n * q_heads][stats_pitch], +infinity and 0 behind the last cell.
+    // [2][n * q_heads][stats_pitch], +infinity and 0 behind the last cell (of q_side, where there is one).
     float* stats;
     long long stats_pitch;
     // Parts of a split axis, joined by a kernel of their own:
     //   forward  [splits][n * q_heads][d][sq] sums and [splits][2][n * q_heads][sq] maxima, sums of weights
     //   backward [splits][n * heads][d][cells] sums
     float *part_o, *part_ml, *part_dq, *part_dk, *part_dv;
-    // Tensor cores: copies of tensors that bulk copies cannot address or whose masked cells have to be zeros, [n][heads *
-    // d][pitch] with rows of whole 16 bytes, and the keys' mask as bits.
+    // Tensor cores: what the masks leave, and copies of tensors that bulk copies cannot address or whose cells a mask
+    // picks, [n][heads * d][pitch] with rows of whole 16 bytes.
+    AttnSide q_side, kv_side;
     bf16 *copy_q, *copy_k, *copy_v, *copy_do;
-    uint32_t* bits;
     int q_splits, kv_splits; // of the queries' axis (dk, dv), of the keys' axis (o, dq)
 };
 
@@ -58,6 +65,7 @@ inline int attn_splits(long long work, int steps, long long slots, int least)
 }
 
 // Kernels of attention_tc.cu (bf16) and attention_simt.cu (fp32).
+int32_t attn_tc_index(const AttnProblem& p, cudaStream_t stream); // fills the sides; before the others
 int32_t attn_tc_fwd(const AttnProblem& p, cudaStream_t stream);
 int32_t attn_tc_bwd(const AttnProblem& p, cudaStream_t stream);
 void attn_tc_splits(AttnProblem* p, bool backward);

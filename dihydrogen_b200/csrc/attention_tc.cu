@@ -9,65 +9,145 @@ namespace
 
 __device__ int at_status_word; // a kernel gave up on a wait
 
-constexpr int AT_JOBS = 4;
+constexpr int AT_JOBS = 7;
+constexpr int AT_INDEX_THREADS = 1024, AT_INDEX_CELLS = 8; // cells of a thread at a time
 
-// Copies with rows of whole 16 bytes; cells that a mask takes out, and those behind the last, as zeros.
-struct AtCopy
+// What a mask leaves of a sample's cells, in order.  A block a sample and side.
+__global__ void __launch_bounds__(AT_INDEX_THREADS) attn_index_kernel(const __grid_constant__ AttnProblem p)
 {
+    __shared__ int of_warp[32];
+    __shared__ int all;
+    const uint8_t* mask = blockIdx.y ? p.kv_mask : p.q_mask;
+    const AttnSide side = blockIdx.y ? p.kv_side : p.q_side;
+    const int cells = blockIdx.y ? p.sk : p.sq;
+    if (!mask)
+        return;
+    wait_for_previous_kernel(mask);
+    dependents_may_start();
+    const long long n = blockIdx.x;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    mask += n * cells;
+    int* index = side.index + n * cells;
+    int* before = side.before + n * (cells + 1ll);
+    int base = 0;
+    for (long long c0 = 0; c0 < cells; c0 += AT_INDEX_THREADS * AT_INDEX_CELLS)
+    {
+        const long long i0 = c0 + threadIdx.x * AT_INDEX_CELLS;
+        uint32_t bits = 0;
+        for (int e = 0; e < AT_INDEX_CELLS; ++e)
+            if (i0 + e < cells && mask[i0 + e])
+                bits |= 1u << e;
+        const int mine = __popc(bits);
+        int sum = mine; // of this lane and those before
+        for (int h = 1; h < 32; h *= 2)
+        {
+            const int other = __shfl_up_sync(~0u, sum, h);
+            sum += lane >= h ? other : 0;
+        }
+        if (lane == 31)
+            of_warp[warp] = sum;
+        __syncthreads();
+        if (warp == 0)
+        {
+            int w = of_warp[lane];
+            for (int h = 1; h < 32; h *= 2)
+            {
+                const int other = __shfl_up_sync(~0u, w, h);
+                w += lane >= h ? other : 0;
+            }
+            of_warp[lane] = w;
+            if (lane == 31)
+                all = w;
+        }
+        __syncthreads();
+        int at = base + sum - mine + (warp > 0 ? of_warp[warp - 1] : 0);
+        for (int e = 0; e < AT_INDEX_CELLS; ++e)
+            if (i0 + e < cells)
+            {
+                before[i0 + e] = at;
+                if (bits >> e & 1)
+                    index[at++] = (int) (i0 + e);
+            }
+        base += all;
+        __syncthreads();
+    }
+    if (threadIdx.x == 0)
+    {
+        before[cells] = base;
+        side.count[n] = base;
+    }
+}
+
+// AT_COPY: a copy with rows of whole 16 bytes, of the cells that a mask leaves; zeros behind the last.
+// AT_ZERO: zeros in the cells that a mask takes out.  AT_LSE: their lse.
+enum AtJobKind
+{
+    AT_COPY,
+    AT_ZERO,
+    AT_LSE
+};
+
+struct AtJob
+{
+    AtJobKind kind;
     const bf16* from;
     bf16* to;
+    float* lse;
     long long sn, sc;
     const uint8_t* mask;
-    int channels, cells;
-    long long units; // of 8 cells, all samples
+    AttnSide side;
+    int channels, cells; // rows of a sample
+    int chunks;          // of 256 cells a row: a warp each
 };
 
 struct AtPrepare
 {
-    AtCopy job[AT_JOBS];
+    AtJob job[AT_JOBS];
     int jobs;
-    const uint8_t* mask; // to bits
-    uint32_t* bits;
-    int cells;
-    long long words, words_total;
+    int n;
 };
 
 __global__ void __launch_bounds__(256) attn_prepare_kernel(const __grid_constant__ AtPrepare a)
 {
-    const uint8_t* mask = a.mask;
-    wait_for_previous_kernel(mask);
+    const AtJob& c = a.job[blockIdx.y];
+    const bf16* source = c.from;
+    wait_for_previous_kernel(source);
     dependents_may_start();
-    const long long step = (long long) gridDim.x * 256, first = (long long) blockIdx.x * 256 + threadIdx.x;
-    if (blockIdx.y == (unsigned) a.jobs)
+    const int lane = threadIdx.x & 31;
+    const long long total = (long long) a.n * c.channels * c.chunks;
+    const int pitch = (c.cells + 7) / 8 * 8;
+    for (long long u = (long long) blockIdx.x * 8 + (threadIdx.x >> 5); u < total; u += (long long) gridDim.x * 8)
     {
-        for (long long w = first; w < a.words_total; w += step)
+        const long long row = u / c.chunks, n = row / c.channels;
+        const long long first = n * c.sn + (row - n * c.channels) * c.sc;
+        const int i0 = (int) (u - row * c.chunks) * 256 + lane;
+        if (c.kind == AT_COPY)
         {
-            const long long n = w / a.words;
-            const long long j0 = (w - n * a.words) * 32;
-            uint32_t bits = 0;
-            for (int e = 0; e < 32; ++e)
-                if (j0 + e < a.cells && mask[n * a.cells + j0 + e])
-                    bits |= 1u << e;
-            a.bits[w] = bits;
-        }
-        return;
-    }
-    const AtCopy& c = a.job[blockIdx.y];
-    const int per_row = (c.cells + 7) / 8;
-    for (long long u = first; u < c.units; u += step)
-    {
-        const long long row = u / per_row, n = row / c.channels;
-        const int i0 = (int) (u - row * per_row) * 8;
-        const bf16* from = c.from + n * c.sn + (row - n * c.channels) * c.sc + i0;
-        uint32_t v[4];
+            const int count = c.side.index ? c.side.count[n] : c.cells;
+            uint16_t v[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e)
-        {
-            const bool there = i0 + e < c.cells && (!c.mask || c.mask[n * c.cells + i0 + e]);
-            const uint32_t x = there ? reinterpret_cast<const uint16_t*>(from)[e] : 0u;
-            v[e / 2] = e & 1 ? v[e / 2] | x << 16 : x;
+            for (int e = 0; e < 8; ++e)
+            {
+                const int i = i0 + 32 * e;
+                const int cell = i < count && c.side.index ? c.side.index[n * c.cells + i] : i;
+                v[e] = i < count ? reinterpret_cast<const uint16_t*>(source)[first + cell] : (uint16_t) 0;
+            }
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (i0 + 32 * e < pitch)
+                    reinterpret_cast<uint16_t*>(c.to)[row * pitch + i0 + 32 * e] = v[e];
         }
-        reinterpret_cast<uint4*>(c.to)[u] = make_uint4(v[0], v[1], v[2], v[3]);
+        else
+            for (int e = 0; e < 8; ++e)
+            {
+                const int i = i0 + 32 * e;
+                if (i >= c.cells || c.mask[n * c.cells + i])
+                    continue;
+                if (c.kind == AT_ZERO)
+                    reinterpret_cast<uint16_t*>(c.to)[first + i] = 0;
+                else
+                    c.lse[row * c.cells + i] = -INFINITY;
+            }
     }
 }
 
@@ -78,23 +158,40 @@ struct AtHost
     AtExtra ex = {};
 };
 
-// The tensor as bulk copies see it, copied first where they cannot or where masked cells have to be zeros.
-int32_t at_operand(const AttnProblem& p, const AttnTensor& t, int heads, int cells, const uint8_t* zeros, bf16* copy,
+void at_job(AtHost* h, const AtJob& job)
+{
+    h->prepare.job[h->prepare.jobs++] = job;
+}
+
+int at_chunks(int cells)
+{
+    return (cells + 255) / 256;
+}
+
+// A result's cells that its mask takes out.
+void at_zeros(const AttnTensor& t, int channels, int cells, const uint8_t* mask, AtHost* h)
+{
+    if (mask)
+        at_job(h, AtJob{AT_ZERO, nullptr, static_cast<bf16*>(t.p), nullptr, t.sn, t.sc, mask, {}, channels, cells,
+                        at_chunks(cells)});
+}
+
+// The tensor as bulk copies see it, copied first where they cannot or where a mask picks cells.
+int32_t at_operand(const AttnProblem& p, const AttnTensor& t, int heads, int cells, const AttnSide& side, bf16* copy,
                    int box_channels, AtHost* h, CUtensorMap* map)
 {
     const void* at = t.p;
     long long sc = t.sc, sn = t.sn;
     const bool fits = reinterpret_cast<uintptr_t>(at) % 16 == 0 && sc % 8 == 0 && (p.n == 1 || sn % 8 == 0) && sc > 0
                       && (p.n == 1 || sn > 0);
-    if (!fits || zeros)
+    if (!fits || side.index)
     {
         const int channels = heads * p.d;
-        const long long pitch = (cells + 7) / 8 * 8;
-        h->prepare.job[h->prepare.jobs++] = AtCopy{static_cast<const bf16*>(at), copy, sn, sc, zeros, channels, cells,
-                                                   (long long) p.n * channels * (pitch / 8)};
+        at_job(h, AtJob{AT_COPY, static_cast<const bf16*>(at), copy, nullptr, sn, sc, nullptr, side, channels, cells,
+                        at_chunks(cells)});
         at = copy;
-        sc = pitch;
-        sn = pitch * channels;
+        sc = (cells + 7) / 8 * 8;
+        sn = sc * channels;
     }
     const cuuint64_t dims[4] = {(cuuint64_t) cells, (cuuint64_t) p.d, (cuuint64_t) heads, (cuuint64_t) p.n};
     // a dimension of extent 1 may carry any stride; give it a valid one
@@ -119,24 +216,14 @@ int32_t at_prepare(const AttnProblem& p, AtHost* h, cudaStream_t stream)
     AtPrepare& a = h->prepare;
     h->ex.status = attn_tc_status();
     DCB_REQUIRE(h->ex.status, "no status word on this device");
-    if (p.kv_mask)
-    {
-        a.mask = p.kv_mask;
-        a.bits = p.bits;
-        a.cells = p.sk;
-        a.words = 4ll * attn_tiles(p.sk, AT_TILE);
-        a.words_total = a.words * p.n;
-        h->ex.kv_bits = p.bits;
-        h->ex.words = a.words;
-    }
-    const int rows = a.jobs + (p.kv_mask ? 1 : 0);
-    if (rows == 0)
+    if (a.jobs == 0)
         return DCB_OK;
-    long long units = a.words_total;
+    a.n = p.n;
+    long long warps = 0;
     for (int i = 0; i < a.jobs; ++i)
-        units = std::max(units, a.job[i].units);
-    const unsigned blocks = (unsigned) std::min<long long>((units + 255) / 256, 16ll * num_sms());
-    DCB_CUDA_TRY(launch_overlapped(attn_prepare_kernel, dim3(blocks, rows), 256, 0, stream, a));
+        warps = std::max(warps, (long long) a.n * a.job[i].channels * a.job[i].chunks);
+    const unsigned blocks = (unsigned) std::min<long long>((warps + 7) / 8, 16ll * num_sms());
+    DCB_CUDA_TRY(launch_overlapped(attn_prepare_kernel, dim3(blocks, a.jobs), 256, 0, stream, a));
     return DCB_OK;
 }
 
@@ -182,18 +269,30 @@ void attn_tc_splits(AttnProblem* p, bool backward)
         p->kv_splits = attn_splits(qh * (backward ? q_tiles : (q_tiles + 1) / 2), (int) k_tiles, slots, 2);
 }
 
+int32_t attn_tc_index(const AttnProblem& p, cudaStream_t stream)
+{
+    if (!p.q_mask && !p.kv_mask)
+        return DCB_OK;
+    DCB_CUDA_TRY(launch_overlapped(attn_index_kernel, dim3(p.n, 2), AT_INDEX_THREADS, 0, stream, p));
+    return DCB_OK;
+}
+
 int32_t attn_tc_fwd(const AttnProblem& p, cudaStream_t stream)
 {
     AtHost h;
     const int box = p.d <= 64 ? 64 : 128;
-    // masked keys have weight 0, but 0 times what they hold has to be 0: their values are copied as zeros
-    if (int32_t e = at_operand(p, p.q, p.q_heads, p.sq, nullptr, p.copy_q, box, &h, &h.maps.q))
+    if (int32_t e = at_operand(p, p.q, p.q_heads, p.sq, p.q_side, p.copy_q, box, &h, &h.maps.q))
         return e;
-    if (int32_t e = at_operand(p, p.k, p.kv_heads, p.sk, nullptr, p.copy_k, box, &h, &h.maps.k))
+    if (int32_t e = at_operand(p, p.k, p.kv_heads, p.sk, p.kv_side, p.copy_k, box, &h, &h.maps.k))
         return e;
-    if (int32_t e = at_operand(p, p.v, p.kv_heads, p.sk, p.kv_mask, p.copy_v, box, &h, &h.maps.v))
+    if (int32_t e = at_operand(p, p.v, p.kv_heads, p.sk, p.kv_side, p.copy_v, box, &h, &h.maps.v))
         return e;
     h.maps.d_o = h.maps.q;
+    if (p.q_mask && p.kv_splits == 1) // else the join writes them
+    {
+        at_zeros(p.o, p.q_heads * p.d, p.sq, p.q_mask, &h);
+        at_job(&h, AtJob{AT_LSE, nullptr, nullptr, p.lse, 0, 0, p.q_mask, {}, p.q_heads, p.sq, at_chunks(p.sq)});
+    }
     if (int32_t e = at_prepare(p, &h, stream))
         return e;
     return attn_tc_fwd_launch(p, h.maps, h.ex, stream);
@@ -203,15 +302,21 @@ int32_t attn_tc_bwd(const AttnProblem& p, cudaStream_t stream)
 {
     AtHost h;
     const int box = p.d <= 64 ? 64 : 128;
-    // whatever a gradient that is 0 is multiplied with has to be finite
-    if (int32_t e = at_operand(p, p.q, p.q_heads, p.sq, p.q_mask, p.copy_q, box, &h, &h.maps.q))
+    if (int32_t e = at_operand(p, p.q, p.q_heads, p.sq, p.q_side, p.copy_q, box, &h, &h.maps.q))
         return e;
-    if (int32_t e = at_operand(p, p.k, p.kv_heads, p.sk, p.kv_mask, p.copy_k, box, &h, &h.maps.k))
+    if (int32_t e = at_operand(p, p.k, p.kv_heads, p.sk, p.kv_side, p.copy_k, box, &h, &h.maps.k))
         return e;
-    if (int32_t e = at_operand(p, p.v, p.kv_heads, p.sk, nullptr, p.copy_v, box, &h, &h.maps.v))
+    if (int32_t e = at_operand(p, p.v, p.kv_heads, p.sk, p.kv_side, p.copy_v, box, &h, &h.maps.v))
         return e;
-    if (int32_t e = at_operand(p, p.d_o, p.q_heads, p.sq, p.q_mask, p.copy_do, box, &h, &h.maps.d_o))
+    if (int32_t e = at_operand(p, p.d_o, p.q_heads, p.sq, p.q_side, p.copy_do, box, &h, &h.maps.d_o))
         return e;
+    if (p.kv_splits == 1) // else the joins write them
+        at_zeros(p.dq, p.q_heads * p.d, p.sq, p.q_mask, &h);
+    if (p.q_splits == 1)
+    {
+        at_zeros(p.dk, p.kv_heads * p.d, p.sk, p.kv_mask, &h);
+        at_zeros(p.dv, p.kv_heads * p.d, p.sk, p.kv_mask, &h);
+    }
     if (int32_t e = at_prepare(p, &h, stream))
         return e;
     return attn_tc_bwd_launch(p, h.maps, h.ex, stream);

@@ -307,24 +307,43 @@ __device__ __forceinline__ void at_warp_arrive(uint64_t* bar, int lane)
         mbar_arrive(bar);
 }
 
-// Which of 128 cells from j0 on are there: 32 to a word.
-__device__ __forceinline__ uint32_t at_there(const AttnProblem& p, const uint32_t* bits, int j0, int w)
+// One sample's cells on one side, as the kernels count them: all, or those that a mask leaves.
+struct AtCells
 {
-    const int left = p.sk - (j0 + 32 * w);
-    if (bits)
-        return left > 0 ? bits[(j0 >> 5) + w] : 0u;
-    return left >= 32 ? ~0u : left <= 0 ? 0u : (1u << left) - 1u;
+    int count, cells;
+    const int *index, *counted;
+    __device__ __forceinline__ AtCells(const AttnSide& s, long long n, int cells_) : cells(cells_)
+    {
+        index = s.index ? s.index + n * cells : nullptr;
+        counted = s.index ? s.before + n * (cells + 1ll) : nullptr;
+        count = s.index ? s.count[n] : cells;
+    }
+    __device__ __forceinline__ int cell(int r) const { return index ? index[r] : r; }
+    // How many lie before cell x of the grid.
+    __device__ __forceinline__ int before(long long x) const
+    {
+        const int c = (int) (x < 0 ? 0 : x > cells ? cells : x);
+        return counted ? counted[c] : c;
+    }
+};
+
+// Row r of the queries sees the first so many keys; later rows see no fewer.
+__device__ __forceinline__ int at_limit(const AttnProblem& p, const AtCells& q, const AtCells& kv, int r)
+{
+    if (r < 0 || r >= q.count)
+        return 0;
+    return p.causal ? kv.before((long long) q.cell(r) + p.offset + 1) : kv.count;
 }
 
-// ... and up to cell j0 + last.
+// The columns up to `last` among 32, the w-th word from column 0 on.
 __device__ __forceinline__ uint32_t at_up_to(int last, int w)
 {
     const int left = last - 32 * w + 1;
     return left >= 32 ? ~0u : left <= 0 ? 0u : (1u << left) - 1u;
 }
 
-// Channels [c_lo, c_hi) of an accumulator's rows to a tensor ([channel][cell], this thread's cell is i), or as a part in
-// fp32.  nothing: no product was taken; zero: this row's result is 0 whatever it holds.
+// Channels [c_lo, c_hi) of an accumulator's rows to a tensor ([channel][cell], this thread's cell is i, negative: none), or
+// as a part in fp32.  nothing: no product was taken; zero: this row's result is 0 whatever it holds.
 __device__ __forceinline__ void at_store(const AttnTensor& t, float* part, long long nh, long long n, int head, int d,
                                          int i, int cells, float factor, bool zero, bool nothing, uint32_t taddr,
                                          int c_lo, int c_hi)
@@ -339,7 +358,7 @@ __device__ __forceinline__ void at_store(const AttnTensor& t, float* part, long 
             at_tmem_ld32(taddr + c0, v);
             at_tmem_wait_ld();
         }
-        if (i >= cells)
+        if (i < 0)
             continue;
 #pragma unroll
         for (int c = 0; c < 32; ++c)
@@ -361,8 +380,6 @@ struct AtMaps
 
 struct AtExtra
 {
-    const uint32_t* kv_bits; // mask of the keys, 32 to a word, [n][words]; null without a mask
-    long long words;
     int* status;
 };
 

@@ -134,25 +134,27 @@ __global__ void __launch_bounds__(AT_THREADS, AbShape<D>::BLOCKS)
         return;
 
     long long at = blockIdx.x;
-    const int tiles_k = attn_tiles(p.sk, AT_TILE), steps_q = attn_tiles(p.sq, S::STEP);
+    const int tiles_k = attn_tiles(p.sk, AT_TILE);
     const int tile = (int) (at % tiles_k); // causal: the first keys have the longest walks
     at /= tiles_k;
     const int split = (int) (at % p.q_splits);
     const long long nh = at / p.q_splits, n = nh / p.kv_heads;
     const int head = (int) (nh - n * p.kv_heads);
     const int j0 = tile * AT_TILE;
-    // the walk: steps of queries from t0 on, of every query head of the group
-    int t0 = 0;
-    if (p.causal)
-        t0 = (int) min((long long) steps_q, max(0ll, (long long) j0 - p.offset) / S::STEP);
-    const int per_head = steps_q - t0;
-    const long long all = (long long) per_head * p.group;
-    const int lo = (int) (all * split / p.q_splits), steps = (int) (all * (split + 1) / p.q_splits) - lo;
-
     ab_init<S::COLUMNS>(b, warp);
     const uint32_t tmem = __shfl_sync(~0u, b.tmem, 0); // known to be uniform
     const float* stats = p.stats;
     wait_for_previous_kernel(stats);
+    const AtCells q(p.q_side, n, p.sq), kv(p.kv_side, n, p.sk);
+    // a key is seen from this row of the queries on
+    const auto first_row = [&](int r) {
+        return r >= kv.count ? q.count : p.causal ? q.before((long long) kv.cell(r) - p.offset) : 0;
+    };
+    // the walk: steps of queries from t0 on, of every query head of the group
+    const int t0 = first_row(j0) / S::STEP;
+    const int per_head = max(0, attn_tiles(q.count, S::STEP) - t0);
+    const long long all = j0 < kv.count ? (long long) per_head * p.group : 0;
+    const int lo = (int) (all * split / p.q_splits), steps = (int) (all * (split + 1) / p.q_splits) - lo;
     bool ok = true;
     const uint32_t s_at = tmem, dp_at = tmem + S::DKV_DP, dv_at = tmem + S::DKV_DV, dk_at = tmem + S::DKV_DK;
 
@@ -265,7 +267,7 @@ __global__ void __launch_bounds__(AT_THREADS, AbShape<D>::BLOCKS)
         at_more_registers<S::TEAM_REGS>();
         const int team = warp >> 2;
         const uint32_t lanes = (uint32_t) (warp & 3) << 21;
-        const int j = j0 + (threadIdx.x & 127);
+        const int row = j0 + (threadIdx.x & 127), j = row < kv.count ? kv.cell(row) : -1, from = first_row(row);
         const uint32_t s_mine = s_at + lanes + S::MINE * team, dp_mine = dp_at + lanes + S::MINE * team;
         AtRing rb;
         for (int u = 0; u < steps; ++u)
@@ -282,7 +284,7 @@ __global__ void __launch_bounds__(AT_THREADS, AbShape<D>::BLOCKS)
             ab_fetch<S::MINE>(s_mine, w);
             at_tmem_wait_ld();
             // this key is seen by the cells from `first` on of this team's
-            const int first = p.causal ? j - p.offset - i0 : 0;
+            const int first = j < 0 ? 0 : from - i0;
             const bool cut = __any_sync(~0u, first > 0);
 #pragma unroll
             for (int c = 0; c < S::MINE; c += 4)
@@ -344,14 +346,13 @@ __global__ void __launch_bounds__(AT_THREADS, AbShape<D>::BLOCKS)
         tc_fence_after();
         if (ok)
         {
-            const bool gone = p.kv_mask && j < p.sk && !p.kv_mask[n * p.sk + j];
             const long long part = (long long) p.n * p.kv_heads * p.d * p.sk * split;
             if (team == 0)
-                at_store(p.dv, p.q_splits > 1 ? p.part_dv + part : nullptr, nh, n, head, p.d, j, p.sk, 1.f, gone,
+                at_store(p.dv, p.q_splits > 1 ? p.part_dv + part : nullptr, nh, n, head, p.d, j, p.sk, 1.f, false,
                          steps == 0, dv_at + lanes, 0, D);
             else
                 at_store(p.dk, p.q_splits > 1 ? p.part_dk + part : nullptr, nh, n, head, p.d, j, p.sk,
-                         p.scale / ATTN_LOG2E, gone, steps == 0, dk_at + lanes, 0, D);
+                         p.scale / ATTN_LOG2E, false, steps == 0, dk_at + lanes, 0, D);
         }
     }
     at_finish<S::COLUMNS>(ok, ex.status, warp, lane, tmem);
@@ -372,24 +373,24 @@ __global__ void __launch_bounds__(AT_THREADS, AbShape<D>::BLOCKS)
         return;
 
     long long at = blockIdx.x;
-    const int steps_k = attn_tiles(p.sk, S::STEP), tiles_q = attn_tiles(p.sq, AT_TILE);
+    const int tiles_q = attn_tiles(p.sq, AT_TILE);
     const int tile = tiles_q - 1 - (int) (at % tiles_q); // causal: the longest walks first
     at /= tiles_q;
     const int split = (int) (at % p.kv_splits);
     const long long nh = at / p.kv_splits, n = nh / p.q_heads;
     const int head = (int) (nh - n * p.q_heads), kv_head = head / p.group;
     const int i0 = tile * AT_TILE;
-    const int lo = (int) ((long long) steps_k * split / p.kv_splits);
-    int hi = (int) ((long long) steps_k * (split + 1) / p.kv_splits);
-    if (p.causal)
-        hi = (int) min((long long) hi, max(0ll, (long long) i0 + AT_TILE - 1 + p.offset + S::STEP) / S::STEP);
-    const int steps = max(0, hi - lo);
 
     ab_init<S::COLUMNS>(b, warp);
     const uint32_t tmem = __shfl_sync(~0u, b.tmem, 0); // known to be uniform
-    const uint32_t* bits = ex.kv_bits ? ex.kv_bits + n * ex.words : nullptr;
     const float* stats = p.stats;
-    wait_for_previous_kernel(bits, stats);
+    wait_for_previous_kernel(stats);
+    const AtCells q(p.q_side, n, p.sq), kv(p.kv_side, n, p.sk);
+    const int steps_k = attn_tiles(kv.count, S::STEP);
+    const int lo = (int) ((long long) steps_k * split / p.kv_splits);
+    const int hi = min((int) ((long long) steps_k * (split + 1) / p.kv_splits),
+                       attn_tiles(at_limit(p, q, kv, min(i0 + AT_TILE, q.count) - 1), S::STEP));
+    const int steps = i0 < q.count ? max(0, hi - lo) : 0;
     bool ok = true;
     const uint32_t s_at = tmem, dp_at = tmem + S::DQ_DP, dq_at = tmem + S::DQ_DQ;
 
@@ -490,9 +491,11 @@ __global__ void __launch_bounds__(AT_THREADS, AbShape<D>::BLOCKS)
         at_more_registers<S::TEAM_REGS>();
         const int team = warp >> 2;
         const uint32_t lanes = (uint32_t) (warp & 3) << 21;
-        const int i = i0 + (threadIdx.x & 127);
+        const int row0 = i0 + (warp & 3) * 32, r = row0 + lane;
+        const int i = r < q.count ? q.cell(r) : -1, limit = at_limit(p, q, kv, r);
+        const int open = max(0, at_limit(p, q, kv, row0) - lo * S::STEP) / S::STEP; // steps that all its rows see whole
         const uint32_t dp_mine = dp_at + lanes + S::MINE * team;
-        const float* row = stats + nh * p.stats_pitch + i; // up to a multiple of 128 cells
+        const float* row = stats + nh * p.stats_pitch + r; // up to a multiple of 128 cells
         const float lse = row[0], delta = row[(long long) p.n * p.q_heads * p.stats_pitch];
         for (int u = 0; u < steps; ++u)
         {
@@ -515,21 +518,15 @@ __global__ void __launch_bounds__(AT_THREADS, AbShape<D>::BLOCKS)
             float d[S::MINE];
             ab_fetch<S::MINE>(dp_mine, d);
             at_tmem_wait_ld();
-            uint32_t see[S::MINE / 32];
-            bool all = true;
-#pragma unroll
-            for (int k = 0; k < S::MINE / 32; ++k)
-            {
-                see[k] = at_there(p, bits, j0, k);
-                if (p.causal)
-                    see[k] &= at_up_to(i + p.offset - j0, k);
-                all = all && see[k] == ~0u;
-            }
 #pragma unroll
             for (int c = 0; c < S::MINE; ++c)
                 d[c] = w[c] * (d[c] - delta);
-            if (__any_sync(~0u, !all))
+            if (u >= open)
             {
+                uint32_t see[S::MINE / 32];
+#pragma unroll
+                for (int k = 0; k < S::MINE / 32; ++k)
+                    see[k] = at_up_to(limit - 1 - j0, k);
 #pragma unroll
                 for (int c = 0; c < S::MINE; ++c)
                     d[c] = see[c >> 5] >> (c & 31) & 1 ? d[c] : 0.f;

@@ -76,19 +76,6 @@ __global__ void __launch_bounds__(AT_THREADS, AfShape<D, APART>::BLOCKS)
     const long long nh = at / splits, n = nh / p.q_heads;
     const int head = (int) (nh - n * p.q_heads), kv_head = head / p.group;
     const int i0 = block_q * 2 * AT_TILE;
-    const int tiles = attn_tiles(p.sk, AT_TILE);
-    int lo[2], steps[2]; // of either team: first tile of keys, steps of 64 keys
-    for (int t = 0; t < 2; ++t)
-    {
-        const int part = APART ? 2 * split + t : split, first = APART ? 0 : i0 + t * AT_TILE;
-        lo[t] = (int) ((long long) tiles * part / p.kv_splits);
-        const int hi = (int) ((long long) tiles * (part + 1) / p.kv_splits);
-        int end = min(p.sk, hi * AT_TILE); // cells
-        if (p.causal)
-            end = (int) min((long long) end, max(0ll, (long long) first + AT_TILE + p.offset));
-        steps[t] = first < p.sq ? max(0, end - lo[t] * AT_TILE + 63) / 64 : 0;
-    }
-    const int most = max(steps[0], steps[1]);
     // K and V tiles in the order that they are needed in: number of team t's, of the j-th tile
     const auto k_number = [&](int t, int j) { return (uint32_t) (APART ? 4 * j + t : 2 * j); };
     const auto v_number = [&](int t, int j) { return (uint32_t) (APART ? 4 * j + 2 + t : 2 * j + 1); };
@@ -114,8 +101,20 @@ __global__ void __launch_bounds__(AT_THREADS, AfShape<D, APART>::BLOCKS)
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = __shfl_sync(~0u, b.tmem, 0); // known to be uniform
-    const uint32_t* bits = ex.kv_bits ? ex.kv_bits + n * ex.words : nullptr;
-    wait_for_previous_kernel(bits);
+    const int* p_index = p.q_side.count;
+    wait_for_previous_kernel(p_index); // the sides' counts
+    const AtCells q(p.q_side, n, p.sq), kv(p.kv_side, n, p.sk);
+    const int tiles = attn_tiles(kv.count, AT_TILE);
+    int lo[2], steps[2]; // of either team: first tile of keys, steps of 64 keys
+    for (int t = 0; t < 2; ++t)
+    {
+        const int part = APART ? 2 * split + t : split, first = APART ? 0 : i0 + t * AT_TILE;
+        lo[t] = (int) ((long long) tiles * part / p.kv_splits);
+        const int hi = (int) ((long long) tiles * (part + 1) / p.kv_splits);
+        const int end = min(hi * AT_TILE, at_limit(p, q, kv, min(first + AT_TILE, q.count) - 1)); // keys
+        steps[t] = first < q.count ? max(0, end - lo[t] * AT_TILE + 63) / 64 : 0;
+    }
+    const int most = max(steps[0], steps[1]);
     bool ok = true;
 
     if (warp >= AT_MMA_WARP)
@@ -250,9 +249,10 @@ __global__ void __launch_bounds__(AT_THREADS, AfShape<D, APART>::BLOCKS)
         const int t = warp >> 2;
         const uint32_t lanes = (uint32_t) (warp & 3) << 21; // 32 lanes of tensor memory a warp
         const uint32_t o_at = tmem + lanes + S::O_AT + t * D;
-        const int row0 = (APART ? 0 : i0 + t * AT_TILE) + (warp & 3) * 32, i = row0 + lane;
+        const int row0 = (APART ? 0 : i0 + t * AT_TILE) + (warp & 3) * 32, row = row0 + lane;
+        const int i = row < q.count ? q.cell(row) : -1, limit = at_limit(p, q, kv, row);
         const int part = APART ? 2 * split + t : split;
-        const bool rows = row0 < p.sq; // else no row of this warp is a cell: what its weights are reaches nobody
+        const bool rows = row0 < q.count; // else no row of this warp is a cell: what its weights are reaches nobody
         float top = -INFINITY, sum = 0.f; // the base of the weights so far and their sum
         float mine = -INFINITY;           // the largest score of the step that comes next
         const auto score_at = [&](int u) { return tmem + lanes + (t * S::PLACES + u % S::PLACES) * 64; };
@@ -263,11 +263,7 @@ __global__ void __launch_bounds__(AT_THREADS, AfShape<D, APART>::BLOCKS)
         };
         uint32_t see[2];  // which keys of the coming step this row may see
         bool cut = false; // whether some row of the warp may not see all of them
-        // steps whose keys are there and, where the order is causal, not behind the warp's first row
-        int open = 0;
-        if (!bits)
-            open = (int) min((long long) p.sk, p.causal ? (long long) row0 + p.offset + 1 : (long long) p.sk) - lo[t] * AT_TILE;
-        open = open > 0 ? open / 64 : 0;
+        const int open = max(0, at_limit(p, q, kv, row0) - lo[t] * AT_TILE) / 64; // steps that all its rows see whole
         const auto mask = [&](int c, float x) { return see[c >> 5] >> (c & 31) & 1 ? x : -INFINITY; };
         // masks and maximum of a step's scores, which have arrived
         const auto look = [&](int u, float (&s)[64]) {
@@ -277,11 +273,7 @@ __global__ void __launch_bounds__(AT_THREADS, AfShape<D, APART>::BLOCKS)
                 const int j0 = lo[t] * AT_TILE + u * 64;
 #pragma unroll
                 for (int w = 0; w < 2; ++w)
-                {
-                    see[w] = at_there(p, bits, j0, w);
-                    if (p.causal)
-                        see[w] &= at_up_to(i + p.offset - j0, w);
-                }
+                    see[w] = at_up_to(limit - 1 - j0, w);
 #pragma unroll
                 for (int c = 0; c < 64; ++c)
                     s[c] = mask(c, s[c]);
@@ -452,7 +444,7 @@ __global__ void __launch_bounds__(AT_THREADS, AfShape<D, APART>::BLOCKS)
             const long long heads = (long long) p.n * p.q_heads;
             if (p.kv_splits > 1)
             {
-                if (i < p.sq)
+                if (i >= 0)
                 {
                     float* ml = p.part_ml + (2 * heads * part + nh) * p.sq + i;
                     ml[0] = top;
@@ -463,9 +455,9 @@ __global__ void __launch_bounds__(AT_THREADS, AfShape<D, APART>::BLOCKS)
             }
             else
             {
-                const bool none = sum == 0.f || (p.q_mask && i < p.sq && !p.q_mask[n * p.sq + i]);
+                const bool none = sum == 0.f;
                 at_store(p.o, nullptr, nh, n, head, p.d, i, p.sq, 1.f / sum, none, nothing, o_at, 0, D);
-                if (i < p.sq)
+                if (i >= 0)
                     p.lse[nh * p.sq + i] = none ? -INFINITY : (top + log2f(sum)) / ATTN_LOG2E;
             }
         }
