@@ -38,21 +38,41 @@ __global__ void __launch_bounds__(256) attn_join_fwd_kernel(AttnProblem p)
     }
 }
 
-// Adds up the parts of a gradient in order.
+// Adds up the parts of a gradient in order: a block a row of cells, or a piece of one.
+constexpr int ATTN_JOIN_CELLS = 1024; // of a block: four a thread, 256 apart
+
 template <class T>
 __global__ void __launch_bounds__(256) attn_join_grad_kernel(const float* part, int splits, AttnTensor t, int n,
                                                              int heads, int d, int cells, const uint8_t* mask)
 {
     wait_for_previous_kernel(part, mask);
-    const long long total = (long long) n * heads * d * cells;
-    for (long long at = (long long) blockIdx.x * 256 + threadIdx.x; at < total; at += (long long) gridDim.x * 256)
+    dependents_may_start();
+    const long long rows = (long long) n * heads * d, total = rows * cells;
+    const int pieces = (cells + ATTN_JOIN_CELLS - 1) / ATTN_JOIN_CELLS;
+    for (long long u = blockIdx.x; u < rows * pieces; u += gridDim.x)
     {
-        float v[1] = {0.f};
-        const long long row = at / cells, b = row / ((long long) heads * d);
-        if (!mask || mask[b * cells + (at - row * cells)])
-            for (int s = 0; s < splits; ++s)
-                v[0] += part[s * total + at];
-        store_elems<1>(static_cast<T*>(t.p) + b * t.sn + (row - b * heads * d) * t.sc + (at - row * cells), v);
+        const long long row = u / pieces, b = row / ((long long) heads * d);
+        const int i0 = (int) (u - row * pieces) * ATTN_JOIN_CELLS + threadIdx.x;
+        const float* from = part + row * cells;
+        T* to = static_cast<T*>(t.p) + b * t.sn + (row - b * heads * d) * t.sc;
+        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+        bool there[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            there[e] = i0 + 256 * e < cells && (!mask || mask[b * cells + i0 + 256 * e]);
+#pragma unroll 2
+        for (int s = 0; s < splits; ++s, from += total)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (there[e])
+                    sum[e] += from[i0 + 256 * e];
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (i0 + 256 * e < cells)
+            {
+                const float v[1] = {sum[e]};
+                store_elems<1>(to + i0 + 256 * e, v);
+            }
     }
 }
 
@@ -301,7 +321,10 @@ int32_t attn_join_grad(int32_t dtype, const float* part, int splits, const AttnT
 {
     return with_type(dtype, [&](auto e) -> int32_t {
         DCB_CUDA_TRY(launch_overlapped(attn_join_grad_kernel<decltype(e)>,
-                                       dim3(flat_blocks((long long) n * heads * d * cells, 256)), 256, 0, s, part,
+                                       dim3((unsigned) std::min<long long>((long long) n * heads * d
+                                                                               * ((cells + ATTN_JOIN_CELLS - 1) / ATTN_JOIN_CELLS),
+                                                                           32ll * num_sms())),
+                                       256, 0, s, part,
                                        splits, t, n, heads, d, cells, mask));
         return DCB_OK;
     });
@@ -320,7 +343,10 @@ int64_t dcb_attention_workspace_bytes(const dcb_attention_desc* ad, const dcb_nd
     AttnProblem p;
     if (attn_shapes(ad, qd, kd, &p))
         return -1;
-    return attn_carve(&p, ad->dtype, backward != 0, nullptr);
+    const int64_t plain = attn_carve(&p, ad->dtype, backward != 0, nullptr);
+    static const uint8_t any = 0;
+    p.q_mask = p.kv_mask = &any; // only asked for: masked walks may be cut in other parts
+    return std::max(plain, attn_carve(&p, ad->dtype, backward != 0, nullptr));
 }
 
 int32_t dcb_attention_fwd(const dcb_attention_desc* ad, const dcb_nd_desc* qd, const void* q, const dcb_nd_desc* kd,

@@ -2,6 +2,8 @@
 #include "attention_tc.cuh"
 #include "conv_tc_encode.cuh"
 
+#include <cmath>
+
 namespace dcb
 {
 namespace
@@ -10,6 +12,7 @@ namespace
 __device__ int at_status_word; // a kernel gave up on a wait
 
 constexpr int AT_JOBS = 7;
+constexpr int AT_ROWS = 8; // rows of a tensor that a warp copies with the same indices
 constexpr int AT_INDEX_THREADS = 1024, AT_INDEX_CELLS = 8; // cells of a thread at a time
 
 // What a mask leaves of a sample's cells, in order.  A block a sample and side.
@@ -114,40 +117,55 @@ __global__ void __launch_bounds__(256) attn_prepare_kernel(const __grid_constant
     wait_for_previous_kernel(source);
     dependents_may_start();
     const int lane = threadIdx.x & 31;
-    const long long total = (long long) a.n * c.channels * c.chunks;
+    const int groups = (c.channels + AT_ROWS - 1) / AT_ROWS;
+    const long long total = (long long) a.n * groups * c.chunks;
     const int pitch = (c.cells + 7) / 8 * 8;
     for (long long u = (long long) blockIdx.x * 8 + (threadIdx.x >> 5); u < total; u += (long long) gridDim.x * 8)
     {
-        const long long row = u / c.chunks, n = row / c.channels;
-        const long long first = n * c.sn + (row - n * c.channels) * c.sc;
-        const int i0 = (int) (u - row * c.chunks) * 256 + lane;
+        const long long m = u / c.chunks, n = m / groups;
+        const int row0 = (int) (m - n * groups) * AT_ROWS, row1 = min(row0 + AT_ROWS, c.channels);
+        const int i0 = (int) (u - m * c.chunks) * 256 + lane;
+        int cell[8]; // negative: nothing
         if (c.kind == AT_COPY)
         {
             const int count = c.side.index ? c.side.count[n] : c.cells;
-            uint16_t v[8];
 #pragma unroll
             for (int e = 0; e < 8; ++e)
             {
                 const int i = i0 + 32 * e;
-                const int cell = i < count && c.side.index ? c.side.index[n * c.cells + i] : i;
-                v[e] = i < count ? reinterpret_cast<const uint16_t*>(source)[first + cell] : (uint16_t) 0;
+                cell[e] = i >= count ? -1 : c.side.index ? c.side.index[n * c.cells + i] : i;
             }
+            for (int row = row0; row < row1; ++row)
+            {
+                const uint16_t* from = reinterpret_cast<const uint16_t*>(source) + n * c.sn + row * c.sc;
+                uint16_t* to = reinterpret_cast<uint16_t*>(c.to) + (n * c.channels + row) * (long long) pitch + i0;
+                uint16_t v[8];
 #pragma unroll
-            for (int e = 0; e < 8; ++e)
-                if (i0 + 32 * e < pitch)
-                    reinterpret_cast<uint16_t*>(c.to)[row * pitch + i0 + 32 * e] = v[e];
+                for (int e = 0; e < 8; ++e)
+                    v[e] = cell[e] >= 0 ? from[cell[e]] : (uint16_t) 0;
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    if (i0 + 32 * e < pitch)
+                        to[32 * e] = v[e];
+            }
+            continue;
         }
-        else
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+        {
+            const int i = i0 + 32 * e;
+            cell[e] = i < c.cells && !c.mask[n * c.cells + i] ? i : -1;
+        }
+        for (int row = row0; row < row1; ++row)
+#pragma unroll
             for (int e = 0; e < 8; ++e)
-            {
-                const int i = i0 + 32 * e;
-                if (i >= c.cells || c.mask[n * c.cells + i])
-                    continue;
-                if (c.kind == AT_ZERO)
-                    reinterpret_cast<uint16_t*>(c.to)[first + i] = 0;
-                else
-                    c.lse[row * c.cells + i] = -INFINITY;
-            }
+                if (cell[e] >= 0)
+                {
+                    if (c.kind == AT_ZERO)
+                        reinterpret_cast<uint16_t*>(c.to)[n * c.sn + row * c.sc + cell[e]] = 0;
+                    else
+                        c.lse[(n * c.channels + row) * (long long) c.cells + cell[e]] = -INFINITY;
+                }
     }
 }
 
@@ -221,7 +239,7 @@ int32_t at_prepare(const AttnProblem& p, AtHost* h, cudaStream_t stream)
     a.n = p.n;
     long long warps = 0;
     for (int i = 0; i < a.jobs; ++i)
-        warps = std::max(warps, (long long) a.n * a.job[i].channels * a.job[i].chunks);
+        warps = std::max(warps, (long long) a.n * ((a.job[i].channels + AT_ROWS - 1) / AT_ROWS) * a.job[i].chunks);
     const unsigned blocks = (unsigned) std::min<long long>((warps + 7) / 8, 16ll * num_sms());
     DCB_CUDA_TRY(launch_overlapped(attn_prepare_kernel, dim3(blocks, a.jobs), 256, 0, stream, a));
     return DCB_OK;
@@ -256,17 +274,54 @@ bool attn_tc_apart(const AttnProblem& p)
     return p.sq <= AT_TILE && attn_tiles(p.sk, AT_TILE) >= 4;
 }
 
+namespace
+{
+
+// In how many parts every walk is cut, for `work` walks of `steps` tiles of 128 cells on `slots` blocks at a time: what
+// the longest of the slots' queues takes, with `step_us` a tile, and what the parts' sums of `part_bytes` a part cost.
+// Causal walks are half as long on average and start with the longest, so that the queues are even but for one walk's
+// length (12288 cells, 2 key heads of 128 channels: dk, dv in one part 617 us, in three 450).  Masks are taken to
+// leave half of either side.
+int at_best_splits(long long work, long long steps, long long slots, bool causal, bool masked, double step_us,
+                   double part_bytes)
+{
+    const double left = masked ? 0.5 : 1.;
+    int best = 1;
+    double least = 0.;
+    for (int s = 1; s <= 64 && (s == 1 || steps >= 2 * s); ++s)
+    {
+        const double length = std::ceil(left * steps / s);
+        const double blocks = std::ceil(left * work * s / slots); // of a queue; each starts and ends for about 4 us
+        const double queue = causal ? std::max(length, 0.5 * left * left * work * steps / slots) + 0.2 * length
+                                    : blocks * length;
+        const double us = queue * step_us + 4. * blocks + (s > 1 ? 4. + 2. * s * part_bytes / 4e6 : 0.);
+        if (s == 1 || us < 0.97 * least)
+            best = s, least = us;
+    }
+    return best;
+}
+
+} // namespace
+
 void attn_tc_splits(AttnProblem* p, bool backward)
 {
-    const long long slots = (p->d <= 64 ? 2 : 1) * num_sms(); // blocks at a time
+    const bool small = p->d <= 64, masked = p->q_mask || p->kv_mask;
+    const long long slots = (small ? 2 : 1) * num_sms(); // blocks at a time
     const long long q_tiles = attn_tiles(p->sq, AT_TILE), k_tiles = attn_tiles(p->sk, AT_TILE);
     const long long qh = (long long) p->n * p->q_heads, kh = (long long) p->n * p->kv_heads;
-    p->q_splits = backward ? attn_splits(kh * k_tiles, (int) std::min<long long>(q_tiles * p->group, 1 << 30), slots, 2)
-                           : 1;
-    if (!backward && attn_tc_apart(*p))
-        p->kv_splits = 2 * attn_splits(qh, (int) k_tiles / 2, num_sms(), 2);
+    const double q_bytes = 4. * qh * p->d * p->sq, kv_bytes = 8. * kh * p->d * p->sk;
+    p->q_splits = 1;
+    if (backward)
+    {
+        p->kv_splits = at_best_splits(qh * q_tiles, k_tiles, slots, p->causal, masked, small ? 2.1 : 1., q_bytes);
+        p->q_splits = at_best_splits(kh * k_tiles, q_tiles * p->group, slots, p->causal, masked, small ? 2.8 : 1.4,
+                                     kv_bytes);
+    }
+    else if (attn_tc_apart(*p))
+        p->kv_splits = 2 * at_best_splits(qh, k_tiles / 2, num_sms(), false, masked, 1.2, 2. * q_bytes);
     else
-        p->kv_splits = attn_splits(qh * (backward ? q_tiles : (q_tiles + 1) / 2), (int) k_tiles, slots, 2);
+        p->kv_splits = at_best_splits(qh * ((q_tiles + 1) / 2), k_tiles, slots, p->causal, masked, small ? 3.4 : 2.1,
+                                      q_bytes);
 }
 
 int32_t attn_tc_index(const AttnProblem& p, cudaStream_t stream)

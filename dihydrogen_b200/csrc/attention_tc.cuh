@@ -373,6 +373,15 @@ __device__ __forceinline__ void at_store(const AttnTensor& t, float* part, long 
     }
 }
 
+// Which tile and walk (head and part) a block has.  Causal walks differ in length: all heads' longest ones first; else a
+// head's blocks lie together, whose keys then stay in L2.
+__device__ __forceinline__ int at_block(bool causal, int tiles, long long walks, long long* walk)
+{
+    const long long b = blockIdx.x;
+    *walk = causal ? b % walks : b / tiles;
+    return (int) (causal ? b / walks : b % tiles);
+}
+
 struct AtMaps
 {
     CUtensorMap q, k, v, d_o;

@@ -133,10 +133,9 @@ __global__ void __launch_bounds__(AT_THREADS, AbShape<D>::BLOCKS)
     if (at_misplaced(base, ex.status))
         return;
 
-    long long at = blockIdx.x;
     const int tiles_k = attn_tiles(p.sk, AT_TILE);
-    const int tile = (int) (at % tiles_k); // causal: the first keys have the longest walks
-    at /= tiles_k;
+    long long at;
+    const int tile = at_block(p.causal, tiles_k, (long long) p.n * p.kv_heads * p.q_splits, &at); // the first keys' are longest
     const int split = (int) (at % p.q_splits);
     const long long nh = at / p.q_splits, n = nh / p.kv_heads;
     const int head = (int) (nh - n * p.kv_heads);
@@ -372,10 +371,9 @@ __global__ void __launch_bounds__(AT_THREADS, AbShape<D>::BLOCKS)
     if (at_misplaced(base, ex.status))
         return;
 
-    long long at = blockIdx.x;
     const int tiles_q = attn_tiles(p.sq, AT_TILE);
-    const int tile = tiles_q - 1 - (int) (at % tiles_q); // causal: the longest walks first
-    at /= tiles_q;
+    long long at;
+    const int tile = tiles_q - 1 - at_block(p.causal, tiles_q, (long long) p.n * p.q_heads * p.kv_splits, &at);
     const int split = (int) (at % p.kv_splits);
     const long long nh = at / p.kv_splits, n = nh / p.q_heads;
     const int head = (int) (nh - n * p.q_heads), kv_head = head / p.group;

@@ -67,11 +67,10 @@ __global__ void __launch_bounds__(AT_THREADS, AfShape<D, APART>::BLOCKS)
     if (at_misplaced(base, ex.status))
         return;
 
-    long long at = blockIdx.x;
     const int blocks_q = APART ? 1 : attn_tiles(p.sq, 2 * AT_TILE);
-    const int block_q = blocks_q - 1 - (int) (at % blocks_q); // causal: the longest walks first
-    at /= blocks_q;
     const int splits = APART ? p.kv_splits / 2 : p.kv_splits;
+    long long at;
+    const int block_q = blocks_q - 1 - at_block(p.causal, blocks_q, (long long) p.n * p.q_heads * splits, &at);
     const int split = (int) (at % splits);
     const long long nh = at / splits, n = nh / p.q_heads;
     const int head = (int) (nh - n * p.q_heads), kv_head = head / p.group;
