@@ -6,6 +6,8 @@
 
 #include <cuda_bf16.h>
 
+#include <algorithm>
+
 namespace dcb
 {
 
@@ -21,14 +23,15 @@ inline bool known_dtype(int32_t dtype)
     return dtype == DCB_F32 || dtype == DCB_BF16;
 }
 
-// Largest of 4, 2, 1 elements that every run start of a tensor honours as one access.
-inline int run_vec_of(const RunGeom& g, const RunStrides& s, const void* p, int bytes)
+// Largest of `most` (8 or 4), 4, 2, 1 elements that every run start of a tensor honours as accesses of 16 bytes or less.
+inline int run_vec_of(const RunGeom& g, const RunStrides& s, const void* p, int bytes, int most = 4)
 {
     auto ok = [&](long long v) {
-        return g.len % v == 0 && s.sn % v == 0 && s.sc % v == 0 && s.s_inner % v == 0 && s.s_outer % v == 0
-               && reinterpret_cast<uintptr_t>(p) % (bytes * v) == 0;
+        const long long aligned = std::min<long long>(v, 16 / bytes); // elements
+        return g.len % v == 0 && s.sn % aligned == 0 && s.sc % aligned == 0 && s.s_inner % aligned == 0
+               && s.s_outer % aligned == 0 && reinterpret_cast<uintptr_t>(p) % (bytes * aligned) == 0;
     };
-    return ok(4) ? 4 : (ok(2) ? 2 : 1);
+    return most == 8 && ok(8) ? 8 : ok(4) ? 4 : (ok(2) ? 2 : 1);
 }
 
 // A row's stride that nothing ever steps over says nothing about alignment.
@@ -83,6 +86,13 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi)
 {
     const __nv_bfloat162 t = __floats2bfloat162_rn(lo, hi);
     return *reinterpret_cast<const uint32_t*>(&t);
+}
+
+template <>
+__device__ __forceinline__ void load_elems<8>(const float* p, float (&v)[8])
+{
+    const float4 t = *reinterpret_cast<const float4*>(p), u = *reinterpret_cast<const float4*>(p + 4);
+    v[0] = t.x, v[1] = t.y, v[2] = t.z, v[3] = t.w, v[4] = u.x, v[5] = u.y, v[6] = u.z, v[7] = u.w;
 }
 
 // V neighbours as they are stored.  Loads that are taken ahead keep these and are converted where they are used: a
@@ -141,7 +151,12 @@ struct RawElems<bf16, V>
 template <int V>
 __device__ __forceinline__ void store_elems(float* p, const float (&v)[V])
 {
-    if constexpr (V == 4)
+    if constexpr (V == 8)
+    {
+        *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
+        *reinterpret_cast<float4*>(p + 4) = make_float4(v[4], v[5], v[6], v[7]);
+    }
+    else if constexpr (V == 4)
         *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
     else if constexpr (V == 2)
         *reinterpret_cast<float2*>(p) = make_float2(v[0], v[1]);
@@ -152,12 +167,46 @@ __device__ __forceinline__ void store_elems(float* p, const float (&v)[V])
 template <int V>
 __device__ __forceinline__ void store_elems(bf16* p, const float (&v)[V])
 {
-    if constexpr (V == 4)
+    if constexpr (V == 8)
+        *reinterpret_cast<uint4*>(p) = make_uint4(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]), pack_bf16(v[4], v[5]),
+                                                  pack_bf16(v[6], v[7]));
+    else if constexpr (V == 4)
         *reinterpret_cast<uint2*>(p) = make_uint2(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]));
     else if constexpr (V == 2)
         *reinterpret_cast<uint32_t*>(p) = pack_bf16(v[0], v[1]);
     else
         *p = __float2bfloat16_rn(v[0]);
+}
+
+// V elements 32 apart, of which the first `have` are there: a lane's share of 32 V neighbours where a run starts off the
+// alignment of wider accesses.  They share an address but for a constant.
+template <class T, int V>
+struct SplitElems
+{
+    RawElems<T, 1> r[V];
+    template <bool FULL>
+    __device__ __forceinline__ void load(const T* p, int have)
+    {
+#pragma unroll
+        for (int e = 0; e < V; ++e)
+            if (FULL || e < have)
+                r[e].load(p + 32 * e);
+            else
+                r[e].clear();
+    }
+    __device__ __forceinline__ float get(int e) const { return r[e].get(0); }
+};
+
+template <int V, bool FULL, class T>
+__device__ __forceinline__ void store_split(T* p, const float (&v)[V], int have)
+{
+#pragma unroll
+    for (int e = 0; e < V; ++e)
+        if (FULL || e < have)
+        {
+            const float t[1] = {v[e]};
+            store_elems<1>(p + 32 * e, t);
+        }
 }
 
 // Units of V neighbouring cells of all samples, numbered through: which cells a unit is.

@@ -98,35 +98,14 @@ struct LnRaw
 };
 
 template <class T, int V>
-struct LnRaw<T, V, LN_SPLIT>
-{
-    RawElems<T, 1> r[V];
-    template <bool FULL>
-    __device__ __forceinline__ void load(const T* p, int have)
-    {
-#pragma unroll
-        for (int e = 0; e < V; ++e)
-            if (FULL || e < have)
-                r[e].load(p + 32 * e);
-            else
-                r[e].clear();
-    }
-    __device__ __forceinline__ float get(int e) const { return r[e].get(0); }
-};
+struct LnRaw<T, V, LN_SPLIT> : SplitElems<T, V>
+{};
 
 template <int V, int MODE, bool FULL, class T>
 __device__ __forceinline__ void ln_store(T* p, const float (&v)[V], int have)
 {
     if constexpr (MODE == LN_SPLIT)
-    {
-#pragma unroll
-        for (int e = 0; e < V; ++e)
-            if (FULL || e < have)
-            {
-                const float t[1] = {v[e]};
-                store_elems<1>(p + 32 * e, t);
-            }
-    }
+        store_split<V, FULL>(p, v, have);
     else if (FULL || have > 0)
         store_elems<V>(p, v);
 }

@@ -25,7 +25,7 @@ namespace dcb
 namespace
 {
 
-constexpr int ROT_UNROLL = 4; // heads in flight a thread
+constexpr int ROT_HEADS = 4; // in flight a thread
 
 struct RotArgs
 {
@@ -44,21 +44,49 @@ struct RotArgs
     float sign;
 };
 
-// Slots of a head: its turned pairs, then the channels of no axis two at a time (the last may be alone).
-template <class TX, class TY, int V>
+template <class T, int V, bool SPLIT>
+struct RotRaw
+{
+    RawElems<T, V> r;
+    template <bool FULL>
+    __device__ __forceinline__ void load(const T* p, int)
+    {
+        r.load(p);
+    }
+    __device__ __forceinline__ float get(int e) const { return r.get(e); }
+};
+
+template <class T, int V>
+struct RotRaw<T, V, true> : SplitElems<T, V>
+{};
+
+// Slots of a head: its turned pairs, then the channels of no axis two at a time (the last may be alone).  A thread has V
+// neighbours (units), or, SPLIT, V cells 32 apart of its warp's 32 V (units are a warp's).
+template <class TX, class TY, int V, bool SPLIT>
 __global__ void __launch_bounds__(256) rotary_kernel(const TX* x, RunStrides xs, TY* y, RunStrides ys, RotArgs a)
 {
     wait_for_previous_kernel(x);
     dependents_may_start();
-    const long long unit = (long long) blockIdx.x * 256 + threadIdx.x;
+    const int lane = threadIdx.x & 31;
+    const long long unit = SPLIT ? (long long) blockIdx.x * 8 + __shfl_sync(~0u, (int) threadIdx.x >> 5, 0)
+                                 : (long long) blockIdx.x * 256 + threadIdx.x;
     if (unit >= a.units.total)
         return;
     const int slot = blockIdx.y;
     const long long n = blockIdx.z / a.head_chunks;
     const int head0 = (int) (blockIdx.z - n * a.head_chunks) * a.chunk;
     const int head1 = min(head0 + a.chunk, a.heads);
-    CellAt at = cell_at<V>(a.units, a.per_run, a.rows, a.rows_inner, unit);
+    CellAt at = cell_at<SPLIT ? 32 * V : V>(a.units, a.per_run, a.rows, a.rows_inner, unit);
     at.n = n;
+    int have = V;
+    if (SPLIT)
+    {
+        const long long left = a.units.len - at.pos - lane;
+        have = left <= 0 ? 0 : (int) min((long long) V, (left + 31) / 32);
+        at.cell += lane;
+    }
+    const bool full = !SPLIT || at.pos + 32 * V <= a.units.len;
+    const int lane_at = SPLIT ? lane : 0;
 
     int c0, c1;
     float co[V], si[V];
@@ -76,7 +104,7 @@ __global__ void __launch_bounds__(256) rotary_kernel(const TX* x, RunStrides xs,
 #pragma unroll
         for (int e = 0; e < V; ++e)
         {
-            const uint32_t cell = (uint32_t) at.cell + e;
+            const uint32_t cell = (uint32_t) at.cell + (SPLIT ? 32 * min(e, have - 1) : e);
             const uint32_t row = a.w.div(cell), plane = a.h.div(row);
             const uint32_t p = axis == 2 ? cell - row * a.w.d : axis == 1 ? row - plane * a.h.d : plane;
             co[e] = cos_of[p];
@@ -89,47 +117,79 @@ __global__ void __launch_bounds__(256) rotary_kernel(const TX* x, RunStrides xs,
         c1 = c0 + 1 < a.head_dim ? c0 + 1 : -1;
     }
 
-    const long long xo = offset_of(at, xs), yo = offset_of(at, ys);
-    for (int h = head0; h < head1; h += ROT_UNROLL)
-    {
-        float p[ROT_UNROLL][V], q[ROT_UNROLL][V];
+    // heads [lo, hi), several at a time: a whole group's loads go out before anything waits for one
+    const TX* px = x + offset_of(at, xs) + lane_at;
+    TY* py = y + offset_of(at, ys) + lane_at;
+    const long long x_head = a.head_dim * xs.sc, y_head = a.head_dim * ys.sc;
+    const auto heads = [&](int lo, int hi, auto turn, auto pair, auto whole) {
+        constexpr bool TURN = decltype(turn)::value, PAIR = decltype(pair)::value, FULL = decltype(whole)::value;
+        const auto put = [&](TY* to, const float (&v)[V]) {
+            if constexpr (SPLIT)
+                store_split<V, FULL>(to, v, have);
+            else
+                store_elems<V>(to, v);
+        };
+        const auto some = [&](int h, auto count) {
+            constexpr int N = decltype(count)::value;
+            RotRaw<TX, V, SPLIT> rp[N], rq[N];
 #pragma unroll
-        for (int i = 0; i < ROT_UNROLL; ++i)
-        {
-            const int head = h + i;
-            if (head >= head1 || (a.skip_copies && !(turns && head < a.rotated)))
-                continue;
-            const TX* px = x + xo + (long long) head * a.head_dim * xs.sc;
-            load_elems<V>(px + c0 * xs.sc, p[i]);
-            if (c1 >= 0)
-                load_elems<V>(px + c1 * xs.sc, q[i]);
-        }
-#pragma unroll
-        for (int i = 0; i < ROT_UNROLL; ++i)
-        {
-            const int head = h + i;
-            if (head >= head1 || (a.skip_copies && !(turns && head < a.rotated)))
-                continue;
-            if (turns && head < a.rotated)
+            for (int i = 0; i < N; ++i)
             {
+                rp[i].template load<FULL>(px + (h + i) * x_head + c0 * xs.sc, have);
+                if (PAIR)
+                    rq[i].template load<FULL>(px + (h + i) * x_head + c1 * xs.sc, have);
+            }
+#pragma unroll
+            for (int i = 0; i < N; ++i)
+            {
+                float p[V], q[V];
 #pragma unroll
                 for (int e = 0; e < V; ++e)
                 {
-                    const float r = p[i][e] * co[e] - q[i][e] * si[e];
-                    q[i][e] = p[i][e] * si[e] + q[i][e] * co[e];
-                    p[i][e] = r;
+                    p[e] = rp[i].get(e);
+                    if (PAIR)
+                        q[e] = rq[i].get(e);
+                    if (TURN)
+                    {
+                        const float r = p[e] * co[e] - q[e] * si[e];
+                        q[e] = p[e] * si[e] + q[e] * co[e];
+                        p[e] = r;
+                    }
                 }
+                put(py + (h + i) * y_head + c0 * ys.sc, p);
+                if (PAIR)
+                    put(py + (h + i) * y_head + c1 * ys.sc, q);
             }
-            TY* py = y + yo + (long long) head * a.head_dim * ys.sc;
-            store_elems<V>(py + c0 * ys.sc, p[i]);
-            if (c1 >= 0)
-                store_elems<V>(py + c1 * ys.sc, q[i]);
-        }
-    }
+        };
+        int h = lo;
+#pragma unroll 1
+        for (; h + ROT_HEADS <= hi; h += ROT_HEADS)
+            some(h, std::integral_constant<int, ROT_HEADS>());
+        if (h + 2 <= hi)
+            some(h, std::integral_constant<int, 2>()), h += 2;
+        if (h < hi)
+            some(h, std::integral_constant<int, 1>());
+    };
+    using std::bool_constant;
+    const int turned = turns ? max(head0, min(head1, a.rotated)) : head0; // heads before are turned
+    const auto all = [&](auto whole) {
+        if (turns)
+            heads(head0, turned, bool_constant<true>(), bool_constant<true>(), whole);
+        if (a.skip_copies)
+            return;
+        if (c1 >= 0)
+            heads(turned, head1, bool_constant<false>(), bool_constant<true>(), whole);
+        else
+            heads(turned, head1, bool_constant<false>(), bool_constant<false>(), whole);
+    };
+    if (!SPLIT || full)
+        all(bool_constant<true>());
+    else if (have > 0)
+        all(bool_constant<false>());
 }
 
 template <class TX, class TY>
-int32_t rotary_launch(int v, dim3 grid, const void* x, const RunStrides& xs, void* y, const RunStrides& ys,
+int32_t rotary_launch(int v, bool split, dim3 grid, const void* x, const RunStrides& xs, void* y, const RunStrides& ys,
                       const RotArgs& a, cudaStream_t stream)
 {
     const auto go = [&](auto kernel) -> int32_t {
@@ -137,9 +197,11 @@ int32_t rotary_launch(int v, dim3 grid, const void* x, const RunStrides& xs, voi
                                        static_cast<TY*>(y), ys, a));
         return DCB_OK;
     };
-    return v == 4   ? go(rotary_kernel<TX, TY, 4>)
-           : v == 2 ? go(rotary_kernel<TX, TY, 2>)
-                    : go(rotary_kernel<TX, TY, 1>);
+    if (split)
+        return go(rotary_kernel<TX, TY, 4, true>);
+    return v == 8   ? go(rotary_kernel<TX, TY, 8, false>)
+           : v == 4 ? go(rotary_kernel<TX, TY, 4, false>)
+                    : go(rotary_kernel<TX, TY, 1, false>);
 }
 
 bool same_strides(const dcb_nd_desc& a, const dcb_nd_desc& b)
@@ -279,13 +341,23 @@ int32_t dcb_rotary_apply(const dcb_rotary_plan* plan, const dcb_nd_desc* xd, int
     make_runs(*yd, level, &rg, &ys);
     drop_unused_strides(rg, &xs);
     drop_unused_strides(rg, &ys);
-    const int v = std::min(run_vec_of(rg, xs, x, elem_bytes(x_dtype)), run_vec_of(rg, ys, y, elem_bytes(y_dtype)));
+    const int most = x_dtype == DCB_BF16 || y_dtype == DCB_BF16 ? 8 : 4; // accesses of 16 bytes
+    int v = std::min(run_vec_of(rg, xs, x, elem_bytes(x_dtype), most), run_vec_of(rg, ys, y, elem_bytes(y_dtype), most));
     const dcb_rotary_desc& rd = plan->rd;
+    // Eight cells a thread (16 bytes of bf16) where that leaves 16 blocks for every SM; four, or four 32 apart where
+    // accesses of four are not aligned and runs are long enough that their last 128 cells are no waste; else one.
+    // (2 x 1536 x 40^3 in bf16 with four cells 190 us, with eight 129; 8192 x 1536 values 8.2 and 9.5.)
+    const long long heads_at_once = (xd->c / rd.head_dim + ROT_HEADS - 1) / ROT_HEADS;
+    const long long pairs = (rd.head_dim + 1) / 2;
+    if (v == 8 && rg.rows * rg.len / 8 / 256 * pairs * xd->n * heads_at_once < 16ll * num_sms())
+        v = 4;
+    const bool split = v < 4 && rg.len >= 512;
+    v = split ? 4 : v < 4 ? 1 : v;
     RotArgs a = {};
     RunGeom one = rg;
     one.n = 1;
-    a.units = cell_units(one, v);
-    a.per_run = rg.len / v;
+    a.per_run = split ? (rg.len + 127) / 128 : rg.len / v;
+    a.units = cell_units_of(one, a.per_run);
     a.rows = rg.rows;
     a.rows_inner = rg.rows_inner;
     a.w = FastDiv::of((uint32_t) xd->dims[2]);
@@ -309,13 +381,13 @@ int32_t dcb_rotary_apply(const dcb_rotary_plan* plan, const dcb_nd_desc* xd, int
     a.sign = inverse ? -1.f : 1.f;
     if (a.skip_copies && (a.rotated == 0 || a.turned_pairs == 0))
         return DCB_OK;
-    const long long blocks_x = (a.units.total + 255) / 256;
+    const long long blocks_x = split ? (a.units.total + 7) / 8 : (a.units.total + 255) / 256;
     const int slots = a.turned_pairs + (rd.head_dim - channel + 1) / 2;
     // a thread keeps its angles for as many heads as leave four blocks for every SM's eight
     a.chunk = a.heads;
-    while (a.chunk > ROT_UNROLL
+    while (a.chunk > ROT_HEADS
            && blocks_x * slots * xd->n * ((a.heads + a.chunk - 1) / a.chunk) < 16ll * num_sms())
-        a.chunk = std::max(ROT_UNROLL, a.chunk / 2);
+        a.chunk = std::max(ROT_HEADS, a.chunk / 2);
     a.head_chunks = (a.heads + a.chunk - 1) / a.chunk;
     if (blocks_x >= (1ll << 31) || xd->n * a.head_chunks > 65535)
     {
@@ -325,10 +397,10 @@ int32_t dcb_rotary_apply(const dcb_rotary_plan* plan, const dcb_nd_desc* xd, int
     const dim3 grid((unsigned) blocks_x, slots, (unsigned) (xd->n * a.head_chunks));
     cudaStream_t s = as_stream(stream);
     if (x_dtype == DCB_F32)
-        return y_dtype == DCB_F32 ? rotary_launch<float, float>(v, grid, x, xs, y, ys, a, s)
-                                  : rotary_launch<float, bf16>(v, grid, x, xs, y, ys, a, s);
-    return y_dtype == DCB_F32 ? rotary_launch<bf16, float>(v, grid, x, xs, y, ys, a, s)
-                              : rotary_launch<bf16, bf16>(v, grid, x, xs, y, ys, a, s);
+        return y_dtype == DCB_F32 ? rotary_launch<float, float>(v, split, grid, x, xs, y, ys, a, s)
+                                  : rotary_launch<float, bf16>(v, split, grid, x, xs, y, ys, a, s);
+    return y_dtype == DCB_F32 ? rotary_launch<bf16, float>(v, split, grid, x, xs, y, ys, a, s)
+                              : rotary_launch<bf16, bf16>(v, split, grid, x, xs, y, ys, a, s);
 }
 
 } // extern "C"
