@@ -176,7 +176,7 @@ __device__ __forceinline__ void ln_steps(int count, F f)
     }
 }
 
-template <class T, int V, int MODE, bool FULL>
+template <class T, int V, int MODE, bool FULL, bool KEEP>
 __device__ __forceinline__ void ln_fwd_tile(const T* x, const RunStrides& xs, T* y, const RunStrides& ys,
                                             const float* __restrict__ scale, const float* __restrict__ bias, float eps,
                                             float* mean_out, float* inv_std_out, const LnGeom& geo, const LnSelf& me,
@@ -191,12 +191,13 @@ __device__ __forceinline__ void ln_fwd_tile(const T* x, const RunStrides& xs, T*
     for (int e = 0; e < V; ++e)
         mean[e] = m2[e] = 0.f;
     const T* p = px;
-    ln_steps<FULL>(me.count, [&](int i, auto some) {
-        constexpr int m = decltype(some)::value;
-        LnRaw<T, V, MODE> v[m];
+    const auto fetch = [&](auto& v, auto some) {
 #pragma unroll
-        for (int k = 0; k < m; ++k, p += x_step)
-                v[k].template load<FULL>(p, at.have);
+        for (int k = 0; k < decltype(some)::value; ++k, p += x_step)
+            v[k].template load<FULL>(p, at.have);
+    };
+    const auto take = [&](int i, const auto& v, auto some) {
+        constexpr int m = decltype(some)::value;
         const float inv_m = 1.f / m, f = m / (float) (i + m);
 #pragma unroll
         for (int e = 0; e < V; ++e)
@@ -213,7 +214,19 @@ __device__ __forceinline__ void ln_fwd_tile(const T* x, const RunStrides& xs, T*
             mean[e] = fmaf(d, f, mean[e]);
             m2[e] += fmaf(d * d, f * i, q);
         }
-    });
+    };
+    LnRaw<T, V, MODE> kept[LN_STEP];
+    if (KEEP)
+    {
+        fetch(kept, LnSome<LN_STEP>());
+        take(0, kept, LnSome<LN_STEP>());
+    }
+    else
+        ln_steps<FULL>(me.count, [&](int i, auto some) {
+            LnRaw<T, V, MODE> v[decltype(some)::value];
+            fetch(v, some);
+            take(i, v, some);
+        });
     if (geo.g > 1)
     {
         float all[V];
@@ -249,32 +262,38 @@ __device__ __forceinline__ void ln_fwd_tile(const T* x, const RunStrides& xs, T*
     p = px;
     T* py = y + (offset_of(at.cell, ys) + me.cg * ys.sc) + at.lane;
     const long long y_step = geo.g * ys.sc;
-    ln_steps<FULL>(me.count, [&](int i, auto some) {
+    const auto give = [&](int i, const auto& v, auto some) {
         constexpr int m = decltype(some)::value;
-        LnRaw<T, V, MODE> v[m];
         float w[m], b[m];
 #pragma unroll
-        for (int k = 0; k < m; ++k, p += x_step)
-            {
-                v[k].template load<FULL>(p, at.have);
-                const int c = me.cg + (i + k) * geo.g;
-                w[k] = scale ? __ldg(scale + c) : 1.f;
-                b[k] = bias ? __ldg(bias + c) : 0.f;
-            }
+        for (int k = 0; k < m; ++k)
+        {
+            const int c = me.cg + (i + k) * geo.g;
+            w[k] = scale ? __ldg(scale + c) : 1.f;
+            b[k] = bias ? __ldg(bias + c) : 0.f;
+        }
 #pragma unroll
         for (int k = 0; k < m; ++k, py += y_step)
-            {
-                float out[V];
+        {
+            float out[V];
 #pragma unroll
-                for (int e = 0; e < V; ++e)
-                    out[e] = fmaf((v[k].get(e) - mean[e]) * inv[e], w[k], b[k]);
-                ln_store<V, MODE, FULL>(py, out, at.have);
-            }
-    });
+            for (int e = 0; e < V; ++e)
+                out[e] = fmaf((v[k].get(e) - mean[e]) * inv[e], w[k], b[k]);
+            ln_store<V, MODE, FULL>(py, out, at.have);
+        }
+    };
+    if (KEEP)
+        give(0, kept, LnSome<LN_STEP>());
+    else
+        ln_steps<FULL>(me.count, [&](int i, auto some) {
+            LnRaw<T, V, MODE> v[decltype(some)::value];
+            fetch(v, some);
+            give(i, v, some);
+        });
 }
 
 // Shared memory: the groups' sums and their centred sums of squares.
-template <class T, int V, int MODE>
+template <class T, int V, int MODE, bool KEEP>
 __global__ void __launch_bounds__(32 * LN_WARPS, 4)
     ln_fwd_kernel(const T* x, RunStrides xs, T* y, RunStrides ys, const float* scale, const float* bias, float eps,
                   float* mean_out, float* inv_std_out, LnGeom geo)
@@ -294,10 +313,10 @@ __global__ void __launch_bounds__(32 * LN_WARPS, 4)
         }
         const LnAt<V, MODE> at(geo, (tile * me.groups + me.group) * 32, me.lane);
         if (at.full)
-            ln_fwd_tile<T, V, MODE, true>(x, xs, y, ys, scale, bias, eps, mean_out, inv_std_out, geo, me, at, sums,
+            ln_fwd_tile<T, V, MODE, true, KEEP>(x, xs, y, ys, scale, bias, eps, mean_out, inv_std_out, geo, me, at, sums,
                                           squares);
         else
-            ln_fwd_tile<T, V, MODE, false>(x, xs, y, ys, scale, bias, eps, mean_out, inv_std_out, geo, me, at, sums,
+            ln_fwd_tile<T, V, MODE, false, KEEP>(x, xs, y, ys, scale, bias, eps, mean_out, inv_std_out, geo, me, at, sums,
                                            squares);
     }
     dependents_may_start();
@@ -327,7 +346,7 @@ __device__ __forceinline__ float ln_lane_sums(float (&v)[K], int lane)
     return r;
 }
 
-template <class T, int V, int MODE, bool FULL>
+template <class T, int V, int MODE, bool FULL, bool KEEP>
 __device__ __forceinline__ void ln_bwd_tile(const T* x, const RunStrides& xs, const T* dy, const RunStrides& dys,
                                             const float* mean_in, const float* inv_std_in,
                                             const float* __restrict__ scale, T* dx, const RunStrides& dxs, bool grads,
@@ -347,16 +366,17 @@ __device__ __forceinline__ void ln_bwd_tile(const T* x, const RunStrides& xs, co
     for (int e = 0; e < V; ++e)
         a[e] = b[e] = 0.f;
     const T *p = px, *d = pd;
-    ln_steps<FULL>(me.count, [&](int i, auto some) {
-        constexpr int m = decltype(some)::value;
-        LnRaw<T, V, MODE> x_of[m], dy_of[m];
-        float sw[m], sb[m];
+    const auto fetch = [&](auto& x_of, auto& dy_of, auto some) {
 #pragma unroll
-        for (int k = 0; k < m; ++k, p += x_step, d += dy_step)
+        for (int k = 0; k < decltype(some)::value; ++k, p += x_step, d += dy_step)
         {
             x_of[k].template load<FULL>(p, at.have);
             dy_of[k].template load<FULL>(d, at.have);
         }
+    };
+    const auto take = [&](int i, const auto& x_of, const auto& dy_of, auto some) {
+        constexpr int m = decltype(some)::value;
+        float sw[m], sb[m];
 #pragma unroll
         for (int k = 0; k < m; ++k)
         {
@@ -382,7 +402,19 @@ __device__ __forceinline__ void ln_bwd_tile(const T* x, const RunStrides& xs, co
                 acc[geo.c + c] += tb;
             }
         }
-    });
+    };
+    LnRaw<T, V, MODE> x_kept[LN_STEP], dy_kept[LN_STEP];
+    if (KEEP)
+    {
+        fetch(x_kept, dy_kept, LnSome<LN_STEP>());
+        take(0, x_kept, dy_kept, LnSome<LN_STEP>());
+    }
+    else
+        ln_steps<FULL>(me.count, [&](int i, auto some) {
+            LnRaw<T, V, MODE> x_of[decltype(some)::value], dy_of[decltype(some)::value];
+            fetch(x_of, dy_of, some);
+            take(i, x_of, dy_of, some);
+        });
     if (geo.g > 1)
     {
         store_elems<V>(mine + (me.cg * 32 + me.lane) * V, a);
@@ -397,35 +429,38 @@ __device__ __forceinline__ void ln_bwd_tile(const T* x, const RunStrides& xs, co
     p = px, d = pd;
     T* po = dx + (offset_of(at.cell, dxs) + me.cg * dxs.sc) + at.lane;
     const long long dx_step = geo.g * dxs.sc;
-    ln_steps<FULL>(me.count, [&](int i, auto some) {
+    const auto give = [&](int i, const auto& x_of, const auto& dy_of, auto some) {
         constexpr int m = decltype(some)::value;
-        LnRaw<T, V, MODE> x_of[m], dy_of[m];
         float w[m];
 #pragma unroll
-        for (int k = 0; k < m; ++k, p += x_step, d += dy_step)
-            {
-                x_of[k].template load<FULL>(p, at.have);
-                dy_of[k].template load<FULL>(d, at.have);
-                w[k] = scale ? __ldg(scale + me.cg + (i + k) * geo.g) : 1.f;
-            }
+        for (int k = 0; k < m; ++k)
+            w[k] = scale ? __ldg(scale + me.cg + (i + k) * geo.g) : 1.f;
 #pragma unroll
         for (int k = 0; k < m; ++k, po += dx_step)
-            {
-                float out[V];
+        {
+            float out[V];
 #pragma unroll
-                for (int e = 0; e < V; ++e)
-                {
-                    const float u = (x_of[k].get(e) - mean.get(e)) * inv.get(e);
-                    out[e] = inv.get(e) * (fmaf(dy_of[k].get(e), w[k], -a[e]) - u * b[e]);
-                }
-                ln_store<V, MODE, FULL>(po, out, at.have);
+            for (int e = 0; e < V; ++e)
+            {
+                const float u = (x_of[k].get(e) - mean.get(e)) * inv.get(e);
+                out[e] = inv.get(e) * (fmaf(dy_of[k].get(e), w[k], -a[e]) - u * b[e]);
             }
-    });
+            ln_store<V, MODE, FULL>(po, out, at.have);
+        }
+    };
+    if (KEEP)
+        give(0, x_kept, dy_kept, LnSome<LN_STEP>());
+    else
+        ln_steps<FULL>(me.count, [&](int i, auto some) {
+            LnRaw<T, V, MODE> x_of[decltype(some)::value], dy_of[decltype(some)::value];
+            fetch(x_of, dy_of, some);
+            give(i, x_of, dy_of, some);
+        });
 }
 
 // Blocks walk over the tiles.  The gradients of scale and bias are added up over a tile's cells by exchanges between
 // the lanes, over the tiles in shared memory, [group][2][c], and leave as partial[which][channel][block].
-template <class T, int V, int MODE>
+template <class T, int V, int MODE, bool KEEP>
 __global__ void __launch_bounds__(32 * LN_WARPS, ln_bwd_blocks(V))
     ln_bwd_kernel(const T* x, RunStrides xs, const T* dy, RunStrides dys, const float* mean_in,
                   const float* inv_std_in, const float* scale, T* dx, RunStrides dxs, float* partial, LnGeom geo)
@@ -451,10 +486,10 @@ __global__ void __launch_bounds__(32 * LN_WARPS, ln_bwd_blocks(V))
         float* mine = reinterpret_cast<float*>(room[turn]) + me.group * geo.g * 32 * V;
         float* sums = acc + me.group * 2 * geo.c;
         if (at.full)
-            ln_bwd_tile<T, V, MODE, true>(x, xs, dy, dys, mean_in, inv_std_in, scale, dx, dxs, partial != nullptr, geo,
+            ln_bwd_tile<T, V, MODE, true, KEEP>(x, xs, dy, dys, mean_in, inv_std_in, scale, dx, dxs, partial != nullptr, geo,
                                           me, at, mine, sums);
         else
-            ln_bwd_tile<T, V, MODE, false>(x, xs, dy, dys, mean_in, inv_std_in, scale, dx, dxs, partial != nullptr,
+            ln_bwd_tile<T, V, MODE, false, KEEP>(x, xs, dy, dys, mean_in, inv_std_in, scale, dx, dxs, partial != nullptr,
                                            geo, me, at, mine, sums);
     }
     dependents_may_start();
@@ -501,6 +536,7 @@ __global__ void __launch_bounds__(256) ln_zero_kernel(float* dscale, float* dbia
 struct LnChoice
 {
     int v, g, mode;
+    bool keep; // every thread has eight channels: they stay in registers
 };
 
 // vmax: neighbours that one access may fetch.  len: cells of a run.
@@ -517,6 +553,7 @@ LnChoice ln_choose(int c, int vmax, long long len, long long cells)
     h.g = 1;
     while (h.g < LN_WARPS && (c > LN_STEP * h.g || (c >= 2 * h.g && tiles * h.g < 8ll * num_sms())))
         h.g *= 2;
+    h.keep = c == LN_STEP * h.g;
     return h;
 }
 
@@ -570,45 +607,48 @@ LnGeom ln_geometry(const RunGeom& rg, const LnChoice& h)
     return g;
 }
 
-template <class T, int V, int MODE>
+template <class T, int V, int MODE, bool KEEP>
 int32_t ln_launch_fwd(const LnGeom& g, const void* x, const RunStrides& xs, void* y, const RunStrides& ys,
                       const void* scale, const void* bias, float eps, void* mean, void* inv_std, cudaStream_t stream)
 {
     const unsigned blocks = (unsigned) std::min<long long>(g.tiles, 4ll * num_sms());
-    DCB_CUDA_TRY(launch_overlapped(ln_fwd_kernel<T, V, MODE>, dim3(blocks), 32 * LN_WARPS, 0, stream,
+    DCB_CUDA_TRY(launch_overlapped(ln_fwd_kernel<T, V, MODE, KEEP>, dim3(blocks), 32 * LN_WARPS, 0, stream,
                                    static_cast<const T*>(x), xs, static_cast<T*>(y), ys,
                                    static_cast<const float*>(scale), static_cast<const float*>(bias), eps,
                                    static_cast<float*>(mean), static_cast<float*>(inv_std), g));
     return DCB_OK;
 }
 
-template <class T, int V, int MODE>
+template <class T, int V, int MODE, bool KEEP>
 int32_t ln_launch_bwd(const LnGeom& g, unsigned blocks, const void* x, const RunStrides& xs, const void* dy,
                       const RunStrides& dys, const void* mean, const void* inv_std, const void* scale, void* dx,
                       const RunStrides& dxs, float* partial, cudaStream_t stream)
 {
     const int smem = partial ? 8 * g.c * (LN_WARPS / g.g) : 0;
     if (smem > 32 * 1024)
-        if (int32_t e = allow_dynamic_smem((const void*) ln_bwd_kernel<T, V, MODE>, 8 * LN_MAX_CHANNELS))
+        if (int32_t e = allow_dynamic_smem((const void*) ln_bwd_kernel<T, V, MODE, KEEP>, 8 * LN_MAX_CHANNELS))
             return e;
-    DCB_CUDA_TRY(launch_overlapped(ln_bwd_kernel<T, V, MODE>, dim3(blocks), 32 * LN_WARPS, smem, stream,
+    DCB_CUDA_TRY(launch_overlapped(ln_bwd_kernel<T, V, MODE, KEEP>, dim3(blocks), 32 * LN_WARPS, smem, stream,
                                    static_cast<const T*>(x), xs, static_cast<const T*>(dy), dys,
                                    static_cast<const float*>(mean), static_cast<const float*>(inv_std),
                                    static_cast<const float*>(scale), static_cast<T*>(dx), dxs, partial, g));
     return DCB_OK;
 }
 
-// f(V, MODE) for the choice.
+// f(V, MODE, KEEP) for the choice.
 template <class F>
 int32_t ln_with_shape(const LnChoice& h, F f)
 {
     using std::integral_constant;
-    if (h.mode == LN_ROWS)
-        return f(integral_constant<int, 4>(), integral_constant<int, LN_ROWS>());
-    if (h.mode == LN_SPLIT)
-        return f(integral_constant<int, 4>(), integral_constant<int, LN_SPLIT>());
-    return h.v == 4 ? f(integral_constant<int, 4>(), integral_constant<int, LN_FLAT>())
-                    : f(integral_constant<int, 1>(), integral_constant<int, LN_FLAT>());
+    const auto shape = [&](auto keep) -> int32_t {
+        if (h.mode == LN_ROWS)
+            return f(integral_constant<int, 4>(), integral_constant<int, LN_ROWS>(), keep);
+        if (h.mode == LN_SPLIT)
+            return f(integral_constant<int, 4>(), integral_constant<int, LN_SPLIT>(), keep);
+        return h.v == 4 ? f(integral_constant<int, 4>(), integral_constant<int, LN_FLAT>(), keep)
+                        : f(integral_constant<int, 1>(), integral_constant<int, LN_FLAT>(), keep);
+    };
+    return h.keep ? shape(std::bool_constant<true>()) : shape(std::bool_constant<false>());
 }
 
 } // namespace
@@ -646,8 +686,9 @@ int32_t dcb_ln_fwd(const dcb_nd_desc* xd, int32_t dtype, const void* x, const vo
     const LnGeom g = ln_geometry(rg, h);
     return ln_with_types(dtype, [&](auto t) -> int32_t {
         using T = decltype(t);
-        return ln_with_shape(h, [&](auto v, auto mode) {
-            return ln_launch_fwd<T, decltype(v)::value, decltype(mode)::value>(g, x, xs, y, ys, scale, bias, eps, mean,
+        return ln_with_shape(h, [&](auto v, auto mode, auto keep) {
+            return ln_launch_fwd<T, decltype(v)::value, decltype(mode)::value, decltype(keep)::value>(
+                g, x, xs, y, ys, scale, bias, eps, mean,
                                                                                inv_std, as_stream(stream));
         });
     });
@@ -709,8 +750,9 @@ int32_t dcb_ln_bwd(const dcb_nd_desc* xd, int32_t dtype, const void* x, const dc
     const unsigned blocks = (unsigned) std::min<long long>(g.tiles, (long long) ln_bwd_blocks(h.v) * num_sms());
     const int32_t e = ln_with_types(dtype, [&](auto t) -> int32_t {
         using T = decltype(t);
-        return ln_with_shape(h, [&](auto v, auto mode) {
-            return ln_launch_bwd<T, decltype(v)::value, decltype(mode)::value>(g, blocks, x, xs, dy, dys, mean,
+        return ln_with_shape(h, [&](auto v, auto mode, auto keep) {
+            return ln_launch_bwd<T, decltype(v)::value, decltype(mode)::value, decltype(keep)::value>(
+                g, blocks, x, xs, dy, dys, mean,
                                                                                inv_std, scale, dx, dxs, partial, s);
         });
     });

@@ -199,9 +199,10 @@ int32_t rotary_launch(int v, bool split, dim3 grid, const void* x, const RunStri
     };
     if (split)
         return go(rotary_kernel<TX, TY, 4, true>);
-    return v == 8   ? go(rotary_kernel<TX, TY, 8, false>)
-           : v == 4 ? go(rotary_kernel<TX, TY, 4, false>)
-                    : go(rotary_kernel<TX, TY, 1, false>);
+    if constexpr (sizeof(TX) == 2 || sizeof(TY) == 2)
+        if (v == 8)
+            return go(rotary_kernel<TX, TY, 8, false>);
+    return v == 4 ? go(rotary_kernel<TX, TY, 4, false>) : go(rotary_kernel<TX, TY, 1, false>);
 }
 
 bool same_strides(const dcb_nd_desc& a, const dcb_nd_desc& b)
