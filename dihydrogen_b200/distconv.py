@@ -64,6 +64,9 @@ class _Geometry:
         self.base = t.dtype.itemsize * t.get_local_offset([0] * t.nd)
         self.split_root = t.is_split_root()
         self.owned = tuple(slice(o, o + l) for o, l in reversed(list(zip(self.overlap, self.local))))
+        # all cells and channels of a sample are here
+        self.whole = not any(t.dist.is_distributed(d) and t.dist.locale_shape[d] > 1 for d in range(t.nd - 1))
+        self.operand = None  # descriptor of the owned cells, by reference
         self.descs = {}    # widths -> NdDesc
         self.offsets = {}  # widths -> byte offset of the window
 
@@ -358,8 +361,14 @@ class Tensor:
         if self.dtype is not torch.float32:
             raise TypeError(f"this operator takes tensors of torch.float32, not {self.dtype}")
 
+    def _operand(self):
+        """Descriptor and address of the owned cells, for the operators that take every type."""
+        g = self._geo()
+        if g.operand is None:
+            g.operand = ctypes.byref(self._make_nd_desc())
+        return g.operand, self.buffer.data_ptr() + g.base
+
     def _nd_any(self, lo=None, hi=None):
-        """The same for the operators that take every type."""
         descs = self._geo().descs
         key = (tuple(lo), tuple(hi)) if lo is not None else None
         d = descs.get(key)
@@ -512,17 +521,20 @@ class ChannelSlice:
         self.local_shape = tensor.local_shape[:-2] + [count, tensor.local_shape[-1]]
         self._of = None
 
-    def _nd_any(self):
+    def _geo(self):
+        return self.tensor._geo()
+
+    def _operand(self):
         geo = self.tensor._geo()
         if self._of is not geo:
-            self._of, self._desc = geo, self.tensor._make_nd_desc()
-            self._desc.c = self.count
-            self._base = self.dtype.itemsize * self.first * geo.strides[-2]
-        return ctypes.byref(self._desc)
+            desc = self.tensor._make_nd_desc()
+            desc.c = self.count
+            self._of, self._ref = geo, ctypes.byref(desc)
+            self._base = geo.base + self.dtype.itemsize * self.first * geo.strides[-2]
+        return self._ref, self.tensor.buffer.data_ptr() + self._base
 
     def get_base_ptr(self) -> int:
-        self._nd_any()
-        return self.tensor.get_base_ptr() + self._base
+        return self._operand()[1]
 
 
 # ---------------------------------------------------------------------------
@@ -1509,21 +1521,24 @@ def _workspace(nbytes: int, stream, device):
     return ws, ws.data_ptr()
 
 
-def _check_vector(name, t, shape, dtypes=(torch.float32,), optional=False):
-    """A plain torch operand: the kernels take it as a dense array."""
+def _vector(name, t, count, dtypes=(torch.float32,)):
+    """Address of a plain torch operand, which the kernels take as a dense array; 0 for None."""
     if t is None:
-        if optional:
-            return 0
-        raise ValueError(f"{name} is missing")
-    if t.dtype not in dtypes or not t.is_contiguous() or t.numel() != math.prod(shape):
-        raise ValueError(f"{name} must be a contiguous array of {math.prod(shape)} {dtypes[0]}, not "
-                         f"{list(t.shape)} {t.dtype}")
+        return 0
+    if t.dtype not in dtypes or t.numel() != count or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous array of {count} {dtypes[0]}, not {list(t.shape)} {t.dtype}")
     return t.data_ptr()
+
+
+def _needed(name, t, count):
+    if t is None:
+        raise ValueError(f"{name} is missing")
+    return _vector(name, t, count)
 
 
 def _check_alike(what, first, *others):
     for t in others:
-        if t.local_shape != first.local_shape or t.dtype != first.dtype:
+        if t.local_shape != first.local_shape or t.dtype is not first.dtype:
             raise ValueError(f"{what}: local shapes and types must agree: {first.local_shape} {first.dtype} and "
                              f"{t.local_shape} {t.dtype}")
 
@@ -1543,13 +1558,9 @@ class LayerNormalization:
         self.be, self.num_dims, self.epsilon = backend, num_dims, float(epsilon)
         self._last = (None, 0)
 
-    @staticmethod
-    def _cells(t):
-        return [t.local_shape[-1]] + t.local_shape[:-2]
-
     def new_statistics(self, input: Tensor):
         """Memory for ``mean`` and ``inv_std`` of a tensor like ``input``."""
-        both = torch.empty([2] + [self._cells(input)[0], math.prod(self._cells(input)[1:])], dtype=torch.float32,
+        both = torch.empty([2, input.local_shape[-1], math.prod(input.local_shape[:-2])], dtype=torch.float32,
                            device=input.buffer.device)
         return both[0], both[1]
 
@@ -1557,15 +1568,14 @@ class LayerNormalization:
         """``scale`` and ``bias`` may be None (1 and 0); so may ``mean`` and
         ``inv_std`` where no backward pass follows.  ``output`` may be ``input``."""
         _check_alike("layer normalisation", input, output)
-        C = input.local_shape[-2]
-        cells = self._cells(input)
-        pw, pb = _check_vector("scale", scale, [C], optional=True), _check_vector("bias", bias, [C], optional=True)
-        pm = _check_vector("mean", mean, cells, optional=True)
-        pi = _check_vector("inv_std", inv_std, cells, optional=True)
-        if input.get_local_size() == 0:
+        C, size = input.local_shape[-2], input._geo().size
+        if size == 0:
             return 0
-        call("dcb_ln_fwd", input._nd_any(), _DTYPES[input.dtype], input.get_base_ptr(), pw, pb, self.epsilon,
-             output._nd_any(), output.get_base_ptr(), pm, pi, _stream_ptr(self.be.stream))
+        xd, x = input._operand()
+        yd, y = output._operand()
+        call("dcb_ln_fwd", xd, _DTYPES[input.dtype], x, _vector("scale", scale, C), _vector("bias", bias, C),
+             self.epsilon, yd, y, _vector("mean", mean, size // C), _vector("inv_std", inv_std, size // C),
+             _stream_ptr(self.be.stream))
         return 0
 
     def backward_stage1(self, input: Tensor, d_output: Tensor, mean, inv_std, scale, scale_gradient, bias_gradient,
@@ -1573,29 +1583,29 @@ class LayerNormalization:
         """``d_input`` and this rank's sums of the gradients of scale and bias
         (None: not wanted).  ``d_input`` may be ``d_output`` or ``input``."""
         _check_alike("layer normalisation", input, d_output, d_input)
-        C, s = input.local_shape[-2], self.be.stream
-        cells = self._cells(input)
-        pm, pi = _check_vector("mean", mean, cells), _check_vector("inv_std", inv_std, cells)
-        pw = _check_vector("scale", scale, [C], optional=True)
+        C, s, geo = input.local_shape[-2], self.be.stream, input._geo()
         if (scale_gradient is None) != (bias_gradient is None):
             raise ValueError("the gradients of scale and bias are wanted together")
-        gw = _check_vector("scale_gradient", scale_gradient, [C], optional=True)
-        gb = _check_vector("bias_gradient", bias_gradient, [C], optional=True)
-        if input.get_local_size() == 0:
+        gw, gb = _vector("scale_gradient", scale_gradient, C), _vector("bias_gradient", bias_gradient, C)
+        if geo.size == 0:
             if gw:
                 _zero_on(s, scale_gradient, bias_gradient)
             return 0
-        xd, dtype = input._nd_any(), _DTYPES[input.dtype]
-        nbytes = 0
+        cells = geo.size // C
+        pm, pi = _needed("mean", mean, cells), _needed("inv_std", inv_std, cells)
+        xd, x = input._operand()
+        dyd, dy = d_output._operand()
+        dxd, dx = d_input._operand()
+        dtype = _DTYPES[input.dtype]
+        keep, ws, nbytes = None, 0, 0
         if gw:
-            geo = input._geo()
             if self._last[0] is not geo:
                 self._last = (geo, _abi.lib().dcb_ln_bwd_workspace_bytes(xd, dtype))
             nbytes = self._last[1]
-        keep, ws = _workspace(nbytes, s, input.buffer.device)
-        call("dcb_ln_bwd", xd, dtype, input.get_base_ptr(), d_output._nd_any(), d_output.get_base_ptr(), pm, pi, pw,
-             d_input._nd_any(), d_input.get_base_ptr(), gw, gb, ws, nbytes, _stream_ptr(s))
-        if gw and not input._geo().split_root:  # a replica: its cells count once
+            keep, ws = _workspace(nbytes, s, input.buffer.device)
+        call("dcb_ln_bwd", xd, dtype, x, dyd, dy, pm, pi, _vector("scale", scale, C), dxd, dx, gw, gb, ws, nbytes,
+             _stream_ptr(s))
+        if gw and not geo.split_root:  # a replica: its cells count once
             _zero_on(s, scale_gradient, bias_gradient)
         return 0
 
@@ -1655,15 +1665,17 @@ class RotaryPositions:
             rd.axis_channels[2 - i], rd.origin[2 - i] = axis_channels[i], input.offset[i]
             rd.step[2 - i] = 1.0 if step is None else float(step[i])
         self._local = list(input.local_shape)
-        call("dcb_rotary_plan_create", ctypes.byref(rd), input._nd_any(), ctypes.byref(self._plan))
+        call("dcb_rotary_plan_create", ctypes.byref(rd), ctypes.byref(input._make_nd_desc()), ctypes.byref(self._plan))
 
     def _apply(self, x: Tensor, y: Tensor, inverse):
         if x.local_shape[:-1] != self._local[:-1] or y.local_shape != x.local_shape:
             raise ValueError(f"local shapes {x.local_shape} and {y.local_shape}, set up for {self._local}")
-        if math.prod(x.local_shape) == 0:
+        if x._geo().size == 0:
             return 0
-        call("dcb_rotary_apply", self._plan, x._nd_any(), _DTYPES[x.dtype], x.get_base_ptr(), y._nd_any(),
-             _DTYPES[y.dtype], y.get_base_ptr(), inverse, _stream_ptr(self.be.stream))
+        xd, px = x._operand()
+        yd, py = y._operand()
+        call("dcb_rotary_apply", self._plan, xd, _DTYPES[x.dtype], px, yd, _DTYPES[y.dtype], py, inverse,
+             _stream_ptr(self.be.stream))
         return 0
 
     def forward(self, input: Tensor, output: Tensor):
@@ -1712,30 +1724,28 @@ class Attention:
                                     1.0 / math.sqrt(head_dim) if self.scale is None else self.scale)
             size = []
             for backward in (0, 1):
-                n = _abi.lib().dcb_attention_workspace_bytes(ctypes.byref(ad), q._nd_any(), k._nd_any(), backward)
+                n = _abi.lib().dcb_attention_workspace_bytes(ctypes.byref(ad), q._operand()[0], k._operand()[0], backward)
                 if n < 0:
                     raise ValueError("attention: " + _abi.lib().dcb_last_error().decode())
                 size.append(n)
-            got = self._known[key] = (ad, size)
+            got = self._known[key] = (ctypes.byref(ad), size)
         return got
 
     def _checked(self, q, k, v, q_like, kv_like, lse, q_mask, kv_mask):
         if q.nd != self.num_dims:
             raise ValueError(f"queries of {q.nd} dimensions, set up for {self.num_dims}")
         for t in (q, k, v) + q_like + kv_like:
-            for dim in range(t.nd - 1):
-                if t.dist.is_distributed(dim) and t.dist.locale_shape[dim] > 1:
-                    raise ValueError("attention needs all cells and channels of a sample on one rank: "
-                                     "re-distribute the tensor (TensorShuffler)")
+            if not t._geo().whole:
+                raise ValueError("attention needs all cells and channels of a sample on one rank: re-distribute the "
+                                 "tensor (TensorShuffler)")
         _check_alike("attention", q, *q_like)
         _check_alike("attention", k, v, *kv_like)
-        if q.dtype != k.dtype or q.local_shape[-1] != k.local_shape[-1]:
+        if q.dtype is not k.dtype or q.local_shape[-1] != k.local_shape[-1]:
             raise ValueError("attention: queries and keys differ in type or samples")
         n, cells_q, cells_k = q.local_shape[-1], math.prod(q.local_shape[:-2]), math.prod(k.local_shape[:-2])
-        masks = (torch.bool, torch.uint8)
-        return (_check_vector("lse", lse, [n, self.q_heads, cells_q]),
-                _check_vector("q_mask", q_mask, [n, cells_q], masks, True),
-                _check_vector("kv_mask", kv_mask, [n, cells_k], masks, True))
+        return (_needed("lse", lse, n * self.q_heads * cells_q),
+                _vector("q_mask", q_mask, n * cells_q, (torch.bool, torch.uint8)),
+                _vector("kv_mask", kv_mask, n * cells_k, (torch.bool, torch.uint8)))
 
     def forward(self, q, k, v, output: Tensor, lse, q_mask=None, kv_mask=None):
         pl, pq, pk = self._checked(q, k, v, (output,), (), lse, q_mask, kv_mask)
@@ -1744,9 +1754,8 @@ class Attention:
         ad, size = self._desc(q, k)
         s = self.be.stream
         keep, ws = _workspace(size[0], s, lse.device)
-        call("dcb_attention_fwd", ctypes.byref(ad), q._nd_any(), q.get_base_ptr(), k._nd_any(), k.get_base_ptr(),
-             v._nd_any(), v.get_base_ptr(), pq, pk, output._nd_any(), output.get_base_ptr(), pl, ws, size[0],
-             _stream_ptr(s))
+        call("dcb_attention_fwd", ad, *q._operand(), *k._operand(), *v._operand(), pq, pk, *output._operand(), pl, ws,
+             size[0], _stream_ptr(s))
         return 0
 
     def backward(self, q, k, v, output: Tensor, lse, d_output: Tensor, d_q, d_k, d_v, q_mask=None, kv_mask=None):
@@ -1757,10 +1766,8 @@ class Attention:
         ad, size = self._desc(q, k)
         s = self.be.stream
         keep, ws = _workspace(size[1], s, lse.device)
-        call("dcb_attention_bwd", ctypes.byref(ad), q._nd_any(), q.get_base_ptr(), k._nd_any(), k.get_base_ptr(),
-             v._nd_any(), v.get_base_ptr(), pq, pk, output._nd_any(), output.get_base_ptr(), pl, d_output._nd_any(),
-             d_output.get_base_ptr(), d_q._nd_any(), d_q.get_base_ptr(), d_k._nd_any(), d_k.get_base_ptr(),
-             d_v._nd_any(), d_v.get_base_ptr(), ws, size[1], _stream_ptr(s))
+        call("dcb_attention_bwd", ad, *q._operand(), *k._operand(), *v._operand(), pq, pk, *output._operand(), pl,
+             *d_output._operand(), *d_q._operand(), *d_k._operand(), *d_v._operand(), ws, size[1], _stream_ptr(s))
         return 0
 
     def status(self) -> int:
