@@ -24,15 +24,20 @@ template <int D>
 __device__ __forceinline__ void as_load(float* to, const AttnTensor& t, long long n, int head, int d, int cell0,
                                         int cells, const uint8_t* mask)
 {
-    const float* p = static_cast<const float*>(t.p) + n * t.sn + (long long) head * d * t.sc + cell0;
-    const int j = threadIdx.x & 63;
-    const bool there = cell0 + j < cells && (!mask || mask[cell0 + j]);
-    for (int c = threadIdx.x >> 6; c < D; c += AS_THREADS / 64)
+    const int j = threadIdx.x & 63, c0 = threadIdx.x >> 6;
+    const bool in = cell0 + j < cells, there = in && (!mask || mask[cell0 + j]);
+    const float* p = static_cast<const float*>(t.p) + n * t.sn + ((long long) head * d + c0) * t.sc + cell0 + j;
+    // eight loads go out before the first is waited for
+#pragma unroll
+    for (int k0 = 0; k0 < D / 4; k0 += 8)
     {
-        float v[1] = {0.f};
-        if (there && c < d)
-            load_elems<1>(p + c * t.sc + j, v);
-        to[c * AS_PITCH + j] = v[0];
+        float v[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+            v[k] = in && c0 + 4 * (k0 + k) < d ? p[4 * (k0 + k) * t.sc] : 0.f;
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+            to[(c0 + 4 * (k0 + k)) * AS_PITCH + j] = there ? v[k] : 0.f;
     }
 }
 
@@ -59,6 +64,13 @@ __device__ __forceinline__ void as_scores(const float* A, const float* B, int tx
     }
 }
 
+// Row t of a tile of weights lies at as_row(t): the rows that neighbouring threads write are neighbours then, four banks
+// apart, and are written as 16 bytes.
+__device__ __forceinline__ int as_row(int t)
+{
+    return ((t & 3) * 16 + (t >> 2)) * AS_PITCH;
+}
+
 // acc[e][r] += sum_t W[t][4 ty + e] X[tx + 16 r][t]
 template <int D>
 __device__ __forceinline__ void as_accumulate(const float* W, const float* X, int tx, int ty, float (&acc)[4][D / 16])
@@ -69,7 +81,7 @@ __device__ __forceinline__ void as_accumulate(const float* W, const float* X, in
         float w[4][4];
 #pragma unroll
         for (int u = 0; u < 4; ++u)
-            load_elems<4>(W + (t + u) * AS_PITCH + 4 * ty, w[u]);
+            load_elems<4>(W + as_row(t + u) + 4 * ty, w[u]);
 #pragma unroll
         for (int r = 0; r < D / 16; ++r)
         {
@@ -107,6 +119,17 @@ __device__ __forceinline__ void as_store(const AttnTensor& t, float* part, long 
             else
                 store_elems<1>(static_cast<float*>(t.p) + n * t.sn + ((long long) head * d + c) * t.sc + i, v);
         }
+    }
+}
+
+// A thread's 4 x 4 scores as rows 4 tx ... of a tile [key][query].
+__device__ __forceinline__ void as_put_by_column(float* W, int tx, int ty, const float (&s)[4][4])
+{
+#pragma unroll
+    for (int b = 0; b < 4; ++b)
+    {
+        const float v[4] = {s[0][b], s[1][b], s[2][b], s[3][b]};
+        store_elems<4>(W + as_row(4 * tx + b) + 4 * ty, v);
     }
 }
 
@@ -204,10 +227,8 @@ __global__ void __launch_bounds__(AS_THREADS) attn_simt_fwd_kernel(AttnProblem p
 #pragma unroll
             for (int r = 0; r < D / 16; ++r)
                 acc[a][r] *= shrink;
-#pragma unroll
-            for (int b = 0; b < 4; ++b)
-                P[(4 * tx + b) * AS_PITCH + 4 * ty + a] = s[a][b];
         }
+        as_put_by_column(P, tx, ty, s);
         __syncthreads();
         as_accumulate<D>(P, V, tx, ty, acc);
     }
@@ -262,16 +283,17 @@ __device__ __forceinline__ void as_weights(const AttnProblem& p, const float* Q,
             const int j = 4 * tx + b;
             const bool ok = see[j] && (!p.causal || j0 + j <= i0 + i + p.offset);
             const float w = ok ? exp2f(fmaf(s[a][b], p.scale, -top)) : 0.f;
-            const float g = w == 0.f ? 0.f : w * (dp[a][b] - del);
-            if (BY_KEY)
-            {
-                P[i * AS_PITCH + j] = w;
-                dS[i * AS_PITCH + j] = g;
-            }
-            else
-                dS[j * AS_PITCH + i] = g;
+            dp[a][b] = w == 0.f ? 0.f : w * (dp[a][b] - del);
+            s[a][b] = w;
+        }
+        if (BY_KEY) // [query][key]
+        {
+            store_elems<4>(P + as_row(i) + 4 * tx, s[a]);
+            store_elems<4>(dS + as_row(i) + 4 * tx, dp[a]);
         }
     }
+    if (!BY_KEY)
+        as_put_by_column(dS, tx, ty, dp);
 }
 
 __device__ __forceinline__ void as_load_stats(const AttnProblem& p, long long nh, int i0, float* lse, float* delta)
