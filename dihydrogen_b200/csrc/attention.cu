@@ -6,6 +6,120 @@ namespace dcb
 namespace
 {
 
+constexpr int ATTN_INDEX_THREADS = 1024, ATTN_INDEX_CELLS = 8; // cells of a thread at a time
+
+// What a mask leaves of a sample's cells, in order.  A block a sample and side.
+__global__ void __launch_bounds__(ATTN_INDEX_THREADS) attn_index_kernel(const __grid_constant__ AttnProblem p)
+{
+    __shared__ int of_warp[32];
+    __shared__ int all;
+    const uint8_t* mask = blockIdx.y ? p.kv_mask : p.q_mask;
+    const AttnSide side = blockIdx.y ? p.kv_side : p.q_side;
+    const int cells = blockIdx.y ? p.sk : p.sq;
+    if (!mask)
+        return;
+    wait_for_previous_kernel(mask);
+    dependents_may_start();
+    const long long n = blockIdx.x;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    mask += n * cells;
+    int* index = side.index + n * cells;
+    int* before = side.before + n * (cells + 1ll);
+    int base = 0;
+    for (long long c0 = 0; c0 < cells; c0 += ATTN_INDEX_THREADS * ATTN_INDEX_CELLS)
+    {
+        const long long i0 = c0 + threadIdx.x * ATTN_INDEX_CELLS;
+        uint32_t bits = 0;
+        for (int e = 0; e < ATTN_INDEX_CELLS; ++e)
+            if (i0 + e < cells && mask[i0 + e])
+                bits |= 1u << e;
+        const int mine = __popc(bits);
+        int sum = mine; // of this lane and those before
+        for (int h = 1; h < 32; h *= 2)
+        {
+            const int other = __shfl_up_sync(~0u, sum, h);
+            sum += lane >= h ? other : 0;
+        }
+        if (lane == 31)
+            of_warp[warp] = sum;
+        __syncthreads();
+        if (warp == 0)
+        {
+            int w = of_warp[lane];
+            for (int h = 1; h < 32; h *= 2)
+            {
+                const int other = __shfl_up_sync(~0u, w, h);
+                w += lane >= h ? other : 0;
+            }
+            of_warp[lane] = w;
+            if (lane == 31)
+                all = w;
+        }
+        __syncthreads();
+        int at = base + sum - mine + (warp > 0 ? of_warp[warp - 1] : 0);
+        for (int e = 0; e < ATTN_INDEX_CELLS; ++e)
+            if (i0 + e < cells)
+            {
+                before[i0 + e] = at;
+                if (bits >> e & 1)
+                    index[at++] = (int) (i0 + e);
+            }
+        base += all;
+        __syncthreads();
+    }
+    if (threadIdx.x == 0)
+    {
+        before[cells] = base;
+        side.count[n] = base;
+    }
+}
+
+// Zeros (and lse = -infinity) in the cells that a mask takes out of a result.
+struct AttnZeros
+{
+    AttnTensor t;
+    const uint8_t* mask;
+    long long rows; // of a sample
+    int cells;
+    float* lse;     // with as many rows as heads; null
+    int heads;
+};
+
+constexpr int ATTN_ZERO_ROWS = 16; // that a thread writes for one look at the mask
+
+struct AttnZeroJobs
+{
+    AttnZeros job[3];
+    int n;
+};
+
+template <class T>
+__global__ void __launch_bounds__(256) attn_zero_kernel(const __grid_constant__ AttnZeroJobs a)
+{
+    const AttnZeros& z = a.job[blockIdx.y];
+    const uint8_t* mask = z.mask;
+    wait_for_previous_kernel(mask);
+    dependents_may_start();
+    const int chunks = (z.cells + 255) / 256;
+    const long long rows = z.rows + z.heads; // of a sample: the tensor's, then lse's
+    const long long groups = (rows + ATTN_ZERO_ROWS - 1) / ATTN_ZERO_ROWS;
+    for (long long u = blockIdx.x; u < a.n * groups * chunks; u += gridDim.x)
+    {
+        const long long m = u / chunks, n = m / groups, row0 = (m - n * groups) * ATTN_ZERO_ROWS;
+        const int i = (int) (u - m * chunks) * 256 + threadIdx.x;
+        if (i >= z.cells || mask[n * z.cells + i])
+            continue;
+        T* to = static_cast<T*>(z.t.p) + n * z.t.sn + i;
+        const float v[1] = {0.f};
+#pragma unroll 4
+        for (long long row = row0; row < row0 + ATTN_ZERO_ROWS; ++row)
+            if (row < z.rows)
+                store_elems<1>(to + row * z.t.sc, v);
+            else if (row < rows)
+                z.lse[(n * z.heads + row - z.rows) * z.cells + i] = -INFINITY;
+    }
+}
+
 // Joins the parts of a split axis of keys: o = sum_s part_s 2^(m_s - m) / sum_s l_s 2^(m_s - m).
 template <class T>
 __global__ void __launch_bounds__(256) attn_join_fwd_kernel(AttnProblem p)
@@ -130,7 +244,7 @@ __global__ void __launch_bounds__(32 * ATTN_STATS_WARPS) attn_stats_kernel(AttnP
                 delta += part[w][threadIdx.x];
             const int at_cell = i < count && index ? index[i] : i;
             const float lse = i < count ? p.lse[nh * p.sq + at_cell] : -INFINITY;
-            const bool none = lse == -INFINITY || (p.q_mask && !p.q_mask[n * p.sq + at_cell]);
+            const bool none = lse == -INFINITY;
             p.stats[nh * p.stats_pitch + i] = none ? INFINITY : lse * ATTN_LOG2E;
             p.stats[heads * p.stats_pitch + nh * p.stats_pitch + i] = none ? 0.f : delta;
         }
@@ -265,6 +379,15 @@ int64_t attn_carve(AttnProblem* p, int32_t dtype, bool backward, void* workspace
     (tc ? attn_tc_splits : attn_simt_splits)(p, backward);
     const long long qh = (long long) p->n * p->q_heads, kh = (long long) p->n * p->kv_heads;
     p->stats_pitch = tc ? (long long) attn_tiles(p->sq, 128) * 128 : p->sq;
+    const auto side = [&](int cells, bool masked) {
+        AttnSide t;
+        t.index = reinterpret_cast<int*>(w.floats((long long) p->n * cells));
+        t.before = reinterpret_cast<int*>(w.floats((long long) p->n * (cells + 1)));
+        t.count = reinterpret_cast<int*>(w.floats(p->n));
+        return masked ? t : AttnSide{};
+    };
+    p->q_side = side(p->sq, p->q_mask != nullptr);
+    p->kv_side = side(p->sk, p->kv_mask != nullptr);
     if (tc)
     {
         const auto copy = [&](long long heads, int cells) {
@@ -274,15 +397,6 @@ int64_t attn_carve(AttnProblem* p, int32_t dtype, bool backward, void* workspace
         p->copy_k = copy(kh, p->sk);
         p->copy_v = copy(kh, p->sk);
         p->copy_do = backward ? copy(qh, p->sq) : nullptr;
-        const auto side = [&](int cells, bool masked) {
-            AttnSide t;
-            t.index = reinterpret_cast<int*>(w.floats((long long) p->n * cells));
-            t.before = reinterpret_cast<int*>(w.floats((long long) p->n * (cells + 1)));
-            t.count = reinterpret_cast<int*>(w.floats(p->n));
-            return masked ? t : AttnSide{};
-        };
-        p->q_side = side(p->sq, p->q_mask != nullptr);
-        p->kv_side = side(p->sk, p->kv_mask != nullptr);
     }
     if (!backward)
     {
@@ -326,6 +440,47 @@ int32_t attn_join_grad(int32_t dtype, const float* part, int splits, const AttnT
                                                                            32ll * num_sms())),
                                        256, 0, s, part,
                                        splits, t, n, heads, d, cells, mask));
+        return DCB_OK;
+    });
+}
+
+// What the masks leave of both sides.
+int32_t attn_index(const AttnProblem& p, cudaStream_t s)
+{
+    if (!p.q_mask && !p.kv_mask)
+        return DCB_OK;
+    DCB_CUDA_TRY(launch_overlapped(attn_index_kernel, dim3(p.n, 2), ATTN_INDEX_THREADS, 0, s, p));
+    return DCB_OK;
+}
+
+// The results' cells that the masks take out, of those that no join writes.
+int32_t attn_zeros(const AttnProblem& p, int32_t dtype, bool backward, cudaStream_t s)
+{
+    AttnZeroJobs a = {};
+    int jobs = 0;
+    long long units = 0;
+    const auto add = [&](const AttnTensor& t, int heads, int cells, const uint8_t* mask, float* lse) {
+        if (!mask)
+            return;
+        a.job[jobs++] = AttnZeros{t, mask, (long long) heads * p.d, cells, lse, lse ? heads : 0};
+        units = std::max(units, (long long) p.n * (heads * (p.d + 1ll) / ATTN_ZERO_ROWS + 1) * ((cells + 255) / 256));
+    };
+    if (!backward && p.kv_splits == 1)
+        add(p.o, p.q_heads, p.sq, p.q_mask, p.lse);
+    if (backward && p.kv_splits == 1)
+        add(p.dq, p.q_heads, p.sq, p.q_mask, nullptr);
+    if (backward && p.q_splits == 1)
+    {
+        add(p.dk, p.kv_heads, p.sk, p.kv_mask, nullptr);
+        add(p.dv, p.kv_heads, p.sk, p.kv_mask, nullptr);
+    }
+    if (jobs == 0)
+        return DCB_OK;
+    a.n = p.n;
+    return with_type(dtype, [&](auto e) -> int32_t {
+        DCB_CUDA_TRY(launch_overlapped(attn_zero_kernel<decltype(e)>,
+                                       dim3((unsigned) std::min<long long>(units, 16ll * num_sms()), jobs), 256, 0, s,
+                                       a));
         return DCB_OK;
     });
 }
@@ -377,9 +532,10 @@ int32_t dcb_attention_fwd(const dcb_attention_desc* ad, const dcb_nd_desc* qd, c
                          (long long) p.n * p.q_heads * p.sq, s);
     if (int32_t e = attn_workspace(&p, ad->dtype, false, workspace, workspace_bytes))
         return e;
-    if (ad->dtype == DCB_BF16)
-        if (int32_t e = attn_tc_index(p, s))
-            return e;
+    if (int32_t e = attn_index(p, s))
+        return e;
+    if (int32_t e = attn_zeros(p, ad->dtype, false, s))
+        return e;
     if (int32_t e = ad->dtype == DCB_BF16 ? attn_tc_fwd(p, s) : attn_simt_fwd(p, s))
         return e;
     if (p.kv_splits == 1)
@@ -429,9 +585,10 @@ int32_t dcb_attention_bwd(const dcb_attention_desc* ad, const dcb_nd_desc* qd, c
     p.kv_mask = static_cast<const uint8_t*>(kv_mask);
     if (int32_t e = attn_workspace(&p, ad->dtype, true, workspace, workspace_bytes))
         return e;
-    if (ad->dtype == DCB_BF16)
-        if (int32_t err = attn_tc_index(p, s))
-            return err;
+    if (int32_t err = attn_index(p, s))
+        return err;
+    if (int32_t err = attn_zeros(p, ad->dtype, true, s))
+        return err;
     const int32_t e = with_type(ad->dtype, [&](auto t) -> int32_t {
         DCB_CUDA_TRY(launch_overlapped(attn_stats_kernel<decltype(t)>,
                                        dim3((unsigned) std::min<long long>(

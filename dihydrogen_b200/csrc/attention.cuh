@@ -19,7 +19,7 @@ struct AttnTensor
     long long sn, sc; // element strides of samples and channels
 };
 
-// The cells of a side that a mask leaves, for the tensor-core kernels: they see those cells only, one after the other.
+// The cells of a side that a mask leaves: the kernels see those only, one after the other.
 // Per sample the cells' indices, how many lie before a cell, how many there are.  Null without a mask.
 struct AttnSide
 {
@@ -44,12 +44,40 @@ struct AttnProblem
     //   forward  [splits][n * q_heads][d][sq] sums and [splits][2][n * q_heads][sq] maxima, sums of weights
     //   backward [splits][n * heads][d][cells] sums
     float *part_o, *part_ml, *part_dq, *part_dk, *part_dv;
-    // Tensor cores: what the masks leave, and copies of tensors that bulk copies cannot address or whose cells a mask
-    // picks, [n][heads * d][pitch] with rows of whole 16 bytes.
     AttnSide q_side, kv_side;
+    // Tensor cores: copies of tensors that bulk copies cannot address or whose cells a mask picks, [n][heads * d][pitch]
+    // with rows of whole 16 bytes.
     bf16 *copy_q, *copy_k, *copy_v, *copy_do;
     int q_splits, kv_splits; // of the queries' axis (dk, dv), of the keys' axis (o, dq)
 };
+
+// One sample's cells on one side, as the kernels count them: all, or those that a mask leaves.
+struct AttnCells
+{
+    int count, cells;
+    const int *index, *counted;
+    __device__ __forceinline__ AttnCells(const AttnSide& s, long long n, int cells_) : cells(cells_)
+    {
+        index = s.index ? s.index + n * cells : nullptr;
+        counted = s.index ? s.before + n * (cells + 1ll) : nullptr;
+        count = s.index ? s.count[n] : cells;
+    }
+    __device__ __forceinline__ int cell(int r) const { return index ? index[r] : r; }
+    // How many lie before cell x of the grid.
+    __device__ __forceinline__ int before(long long x) const
+    {
+        const int c = (int) (x < 0 ? 0 : x > cells ? cells : x);
+        return counted ? counted[c] : c;
+    }
+};
+
+// Row r of the queries sees the first so many keys; later rows see no fewer.
+__device__ __forceinline__ int attn_limit(const AttnProblem& p, const AttnCells& q, const AttnCells& kv, int r)
+{
+    if (r < 0 || r >= q.count)
+        return 0;
+    return p.causal ? kv.before((long long) q.cell(r) + p.offset + 1) : kv.count;
+}
 
 __host__ __device__ inline int attn_tiles(int cells, int tile)
 {
@@ -64,13 +92,11 @@ inline int attn_splits(long long work, int steps, long long slots, int least)
     return (int) std::max<long long>(1, std::min<long long>(slots / work, steps / least));
 }
 
-// Kernels of attention_tc.cu (bf16) and attention_simt.cu (fp32).
-int32_t attn_tc_index(const AttnProblem& p, cudaStream_t stream); // fills the sides; before the others
+// Kernels of attention_tc.cu (bf16) and attention_simt.cu (fp32), both behind attn_index, which fills the sides.
 int32_t attn_tc_fwd(const AttnProblem& p, cudaStream_t stream);
 int32_t attn_tc_bwd(const AttnProblem& p, cudaStream_t stream);
 void attn_tc_splits(AttnProblem* p, bool backward);
 int* attn_tc_status(); // device word of the current device
-
 int32_t attn_simt_fwd(const AttnProblem& p, cudaStream_t stream);
 int32_t attn_simt_bwd(const AttnProblem& p, cudaStream_t stream);
 void attn_simt_splits(AttnProblem* p, bool backward);

@@ -18,15 +18,16 @@ constexpr int AS_PITCH = 68; // floats: rows 16-byte aligned, four rows on diffe
 constexpr int AS_THREADS = 256;
 constexpr int AS_LEAST = 4;  // tiles a part of a split axis walks at least
 
-// One head's cells [cell0, cell0 + 64) to shared memory as [channel][cell]; cells that are not there, and channels up to
-// D, as zeros.
+// One head's cells, 64 from the r0-th on of those that are there, to shared memory as [channel][cell]; cells that are not,
+// and channels up to D, as zeros.
 template <int D>
-__device__ __forceinline__ void as_load(float* to, const AttnTensor& t, long long n, int head, int d, int cell0,
-                                        int cells, const uint8_t* mask)
+__device__ __forceinline__ void as_load(float* to, const AttnTensor& t, long long n, int head, int d, int r0,
+                                        const AttnCells& cells)
 {
     const int j = threadIdx.x & 63, c0 = threadIdx.x >> 6;
-    const bool in = cell0 + j < cells, there = in && (!mask || mask[cell0 + j]);
-    const float* p = static_cast<const float*>(t.p) + n * t.sn + ((long long) head * d + c0) * t.sc + cell0 + j;
+    const bool in = r0 + j < cells.count;
+    const float* p = static_cast<const float*>(t.p) + n * t.sn + ((long long) head * d + c0) * t.sc
+                     + (in ? cells.cell(r0 + j) : 0);
     // eight loads go out before the first is waited for
 #pragma unroll
     for (int k0 = 0; k0 < D / 4; k0 += 8)
@@ -37,7 +38,7 @@ __device__ __forceinline__ void as_load(float* to, const AttnTensor& t, long lon
             v[k] = in && c0 + 4 * (k0 + k) < d ? p[4 * (k0 + k) * t.sc] : 0.f;
 #pragma unroll
         for (int k = 0; k < 8; ++k)
-            to[(c0 + 4 * (k0 + k)) * AS_PITCH + j] = there ? v[k] : 0.f;
+            to[(c0 + 4 * (k0 + k)) * AS_PITCH + j] = v[k];
     }
 }
 
@@ -99,25 +100,23 @@ __device__ __forceinline__ void as_accumulate(const float* W, const float* X, in
 // Results of 4 cells x D / 16 channels: to the tensor, or as a part to [head][channel][cell].
 template <int D>
 __device__ __forceinline__ void as_store(const AttnTensor& t, float* part, long long nh, long long n, int head, int d,
-                                         int cell0, int cells, int tx, int ty, const float (&acc)[4][D / 16])
+                                         int r0, const AttnCells& side, int tx, int ty, const float (&acc)[4][D / 16])
 {
 #pragma unroll
-    for (int r = 0; r < D / 16; ++r)
+    for (int e = 0; e < 4; ++e)
     {
-        const int c = tx + 16 * r;
-        if (c >= d)
+        const int row = r0 + 4 * ty + e;
+        if (row >= side.count)
             continue;
+        const int i = side.cell(row);
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
+        for (int r = 0; r < D / 16; ++r)
         {
-            const int i = cell0 + 4 * ty + e;
-            if (i >= cells)
-                continue;
-            const float v[1] = {acc[e][r]};
-            if (part)
-                part[(nh * d + c) * cells + i] = v[0];
-            else
-                store_elems<1>(static_cast<float*>(t.p) + n * t.sn + ((long long) head * d + c) * t.sc + i, v);
+            const int c = tx + 16 * r;
+            if (c < d)
+                (part ? part + (nh * d + c) * side.cells
+                      : static_cast<float*>(t.p) + n * t.sn + ((long long) head * d + c) * t.sc)[i]
+                    = acc[e][r];
         }
     }
 }
@@ -165,13 +164,17 @@ __global__ void __launch_bounds__(AS_THREADS) attn_simt_fwd_kernel(AttnProblem p
 {
     extern __shared__ float smem[];
     float *Q = smem, *K = Q + D * AS_PITCH, *V = K + D * AS_PITCH, *P = V + D * AS_PITCH;
-    __shared__ uint8_t see[AS_TILE];
     const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
     const AsAt at = as_at(attn_tiles(p.sq, AS_TILE), p.kv_splits, p.q_heads);
     const int i0 = at.tile * AS_TILE, kv_head = at.head / p.group;
-    const uint8_t* qm = p.q_mask ? p.q_mask + at.n * p.sq : nullptr;
-    const uint8_t* km = p.kv_mask ? p.kv_mask + at.n * p.sk : nullptr;
-    as_load<D>(Q, p.q, at.n, at.head, p.d, i0, p.sq, qm);
+    const AttnCells q(p.q_side, at.n, p.sq), kv(p.kv_side, at.n, p.sk);
+    if (i0 >= q.count)
+        return;
+    as_load<D>(Q, p.q, at.n, at.head, p.d, i0, q);
+    int limit[4]; // keys that a row sees
+#pragma unroll
+    for (int a = 0; a < 4; ++a)
+        limit[a] = attn_limit(p, q, kv, i0 + 4 * ty + a);
     float m[4], l[4], acc[4][D / 16];
 #pragma unroll
     for (int a = 0; a < 4; ++a)
@@ -182,17 +185,14 @@ __global__ void __launch_bounds__(AS_THREADS) attn_simt_fwd_kernel(AttnProblem p
             acc[a][r] = 0.f;
     }
     int lo, hi;
-    as_range(attn_tiles(p.sk, AS_TILE), p.kv_splits, at.split, &lo, &hi);
-    if (p.causal)
-        hi = (int) min((long long) hi, max(0ll, (long long) i0 + AS_TILE - 1 + p.offset + AS_TILE) / AS_TILE);
+    as_range(attn_tiles(kv.count, AS_TILE), p.kv_splits, at.split, &lo, &hi);
+    hi = min(hi, attn_tiles(attn_limit(p, q, kv, min(i0 + AS_TILE, q.count) - 1), AS_TILE));
     for (int t = lo; t < hi; ++t)
     {
         const int j0 = t * AS_TILE;
         __syncthreads();
-        as_load<D>(K, p.k, at.n, kv_head, p.d, j0, p.sk, km);
-        as_load<D>(V, p.v, at.n, kv_head, p.d, j0, p.sk, km);
-        if (threadIdx.x < AS_TILE)
-            see[threadIdx.x] = j0 + (int) threadIdx.x < p.sk && (!km || km[j0 + threadIdx.x]);
+        as_load<D>(K, p.k, at.n, kv_head, p.d, j0, kv);
+        as_load<D>(V, p.v, at.n, kv_head, p.d, j0, kv);
         __syncthreads();
         float s[4][4];
         as_scores<D>(Q, K, tx, ty, s);
@@ -203,9 +203,7 @@ __global__ void __launch_bounds__(AS_THREADS) attn_simt_fwd_kernel(AttnProblem p
 #pragma unroll
             for (int b = 0; b < 4; ++b)
             {
-                const int j = 4 * tx + b;
-                const bool ok = see[j] && (!p.causal || j0 + j <= i0 + 4 * ty + a + p.offset);
-                s[a][b] = ok ? s[a][b] * p.scale : -INFINITY;
+                s[a][b] = j0 + 4 * tx + b < limit[a] ? s[a][b] * p.scale : -INFINITY;
                 top = fmaxf(top, s[a][b]);
             }
 #pragma unroll
@@ -238,36 +236,36 @@ __global__ void __launch_bounds__(AS_THREADS) attn_simt_fwd_kernel(AttnProblem p
         if (tx == 0)
 #pragma unroll
             for (int a = 0; a < 4; ++a)
-                if (i0 + 4 * ty + a < p.sq)
+                if (i0 + 4 * ty + a < q.count)
                 {
-                    float* ml = p.part_ml + (2 * heads * at.split + at.nh) * p.sq + i0 + 4 * ty + a;
+                    float* ml = p.part_ml + (2 * heads * at.split + at.nh) * p.sq + q.cell(i0 + 4 * ty + a);
                     ml[0] = m[a];
                     ml[heads * p.sq] = l[a];
                 }
-        as_store<D>(p.o, p.part_o + at.split * heads * p.d * p.sq, at.nh, at.n, at.head, p.d, i0, p.sq, tx, ty,
-                       acc);
+        as_store<D>(p.o, p.part_o + at.split * heads * p.d * p.sq, at.nh, at.n, at.head, p.d, i0, q, tx, ty,
+                    acc);
         return;
     }
 #pragma unroll
     for (int a = 0; a < 4; ++a)
     {
         const int i = i0 + 4 * ty + a;
-        const bool none = l[a] == 0.f || (qm && i < p.sq && !qm[i]);
+        const bool none = l[a] == 0.f;
         const float f = none ? 0.f : 1.f / l[a];
 #pragma unroll
         for (int r = 0; r < D / 16; ++r)
             acc[a][r] = none ? 0.f : acc[a][r] * f;
-        if (tx == 0 && i < p.sq)
-            p.lse[at.nh * p.sq + i] = none ? -INFINITY : (m[a] + log2f(l[a])) / ATTN_LOG2E;
+        if (tx == 0 && i < q.count)
+            p.lse[at.nh * p.sq + q.cell(i)] = none ? -INFINITY : (m[a] + log2f(l[a])) / ATTN_LOG2E;
     }
-    as_store<D>(p.o, nullptr, at.nh, at.n, at.head, p.d, i0, p.sq, tx, ty, acc);
+    as_store<D>(p.o, nullptr, at.nh, at.n, at.head, p.d, i0, q, tx, ty, acc);
 }
 
 // The weights and their gradients of a tile, P = exp2(s - lse), dS = P (dP - delta): [query][key] or [key][query].
 template <int D, bool BY_KEY>
 __device__ __forceinline__ void as_weights(const AttnProblem& p, const float* Q, const float* K, const float* V,
-                                           const float* dO, const float* lse, const float* delta, const uint8_t* see,
-                                           int i0, int j0, int tx, int ty, float* P, float* dS)
+                                           const float* dO, const float* lse, const float* delta,
+                                           const int* limit, int j0, int tx, int ty, float* P, float* dS)
 {
     float s[4][4], dp[4][4];
     as_scores<D>(Q, K, tx, ty, s);
@@ -277,12 +275,11 @@ __device__ __forceinline__ void as_weights(const AttnProblem& p, const float* Q,
     {
         const int i = 4 * ty + a;
         const float top = lse[i], del = delta[i];
+        const int seen = limit[i];
 #pragma unroll
         for (int b = 0; b < 4; ++b)
         {
-            const int j = 4 * tx + b;
-            const bool ok = see[j] && (!p.causal || j0 + j <= i0 + i + p.offset);
-            const float w = ok ? exp2f(fmaf(s[a][b], p.scale, -top)) : 0.f;
+            const float w = j0 + 4 * tx + b < seen ? exp2f(fmaf(s[a][b], p.scale, -top)) : 0.f;
             dp[a][b] = w == 0.f ? 0.f : w * (dp[a][b] - del);
             s[a][b] = w;
         }
@@ -296,13 +293,15 @@ __device__ __forceinline__ void as_weights(const AttnProblem& p, const float* Q,
         as_put_by_column(dS, tx, ty, dp);
 }
 
-__device__ __forceinline__ void as_load_stats(const AttnProblem& p, long long nh, int i0, float* lse, float* delta)
+__device__ __forceinline__ void as_load_stats(const AttnProblem& p, const AttnCells& q, const AttnCells& kv,
+                                              long long nh, int i0, float* lse, float* delta, int* limit)
 {
     if (threadIdx.x < AS_TILE)
     {
         const int i = i0 + threadIdx.x;
-        lse[threadIdx.x] = i < p.sq ? p.stats[nh * p.stats_pitch + i] : INFINITY;
-        delta[threadIdx.x] = i < p.sq ? p.stats[((long long) p.n * p.q_heads + nh) * p.stats_pitch + i] : 0.f;
+        limit[threadIdx.x] = attn_limit(p, q, kv, i);
+        lse[threadIdx.x] = i < q.count ? p.stats[nh * p.stats_pitch + i] : INFINITY;
+        delta[threadIdx.x] = i < q.count ? p.stats[((long long) p.n * p.q_heads + nh) * p.stats_pitch + i] : 0.f;
     }
 }
 
@@ -313,36 +312,35 @@ __global__ void __launch_bounds__(AS_THREADS) attn_simt_dkv_kernel(AttnProblem p
     float *K = smem, *V = K + D * AS_PITCH, *Q = V + D * AS_PITCH, *dO = Q + D * AS_PITCH, *P = dO + D * AS_PITCH,
           *dS = P + AS_TILE * AS_PITCH;
     __shared__ float lse[AS_TILE], delta[AS_TILE];
-    __shared__ uint8_t see[AS_TILE];
+    __shared__ int limit[AS_TILE];
     const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
     const AsAt at = as_at(attn_tiles(p.sk, AS_TILE), p.q_splits, p.kv_heads);
     const int j0 = at.tile * AS_TILE;
-    const uint8_t* qm = p.q_mask ? p.q_mask + at.n * p.sq : nullptr;
-    const uint8_t* km = p.kv_mask ? p.kv_mask + at.n * p.sk : nullptr;
-    as_load<D>(K, p.k, at.n, at.head, p.d, j0, p.sk, km);
-    as_load<D>(V, p.v, at.n, at.head, p.d, j0, p.sk, km);
-    if (threadIdx.x < AS_TILE)
-        see[threadIdx.x] = j0 + (int) threadIdx.x < p.sk && (!km || km[j0 + threadIdx.x]);
+    const AttnCells q(p.q_side, at.n, p.sq), kv(p.kv_side, at.n, p.sk);
+    if (j0 >= kv.count)
+        return;
+    as_load<D>(K, p.k, at.n, at.head, p.d, j0, kv);
+    as_load<D>(V, p.v, at.n, at.head, p.d, j0, kv);
     float gk[4][D / 16], gv[4][D / 16];
 #pragma unroll
     for (int a = 0; a < 4; ++a)
 #pragma unroll
         for (int r = 0; r < D / 16; ++r)
             gk[a][r] = gv[a][r] = 0.f;
-    const int tiles = attn_tiles(p.sq, AS_TILE);
+    // tiles of queries from the first that sees a key of this tile on, of every query head of the group
+    const int t0 = p.causal ? q.before((long long) kv.cell(j0) - p.offset) / AS_TILE : 0;
+    const int tiles = max(0, attn_tiles(q.count, AS_TILE) - t0);
     int lo, hi;
     as_range(tiles * p.group, p.q_splits, at.split, &lo, &hi);
     for (int u = lo; u < hi; ++u)
     {
-        const int g = u / tiles, i0 = (u - g * tiles) * AS_TILE, head = at.head * p.group + g;
-        if (p.causal && j0 > (long long) i0 + AS_TILE - 1 + p.offset)
-            continue;
+        const int g = u / tiles, i0 = (t0 + u - g * tiles) * AS_TILE, head = at.head * p.group + g;
         __syncthreads();
-        as_load<D>(Q, p.q, at.n, head, p.d, i0, p.sq, qm);
-        as_load<D>(dO, p.d_o, at.n, head, p.d, i0, p.sq, qm);
-        as_load_stats(p, at.n * p.q_heads + head, i0, lse, delta);
+        as_load<D>(Q, p.q, at.n, head, p.d, i0, q);
+        as_load<D>(dO, p.d_o, at.n, head, p.d, i0, q);
+        as_load_stats(p, q, kv, at.n * p.q_heads + head, i0, lse, delta, limit);
         __syncthreads();
-        as_weights<D, true>(p, Q, K, V, dO, lse, delta, see, i0, j0, tx, ty, P, dS);
+        as_weights<D, true>(p, Q, K, V, dO, lse, delta, limit, j0, tx, ty, P, dS);
         __syncthreads();
         as_accumulate<D>(P, dO, tx, ty, gv);
         as_accumulate<D>(dS, Q, tx, ty, gk);
@@ -353,8 +351,8 @@ __global__ void __launch_bounds__(AS_THREADS) attn_simt_dkv_kernel(AttnProblem p
         for (int r = 0; r < D / 16; ++r)
             gk[a][r] *= p.scale / ATTN_LOG2E;
     const long long size = (long long) p.n * p.kv_heads * p.d * p.sk * at.split;
-    as_store<D>(p.dk, p.q_splits > 1 ? p.part_dk + size : nullptr, at.nh, at.n, at.head, p.d, j0, p.sk, tx, ty, gk);
-    as_store<D>(p.dv, p.q_splits > 1 ? p.part_dv + size : nullptr, at.nh, at.n, at.head, p.d, j0, p.sk, tx, ty, gv);
+    as_store<D>(p.dk, p.q_splits > 1 ? p.part_dk + size : nullptr, at.nh, at.n, at.head, p.d, j0, kv, tx, ty, gk);
+    as_store<D>(p.dv, p.q_splits > 1 ? p.part_dv + size : nullptr, at.nh, at.n, at.head, p.d, j0, kv, tx, ty, gv);
 }
 
 template <int D>
@@ -363,15 +361,16 @@ __global__ void __launch_bounds__(AS_THREADS) attn_simt_dq_kernel(AttnProblem p)
     extern __shared__ float smem[];
     float *Q = smem, *dO = Q + D * AS_PITCH, *K = dO + D * AS_PITCH, *V = K + D * AS_PITCH, *dS = V + D * AS_PITCH;
     __shared__ float lse[AS_TILE], delta[AS_TILE];
-    __shared__ uint8_t see[AS_TILE];
+    __shared__ int limit[AS_TILE];
     const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
     const AsAt at = as_at(attn_tiles(p.sq, AS_TILE), p.kv_splits, p.q_heads);
     const int i0 = at.tile * AS_TILE, kv_head = at.head / p.group;
-    const uint8_t* qm = p.q_mask ? p.q_mask + at.n * p.sq : nullptr;
-    const uint8_t* km = p.kv_mask ? p.kv_mask + at.n * p.sk : nullptr;
-    as_load<D>(Q, p.q, at.n, at.head, p.d, i0, p.sq, qm);
-    as_load<D>(dO, p.d_o, at.n, at.head, p.d, i0, p.sq, qm);
-    as_load_stats(p, at.nh, i0, lse, delta);
+    const AttnCells q(p.q_side, at.n, p.sq), kv(p.kv_side, at.n, p.sk);
+    if (i0 >= q.count)
+        return;
+    as_load<D>(Q, p.q, at.n, at.head, p.d, i0, q);
+    as_load<D>(dO, p.d_o, at.n, at.head, p.d, i0, q);
+    as_load_stats(p, q, kv, at.nh, i0, lse, delta, limit);
     float gq[4][D / 16];
 #pragma unroll
     for (int a = 0; a < 4; ++a)
@@ -379,19 +378,16 @@ __global__ void __launch_bounds__(AS_THREADS) attn_simt_dq_kernel(AttnProblem p)
         for (int r = 0; r < D / 16; ++r)
             gq[a][r] = 0.f;
     int lo, hi;
-    as_range(attn_tiles(p.sk, AS_TILE), p.kv_splits, at.split, &lo, &hi);
-    if (p.causal)
-        hi = (int) min((long long) hi, max(0ll, (long long) i0 + AS_TILE - 1 + p.offset + AS_TILE) / AS_TILE);
+    as_range(attn_tiles(kv.count, AS_TILE), p.kv_splits, at.split, &lo, &hi);
+    hi = min(hi, attn_tiles(attn_limit(p, q, kv, min(i0 + AS_TILE, q.count) - 1), AS_TILE));
     for (int t = lo; t < hi; ++t)
     {
         const int j0 = t * AS_TILE;
         __syncthreads();
-        as_load<D>(K, p.k, at.n, kv_head, p.d, j0, p.sk, km);
-        as_load<D>(V, p.v, at.n, kv_head, p.d, j0, p.sk, km);
-        if (threadIdx.x < AS_TILE)
-            see[threadIdx.x] = j0 + (int) threadIdx.x < p.sk && (!km || km[j0 + threadIdx.x]);
+        as_load<D>(K, p.k, at.n, kv_head, p.d, j0, kv);
+        as_load<D>(V, p.v, at.n, kv_head, p.d, j0, kv);
         __syncthreads();
-        as_weights<D, false>(p, Q, K, V, dO, lse, delta, see, i0, j0, tx, ty, nullptr, dS);
+        as_weights<D, false>(p, Q, K, V, dO, lse, delta, limit, j0, tx, ty, nullptr, dS);
         __syncthreads();
         as_accumulate<D>(dS, K, tx, ty, gq);
     }
@@ -401,7 +397,7 @@ __global__ void __launch_bounds__(AS_THREADS) attn_simt_dq_kernel(AttnProblem p)
         for (int r = 0; r < D / 16; ++r)
             gq[a][r] *= p.scale / ATTN_LOG2E;
     float* part = p.kv_splits > 1 ? p.part_dq + (long long) at.split * p.n * p.q_heads * p.d * p.sq : nullptr;
-    as_store<D>(p.dq, part, at.nh, at.n, at.head, p.d, i0, p.sq, tx, ty, gq);
+    as_store<D>(p.dq, part, at.nh, at.n, at.head, p.d, i0, q, tx, ty, gq);
 }
 
 int32_t as_launch(void (*kernel)(AttnProblem), const AttnProblem& p, long long blocks, int smem, cudaStream_t stream)
@@ -431,11 +427,13 @@ int32_t as_with(int d, F f)
 void attn_simt_splits(AttnProblem* p, bool backward)
 {
     const long long slots = 2ll * num_sms(); // two blocks an SM, of tiles of 64 channels
-    p->kv_splits = attn_splits((long long) p->n * p->q_heads * attn_tiles(p->sq, AS_TILE), attn_tiles(p->sk, AS_TILE),
-                               slots, AS_LEAST);
+    const int left = p->q_mask || p->kv_mask ? 2 : 1; // masks are taken to leave half of either side
+    const int q_tiles = attn_tiles(p->sq, AS_TILE), k_tiles = attn_tiles(p->sk, AS_TILE);
+    const auto walks = [&](long long n) { return (n + left - 1) / left; };
+    p->kv_splits = attn_splits(walks((long long) p->n * p->q_heads * q_tiles), k_tiles / left, slots, AS_LEAST);
     p->q_splits = !backward ? 1
-                            : attn_splits((long long) p->n * p->kv_heads * attn_tiles(p->sk, AS_TILE),
-                                          attn_tiles(p->sq, AS_TILE) * p->group, slots, AS_LEAST);
+                            : attn_splits(walks((long long) p->n * p->kv_heads * k_tiles), q_tiles * p->group / left,
+                                          slots, AS_LEAST);
 }
 
 int32_t attn_simt_fwd(const AttnProblem& p, cudaStream_t stream)

@@ -11,93 +11,14 @@ namespace
 
 __device__ int at_status_word; // a kernel gave up on a wait
 
-constexpr int AT_JOBS = 7;
+constexpr int AT_JOBS = 4;
 constexpr int AT_ROWS = 8; // rows of a tensor that a warp copies with the same indices
-constexpr int AT_INDEX_THREADS = 1024, AT_INDEX_CELLS = 8; // cells of a thread at a time
-
-// What a mask leaves of a sample's cells, in order.  A block a sample and side.
-__global__ void __launch_bounds__(AT_INDEX_THREADS) attn_index_kernel(const __grid_constant__ AttnProblem p)
-{
-    __shared__ int of_warp[32];
-    __shared__ int all;
-    const uint8_t* mask = blockIdx.y ? p.kv_mask : p.q_mask;
-    const AttnSide side = blockIdx.y ? p.kv_side : p.q_side;
-    const int cells = blockIdx.y ? p.sk : p.sq;
-    if (!mask)
-        return;
-    wait_for_previous_kernel(mask);
-    dependents_may_start();
-    const long long n = blockIdx.x;
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    mask += n * cells;
-    int* index = side.index + n * cells;
-    int* before = side.before + n * (cells + 1ll);
-    int base = 0;
-    for (long long c0 = 0; c0 < cells; c0 += AT_INDEX_THREADS * AT_INDEX_CELLS)
-    {
-        const long long i0 = c0 + threadIdx.x * AT_INDEX_CELLS;
-        uint32_t bits = 0;
-        for (int e = 0; e < AT_INDEX_CELLS; ++e)
-            if (i0 + e < cells && mask[i0 + e])
-                bits |= 1u << e;
-        const int mine = __popc(bits);
-        int sum = mine; // of this lane and those before
-        for (int h = 1; h < 32; h *= 2)
-        {
-            const int other = __shfl_up_sync(~0u, sum, h);
-            sum += lane >= h ? other : 0;
-        }
-        if (lane == 31)
-            of_warp[warp] = sum;
-        __syncthreads();
-        if (warp == 0)
-        {
-            int w = of_warp[lane];
-            for (int h = 1; h < 32; h *= 2)
-            {
-                const int other = __shfl_up_sync(~0u, w, h);
-                w += lane >= h ? other : 0;
-            }
-            of_warp[lane] = w;
-            if (lane == 31)
-                all = w;
-        }
-        __syncthreads();
-        int at = base + sum - mine + (warp > 0 ? of_warp[warp - 1] : 0);
-        for (int e = 0; e < AT_INDEX_CELLS; ++e)
-            if (i0 + e < cells)
-            {
-                before[i0 + e] = at;
-                if (bits >> e & 1)
-                    index[at++] = (int) (i0 + e);
-            }
-        base += all;
-        __syncthreads();
-    }
-    if (threadIdx.x == 0)
-    {
-        before[cells] = base;
-        side.count[n] = base;
-    }
-}
-
-// AT_COPY: a copy with rows of whole 16 bytes, of the cells that a mask leaves; zeros behind the last.
-// AT_ZERO: zeros in the cells that a mask takes out.  AT_LSE: their lse.
-enum AtJobKind
-{
-    AT_COPY,
-    AT_ZERO,
-    AT_LSE
-};
-
+// A copy with rows of whole 16 bytes, of the cells that a mask leaves; zeros behind the last.
 struct AtJob
 {
-    AtJobKind kind;
     const bf16* from;
     bf16* to;
-    float* lse;
     long long sn, sc;
-    const uint8_t* mask;
     AttnSide side;
     int channels, cells; // rows of a sample
     int chunks;          // of 256 cells a row: a warp each
@@ -125,47 +46,27 @@ __global__ void __launch_bounds__(256) attn_prepare_kernel(const __grid_constant
         const long long m = u / c.chunks, n = m / groups;
         const int row0 = (int) (m - n * groups) * AT_ROWS, row1 = min(row0 + AT_ROWS, c.channels);
         const int i0 = (int) (u - m * c.chunks) * 256 + lane;
+        const int count = c.side.index ? c.side.count[n] : c.cells;
         int cell[8]; // negative: nothing
-        if (c.kind == AT_COPY)
-        {
-            const int count = c.side.index ? c.side.count[n] : c.cells;
-#pragma unroll
-            for (int e = 0; e < 8; ++e)
-            {
-                const int i = i0 + 32 * e;
-                cell[e] = i >= count ? -1 : c.side.index ? c.side.index[n * c.cells + i] : i;
-            }
-            for (int row = row0; row < row1; ++row)
-            {
-                const uint16_t* from = reinterpret_cast<const uint16_t*>(source) + n * c.sn + row * c.sc;
-                uint16_t* to = reinterpret_cast<uint16_t*>(c.to) + (n * c.channels + row) * (long long) pitch + i0;
-                uint16_t v[8];
-#pragma unroll
-                for (int e = 0; e < 8; ++e)
-                    v[e] = cell[e] >= 0 ? from[cell[e]] : (uint16_t) 0;
-#pragma unroll
-                for (int e = 0; e < 8; ++e)
-                    if (i0 + 32 * e < pitch)
-                        to[32 * e] = v[e];
-            }
-            continue;
-        }
 #pragma unroll
         for (int e = 0; e < 8; ++e)
         {
             const int i = i0 + 32 * e;
-            cell[e] = i < c.cells && !c.mask[n * c.cells + i] ? i : -1;
+            cell[e] = i >= count ? -1 : c.side.index ? c.side.index[n * c.cells + i] : i;
         }
         for (int row = row0; row < row1; ++row)
+        {
+            const uint16_t* from = reinterpret_cast<const uint16_t*>(source) + n * c.sn + row * c.sc;
+            uint16_t* to = reinterpret_cast<uint16_t*>(c.to) + (n * c.channels + row) * (long long) pitch + i0;
+            uint16_t v[8];
 #pragma unroll
             for (int e = 0; e < 8; ++e)
-                if (cell[e] >= 0)
-                {
-                    if (c.kind == AT_ZERO)
-                        reinterpret_cast<uint16_t*>(c.to)[n * c.sn + row * c.sc + cell[e]] = 0;
-                    else
-                        c.lse[(n * c.channels + row) * (long long) c.cells + cell[e]] = -INFINITY;
-                }
+                v[e] = cell[e] >= 0 ? from[cell[e]] : (uint16_t) 0;
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (i0 + 32 * e < pitch)
+                    to[32 * e] = v[e];
+        }
     }
 }
 
@@ -175,24 +76,6 @@ struct AtHost
     AtMaps maps;
     AtExtra ex = {};
 };
-
-void at_job(AtHost* h, const AtJob& job)
-{
-    h->prepare.job[h->prepare.jobs++] = job;
-}
-
-int at_chunks(int cells)
-{
-    return (cells + 255) / 256;
-}
-
-// A result's cells that its mask takes out.
-void at_zeros(const AttnTensor& t, int channels, int cells, const uint8_t* mask, AtHost* h)
-{
-    if (mask)
-        at_job(h, AtJob{AT_ZERO, nullptr, static_cast<bf16*>(t.p), nullptr, t.sn, t.sc, mask, {}, channels, cells,
-                        at_chunks(cells)});
-}
 
 // The tensor as bulk copies see it, copied first where they cannot or where a mask picks cells.
 int32_t at_operand(const AttnProblem& p, const AttnTensor& t, int heads, int cells, const AttnSide& side, bf16* copy,
@@ -205,8 +88,8 @@ int32_t at_operand(const AttnProblem& p, const AttnTensor& t, int heads, int cel
     if (!fits || side.index)
     {
         const int channels = heads * p.d;
-        at_job(h, AtJob{AT_COPY, static_cast<const bf16*>(at), copy, nullptr, sn, sc, nullptr, side, channels, cells,
-                        at_chunks(cells)});
+        h->prepare.job[h->prepare.jobs++]
+            = AtJob{static_cast<const bf16*>(at), copy, sn, sc, side, channels, cells, (cells + 255) / 256};
         at = copy;
         sc = (cells + 7) / 8 * 8;
         sn = sc * channels;
@@ -324,14 +207,6 @@ void attn_tc_splits(AttnProblem* p, bool backward)
                                       q_bytes);
 }
 
-int32_t attn_tc_index(const AttnProblem& p, cudaStream_t stream)
-{
-    if (!p.q_mask && !p.kv_mask)
-        return DCB_OK;
-    DCB_CUDA_TRY(launch_overlapped(attn_index_kernel, dim3(p.n, 2), AT_INDEX_THREADS, 0, stream, p));
-    return DCB_OK;
-}
-
 int32_t attn_tc_fwd(const AttnProblem& p, cudaStream_t stream)
 {
     AtHost h;
@@ -343,11 +218,6 @@ int32_t attn_tc_fwd(const AttnProblem& p, cudaStream_t stream)
     if (int32_t e = at_operand(p, p.v, p.kv_heads, p.sk, p.kv_side, p.copy_v, box, &h, &h.maps.v))
         return e;
     h.maps.d_o = h.maps.q;
-    if (p.q_mask && p.kv_splits == 1) // else the join writes them
-    {
-        at_zeros(p.o, p.q_heads * p.d, p.sq, p.q_mask, &h);
-        at_job(&h, AtJob{AT_LSE, nullptr, nullptr, p.lse, 0, 0, p.q_mask, {}, p.q_heads, p.sq, at_chunks(p.sq)});
-    }
     if (int32_t e = at_prepare(p, &h, stream))
         return e;
     return attn_tc_fwd_launch(p, h.maps, h.ex, stream);
@@ -365,13 +235,6 @@ int32_t attn_tc_bwd(const AttnProblem& p, cudaStream_t stream)
         return e;
     if (int32_t e = at_operand(p, p.d_o, p.q_heads, p.sq, p.q_side, p.copy_do, box, &h, &h.maps.d_o))
         return e;
-    if (p.kv_splits == 1) // else the joins write them
-        at_zeros(p.dq, p.q_heads * p.d, p.sq, p.q_mask, &h);
-    if (p.q_splits == 1)
-    {
-        at_zeros(p.dk, p.kv_heads * p.d, p.sk, p.kv_mask, &h);
-        at_zeros(p.dv, p.kv_heads * p.d, p.sk, p.kv_mask, &h);
-    }
     if (int32_t e = at_prepare(p, &h, stream))
         return e;
     return attn_tc_bwd_launch(p, h.maps, h.ex, stream);

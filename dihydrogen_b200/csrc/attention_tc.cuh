@@ -307,34 +307,6 @@ __device__ __forceinline__ void at_warp_arrive(uint64_t* bar, int lane)
         mbar_arrive(bar);
 }
 
-// One sample's cells on one side, as the kernels count them: all, or those that a mask leaves.
-struct AtCells
-{
-    int count, cells;
-    const int *index, *counted;
-    __device__ __forceinline__ AtCells(const AttnSide& s, long long n, int cells_) : cells(cells_)
-    {
-        index = s.index ? s.index + n * cells : nullptr;
-        counted = s.index ? s.before + n * (cells + 1ll) : nullptr;
-        count = s.index ? s.count[n] : cells;
-    }
-    __device__ __forceinline__ int cell(int r) const { return index ? index[r] : r; }
-    // How many lie before cell x of the grid.
-    __device__ __forceinline__ int before(long long x) const
-    {
-        const int c = (int) (x < 0 ? 0 : x > cells ? cells : x);
-        return counted ? counted[c] : c;
-    }
-};
-
-// Row r of the queries sees the first so many keys; later rows see no fewer.
-__device__ __forceinline__ int at_limit(const AttnProblem& p, const AtCells& q, const AtCells& kv, int r)
-{
-    if (r < 0 || r >= q.count)
-        return 0;
-    return p.causal ? kv.before((long long) q.cell(r) + p.offset + 1) : kv.count;
-}
-
 // The columns up to `last` among 32, the w-th word from column 0 on.
 __device__ __forceinline__ uint32_t at_up_to(int last, int w)
 {

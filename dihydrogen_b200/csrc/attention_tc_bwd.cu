@@ -144,7 +144,7 @@ __global__ void __launch_bounds__(AT_THREADS, AbShape<D>::BLOCKS)
     const uint32_t tmem = __shfl_sync(~0u, b.tmem, 0); // known to be uniform
     const float* stats = p.stats;
     wait_for_previous_kernel(stats);
-    const AtCells q(p.q_side, n, p.sq), kv(p.kv_side, n, p.sk);
+    const AttnCells q(p.q_side, n, p.sq), kv(p.kv_side, n, p.sk);
     // a key is seen from this row of the queries on
     const auto first_row = [&](int r) {
         return r >= kv.count ? q.count : p.causal ? q.before((long long) kv.cell(r) - p.offset) : 0;
@@ -383,11 +383,11 @@ __global__ void __launch_bounds__(AT_THREADS, AbShape<D>::BLOCKS)
     const uint32_t tmem = __shfl_sync(~0u, b.tmem, 0); // known to be uniform
     const float* stats = p.stats;
     wait_for_previous_kernel(stats);
-    const AtCells q(p.q_side, n, p.sq), kv(p.kv_side, n, p.sk);
+    const AttnCells q(p.q_side, n, p.sq), kv(p.kv_side, n, p.sk);
     const int steps_k = attn_tiles(kv.count, S::STEP);
     const int lo = (int) ((long long) steps_k * split / p.kv_splits);
     const int hi = min((int) ((long long) steps_k * (split + 1) / p.kv_splits),
-                       attn_tiles(at_limit(p, q, kv, min(i0 + AT_TILE, q.count) - 1), S::STEP));
+                       attn_tiles(attn_limit(p, q, kv, min(i0 + AT_TILE, q.count) - 1), S::STEP));
     const int steps = i0 < q.count ? max(0, hi - lo) : 0;
     bool ok = true;
     const uint32_t s_at = tmem, dp_at = tmem + S::DQ_DP, dq_at = tmem + S::DQ_DQ;
@@ -490,8 +490,8 @@ __global__ void __launch_bounds__(AT_THREADS, AbShape<D>::BLOCKS)
         const int team = warp >> 2;
         const uint32_t lanes = (uint32_t) (warp & 3) << 21;
         const int row0 = i0 + (warp & 3) * 32, r = row0 + lane;
-        const int i = r < q.count ? q.cell(r) : -1, limit = at_limit(p, q, kv, r);
-        const int open = max(0, at_limit(p, q, kv, row0) - lo * S::STEP) / S::STEP; // steps that all its rows see whole
+        const int i = r < q.count ? q.cell(r) : -1, limit = attn_limit(p, q, kv, r);
+        const int open = max(0, attn_limit(p, q, kv, row0) - lo * S::STEP) / S::STEP; // steps that all its rows see whole
         const uint32_t dp_mine = dp_at + lanes + S::MINE * team;
         const float* row = stats + nh * p.stats_pitch + r; // up to a multiple of 128 cells
         const float lse = row[0], delta = row[(long long) p.n * p.q_heads * p.stats_pitch];

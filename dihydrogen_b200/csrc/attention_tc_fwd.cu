@@ -102,7 +102,7 @@ __global__ void __launch_bounds__(AT_THREADS, AfShape<D, APART>::BLOCKS)
     const uint32_t tmem = __shfl_sync(~0u, b.tmem, 0); // known to be uniform
     const int* p_index = p.q_side.count;
     wait_for_previous_kernel(p_index); // the sides' counts
-    const AtCells q(p.q_side, n, p.sq), kv(p.kv_side, n, p.sk);
+    const AttnCells q(p.q_side, n, p.sq), kv(p.kv_side, n, p.sk);
     const int tiles = attn_tiles(kv.count, AT_TILE);
     int lo[2], steps[2]; // of either team: first tile of keys, steps of 64 keys
     for (int t = 0; t < 2; ++t)
@@ -110,7 +110,7 @@ __global__ void __launch_bounds__(AT_THREADS, AfShape<D, APART>::BLOCKS)
         const int part = APART ? 2 * split + t : split, first = APART ? 0 : i0 + t * AT_TILE;
         lo[t] = (int) ((long long) tiles * part / p.kv_splits);
         const int hi = (int) ((long long) tiles * (part + 1) / p.kv_splits);
-        const int end = min(hi * AT_TILE, at_limit(p, q, kv, min(first + AT_TILE, q.count) - 1)); // keys
+        const int end = min(hi * AT_TILE, attn_limit(p, q, kv, min(first + AT_TILE, q.count) - 1)); // keys
         steps[t] = first < q.count ? max(0, end - lo[t] * AT_TILE + 63) / 64 : 0;
     }
     const int most = max(steps[0], steps[1]);
@@ -249,7 +249,7 @@ __global__ void __launch_bounds__(AT_THREADS, AfShape<D, APART>::BLOCKS)
         const uint32_t lanes = (uint32_t) (warp & 3) << 21; // 32 lanes of tensor memory a warp
         const uint32_t o_at = tmem + lanes + S::O_AT + t * D;
         const int row0 = (APART ? 0 : i0 + t * AT_TILE) + (warp & 3) * 32, row = row0 + lane;
-        const int i = row < q.count ? q.cell(row) : -1, limit = at_limit(p, q, kv, row);
+        const int i = row < q.count ? q.cell(row) : -1, limit = attn_limit(p, q, kv, row);
         const int part = APART ? 2 * split + t : split;
         const bool rows = row0 < q.count; // else no row of this warp is a cell: what its weights are reaches nobody
         float top = -INFINITY, sum = 0.f; // the base of the weights so far and their sum
@@ -262,7 +262,7 @@ __global__ void __launch_bounds__(AT_THREADS, AfShape<D, APART>::BLOCKS)
         };
         uint32_t see[2];  // which keys of the coming step this row may see
         bool cut = false; // whether some row of the warp may not see all of them
-        const int open = max(0, at_limit(p, q, kv, row0) - lo[t] * AT_TILE) / 64; // steps that all its rows see whole
+        const int open = max(0, attn_limit(p, q, kv, row0) - lo[t] * AT_TILE) / 64; // steps that all its rows see whole
         const auto mask = [&](int c, float x) { return see[c >> 5] >> (c & 31) & 1 ? x : -INFINITY; };
         // masks and maximum of a step's scores, which have arrived
         const auto look = [&](int u, float (&s)[64]) {
