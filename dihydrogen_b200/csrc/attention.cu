@@ -617,13 +617,11 @@ int32_t dcb_attention_bwd(const dcb_attention_desc* ad, const dcb_nd_desc* qd, c
 int32_t dcb_attention_status(void* stream)
 {
     DCB_CUDA_TRY(cudaStreamSynchronize(as_stream(stream)));
-    int* word = attn_tc_status();
-    int given_up = 0;
-    DCB_REQUIRE(word, "no status word on this device");
-    DCB_CUDA_TRY(cudaMemcpy(&given_up, word, sizeof(int), cudaMemcpyDeviceToHost));
-    if (!given_up)
+    bool gave_up = false;
+    if (int32_t e = attn_tc_status(&gave_up))
+        return e;
+    if (!gave_up)
         return DCB_OK;
-    DCB_CUDA_TRY(cudaMemset(word, 0, sizeof(int)));
     set_last_error("a tensor-core attention kernel gave up on a pipeline wait");
     return DCB_CUDA_ERROR;
 }

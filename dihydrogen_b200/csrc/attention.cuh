@@ -96,7 +96,7 @@ inline int attn_splits(long long work, int steps, long long slots, int least)
 int32_t attn_tc_fwd(const AttnProblem& p, cudaStream_t stream);
 int32_t attn_tc_bwd(const AttnProblem& p, cudaStream_t stream);
 void attn_tc_splits(AttnProblem* p, bool backward);
-int* attn_tc_status(); // device word of the current device
+int32_t attn_tc_status(bool* gave_up); // of the current device, cleared
 int32_t attn_simt_fwd(const AttnProblem& p, cudaStream_t stream);
 int32_t attn_simt_bwd(const AttnProblem& p, cudaStream_t stream);
 void attn_simt_splits(AttnProblem* p, bool backward);

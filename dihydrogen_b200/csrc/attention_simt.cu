@@ -72,10 +72,17 @@ __device__ __forceinline__ int as_row(int t)
     return ((t & 3) * 16 + (t >> 2)) * AS_PITCH;
 }
 
-// acc[e][r] += sum_t W[t][4 ty + e] X[tx + 16 r][t]
+// acc[e][r] += sum_t W[t][4 ty + e] X[tx + 16 r][t].  A tile's 64 terms are added up by themselves first: over n tiles a
+// result is then off by at most (64 + n) roundings, not 64 n.  (2^25 keys of equal weight: 1.7e-3 of the result otherwise.)
 template <int D>
 __device__ __forceinline__ void as_accumulate(const float* W, const float* X, int tx, int ty, float (&acc)[4][D / 16])
 {
+    float sum[4][D / 16];
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+#pragma unroll
+        for (int r = 0; r < D / 16; ++r)
+            sum[e][r] = 0.f;
 #pragma unroll 2
     for (int t = 0; t < AS_TILE; t += 4)
     {
@@ -92,9 +99,14 @@ __device__ __forceinline__ void as_accumulate(const float* W, const float* X, in
             for (int u = 0; u < 4; ++u)
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
-                    acc[e][r] = fmaf(w[u][e], x[u], acc[e][r]);
+                    sum[e][r] = fmaf(w[u][e], x[u], sum[e][r]);
         }
     }
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+#pragma unroll
+        for (int r = 0; r < D / 16; ++r)
+            acc[e][r] += sum[e][r];
 }
 
 // Results of 4 cells x D / 16 channels: to the tensor, or as a part to [head][channel][cell].

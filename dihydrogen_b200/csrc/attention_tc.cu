@@ -9,8 +9,6 @@ namespace dcb
 namespace
 {
 
-__device__ int at_status_word; // a kernel gave up on a wait
-
 constexpr int AT_JOBS = 4;
 constexpr int AT_ROWS = 8; // rows of a tensor that a warp copies with the same indices
 // A copy with rows of whole 16 bytes, of the cells that a mask leaves; zeros behind the last.
@@ -74,7 +72,6 @@ struct AtHost
 {
     AtPrepare prepare = {};
     AtMaps maps;
-    AtExtra ex = {};
 };
 
 // The tensor as bulk copies see it, copied first where they cannot or where a mask picks cells.
@@ -115,8 +112,6 @@ int32_t at_operand(const AttnProblem& p, const AttnTensor& t, int heads, int cel
 int32_t at_prepare(const AttnProblem& p, AtHost* h, cudaStream_t stream)
 {
     AtPrepare& a = h->prepare;
-    h->ex.status = attn_tc_status();
-    DCB_REQUIRE(h->ex.status, "no status word on this device");
     if (a.jobs == 0)
         return DCB_OK;
     a.n = p.n;
@@ -130,26 +125,12 @@ int32_t at_prepare(const AttnProblem& p, AtHost* h, cudaStream_t stream)
 
 } // namespace
 
-// Looked up once per device: a kernel argument must not cost a symbol lookup a call, nor one inside a capture.
-int* attn_tc_status()
+int32_t attn_tc_status(bool* gave_up)
 {
-    static thread_local int known_device = -1;
-    static thread_local int* known = nullptr;
-    int device = 0;
-    if (cudaGetDevice(&device) != cudaSuccess)
-        return nullptr;
-    if (device != known_device)
-    {
-        void* p = nullptr;
-        if (cudaGetSymbolAddress(&p, at_status_word) != cudaSuccess)
-        {
-            (void) cudaGetLastError();
-            return nullptr;
-        }
-        known = static_cast<int*>(p);
-        known_device = device;
-    }
-    return known;
+    *gave_up = false;
+    if (int32_t e = attn_tc_fwd_status(gave_up))
+        return e;
+    return attn_tc_bwd_status(gave_up);
 }
 
 bool attn_tc_apart(const AttnProblem& p)
@@ -220,7 +201,7 @@ int32_t attn_tc_fwd(const AttnProblem& p, cudaStream_t stream)
     h.maps.d_o = h.maps.q;
     if (int32_t e = at_prepare(p, &h, stream))
         return e;
-    return attn_tc_fwd_launch(p, h.maps, h.ex, stream);
+    return attn_tc_fwd_launch(p, h.maps, stream);
 }
 
 int32_t attn_tc_bwd(const AttnProblem& p, cudaStream_t stream)
@@ -237,7 +218,7 @@ int32_t attn_tc_bwd(const AttnProblem& p, cudaStream_t stream)
         return e;
     if (int32_t e = at_prepare(p, &h, stream))
         return e;
-    return attn_tc_bwd_launch(p, h.maps, h.ex, stream);
+    return attn_tc_bwd_launch(p, h.maps, stream);
 }
 
 } // namespace dcb

@@ -359,17 +359,29 @@ struct AtMaps
     CUtensorMap q, k, v, d_o;
 };
 
-struct AtExtra
+// A kernel gave up on a wait: a word of each source file, so that no launch has to look a symbol up.
+static __device__ int at_gave_up;
+
+// Reads and clears this file's word.
+inline int32_t at_read_status(bool* gave_up)
 {
-    int* status;
-};
+    int word = 0;
+    DCB_CUDA_TRY(cudaMemcpyFromSymbol(&word, at_gave_up, sizeof(int)));
+    if (word)
+    {
+        *gave_up = true;
+        word = 0;
+        DCB_CUDA_TRY(cudaMemcpyToSymbol(at_gave_up, &word, sizeof(int)));
+    }
+    return DCB_OK;
+}
 
 // The end of every kernel: who gave up says so, waits for what he started, and the tensor memory goes back.
 template <uint32_t COLUMNS = TC_TMEM_COLS>
-__device__ __forceinline__ void at_finish(bool ok, int* status, int warp, int lane, uint32_t tmem)
+__device__ __forceinline__ void at_finish(bool ok, int warp, int lane, uint32_t tmem)
 {
     if (!ok && lane == 0)
-        atomicExch(status, 1);
+        atomicExch(&at_gave_up, 1);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -379,12 +391,12 @@ __device__ __forceinline__ void at_finish(bool ok, int* status, int warp, int la
 }
 
 // The 128-byte swizzle goes by address bits: tiles start on multiples of 1024 bytes.
-__device__ __forceinline__ bool at_misplaced(uint32_t base, int* status)
+__device__ __forceinline__ bool at_misplaced(uint32_t base)
 {
     if ((base & 1023u) == 0)
         return false;
     if (threadIdx.x == 0)
-        atomicExch(status, 1);
+        atomicExch(&at_gave_up, 1);
     return true;
 }
 
@@ -424,7 +436,9 @@ __device__ __forceinline__ void at_drain(uint64_t* full, uint32_t slots, const A
 
 // Few queries against many keys: both teams of a block have the same queries.
 bool attn_tc_apart(const AttnProblem& p);
-int32_t attn_tc_fwd_launch(const AttnProblem& p, const AtMaps& maps, const AtExtra& ex, cudaStream_t stream);
-int32_t attn_tc_bwd_launch(const AttnProblem& p, const AtMaps& maps, const AtExtra& ex, cudaStream_t stream);
+int32_t attn_tc_fwd_launch(const AttnProblem& p, const AtMaps& maps, cudaStream_t stream);
+int32_t attn_tc_bwd_launch(const AttnProblem& p, const AtMaps& maps, cudaStream_t stream);
+int32_t attn_tc_fwd_status(bool* gave_up);
+int32_t attn_tc_bwd_status(bool* gave_up);
 
 } // namespace dcb

@@ -121,8 +121,7 @@ __device__ __forceinline__ void ab_put(uint32_t taddr, const uint32_t (&v)[N])
 
 template <int D>
 __global__ void __launch_bounds__(AT_THREADS, AbShape<D>::BLOCKS)
-    attn_tc_dkv_kernel(const __grid_constant__ AttnProblem p, const __grid_constant__ AtMaps maps,
-                       const __grid_constant__ AtExtra ex)
+    attn_tc_dkv_kernel(const __grid_constant__ AttnProblem p, const __grid_constant__ AtMaps maps)
 {
     using S = AbShape<D>;
     extern __shared__ __align__(1024) uint8_t smem[];
@@ -130,7 +129,7 @@ __global__ void __launch_bounds__(AT_THREADS, AbShape<D>::BLOCKS)
     AbBars& b = *reinterpret_cast<AbBars*>(smem + S::BARS_AT);
     const int warp = __shfl_sync(~0u, (int) threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     volatile int* give_up = &b.give_up;
-    if (at_misplaced(base, ex.status))
+    if (at_misplaced(base))
         return;
 
     const int tiles_k = attn_tiles(p.sk, AT_TILE);
@@ -354,13 +353,12 @@ __global__ void __launch_bounds__(AT_THREADS, AbShape<D>::BLOCKS)
                          p.scale / ATTN_LOG2E, false, steps == 0, dk_at + lanes, 0, D);
         }
     }
-    at_finish<S::COLUMNS>(ok, ex.status, warp, lane, tmem);
+    at_finish<S::COLUMNS>(ok, warp, lane, tmem);
 }
 
 template <int D>
 __global__ void __launch_bounds__(AT_THREADS, AbShape<D>::BLOCKS)
-    attn_tc_dq_kernel(const __grid_constant__ AttnProblem p, const __grid_constant__ AtMaps maps,
-                      const __grid_constant__ AtExtra ex)
+    attn_tc_dq_kernel(const __grid_constant__ AttnProblem p, const __grid_constant__ AtMaps maps)
 {
     using S = AbShape<D>;
     extern __shared__ __align__(1024) uint8_t smem[];
@@ -368,7 +366,7 @@ __global__ void __launch_bounds__(AT_THREADS, AbShape<D>::BLOCKS)
     AbBars& b = *reinterpret_cast<AbBars*>(smem + S::BARS_AT);
     const int warp = __shfl_sync(~0u, (int) threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     volatile int* give_up = &b.give_up;
-    if (at_misplaced(base, ex.status))
+    if (at_misplaced(base))
         return;
 
     const int tiles_q = attn_tiles(p.sq, AT_TILE);
@@ -547,11 +545,11 @@ __global__ void __launch_bounds__(AT_THREADS, AbShape<D>::BLOCKS)
                      dq_at + lanes, team * (D / 2), (team + 1) * (D / 2));
         }
     }
-    at_finish<S::COLUMNS>(ok, ex.status, warp, lane, tmem);
+    at_finish<S::COLUMNS>(ok, warp, lane, tmem);
 }
 
 template <int D>
-int32_t ab_launch(const AttnProblem& p, const AtMaps& maps, const AtExtra& ex, cudaStream_t stream)
+int32_t ab_launch(const AttnProblem& p, const AtMaps& maps, cudaStream_t stream)
 {
     const long long dkv = (long long) p.n * p.kv_heads * attn_tiles(p.sk, AT_TILE) * p.q_splits;
     const long long dq = (long long) p.n * p.q_heads * attn_tiles(p.sq, AT_TILE) * p.kv_splits;
@@ -560,18 +558,21 @@ int32_t ab_launch(const AttnProblem& p, const AtMaps& maps, const AtExtra& ex, c
         return e;
     if (int32_t e = allow_dynamic_smem((const void*) attn_tc_dq_kernel<D>, AbShape<D>::SMEM))
         return e;
-    DCB_CUDA_TRY(launch_overlapped(attn_tc_dkv_kernel<D>, dim3((unsigned) dkv), AT_THREADS, AbShape<D>::SMEM, stream, p,
-                                   maps, ex));
-    DCB_CUDA_TRY(launch_overlapped(attn_tc_dq_kernel<D>, dim3((unsigned) dq), AT_THREADS, AbShape<D>::SMEM, stream, p,
-                                   maps, ex));
+    DCB_CUDA_TRY(launch_overlapped(attn_tc_dkv_kernel<D>, dim3((unsigned) dkv), AT_THREADS, AbShape<D>::SMEM, stream, p, maps));
+    DCB_CUDA_TRY(launch_overlapped(attn_tc_dq_kernel<D>, dim3((unsigned) dq), AT_THREADS, AbShape<D>::SMEM, stream, p, maps));
     return DCB_OK;
 }
 
 } // namespace
 
-int32_t attn_tc_bwd_launch(const AttnProblem& p, const AtMaps& maps, const AtExtra& ex, cudaStream_t stream)
+int32_t attn_tc_bwd_launch(const AttnProblem& p, const AtMaps& maps, cudaStream_t stream)
 {
-    return p.d <= 64 ? ab_launch<64>(p, maps, ex, stream) : ab_launch<128>(p, maps, ex, stream);
+    return p.d <= 64 ? ab_launch<64>(p, maps, stream) : ab_launch<128>(p, maps, stream);
+}
+
+int32_t attn_tc_bwd_status(bool* gave_up)
+{
+    return at_read_status(gave_up);
 }
 
 } // namespace dcb

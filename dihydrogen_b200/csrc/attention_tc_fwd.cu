@@ -55,8 +55,7 @@ static_assert(sizeof(AfBars) <= 256, "the barriers' room");
 
 template <int D, bool APART>
 __global__ void __launch_bounds__(AT_THREADS, AfShape<D, APART>::BLOCKS)
-    attn_tc_fwd_kernel(const __grid_constant__ AttnProblem p, const __grid_constant__ AtMaps maps,
-                       const __grid_constant__ AtExtra ex)
+    attn_tc_fwd_kernel(const __grid_constant__ AttnProblem p, const __grid_constant__ AtMaps maps)
 {
     using S = AfShape<D, APART>;
     extern __shared__ __align__(1024) uint8_t smem[];
@@ -64,7 +63,7 @@ __global__ void __launch_bounds__(AT_THREADS, AfShape<D, APART>::BLOCKS)
     AfBars& b = *reinterpret_cast<AfBars*>(smem + S::BARS_AT);
     const int warp = __shfl_sync(~0u, (int) threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     volatile int* give_up = &b.give_up;
-    if (at_misplaced(base, ex.status))
+    if (at_misplaced(base))
         return;
 
     const int blocks_q = APART ? 1 : attn_tiles(p.sq, 2 * AT_TILE);
@@ -461,11 +460,11 @@ __global__ void __launch_bounds__(AT_THREADS, AfShape<D, APART>::BLOCKS)
             }
         }
     }
-    at_finish<S::COLUMNS>(ok, ex.status, warp, lane, tmem);
+    at_finish<S::COLUMNS>(ok, warp, lane, tmem);
 }
 
 template <int D, bool APART>
-int32_t af_launch(const AttnProblem& p, const AtMaps& maps, const AtExtra& ex, cudaStream_t stream)
+int32_t af_launch(const AttnProblem& p, const AtMaps& maps, cudaStream_t stream)
 {
     const long long blocks = (long long) p.n * p.q_heads
                              * (APART ? p.kv_splits / 2 : (long long) attn_tiles(p.sq, 2 * AT_TILE) * p.kv_splits);
@@ -473,17 +472,22 @@ int32_t af_launch(const AttnProblem& p, const AtMaps& maps, const AtExtra& ex, c
     if (int32_t e = allow_dynamic_smem((const void*) attn_tc_fwd_kernel<D, APART>, AfShape<D, APART>::SMEM))
         return e;
     DCB_CUDA_TRY(launch_overlapped(attn_tc_fwd_kernel<D, APART>, dim3((unsigned) blocks), AT_THREADS, AfShape<D, APART>::SMEM,
-                                   stream, p, maps, ex));
+                                   stream, p, maps));
     return DCB_OK;
 }
 
 } // namespace
 
-int32_t attn_tc_fwd_launch(const AttnProblem& p, const AtMaps& maps, const AtExtra& ex, cudaStream_t stream)
+int32_t attn_tc_fwd_launch(const AttnProblem& p, const AtMaps& maps, cudaStream_t stream)
 {
     if (attn_tc_apart(p))
-        return p.d <= 64 ? af_launch<64, true>(p, maps, ex, stream) : af_launch<128, true>(p, maps, ex, stream);
-    return p.d <= 64 ? af_launch<64, false>(p, maps, ex, stream) : af_launch<128, false>(p, maps, ex, stream);
+        return p.d <= 64 ? af_launch<64, true>(p, maps, stream) : af_launch<128, true>(p, maps, stream);
+    return p.d <= 64 ? af_launch<64, false>(p, maps, stream) : af_launch<128, false>(p, maps, stream);
+}
+
+int32_t attn_tc_fwd_status(bool* gave_up)
+{
+    return at_read_status(gave_up);
 }
 
 } // namespace dcb

@@ -1521,26 +1521,39 @@ def _workspace(nbytes: int, stream, device):
     return ws, ws.data_ptr()
 
 
-def _vector(name, t, count, dtypes=(torch.float32,)):
+def _device(t):
+    """The device of a tensor's memory, which has to be the current one: kernels are launched there."""
+    b = (t.tensor if isinstance(t, ChannelSlice) else t).buffer
+    d = b.device if b is not None else torch.device("cuda", torch._C._cuda_getDevice())  # none: nothing is read
+    if d.type != "cuda" or d.index != torch._C._cuda_getDevice():
+        raise ValueError(f"tensors have to be on the current CUDA device, not on {d}")
+    return d
+
+
+def _vector(name, t, count, device, dtypes=(torch.float32,)):
     """Address of a plain torch operand, which the kernels take as a dense array; 0 for None."""
     if t is None:
         return 0
-    if t.dtype not in dtypes or t.numel() != count or not t.is_contiguous():
-        raise ValueError(f"{name} must be a contiguous array of {count} {dtypes[0]}, not {list(t.shape)} {t.dtype}")
+    if t.dtype not in dtypes or t.numel() != count or not t.is_contiguous() or t.device != device:
+        raise ValueError(f"{name} must be a contiguous array of {count} {dtypes[0]} on {device}, not "
+                         f"{list(t.shape)} {t.dtype} on {t.device}")
     return t.data_ptr()
 
 
-def _needed(name, t, count):
+def _needed(name, t, count, device):
     if t is None:
         raise ValueError(f"{name} is missing")
-    return _vector(name, t, count)
+    return _vector(name, t, count, device)
 
 
 def _check_alike(what, first, *others):
+    """Shapes, types and devices agree."""
+    device = _device(first)
     for t in others:
-        if t.local_shape != first.local_shape or t.dtype is not first.dtype:
+        if t.local_shape != first.local_shape or t.dtype is not first.dtype or _device(t) != device:
             raise ValueError(f"{what}: local shapes and types must agree: {first.local_shape} {first.dtype} and "
                              f"{t.local_shape} {t.dtype}")
+    return device
 
 
 class LayerNormalization:
@@ -1567,32 +1580,32 @@ class LayerNormalization:
     def forward(self, input: Tensor, scale, bias, output: Tensor, mean=None, inv_std=None):
         """``scale`` and ``bias`` may be None (1 and 0); so may ``mean`` and
         ``inv_std`` where no backward pass follows.  ``output`` may be ``input``."""
-        _check_alike("layer normalisation", input, output)
+        dev = _check_alike("layer normalisation", input, output)
         C, size = input.local_shape[-2], input._geo().size
         if size == 0:
             return 0
         xd, x = input._operand()
         yd, y = output._operand()
-        call("dcb_ln_fwd", xd, _DTYPES[input.dtype], x, _vector("scale", scale, C), _vector("bias", bias, C),
-             self.epsilon, yd, y, _vector("mean", mean, size // C), _vector("inv_std", inv_std, size // C),
-             _stream_ptr(self.be.stream))
+        call("dcb_ln_fwd", xd, _DTYPES[input.dtype], x, _vector("scale", scale, C, dev),
+             _vector("bias", bias, C, dev), self.epsilon, yd, y, _vector("mean", mean, size // C, dev),
+             _vector("inv_std", inv_std, size // C, dev), _stream_ptr(self.be.stream))
         return 0
 
     def backward_stage1(self, input: Tensor, d_output: Tensor, mean, inv_std, scale, scale_gradient, bias_gradient,
                         d_input: Tensor):
         """``d_input`` and this rank's sums of the gradients of scale and bias
         (None: not wanted).  ``d_input`` may be ``d_output`` or ``input``."""
-        _check_alike("layer normalisation", input, d_output, d_input)
+        dev = _check_alike("layer normalisation", input, d_output, d_input)
         C, s, geo = input.local_shape[-2], self.be.stream, input._geo()
         if (scale_gradient is None) != (bias_gradient is None):
             raise ValueError("the gradients of scale and bias are wanted together")
-        gw, gb = _vector("scale_gradient", scale_gradient, C), _vector("bias_gradient", bias_gradient, C)
+        gw, gb = _vector("scale_gradient", scale_gradient, C, dev), _vector("bias_gradient", bias_gradient, C, dev)
         if geo.size == 0:
             if gw:
                 _zero_on(s, scale_gradient, bias_gradient)
             return 0
         cells = geo.size // C
-        pm, pi = _needed("mean", mean, cells), _needed("inv_std", inv_std, cells)
+        pm, pi = _needed("mean", mean, cells, dev), _needed("inv_std", inv_std, cells, dev)
         xd, x = input._operand()
         dyd, dy = d_output._operand()
         dxd, dx = d_input._operand()
@@ -1602,9 +1615,9 @@ class LayerNormalization:
             if self._last[0] is not geo:
                 self._last = (geo, _abi.lib().dcb_ln_bwd_workspace_bytes(xd, dtype))
             nbytes = self._last[1]
-            keep, ws = _workspace(nbytes, s, input.buffer.device)
-        call("dcb_ln_bwd", xd, dtype, x, dyd, dy, pm, pi, _vector("scale", scale, C), dxd, dx, gw, gb, ws, nbytes,
-             _stream_ptr(s))
+            keep, ws = _workspace(nbytes, s, dev)
+        call("dcb_ln_bwd", xd, dtype, x, dyd, dy, pm, pi, _vector("scale", scale, C, dev), dxd, dx, gw, gb, ws,
+             nbytes, _stream_ptr(s))
         if gw and not geo.split_root:  # a replica: its cells count once
             _zero_on(s, scale_gradient, bias_gradient)
         return 0
@@ -1670,6 +1683,8 @@ class RotaryPositions:
     def _apply(self, x: Tensor, y: Tensor, inverse):
         if x.local_shape[:-1] != self._local[:-1] or y.local_shape != x.local_shape:
             raise ValueError(f"local shapes {x.local_shape} and {y.local_shape}, set up for {self._local}")
+        if _device(x) != _device(y):
+            raise ValueError("rotary positions: tensors on two devices")
         if x._geo().size == 0:
             return 0
         xd, px = x._operand()
@@ -1738,14 +1753,14 @@ class Attention:
             if not t._geo().whole:
                 raise ValueError("attention needs all cells and channels of a sample on one rank: re-distribute the "
                                  "tensor (TensorShuffler)")
-        _check_alike("attention", q, *q_like)
+        dev = _check_alike("attention", q, *q_like)
         _check_alike("attention", k, v, *kv_like)
         if q.dtype is not k.dtype or q.local_shape[-1] != k.local_shape[-1]:
             raise ValueError("attention: queries and keys differ in type or samples")
         n, cells_q, cells_k = q.local_shape[-1], math.prod(q.local_shape[:-2]), math.prod(k.local_shape[:-2])
-        return (_needed("lse", lse, n * self.q_heads * cells_q),
-                _vector("q_mask", q_mask, n * cells_q, (torch.bool, torch.uint8)),
-                _vector("kv_mask", kv_mask, n * cells_k, (torch.bool, torch.uint8)))
+        return (_needed("lse", lse, n * self.q_heads * cells_q, dev),
+                _vector("q_mask", q_mask, n * cells_q, dev, (torch.bool, torch.uint8)),
+                _vector("kv_mask", kv_mask, n * cells_k, dev, (torch.bool, torch.uint8)))
 
     def forward(self, q, k, v, output: Tensor, lse, q_mask=None, kv_mask=None):
         pl, pq, pk = self._checked(q, k, v, (output,), (), lse, q_mask, kv_mask)

@@ -28,6 +28,7 @@
 
 #include <algorithm>
 #include <array>
+#include <cmath>
 #include <cstdint>
 #include <cstdio>
 #include <cstdlib>
@@ -2440,6 +2441,216 @@ public:
 
 private:
     BackendDNNLib& m_be;
+};
+
+// ---- attention between cells, and what goes with it (no counterpart in the reference) ----
+namespace internal
+{
+// Device memory that a layer keeps for its calls, which have to follow one another (one stream, or ordered streams).
+class Workspace
+{
+public:
+    Workspace() = default;
+    Workspace(const Workspace&) = delete;
+    ~Workspace() { cudaFree(m_p); }
+    void* get(int64_t bytes)
+    {
+        if (bytes > m_bytes)
+        {
+            cudaFree(m_p);
+            m_p = nullptr;
+            m_bytes = 0;
+            if (cudaMalloc(&m_p, (size_t) bytes) != cudaSuccess)
+                throw std::runtime_error("cudaMalloc of a layer's workspace failed");
+            m_bytes = bytes;
+        }
+        return m_p;
+    }
+
+private:
+    void* m_p = nullptr;
+    int64_t m_bytes = 0;
+};
+} // namespace internal
+
+// Layer normalisation over the channels of every cell, partitioned tensors or not.  mean and inv_std: a float per sample
+// and owned cell; scale and bias may be null.
+class LayerNormalization
+{
+public:
+    LayerNormalization(BackendDNNLib& backend, int num_dims, float epsilon)
+        : m_be(backend), m_num_dims(num_dims), m_epsilon(epsilon)
+    {}
+    int forward(TensorF& input, const float* scale, const float* bias, TensorF& output, float* mean = nullptr,
+                float* inv_std = nullptr)
+    {
+        if (input.get_local_size() == 0)
+            return 0;
+        const dcb_nd_desc xd = input.nd_desc(), yd = output.nd_desc();
+        util::check(dcb_ln_fwd(&xd, DCB_F32, input.get_base_ptr(), scale, bias, m_epsilon, &yd, output.get_base_ptr(),
+                               mean, inv_std, m_be.get_stream()),
+                    "layer normalisation");
+        return 0;
+    }
+    // d_input, and this rank's sums of the gradients of scale and bias
+    int backward_stage1(TensorF& input, TensorF& d_output, const float* mean, const float* inv_std, const float* scale,
+                        float* scale_gradient, float* bias_gradient, TensorF& d_input)
+    {
+        const size_t bytes = (size_t) input.get_local_shape()[-2] * sizeof(float);
+        const bool counts = input.get_local_size() != 0 && input.is_split_root();
+        if (input.get_local_size() != 0)
+        {
+            const dcb_nd_desc xd = input.nd_desc(), dyd = d_output.nd_desc(), dxd = d_input.nd_desc();
+            const int64_t ws = dcb_ln_bwd_workspace_bytes(&xd, DCB_F32);
+            util::check(dcb_ln_bwd(&xd, DCB_F32, input.get_base_ptr(), &dyd, d_output.get_base_ptr(), mean, inv_std,
+                                   scale, &dxd, d_input.get_base_ptr(), scale_gradient, bias_gradient, m_ws.get(ws), ws,
+                                   m_be.get_stream()),
+                        "layer normalisation backward");
+        }
+        if (!counts) // nothing here, or a replica, whose cells count once
+            for (float* g : {scale_gradient, bias_gradient})
+                cudaMemsetAsync(g, 0, bytes, m_be.get_stream());
+        return 0;
+    }
+    int backward(TensorF& input, TensorF& d_output, const float* mean, const float* inv_std, const float* scale,
+                 float* scale_gradient, float* bias_gradient, TensorF& d_input)
+    {
+        backward_stage1(input, d_output, mean, inv_std, scale, scale_gradient, bias_gradient, d_input);
+        const index_t C = input.get_local_shape()[-2];
+        m_be.allreduce(scale_gradient, C);
+        m_be.allreduce(bias_gradient, C);
+        return 0;
+    }
+
+private:
+    BackendDNNLib& m_be;
+    int m_num_dims;
+    float m_epsilon;
+    internal::Workspace m_ws;
+};
+
+// Rotary positions on the grid of a tensor's cells; positions are global, so that a shard gets the angles of the whole
+// tensor.  axis_channels (even) in reference order, W first.
+class RotaryPositions
+{
+public:
+    RotaryPositions(BackendDNNLib& backend, int num_dims) : m_be(backend), m_num_dims(num_dims) {}
+    RotaryPositions(const RotaryPositions&) = delete;
+    ~RotaryPositions() { dcb_rotary_plan_destroy(m_plan); }
+    // rotated_heads < 0: all
+    void setup(TensorF& input, int head_dim, const std::vector<int>& axis_channels, int rotated_heads = -1,
+               double base = 10000.0, bool interleaved = false)
+    {
+        const int nsd = m_num_dims - 2;
+        util::require((int) axis_channels.size() == nsd && input.get_num_dims() == m_num_dims && head_dim > 0,
+                      "RotaryPositions::setup: one entry per spatial dimension");
+        dcb_rotary_desc rd{};
+        rd.nsd = nsd;
+        rd.head_dim = head_dim;
+        rd.rotated_heads = rotated_heads < 0 ? (int32_t) (input.get_local_shape()[-2] / head_dim) : rotated_heads;
+        rd.interleaved = interleaved;
+        rd.base = base;
+        for (int i = 0; i < 3; ++i)
+            rd.step[i] = 1.0;
+        for (int i = 0; i < nsd; ++i)
+        {
+            rd.axis_channels[2 - i] = axis_channels[i];
+            rd.origin[2 - i] = input.get_global_index()[i];
+        }
+        const dcb_nd_desc xd = input.nd_desc();
+        dcb_rotary_plan_destroy(m_plan);
+        m_plan = nullptr;
+        util::check(dcb_rotary_plan_create(&rd, &xd, &m_plan), "rotary plan");
+    }
+    int forward(TensorF& input, TensorF& output) { return apply(input, output, 0); }
+    int backward(TensorF& d_output, TensorF& d_input) { return apply(d_output, d_input, 1); }
+
+private:
+    int apply(TensorF& x, TensorF& y, int inverse)
+    {
+        if (x.get_local_size() == 0)
+            return 0;
+        const dcb_nd_desc xd = x.nd_desc(), yd = y.nd_desc();
+        util::check(dcb_rotary_apply(m_plan, &xd, DCB_F32, x.get_base_ptr(), &yd, DCB_F32, y.get_base_ptr(), inverse,
+                                     m_be.get_stream()),
+                    "rotary positions");
+        return 0;
+    }
+    BackendDNNLib& m_be;
+    int m_num_dims;
+    dcb_rotary_plan* m_plan = nullptr;
+};
+
+// Scaled dot-product attention from the cells of one tensor to those of another, or its own.  A sample's cells and
+// channels have to be on one rank (re-distribute with TensorMPICUDAShuffler).  lse: a float per sample, query head and
+// cell; masks: a byte per sample and cell, may be null.
+class Attention
+{
+public:
+    // scale <= 0: 1 / sqrt(channels of a head)
+    Attention(BackendDNNLib& backend, int num_dims, int q_heads, int kv_heads, float scale = 0.f, bool causal = false)
+        : m_be(backend), m_num_dims(num_dims), m_q_heads(q_heads), m_kv_heads(kv_heads), m_scale(scale), m_causal(causal)
+    {
+        util::require(q_heads >= 1 && kv_heads >= 1 && q_heads % kv_heads == 0,
+                      "Attention: q_heads must be a multiple of kv_heads");
+    }
+    int forward(TensorF& q, TensorF& k, TensorF& v, TensorF& output, float* lse, const void* q_mask = nullptr,
+                const void* kv_mask = nullptr)
+    {
+        whole({&q, &k, &v, &output});
+        if (q.get_local_size() == 0)
+            return 0;
+        const dcb_attention_desc ad = desc(q);
+        const dcb_nd_desc qd = q.nd_desc(), kd = k.nd_desc(), vd = v.nd_desc(), od = output.nd_desc();
+        const int64_t ws = workspace(ad, qd, kd, 0);
+        util::check(dcb_attention_fwd(&ad, &qd, q.get_base_ptr(), &kd, k.get_base_ptr(), &vd, v.get_base_ptr(), q_mask,
+                                      kv_mask, &od, output.get_base_ptr(), lse, m_ws.get(ws), ws, m_be.get_stream()),
+                    "attention");
+        return 0;
+    }
+    int backward(TensorF& q, TensorF& k, TensorF& v, TensorF& output, const float* lse, TensorF& d_output, TensorF& d_q,
+                 TensorF& d_k, TensorF& d_v, const void* q_mask = nullptr, const void* kv_mask = nullptr)
+    {
+        whole({&q, &k, &v, &output, &d_output, &d_q, &d_k, &d_v});
+        if (q.get_local_shape()[-1] == 0)
+            return 0;
+        const dcb_attention_desc ad = desc(q);
+        const dcb_nd_desc qd = q.nd_desc(), kd = k.nd_desc(), vd = v.nd_desc(), od = output.nd_desc(),
+                          dod = d_output.nd_desc(), dqd = d_q.nd_desc(), dkd = d_k.nd_desc(), dvd = d_v.nd_desc();
+        const int64_t ws = workspace(ad, qd, kd, 1);
+        util::check(dcb_attention_bwd(&ad, &qd, q.get_base_ptr(), &kd, k.get_base_ptr(), &vd, v.get_base_ptr(), q_mask,
+                                      kv_mask, &od, output.get_base_ptr(), lse, &dod, d_output.get_base_ptr(), &dqd,
+                                      d_q.get_base_ptr(), &dkd, d_k.get_base_ptr(), &dvd, d_v.get_base_ptr(),
+                                      m_ws.get(ws), ws, m_be.get_stream()),
+                    "attention backward");
+        return 0;
+    }
+
+private:
+    static void whole(std::initializer_list<TensorF*> ts)
+    {
+        for (TensorF* t : ts)
+            for (int d = 0; d < t->get_num_dims() - 1; ++d)
+                util::require(!t->get_distribution().is_distributed(d) || t->get_distribution().get_locale_shape()[d] == 1,
+                              "Attention: a sample's cells have to be on one rank");
+    }
+    dcb_attention_desc desc(const TensorF& q) const
+    {
+        const float d = (float) (q.get_local_shape()[-2] / m_q_heads);
+        return dcb_attention_desc{m_q_heads, m_kv_heads, DCB_F32, m_causal, m_scale > 0.f ? m_scale : 1.f / std::sqrt(d)};
+    }
+    static int64_t workspace(const dcb_attention_desc& ad, const dcb_nd_desc& qd, const dcb_nd_desc& kd, int backward)
+    {
+        const int64_t ws = dcb_attention_workspace_bytes(&ad, &qd, &kd, backward);
+        if (ws < 0)
+            throw std::runtime_error(std::string("attention: ") + dcb_last_error());
+        return ws;
+    }
+    BackendDNNLib& m_be;
+    int m_num_dims, m_q_heads, m_kv_heads;
+    float m_scale;
+    bool m_causal;
+    internal::Workspace m_ws;
 };
 
 // ---- dump_tensor / dump_local_tensor (legacy/include/distconv/distconv.hpp:581-671)

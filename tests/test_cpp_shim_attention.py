@@ -1,0 +1,19 @@
+"""The C++ classes for attention between cells: compile and link without a GPU, results on one."""
+import shutil
+import subprocess
+
+import pytest
+
+from test_cpp_shim import _compile
+
+
+@pytest.mark.skipif(shutil.which("g++") is None, reason="no g++")
+def test_attention_classes_compile_and_link(tmp_path):
+    _compile(tmp_path / "shim_attention_check", "shim_attention_check.cpp")
+
+
+@pytest.mark.gpu
+def test_attention_classes(tmp_path):
+    exe = _compile(tmp_path / "shim_attention_check", "shim_attention_check.cpp")
+    r = subprocess.run([exe], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "shim_attention_check OK" in r.stdout, r.stdout + r.stderr

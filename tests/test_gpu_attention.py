@@ -304,3 +304,108 @@ def test_a_block_of_a_network():
     assert rel(heads(o.buffer, h), y.detach()) < 8 * 2 ** -8
     for got, leaf in ((dx.buffer, lx), (dg, lg), (db, lb), (dw, lw)):
         assert rel(got.reshape(leaf.shape), leaf.grad) < 8 * 2 ** -8
+
+
+def test_calls_that_are_refused():
+    be = backend()
+    at = dc.Attention(be, 4, 2, 1)
+    t = lambda c, cells=12, dtype=torch.float32: tensor(torch.zeros(1, c, 1, cells, dtype=dtype, device="cuda"), be)
+    q, k, lse = t(16), t(8), torch.zeros(1, 2, 12, device="cuda")
+    bad = [
+        (t(16), t(16), t(16), q, lse, {}),                                  # heads of another size
+        (q, k, t(8, 11), q, lse, {}),                                       # v has other cells
+        (q, t(8, dtype=torch.bfloat16), t(8, dtype=torch.bfloat16), q, lse, {}),
+        (q, k, k, t(16, 11), lse, {}),
+        (q, k, k, q, lse[:, :1], {}),
+        (q, k, k, q, lse.double(), {}),
+        (q, k, k, q, lse.cpu(), {}),
+        (q, k, k, q, None, {}),
+        (q, k, k, q, lse, {"kv_mask": torch.ones(1, 11, dtype=torch.bool, device="cuda")}),
+        (q, k, k, q, lse, {"q_mask": torch.ones(1, 12, device="cuda")}),
+        (q, k, k, q, lse, {"q_mask": torch.ones(1, 24, dtype=torch.bool, device="cuda")[:, ::2]}),
+    ]
+    for *args, kw in bad:
+        with pytest.raises(ValueError):
+            at.forward(*args, **kw)
+    with pytest.raises(ValueError):
+        dc.Attention(be, 4, 2, 2).forward(t(258), t(258), t(258), t(258), lse)  # 129 channels a head
+    part = dc.Tensor([12, 4, 16, 1], dc.Locale(0, 2), dc.Distribution.make_distribution([2, 1, 1, 1]))
+    part.allocate()
+    with pytest.raises(ValueError):
+        at.forward(part, part, part, part, lse)
+    ln = dc.LayerNormalization(be, 4, 1e-5)
+    with pytest.raises(ValueError):
+        ln.forward(q, torch.ones(16), None, q)  # scale on the host
+    with pytest.raises(ValueError):
+        ln.forward(q, torch.ones(15, device="cuda"), None, q)
+    with pytest.raises(ValueError):
+        ln.backward(q, q, None, None, None, None, None, q)
+    rot = dc.RotaryPositions(be, 4)
+    rot.setup(q, 8, [4, 4])
+    with pytest.raises(ValueError):
+        rot.forward(k, k)
+    with pytest.raises(dc.distconv._abi.DcbError):
+        rot.setup(q, 8, [3, 4])
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=["f32", "bf16"])
+def test_offsets_that_pass_32_bits(dtype):
+    """Keys and values of 2^31 elements and more: weights are equal, values depend on the channel and the half."""
+    cells, d = (1 << 25) + 40, 64
+    be = backend()
+    k = torch.zeros(1, d, 1, cells, dtype=dtype, device="cuda")
+    v = torch.empty_like(k)
+    channel = torch.arange(d, device="cuda", dtype=torch.float32).to(dtype)
+    v[0, :, 0, : cells // 2], v[0, :, 0, cells // 2:] = channel[:, None], -3 * channel[:, None]
+    q, o = torch.ones(1, d, 1, 2, dtype=dtype, device="cuda"), torch.empty(1, d, 1, 2, dtype=dtype, device="cuda")
+    lse = torch.empty(1, 1, 2, device="cuda")
+    at = dc.Attention(be, 4, 1)
+    at.forward(*(tensor(t, be) for t in (q, k, v, o)), lse)
+    # o = -channel: sums of equal weights, in parts of at most 2^25 terms
+    want = -torch.arange(d, dtype=torch.float64)[:, None].expand(d, 2)
+    off = (o[0, :, 0].double().cpu() - want).abs().max()
+    assert float(off) <= 64 * (R.stored(dtype) + 2.0 ** -10), float(off)
+    assert float((lse.double().cpu() - math.log(cells)).abs().max()) < 1e-3
+    # and the other operators over the same memory
+    tv, tk = tensor(v, be), tensor(k, be)
+    ln = dc.LayerNormalization(be, 4, 1e-5)
+    ln.forward(tv, None, None, tk)
+    u = (channel.double() - channel.double().mean()) / channel.double().std(correction=0)
+    for j, sign in ((0, 1), (cells - 1, -1)):
+        assert float((k[0, :, 0, j].double() - sign * u).abs().max()) <= 2 * R.stored(dtype) * 2 + 1e-4
+    rot = dc.RotaryPositions(be, 4)
+    rot.setup(tv, d, [0, 2])
+    rot.forward(tv, tk)
+    assert torch.equal(k[0, 2:, 0, -5:], v[0, 2:, 0, -5:])
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=["f32", "bf16"])
+def test_two_calls_at_once(dtype):
+    """Two layers on two streams, masked and not, many times: neither sees the other's workspace."""
+    g = torch.Generator().manual_seed(12)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    sets = []
+    for s in streams:
+        be = backend(s)
+        q, k, v, do = (tensor(torch.randn(2, 64, 9, 15, generator=g).to(dtype).cuda(), be) for _ in range(4))
+        o, dq, dk, dv = (tensor(torch.empty_like(q.buffer), be) for _ in range(4))
+        lse = torch.empty(2, 2, 135, device="cuda")
+        mask = (torch.rand(2, 135, generator=g) < 0.7).cuda()
+        at = dc.Attention(be, 4, 2)
+
+        def step(at=at, q=q, k=k, v=v, o=o, lse=lse, do=do, dq=dq, dk=dk, dv=dv, mask=mask):
+            at.forward(q, k, v, o, lse, q_mask=mask, kv_mask=mask)
+            at.backward(q, k, v, o, lse, do, dq, dk, dv, q_mask=mask, kv_mask=mask)
+
+        torch.cuda.synchronize()
+        step()
+        torch.cuda.synchronize()
+        out = [o.buffer, dq.buffer, dk.buffer, dv.buffer, lse]
+        sets.append((step, out, [t.clone() for t in out]))
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for step, *_ in sets:
+            step()
+    torch.cuda.synchronize()
+    for _s, out, want in sets:
+        assert all(torch.equal(a, b) for a, b in zip(out, want))
