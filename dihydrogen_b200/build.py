@@ -22,7 +22,7 @@ LIB = os.path.join(PKG, "libdistconv_b200.so")
 SOURCES = ["runtime.cu", "halo.cu", "bn.cu", "conv.cu", "conv_simt.cu", "conv_tc.cu",
            "conv_tc_wgrad_s1.cu", "conv_tc_wgrad_s2.cu", "conv_tc_shift.cu",
            "conv_tc_shift_plan.cu", "conv_tc_wgrad_plan.cu", "comm.cu", "pool.cu", "shuffle.cu",
-           "ln.cu", "rotary.cu", "attention.cu", "attention_simt.cu", "attention_tc.cu",
+           "ln.cu", "rotary.cu", "attention.cu", "attention_thin.cu", "attention_simt.cu", "attention_tc.cu",
            "attention_tc_fwd.cu", "attention_tc_bwd.cu"]
 
 NVCC_FLAGS = [

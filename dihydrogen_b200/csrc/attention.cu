@@ -30,9 +30,13 @@ __global__ void __launch_bounds__(ATTN_INDEX_THREADS) attn_index_kernel(const __
     {
         const long long i0 = c0 + threadIdx.x * ATTN_INDEX_CELLS;
         uint32_t bits = 0;
+        uint8_t m[ATTN_INDEX_CELLS];
+#pragma unroll
         for (int e = 0; e < ATTN_INDEX_CELLS; ++e)
-            if (i0 + e < cells && mask[i0 + e])
-                bits |= 1u << e;
+            m[e] = i0 + e < cells ? mask[i0 + e] : (uint8_t) 0;
+#pragma unroll
+        for (int e = 0; e < ATTN_INDEX_CELLS; ++e)
+            bits |= (m[e] ? 1u : 0u) << e;
         const int mine = __popc(bits);
         int sum = mine; // of this lane and those before
         for (int h = 1; h < 32; h *= 2)
@@ -376,7 +380,11 @@ int64_t attn_carve(AttnProblem* p, int32_t dtype, bool backward, void* workspace
 {
     Carve w{static_cast<char*>(workspace)};
     const bool tc = dtype == DCB_BF16;
-    (tc ? attn_tc_splits : attn_simt_splits)(p, backward);
+    const bool thin = !backward && attn_thin(*p, dtype);
+    if (thin)
+        attn_thin_splits(p, dtype);
+    else
+        (tc ? attn_tc_splits : attn_simt_splits)(p, backward);
     const long long qh = (long long) p->n * p->q_heads, kh = (long long) p->n * p->kv_heads;
     p->stats_pitch = tc ? (long long) attn_tiles(p->sq, 128) * 128 : p->sq;
     const auto side = [&](int cells, bool masked) {
@@ -388,7 +396,7 @@ int64_t attn_carve(AttnProblem* p, int32_t dtype, bool backward, void* workspace
     };
     p->q_side = side(p->sq, p->q_mask != nullptr);
     p->kv_side = side(p->sk, p->kv_mask != nullptr);
-    if (tc)
+    if (tc && !thin)
     {
         const auto copy = [&](long long heads, int cells) {
             return reinterpret_cast<bf16*>(w.floats(heads * p->d * ((cells + 7) / 8) * 4));
@@ -536,12 +544,15 @@ int32_t dcb_attention_fwd(const dcb_attention_desc* ad, const dcb_nd_desc* qd, c
         return e;
     if (int32_t e = attn_zeros(p, ad->dtype, false, s))
         return e;
-    if (int32_t e = ad->dtype == DCB_BF16 ? attn_tc_fwd(p, s) : attn_simt_fwd(p, s))
+    const int32_t e = attn_thin(p, ad->dtype)   ? attn_thin_fwd(p, ad->dtype, s)
+                      : ad->dtype == DCB_BF16 ? attn_tc_fwd(p, s)
+                                              : attn_simt_fwd(p, s);
+    if (e)
         return e;
     if (p.kv_splits == 1)
         return DCB_OK;
-    return with_type(ad->dtype, [&](auto e) -> int32_t {
-        DCB_CUDA_TRY(launch_overlapped(attn_join_fwd_kernel<decltype(e)>,
+    return with_type(ad->dtype, [&](auto t) -> int32_t {
+        DCB_CUDA_TRY(launch_overlapped(attn_join_fwd_kernel<decltype(t)>,
                                        dim3(flat_blocks((long long) p.n * p.q_heads * p.d * p.sq, 256)), 256, 0, s, p));
         return DCB_OK;
     });

@@ -283,4 +283,28 @@ __device__ __forceinline__ long long offset_of(const CellAt& a, const RunStrides
     return a.n * s.sn + a.outer * s.s_outer + a.inner * s.s_inner + a.pos;
 }
 
+// Sums over a warp's lanes of K values a lane, by halves: lane l ends with the sum of value l mod K
+// in v[0].  K - 1 + log2(32 / K) exchanges instead of 5 K.
+template <int K>
+__device__ __forceinline__ float lane_sums(float (&v)[K], int lane)
+{
+#pragma unroll
+    for (int h = K / 2; h >= 1; h /= 2)
+    {
+        const bool upper = lane & h;
+#pragma unroll
+        for (int i = 0; i < h; ++i)
+        {
+            const float send = upper ? v[i] : v[i + h];
+            const float keep = upper ? v[i + h] : v[i];
+            v[i] = keep + __shfl_xor_sync(~0u, send, h);
+        }
+    }
+    float r = v[0];
+#pragma unroll
+    for (int h = K; h < 32; h *= 2)
+        r += __shfl_xor_sync(~0u, r, h);
+    return r;
+}
+
 } // namespace dcb

@@ -322,30 +322,6 @@ __global__ void __launch_bounds__(32 * LN_WARPS, 4)
     dependents_may_start();
 }
 
-// Sums over a warp's lanes of K values a lane, by halves: lane l ends with the sum of value l mod K
-// in v[0].  K - 1 + log2(32 / K) exchanges instead of 5 K.
-template <int K>
-__device__ __forceinline__ float ln_lane_sums(float (&v)[K], int lane)
-{
-#pragma unroll
-    for (int h = K / 2; h >= 1; h /= 2)
-    {
-        const bool upper = lane & h;
-#pragma unroll
-        for (int i = 0; i < h; ++i)
-        {
-            const float send = upper ? v[i] : v[i + h];
-            const float keep = upper ? v[i + h] : v[i];
-            v[i] = keep + __shfl_xor_sync(~0u, send, h);
-        }
-    }
-    float r = v[0];
-#pragma unroll
-    for (int h = K; h < 32; h *= 2)
-        r += __shfl_xor_sync(~0u, r, h);
-    return r;
-}
-
 template <class T, int V, int MODE, bool FULL, bool KEEP>
 __device__ __forceinline__ void ln_bwd_tile(const T* x, const RunStrides& xs, const T* dy, const RunStrides& dys,
                                             const float* mean_in, const float* inv_std_in,
@@ -394,7 +370,7 @@ __device__ __forceinline__ void ln_bwd_tile(const T* x, const RunStrides& xs, co
         }
         if (grads) // a channel belongs to one warp of the group
         {
-            const float tw = ln_lane_sums<m>(sw, me.lane), tb = ln_lane_sums<m>(sb, me.lane);
+            const float tw = lane_sums<m>(sw, me.lane), tb = lane_sums<m>(sb, me.lane);
             const int c = me.cg + (i + me.lane) * geo.g;
             if (me.lane < m)
             {

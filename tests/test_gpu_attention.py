@@ -86,6 +86,21 @@ def test_few_cells_against_many(shape, dtype):
     run(*shape, dtype, causal=True)
 
 
+@pytest.mark.parametrize("dtype", TYPES, ids=["f32", "bf16"])
+@pytest.mark.parametrize("cells", [1, 2, 7, 8, 9])
+def test_few_queries(cells, dtype):
+    """About the counts at which another kernel takes over: channels, keys and orders off every tile, masks."""
+    g = torch.Generator().manual_seed(13)
+    for hq, hk, d, keys in ((4, 2, 64, 4096), (2, 2, 24, 257), (3, 1, 128, 1000), (2, 1, 33, 31), (2, 2, 65, 1336), (1, 1, 1, 8)):
+        run(2, hq, hk, d, (1, cells), (1, keys), dtype)
+        run(2, hq, hk, d, (1, cells), (1, keys), dtype, causal=True, pad=3)
+        qm, km = torch.rand(3, cells, generator=g) < 0.7, torch.rand(3, keys, generator=g) < 0.5
+        km[1], qm[2] = False, False
+        run(3, hq, hk, d, (1, cells), (1, keys), dtype, q_mask=qm, kv_mask=km, poison=NAN)
+        run(3, hq, hk, d, (1, cells), (1, keys), dtype, causal=True, kv_mask=km, poison=float("inf"), pad=8)
+        run(3, hq, hk, d, (1, cells), (1, keys), dtype, q_mask=qm, poison=-3.3e38)
+
+
 @pytest.mark.parametrize("poison", [0.0, NAN, float("inf"), -3.3e38])
 @pytest.mark.parametrize("dtype", TYPES, ids=["f32", "bf16"])
 @pytest.mark.parametrize("causal", [False, True])
