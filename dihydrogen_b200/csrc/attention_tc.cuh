@@ -259,6 +259,29 @@ __device__ __forceinline__ float at_exp2(float x)
     return y;
 }
 
+// 2^x of two numbers of at most 127 without the unit that has ex2: 2^i p(f), i the nearest whole number (from the low
+// bits of x + 1.5 2^23, to which 127 is added: they are the exponent of 2^i), p of degree 4 with the least greatest
+// relative error on [-1/2, 1/2] (Remez exchange; 2.7e-6 with its coefficients in 32 bits).  0 below -126.5, NaN for NaN.
+__device__ __forceinline__ void at_exp2_pair(uint64_t x, float& lo, float& hi)
+{
+    float a, b;
+    at_unpair(x, a, b);
+    asm("max.NaN.f32 %0, %1, 0fC2FE0000;" : "=f"(a) : "f"(a)); // -127
+    asm("max.NaN.f32 %0, %1, 0fC2FE0000;" : "=f"(b) : "f"(b));
+    x = at_pair(a, b);
+    const float magic = 12582912.f + 127.f;
+    const uint64_t i = at_add2(x, at_pair(magic, magic));
+    const uint64_t f = at_fma2(at_add2(i, at_pair(-magic, -magic)), at_pair(-1.f, -1.f), x);
+    uint64_t y = at_fma2(f, at_pair(9.570102e-3f, 9.570102e-3f), at_pair(5.591786e-2f, 5.591786e-2f));
+    y = at_fma2(y, f, at_pair(.24024744f, .24024744f));
+    y = at_fma2(y, f, at_pair(.6931218f, .6931218f));
+    y = at_fma2(y, f, at_pair(.9999993f, .9999993f));
+    at_unpair(i, a, b);
+    a = __uint_as_float(__float_as_uint(a) << 23);
+    b = __uint_as_float(__float_as_uint(b) << 23);
+    at_unpair(at_mul2(y, at_pair(a, b)), lo, hi);
+}
+
 // A wait of a whole warp: it goes on, or gives up, as one.
 __device__ __forceinline__ bool at_warp_wait(uint64_t* bar, uint32_t parity, volatile int* give_up)
 {

@@ -319,7 +319,9 @@ __global__ void __launch_bounds__(AT_THREADS, AfShape<D, APART>::BLOCKS)
             scale2 = at_pair(p.scale, p.scale), base2 = at_pair(-base_of, -base_of);
             l0 = l1 = 0;
         };
-        // weights of 16 scores, to the h-th eight columns
+        // Weights of 16 scores, to the h-th eight columns.  With two blocks on an SM two of them do without ex2, whose
+        // unit is what these warps wait for: 4 x 8 heads x 64^2 cells x 64 take 208 us, 219 with none, 208 with four, 226
+        // with eight.  One block's warps have no issue slots left for it: 128 channels go from 611 us to 623.
         const auto weigh = [&](int u, int h, const float* s) {
             uint32_t w[8];
 #pragma unroll
@@ -328,10 +330,16 @@ __global__ void __launch_bounds__(AT_THREADS, AfShape<D, APART>::BLOCKS)
                 float e[4];
 #pragma unroll
                 for (int k = 0; k < 4; k += 2)
-                    at_unpair(at_fma2(at_pair(s[c + k], s[c + k + 1]), scale2, base2), e[k], e[k + 1]);
-#pragma unroll
-                for (int k = 0; k < 4; ++k)
-                    e[k] = at_exp2(e[k]);
+                {
+                    const uint64_t x = at_fma2(at_pair(s[c + k], s[c + k + 1]), scale2, base2);
+                    if (S::BLOCKS == 2 && c + k == 14)
+                        at_exp2_pair(x, e[k], e[k + 1]);
+                    else
+                    {
+                        at_unpair(x, e[k], e[k + 1]);
+                        e[k] = at_exp2(e[k]), e[k + 1] = at_exp2(e[k + 1]);
+                    }
+                }
                 l0 = at_add2(l0, at_pair(e[0], e[1]));
                 l1 = at_add2(l1, at_pair(e[2], e[3]));
                 w[c / 2] = pack_bf16(e[0], e[1]);

@@ -243,6 +243,24 @@ def test_the_same_bits_every_run_on_streams_and_in_graphs(dtype):
 
 
 @pytest.mark.parametrize("dtype", TYPES, ids=["f32", "bf16"])
+@pytest.mark.parametrize("queries", [1, 6, 150])
+@pytest.mark.parametrize("d", [32, 64, 128])
+def test_a_key_that_is_not_a_number_reaches_the_queries_that_see_it(d, queries, dtype):
+    g = torch.Generator().manual_seed(14)
+    be = backend()
+    keys = 150
+    for bad in (0, 13, 14, 15, 30, 63, 64, 127, 149):
+        for causal in (False, True):
+            q, k, v = (torch.randn(1, d, 1, c, generator=g).to(dtype).cuda() for c in (queries, keys, keys))
+            k[..., bad] = NAN
+            o, lse = torch.zeros_like(q), torch.zeros(1, 1, queries, device="cuda")
+            dc.Attention(be, 4, 1, 1, causal=causal).forward(*(tensor(t, be) for t in (q, k, v, o)), lse)
+            sees = torch.arange(queries) + (keys - queries if causal else keys) >= bad
+            assert torch.equal(lse.flatten().isnan().cpu(), sees)
+            assert torch.equal(o.isnan().all(1).flatten().cpu(), sees) and torch.equal(o.isnan().any(1).flatten().cpu(), sees)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=["f32", "bf16"])
 def test_empty_sides(dtype):
     be = backend()
     at = dc.Attention(be, 4, 2)
