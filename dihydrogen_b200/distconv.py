@@ -355,7 +355,12 @@ class Tensor:
     def _nd(self, lo=None, hi=None):
         """nd_desc() by reference, made once per pair of widths; for the operators on single precision."""
         self._single()
-        return self._nd_any(lo, hi)
+        descs = self._geo().descs
+        key = (tuple(lo), tuple(hi)) if lo is not None else None
+        d = descs.get(key)
+        if d is None:
+            d = descs[key] = self._make_nd_desc(lo, hi)
+        return ctypes.byref(d)
 
     def _single(self):
         if self.dtype is not torch.float32:
@@ -367,14 +372,6 @@ class Tensor:
         if g.operand is None:
             g.operand = ctypes.byref(self._make_nd_desc())
         return g.operand, self.buffer.data_ptr() + g.base
-
-    def _nd_any(self, lo=None, hi=None):
-        descs = self._geo().descs
-        key = (tuple(lo), tuple(hi)) if lo is not None else None
-        d = descs.get(key)
-        if d is None:
-            d = descs[key] = self._make_nd_desc(lo, hi)
-        return ctypes.byref(d)
 
     # -- memory --
     def np_real_shape(self):
@@ -1513,7 +1510,7 @@ def _workspace(nbytes: int, stream, device):
     streams and captured graphs never share it."""
     if nbytes <= 0:
         return None, 0
-    if stream is None:
+    if stream is None or stream.cuda_stream == torch._C._cuda_getCurrentRawStream(device.index):
         ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
     else:
         with torch.cuda.stream(stream):

@@ -242,6 +242,25 @@ def test_the_same_bits_every_run_on_streams_and_in_graphs(dtype):
         assert all(torch.equal(a, b) for a, b in zip(out, want))
 
 
+def test_masks_of_many_cells():
+    """A mask is counted in parts of 8192 cells and more, from any address; any byte that is not zero counts."""
+    g = torch.Generator().manual_seed(15)
+    for keys, first in ((8192, 0), (8193, 1), (40001, 5), (64 * 8192 + 7, 3)):
+        km = (torch.rand(2, keys, generator=g) < 0.3).to(torch.uint8) * torch.randint(1, 256, (2, keys), generator=g).to(torch.uint8)
+        km[0, : keys // 2] = 0
+        q, k, v = (torch.randn(2, 16, 1, c, generator=g) for c in (3, keys, keys))
+        want = R.attention(heads(q, 2), heads(k, 2), heads(v, 2), 1 / math.sqrt(8), kv_mask=km)
+        be = backend()
+        room = torch.zeros(2 * keys + first, dtype=torch.uint8, device="cuda")
+        mask = room[first:].view(2, keys)
+        mask.copy_(km)
+        tq, tk, tv = (tensor(t.cuda(), be) for t in (q, k, v))
+        o, lse = tensor(torch.full_like(q, NAN).cuda(), be), torch.full((2, 2, 3), NAN, device="cuda")
+        dc.Attention(be, 4, 2, 2).forward(tq, tk, tv, o, lse, kv_mask=mask)
+        R.close(lse, want["lse"], "lse")
+        R.close(heads(o.buffer, 2), want["o"], "o")
+
+
 @pytest.mark.parametrize("dtype", TYPES, ids=["f32", "bf16"])
 @pytest.mark.parametrize("queries", [1, 6, 150])
 @pytest.mark.parametrize("d", [32, 64, 128])
