@@ -177,14 +177,15 @@ __global__ void __launch_bounds__(256) attn_join_fwd_kernel(AttnProblem p)
         float m = -INFINITY;
         for (int s = 0; s < p.kv_splits && !gone; ++s)
             m = fmaxf(m, ml[s * step]);
+        // a part whose only keys are NaN has no maximum, but a sum that is NaN
+        const float base = m == -INFINITY ? 0.f : m;
         float l = 0.f, o = 0.f;
-        if (m != -INFINITY)
-            for (int s = 0; s < p.kv_splits; ++s)
-            {
-                const float f = exp2f(ml[s * step] - m);
-                l = fmaf(ml[s * step + heads * p.sq], f, l);
-                o = fmaf(p.part_o[s * total + at], f, o);
-            }
+        for (int s = 0; s < p.kv_splits && !gone; ++s)
+        {
+            const float f = exp2f(ml[s * step] - base);
+            l = fmaf(ml[s * step + heads * p.sq], f, l);
+            o = fmaf(p.part_o[s * total + at], f, o);
+        }
         const bool none = l == 0.f;
         const float v[1] = {none ? 0.f : o / l};
         store_elems<1>(static_cast<T*>(p.o.p) + n * p.o.sn + ((nh - n * p.q_heads) * p.d + c) * p.o.sc + i, v);
