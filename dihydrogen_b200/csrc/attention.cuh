@@ -84,12 +84,12 @@ __host__ __device__ inline int attn_tiles(int cells, int tile)
     return (cells + tile - 1) / tile;
 }
 
-// Splits of a walk over `steps` tiles so that `work` walks fill `slots` blocks; a part walks `least` tiles at least.
-inline int attn_splits(long long work, int steps, long long slots, int least)
+// Splits of a walk over `steps` tiles so that `work` walks fill `slots` blocks; a part walks a tile at least.
+inline int attn_splits(long long work, int steps, long long slots)
 {
     if (work <= 0 || work >= slots)
         return 1;
-    return (int) std::max<long long>(1, std::min<long long>(slots / work, steps / least));
+    return (int) std::max<long long>(1, std::min<long long>(slots / work, steps));
 }
 
 // Kernels of attention_thin.cu: the forward pass of so few queries that it is a pass over the keys.  2 x 8 heads x 64,

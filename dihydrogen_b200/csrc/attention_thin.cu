@@ -247,7 +247,7 @@ void attn_thin_splits(AttnProblem* p, int32_t dtype)
     const int channels = dtype == DCB_BF16 && !p->kv_mask && p->sk % 8 == 0 ? ath_channels<bf16>() : 8;
     const int warps = (p->d <= 32 ? 32 : p->d <= 64 ? 64 : 128) / channels;
     p->kv_splits = attn_splits((long long) p->n * p->q_heads * p->sq, attn_tiles(p->sk, 32 * ATH_KEYS),
-                               (16ll / warps) * num_sms(), 1);
+                               (16ll / warps) * num_sms());
     p->q_splits = 1;
 }
 
