@@ -234,11 +234,6 @@ inline CellUnits cell_units_of(const RunGeom& g, long long per_run)
     return u;
 }
 
-inline CellUnits cell_units(const RunGeom& g, int v)
-{
-    return cell_units_of(g, g.len / v);
-}
-
 struct CellAt
 {
     long long n;
