@@ -582,6 +582,7 @@ int32_t dcb_attention_fwd(const dcb_attention_desc* ad, const dcb_nd_desc* qd, c
     if (p.n == 0 || p.sq == 0)
         return DCB_OK;
     DCB_REQUIRE(lse, "null lse");
+    DCB_REQUIRE(o != q && (p.sk == 0 || (o != k && o != v)), "a result in an operand's place");
     cudaStream_t s = as_stream(stream);
     p.lse = static_cast<float*>(lse);
     p.q_mask = static_cast<const uint8_t*>(q_mask);
@@ -632,6 +633,13 @@ int32_t dcb_attention_bwd(const dcb_attention_desc* ad, const dcb_nd_desc* qd, c
             return e;
     if (p.n == 0)
         return DCB_OK;
+    const void* const results[] = {dq, dk, dv};
+    for (int r = 0; r < 3; ++r)
+    {
+        for (const void* x : {q, k, v, o, d_o, lse})
+            DCB_REQUIRE(!results[r] || results[r] != x, "a result in an operand's place");
+        DCB_REQUIRE(!results[r] || results[r] != results[(r + 1) % 3], "two results in one place");
+    }
     cudaStream_t s = as_stream(stream);
     if (p.sq == 0 || p.sk == 0) // one side is empty: the other's gradients are zero
     {

@@ -491,14 +491,16 @@ int32_t dcb_rotary_apply(const dcb_rotary_plan* plan, const dcb_nd_desc* xd,
  * i may see j if q_mask (n x cells of q bytes, may be null) is not 0 at i, kv_mask
  * (n x cells of k) not at j, and, where `causal`, j <= i + (cells of k - cells of
  * q).  A cell that sees nothing gets o = 0, lse = -infinity and takes no part in
- * any gradient (its d_o has to be finite where no mask takes it out).  Cells that a mask takes out are never interpreted, whatever they
- * hold; `causal` only sets the weight of a later cell to 0, its values have to be
- * finite.  A sample's cells lie contiguous (a shard without halo; re-distribute a
- * spatially partitioned tensor to sample-parallel first); sample and channel
- * strides are free.  All tensors are of desc->dtype; lse is n x q_heads x cells of
- * q floats.  fp32 tensors are multiplied in fp32; bf16 tensors on the tensor cores
- * with fp32 accumulation, and their weights exp(s) are rounded to bf16.  The same
- * bits every run.
+ * any gradient (its d_o has to be finite where no mask takes it out).  What cells
+ * that a mask takes out hold is never interpreted, and their results are 0;
+ * `causal` only sets the weight of a later cell to 0, its values have to be finite.
+ * A sample's cells lie contiguous (a shard without halo; re-distribute a spatially
+ * partitioned tensor to sample-parallel first); sample and channel strides are
+ * free.  All tensors are of desc->dtype; lse is n x q_heads x cells of q floats.
+ * No result overlaps an operand or another result.  fp32 tensors are multiplied in
+ * fp32; bf16 tensors on the tensor cores with fp32 accumulation, and their weights
+ * exp(s) and the gradients of s are rounded to bf16 as operands (a single query's
+ * weights stay fp32).  The same bits every run.
  * ------------------------------------------------------------------------ */
 typedef struct dcb_attention_desc
 {

@@ -113,6 +113,26 @@ def test_attention_refusals():
     assert attention(desc(), nd(0, 16, 3, 5), nd(0, 8, 4, 7), q=None) == _abi.OK
 
 
+def test_results_in_an_operands_place_are_refused():
+    ad, qd, kd = desc(q=2, kv=1), nd(1, 16, 3, 5), nd(1, 8, 4, 7)
+    far = lambda i: FAKE + (i << 20)
+    for taken in range(3):
+        at = [far(1), far(2), far(3)]
+        assert status("dcb_attention_fwd", ad, qd, at[0], kd, at[1], kd, at[2], None, None, qd, at[taken], far(9), far(8),
+                      1 << 40, None) == _abi.BAD_ARG
+        assert b"place" in _abi.lib().dcb_last_error()
+    names = ("q", "k", "v", "o", "lse", "d_o", "dq", "dk", "dv")
+    for result in ("dq", "dk", "dv"):
+        for other in names:
+            if other == result:
+                continue
+            a = {n: far(i + 1) for i, n in enumerate(names)}
+            a[result] = a[other]
+            assert status("dcb_attention_bwd", ad, qd, a["q"], kd, a["k"], kd, a["v"], None, None, qd, a["o"], a["lse"], qd,
+                          a["d_o"], qd, a["dq"], kd, a["dk"], kd, a["dv"], far(12), 1 << 40, None) == _abi.BAD_ARG
+            assert b"place" in _abi.lib().dcb_last_error()
+
+
 @pytest.mark.parametrize("dtype", [_abi.F32, _abi.BF16])
 def test_workspaces_are_whole_units(dtype):
     """Of 256 bytes; how many depends on the parts that walks are cut in, too."""
