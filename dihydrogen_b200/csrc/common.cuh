@@ -310,6 +310,12 @@ inline bool same_extents(const dcb_nd_desc& a, const dcb_nd_desc& b)
            && a.dims[1] == b.dims[1] && a.dims[2] == b.dims[2];
 }
 
+inline bool same_strides(const dcb_nd_desc& a, const dcb_nd_desc& b)
+{
+    return a.sn == b.sn && a.sc == b.sc && a.strides[0] == b.strides[0] && a.strides[1] == b.strides[1]
+           && a.strides[2] == b.strides[2];
+}
+
 // Largest vector width (4, 2, 1 floats) that every run start of a tensor with
 // these strides honours.
 inline int run_vec(const RunGeom& g, const RunStrides& s, const void* p)

@@ -646,6 +646,7 @@ int32_t dcb_ln_fwd(const dcb_nd_desc* xd, int32_t dtype, const void* x, const vo
     if (ln_empty(xd))
         return DCB_OK;
     DCB_REQUIRE(x && y, "null tensor");
+    DCB_REQUIRE(x != y || same_strides(*xd, *yd), "in place the strides must be the same");
     const int level = ln_level({xd, yd});
     DCB_REQUIRE(level >= 0, "W must have unit stride");
     RunGeom rg;
@@ -664,8 +665,7 @@ int32_t dcb_ln_fwd(const dcb_nd_desc* xd, int32_t dtype, const void* x, const vo
         using T = decltype(t);
         return ln_with_shape(h, [&](auto v, auto mode, auto keep) {
             return ln_launch_fwd<T, decltype(v)::value, decltype(mode)::value, decltype(keep)::value>(
-                g, x, xs, y, ys, scale, bias, eps, mean,
-                                                                               inv_std, as_stream(stream));
+                g, x, xs, y, ys, scale, bias, eps, mean, inv_std, as_stream(stream));
         });
     });
 }
@@ -701,6 +701,8 @@ int32_t dcb_ln_bwd(const dcb_nd_desc* xd, int32_t dtype, const void* x, const dc
         return DCB_OK;
     }
     DCB_REQUIRE(x && dy && dx && mean && inv_std, "null tensor");
+    DCB_REQUIRE((dx != x || same_strides(*dxd, *xd)) && (dx != dy || same_strides(*dxd, *dyd)),
+                "in place the strides must be the same");
     const int level = ln_level({xd, dyd, dxd});
     DCB_REQUIRE(level >= 0, "W must have unit stride");
     if (dscale)

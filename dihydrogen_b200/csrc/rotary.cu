@@ -205,12 +205,6 @@ int32_t rotary_launch(int v, bool split, dim3 grid, const void* x, const RunStri
     return v == 4 ? go(rotary_kernel<TX, TY, 4, false>) : go(rotary_kernel<TX, TY, 1, false>);
 }
 
-bool same_strides(const dcb_nd_desc& a, const dcb_nd_desc& b)
-{
-    return a.sn == b.sn && a.sc == b.sc && a.strides[0] == b.strides[0] && a.strides[1] == b.strides[1]
-           && a.strides[2] == b.strides[2];
-}
-
 } // namespace
 } // namespace dcb
 

@@ -418,7 +418,7 @@ int64_t dcb_pool_bwd_workspace_bytes(const dcb_pool_desc* pd,
  * cell, dense in the order N, D, H, W.  All sums are fp32 or wider.
  * ------------------------------------------------------------------------ */
 /* scale and bias may be null (1 and 0), mean and inv_std too (not wanted).  y may
- * be x. */
+ * be x, with its strides. */
 int32_t dcb_ln_fwd(const dcb_nd_desc* xd, int32_t dtype, const void* x,
                    const void* scale, const void* bias, float eps,
                    const dcb_nd_desc* yd, void* y, void* mean, void* inv_std,
@@ -428,8 +428,8 @@ int32_t dcb_ln_fwd(const dcb_nd_desc* xd, int32_t dtype, const void* x,
  *   dscale[c] = sum dy * u,  dbias[c] = sum dy  over the cells xd describes
  * (overwritten; a partitioned tensor's are then all-reduced).  mean and inv_std as
  * dcb_ln_fwd left them; scale may be null; dscale and dbias may both be null (not
- * wanted), and no workspace is needed then.  dx may be dy or x.  The sums over
- * cells are taken in a fixed order: the same bits every run. */
+ * wanted), and no workspace is needed then.  dx may be dy or x, with their strides.
+ * The sums over cells are taken in a fixed order: the same bits every run. */
 int32_t dcb_ln_bwd(const dcb_nd_desc* xd, int32_t dtype, const void* x,
                    const dcb_nd_desc* dyd, const void* dy, const void* mean,
                    const void* inv_std, const void* scale,

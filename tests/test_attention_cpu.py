@@ -54,6 +54,15 @@ def test_layer_norm_refusals():
     assert bwd(FAKE, FAKE, FAKE + 4, need) == _abi.BAD_ARG
 
 
+def test_layer_norm_in_place_needs_the_same_strides():
+    a, b = nd(2, 4, 3, 5), nd(2, 4, 3, 5, sc=16)
+    assert status("dcb_ln_fwd", a, 0, FAKE, None, None, 1e-5, b, FAKE, None, None, None) == _abi.BAD_ARG
+    assert b"strides" in _abi.lib().dcb_last_error()
+    for x, dy, xd, dyd in ((FAKE, 2 * FAKE, b, a), (2 * FAKE, FAKE, a, b)):
+        assert status("dcb_ln_bwd", xd, 0, x, dyd, dy, FAKE, FAKE, None, a, FAKE, None, None, None, 0, None) == _abi.BAD_ARG
+        assert b"strides" in _abi.lib().dcb_last_error()
+
+
 def rotary(**kw):
     rd = _abi.RotaryDesc()
     rd.nsd, rd.head_dim, rd.rotated_heads, rd.base = 2, 8, 2, 100.0
