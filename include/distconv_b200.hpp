@@ -2447,28 +2447,32 @@ private:
 namespace internal
 {
 // Device memory that a layer keeps for its calls, which have to follow one another (one stream, or ordered streams).
+// What it has grown out of stays until the layer goes: a captured graph may still use it.
 class Workspace
 {
 public:
     Workspace() = default;
     Workspace(const Workspace&) = delete;
-    ~Workspace() { cudaFree(m_p); }
+    ~Workspace()
+    {
+        for (void* p : m_all)
+            cudaFree(p);
+    }
     void* get(int64_t bytes)
     {
         if (bytes > m_bytes)
         {
-            cudaFree(m_p);
-            m_p = nullptr;
-            m_bytes = 0;
-            if (cudaMalloc(&m_p, (size_t) bytes) != cudaSuccess)
+            void* p = nullptr;
+            if (cudaMalloc(&p, (size_t) bytes) != cudaSuccess)
                 throw std::runtime_error("cudaMalloc of a layer's workspace failed");
+            m_all.push_back(p);
             m_bytes = bytes;
         }
-        return m_p;
+        return m_all.empty() ? nullptr : m_all.back();
     }
 
 private:
-    void* m_p = nullptr;
+    std::vector<void*> m_all;
     int64_t m_bytes = 0;
 };
 } // namespace internal
@@ -2507,15 +2511,18 @@ public:
                                    m_be.get_stream()),
                         "layer normalisation backward");
         }
-        if (!counts) // nothing here, or a replica, whose cells count once
+        if (!counts && scale_gradient != nullptr) // nothing here, or a replica, whose cells count once
             for (float* g : {scale_gradient, bias_gradient})
                 cudaMemsetAsync(g, 0, bytes, m_be.get_stream());
         return 0;
     }
+    // null gradients of scale and bias: not wanted
     int backward(TensorF& input, TensorF& d_output, const float* mean, const float* inv_std, const float* scale,
                  float* scale_gradient, float* bias_gradient, TensorF& d_input)
     {
         backward_stage1(input, d_output, mean, inv_std, scale, scale_gradient, bias_gradient, d_input);
+        if (scale_gradient == nullptr)
+            return 0;
         const index_t C = input.get_local_shape()[-2];
         m_be.allreduce(scale_gradient, C);
         m_be.allreduce(bias_gradient, C);

@@ -89,7 +89,14 @@ int main()
         LayerNormalization ln(be, 4, (float) EPS);
         ln.forward(x.t, scale, bias, y.t, mean, inv);
         ln.backward(x.t, dy.t, mean, inv, scale, dw, db, dx.t);
+        Field alone(C, 0); // without the gradients of scale and bias
+        ln.backward(x.t, dy.t, mean, inv, scale, nullptr, nullptr, alone.t);
         be.wait();
+        if (alone.host() != dx.host())
+        {
+            std::printf("layer norm: d_input depends on what else is wanted\n");
+            return 1;
+        }
         const Vec vx = x.host(), vd = dy.host();
         Vec ry(vx.size()), rx(vx.size()), rw(C, 0.), rb(C, 0.);
         for (int n = 0; n < N; ++n)
