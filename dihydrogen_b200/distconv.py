@@ -515,8 +515,17 @@ class ChannelSlice:
             raise ValueError(f"channels {first} to {first + count} of {tensor.local_shape[-2]}")
         self.tensor, self.first, self.count = tensor, first, count
         self.dtype, self.dist, self.nd = tensor.dtype, tensor.dist, tensor.nd
-        self.local_shape = tensor.local_shape[:-2] + [count, tensor.local_shape[-1]]
         self._of = None
+
+    @property
+    def local_shape(self):
+        s = self.tensor.local_shape
+        return s[:-2] + [self.count, s[-1]]
+
+    @property
+    def buffer(self):
+        """The whole tensor's."""
+        return self.tensor.buffer
 
     def _geo(self):
         return self.tensor._geo()
@@ -1505,12 +1514,12 @@ class BatchNormalization:
 # ---------------------------------------------------------------------------
 # Attention between cells, and what goes with it
 # ---------------------------------------------------------------------------
-def _workspace(nbytes: int, stream, device):
+def _workspace(nbytes: int, stream, device: int):
     """Device memory for one call, from torch's allocator on the stream the call goes to: calls on other
     streams and captured graphs never share it."""
     if nbytes <= 0:
         return None, 0
-    if stream is None or stream.cuda_stream == torch._C._cuda_getCurrentRawStream(device.index):
+    if stream is None or stream.cuda_stream == torch._C._cuda_getCurrentRawStream(device):
         ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
     else:
         with torch.cuda.stream(stream):
@@ -1518,21 +1527,23 @@ def _workspace(nbytes: int, stream, device):
     return ws, ws.data_ptr()
 
 
-def _device(t):
+def _device(t) -> int:
     """The device of a tensor's memory, which has to be the current one: kernels are launched there."""
-    b = (t.tensor if isinstance(t, ChannelSlice) else t).buffer
-    d = b.device if b is not None else torch.device("cuda", torch._C._cuda_getDevice())  # none: nothing is read
-    if d.type != "cuda" or d.index != torch._C._cuda_getDevice():
-        raise ValueError(f"tensors have to be on the current CUDA device, not on {d}")
-    return d
+    b = t.buffer
+    if b is None:  # nothing is read
+        return torch._C._cuda_getDevice()
+    device = b.get_device()
+    if device < 0 or device != torch._C._cuda_getDevice():
+        raise ValueError(f"tensors have to be on the current CUDA device, not on {b.device}")
+    return device
 
 
 def _vector(name, t, count, device, dtypes=(torch.float32,)):
     """Address of a plain torch operand, which the kernels take as a dense array; 0 for None."""
     if t is None:
         return 0
-    if t.dtype not in dtypes or t.numel() != count or not t.is_contiguous() or t.device != device:
-        raise ValueError(f"{name} must be a contiguous array of {count} {dtypes[0]} on {device}, not "
+    if t.dtype not in dtypes or t.numel() != count or not t.is_contiguous() or t.get_device() != device:
+        raise ValueError(f"{name} must be a contiguous array of {count} {dtypes[0]} on device {device}, not "
                          f"{list(t.shape)} {t.dtype} on {t.device}")
     return t.data_ptr()
 
@@ -1545,10 +1556,10 @@ def _needed(name, t, count, device):
 
 def _check_alike(what, first, *others):
     """Shapes, types and devices agree."""
-    device = _device(first)
+    device, shape, dtype = _device(first), first.local_shape, first.dtype
     for t in others:
-        if t.local_shape != first.local_shape or t.dtype is not first.dtype or _device(t) != device:
-            raise ValueError(f"{what}: local shapes and types must agree: {first.local_shape} {first.dtype} and "
+        if t.local_shape != shape or t.dtype is not dtype or (t.buffer is not None and t.buffer.get_device() != device):
+            raise ValueError(f"{what}: local shapes, types and devices must agree: {shape} {dtype} and "
                              f"{t.local_shape} {t.dtype}")
     return device
 
@@ -1765,7 +1776,7 @@ class Attention:
             return 0
         ad, size = self._desc(q, k)
         s = self.be.stream
-        keep, ws = _workspace(size[0], s, lse.device)
+        keep, ws = _workspace(size[0], s, lse.get_device())
         call("dcb_attention_fwd", ad, *q._operand(), *k._operand(), *v._operand(), pq, pk, *output._operand(), pl, ws,
              size[0], _stream_ptr(s))
         return 0
@@ -1777,7 +1788,7 @@ class Attention:
             return 0
         ad, size = self._desc(q, k)
         s = self.be.stream
-        keep, ws = _workspace(size[1], s, lse.device)
+        keep, ws = _workspace(size[1], s, lse.get_device())
         call("dcb_attention_bwd", ad, *q._operand(), *k._operand(), *v._operand(), pq, pk, *output._operand(), pl,
              *d_output._operand(), *d_q._operand(), *d_k._operand(), *d_v._operand(), ws, size[1], _stream_ptr(s))
         return 0

@@ -186,6 +186,8 @@ def test_channel_slices():
     for first, count in ((-1, 2), (7, 2), (0, 9)):
         with pytest.raises(ValueError):
             t.channel_slice(first, count)
+    t.local_shape[-1] = 1  # fewer samples: the slice follows
+    assert s.local_shape == [6, 4, 2, 1] and s._operand()[0]._obj.n == 1
 
 
 def test_heads():
