@@ -12,6 +12,10 @@
 // under the exponentials of another: P' and dS' are handed over apart, and the scores are taken a step (dkv) or two
 // (dq) ahead.  Heads of 128 channels: steps of 128 columns, one block an SM, whose tensor memory they fill.  Heads of 64:
 // steps of 64 columns and two blocks an SM, whose steps fall under one another's.
+//
+// 8 heads of 128 channels, 2 key heads, 12288 cells, causal: dkv 487 us, dq 332 (1.32 PFLOP/s over the
+// seven products); the tensor pipe is busy 68 and 70 % of the time.  2 x 8 heads of 64 on 64^2 cells: 180 and 140 us; issue slots
+// half full, the tensor pipe 38 %.
 #include "attention_tc.cuh"
 
 namespace dcb

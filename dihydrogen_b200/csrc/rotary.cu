@@ -5,7 +5,7 @@
 // cell, not on the sample or the head: a thread owns a pair of channels at V neighbouring cells,
 // looks up V cosines and sines in the plan's tables (a few hundred kilobytes, in L2) and walks
 // over the heads with them, several heads' loads in flight.  A channel of no axis is a pair with
-// nothing to turn.
+// nothing to turn.  2 x 12 heads of 128 channels on 40^3 cells, bf16: 123 us (6.4 TB/s).
 #include "elem.cuh"
 
 #include <cmath>
