@@ -1710,6 +1710,9 @@ class RotaryPositions:
         return self._apply(d_output, d_input, 1)
 
 
+_MASKS = (torch.bool, torch.uint8)
+
+
 class Attention:
     """Scaled dot-product attention from the cells of one tensor to the cells of
     another (or its own).  No counterpart in the reference.  ``q``, ``k``, ``v``
@@ -1734,15 +1737,19 @@ class Attention:
         if self.q_heads < 1 or self.kv_heads < 1 or self.q_heads % self.kv_heads:
             raise ValueError("q_heads must be a multiple of kv_heads")
         self.scale, self.causal = scale, bool(causal)
-        self._known = {}  # shapes -> (descriptor, workspace bytes forward, backward)
+        self._known = {}  # shapes and type -> (descriptor, workspace bytes forward, backward)
+        self._recent = (None, None, None, None)  # the latest of them
 
-    def _desc(self, q, k):
-        key = (tuple(q.local_shape), tuple(k.local_shape), q.dtype)
+    def _desc(self, q, k, shape_q, shape_k):
+        recent = self._recent
+        if shape_q == recent[0] and shape_k == recent[1] and q.dtype is recent[2]:
+            return recent[3]
+        key = (tuple(shape_q), tuple(shape_k), q.dtype)
         got = self._known.get(key)
         if got is None:
-            if q.local_shape[-2] % self.q_heads or q.local_shape[-2] == 0:
-                raise ValueError(f"{q.local_shape[-2]} channels are not {self.q_heads} heads")
-            head_dim = q.local_shape[-2] // self.q_heads
+            if shape_q[-2] % self.q_heads or shape_q[-2] == 0:
+                raise ValueError(f"{shape_q[-2]} channels are not {self.q_heads} heads")
+            head_dim = shape_q[-2] // self.q_heads
             ad = _abi.AttentionDesc(self.q_heads, self.kv_heads, _DTYPES[q.dtype], self.causal,
                                     1.0 / math.sqrt(head_dim) if self.scale is None else self.scale)
             size = []
@@ -1752,29 +1759,33 @@ class Attention:
                     raise ValueError("attention: " + _abi.lib().dcb_last_error().decode())
                 size.append(n)
             got = self._known[key] = (ctypes.byref(ad), size)
+        self._recent = (list(shape_q), list(shape_k), q.dtype, got)
         return got
 
-    def _checked(self, q, k, v, q_like, kv_like, lse, q_mask, kv_mask):
+    def _checked(self, q, k, q_like, kv_like, lse, q_mask, kv_mask):
+        """Shapes of q and k, and the addresses of lse and the masks."""
         if q.nd != self.num_dims:
             raise ValueError(f"queries of {q.nd} dimensions, set up for {self.num_dims}")
-        for t in (q, k, v) + q_like + kv_like:
+        for t in (q, k, *q_like, *kv_like):
             if not t._geo().whole:
                 raise ValueError("attention needs all cells and channels of a sample on one rank: re-distribute the "
                                  "tensor (TensorShuffler)")
-        dev = _check_alike("attention", q, *q_like)
-        _check_alike("attention", k, v, *kv_like)
-        if q.dtype is not k.dtype or q.local_shape[-1] != k.local_shape[-1]:
+        device = _check_alike("attention", q, *q_like)
+        _check_alike("attention", k, *kv_like)
+        shape_q, shape_k = q.local_shape, k.local_shape
+        n = shape_q[-1]
+        if q.dtype is not k.dtype or n != shape_k[-1]:
             raise ValueError("attention: queries and keys differ in type or samples")
-        n, cells_q, cells_k = q.local_shape[-1], math.prod(q.local_shape[:-2]), math.prod(k.local_shape[:-2])
-        return (_needed("lse", lse, n * self.q_heads * cells_q, dev),
-                _vector("q_mask", q_mask, n * cells_q, dev, (torch.bool, torch.uint8)),
-                _vector("kv_mask", kv_mask, n * cells_k, dev, (torch.bool, torch.uint8)))
+        cells = n * math.prod(shape_q[:-2])
+        return (shape_q, shape_k, _needed("lse", lse, self.q_heads * cells, device),
+                0 if q_mask is None else _vector("q_mask", q_mask, cells, device, _MASKS),
+                0 if kv_mask is None else _vector("kv_mask", kv_mask, n * math.prod(shape_k[:-2]), device, _MASKS))
 
     def forward(self, q, k, v, output: Tensor, lse, q_mask=None, kv_mask=None):
-        pl, pq, pk = self._checked(q, k, v, (output,), (), lse, q_mask, kv_mask)
-        if math.prod(q.local_shape) == 0:
+        shape_q, shape_k, pl, pq, pk = self._checked(q, k, (output,), (v,), lse, q_mask, kv_mask)
+        if 0 in shape_q:
             return 0
-        ad, size = self._desc(q, k)
+        ad, size = self._desc(q, k, shape_q, shape_k)
         s = self.be.stream
         keep, ws = _workspace(size[0], s, lse.get_device())
         call("dcb_attention_fwd", ad, *q._operand(), *k._operand(), *v._operand(), pq, pk, *output._operand(), pl, ws,
@@ -1783,10 +1794,10 @@ class Attention:
 
     def backward(self, q, k, v, output: Tensor, lse, d_output: Tensor, d_q, d_k, d_v, q_mask=None, kv_mask=None):
         """``output`` and ``lse`` as ``forward`` left them, with the same masks."""
-        pl, pq, pk = self._checked(q, k, v, (output, d_output, d_q), (d_k, d_v), lse, q_mask, kv_mask)
-        if q.local_shape[-1] == 0:
+        shape_q, shape_k, pl, pq, pk = self._checked(q, k, (output, d_output, d_q), (v, d_k, d_v), lse, q_mask, kv_mask)
+        if shape_q[-1] == 0:
             return 0
-        ad, size = self._desc(q, k)
+        ad, size = self._desc(q, k, shape_q, shape_k)
         s = self.be.stream
         keep, ws = _workspace(size[1], s, lse.get_device())
         call("dcb_attention_bwd", ad, *q._operand(), *k._operand(), *v._operand(), pq, pk, *output._operand(), pl,
