@@ -93,7 +93,7 @@ inline int attn_splits(long long work, int steps, long long slots)
 }
 
 // Kernels of attention_thin.cu: the forward pass of so few queries that it is a pass over the keys.  2 x 8 heads x 64,
-// against the other kernels: a bf16 query over 64^2 keys 9 us against 16, over 32^3 36 against 43 (31 x 33 x 31: 80
+// against the other kernels: a bf16 query over 64^2 keys 9 us against 16, over 32^3 36 against 43 (31 x 33 x 31: 72
 // against 100), but two queries 52 against 43; eight fp32 queries over 64^2 keys 34 us against 42, over 20 x 20 x 65 227
 // against 243.
 constexpr int ATTN_THIN_BF16 = 1, ATTN_THIN_F32 = 8; // cells of q

@@ -6,8 +6,9 @@
 // their way; every lane then weighs its keys about a maximum of its own and adds up its channels of the values: the
 // lanes' sums meet at the block's end.  Parts are joined by a kernel of their own.  Weights stay fp32.
 //
-// 2 x 8 heads x 64, a query each, parts' join included: bf16, 32^3 keys 36 us (134 MB: 3.7 TB/s), 32 x 64 x 64 keys
-// 102 us (5.3 TB/s); fp32, 20 x 20 x 65 keys 43 us (213 MB: 5 TB/s).
+// 2 x 8 heads x 64, a query each, parts' join included: bf16, 32^3 keys 36 us (134 MB: 3.7 TB/s; start, the
+// parts' last tiles and the join are 12 of it), 32 x 64 x 64 keys 100 us (5.4 TB/s); fp32, 20 x 20 x 65 keys 43 us (213 MB:
+// 5 TB/s).
 #include "attention.cuh"
 
 namespace dcb
@@ -23,13 +24,13 @@ struct AthKeys
 {
     static constexpr int WIDE = GATHER ? 1 : 16 / sizeof(T), LOADS = ATH_KEYS / WIDE;
     int first, at[LOADS]; // the lane's first key, cells
-    __device__ __forceinline__ AthKeys(const AttnCells& kv, int tile, int lane, int limit)
+    __device__ __forceinline__ AthKeys(const AttnCells& kv, int j0, int lane, int end)
     {
-        first = tile * 32 * ATH_KEYS + lane * WIDE;
+        first = j0 + lane * WIDE;
 #pragma unroll
         for (int l = 0; l < LOADS; ++l)
         {
-            const int j = key(l * WIDE) < limit ? key(l * WIDE) : 0;
+            const int j = key(l * WIDE) < end ? key(l * WIDE) : 0;
             at[l] = GATHER ? kv.cell(j) : j;
         }
     }
@@ -73,8 +74,10 @@ __global__ void __launch_bounds__(32 * WARPS, 16 / WARPS) attn_thin_fwd_kernel(c
     if (row >= q.count)
         return;
     const int i = q.cell(row), limit = attn_limit(p, q, kv, row);
-    const int tiles = (limit + 32 * V - 1) / (32 * V);
-    const int lo = (int) ((long long) tiles * split / p.kv_splits), hi = (int) ((long long) tiles * (split + 1) / p.kv_splits);
+    // parts are whole units of 64 keys (a line of 128 bytes of bf16): the last tile of a part may be cut short
+    const int units = attn_tiles(limit, 64);
+    const int lo = 64 * (int) ((long long) units * split / p.kv_splits);
+    const int hi = min(64 * (int) ((long long) units * (split + 1) / p.kv_splits), limit);
     {
         const int c = threadIdx.x;
         if (c < WARPS * CHANNELS)
@@ -94,9 +97,9 @@ __global__ void __launch_bounds__(32 * WARPS, 16 / WARPS) attn_thin_fwd_kernel(c
 #pragma unroll
     for (int c = 0; c < CHANNELS; ++c)
         acc[c] = 0.f;
-    for (int t = lo; t < hi; ++t)
+    for (int j0 = lo; j0 < hi; j0 += 32 * V)
     {
-        const Keys mine(kv, t, lane, limit);
+        const Keys mine(kv, j0, lane, hi);
         typename Keys::Values k[CHANNELS], v[CHANNELS];
 #pragma unroll
         for (int c = 0; c < CHANNELS; ++c)
@@ -133,7 +136,7 @@ __global__ void __launch_bounds__(32 * WARPS, 16 / WARPS) attn_thin_fwd_kernel(c
 #pragma unroll
         for (int e = 0; e < V; ++e)
         {
-            s[e] = mine.key(e) < limit ? s[e] : -INFINITY;
+            s[e] = mine.key(e) < hi ? s[e] : -INFINITY;
             most = fmaxf(most, s[e]);
         }
         if (most > top + ATH_GROWTH)
