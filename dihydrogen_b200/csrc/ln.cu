@@ -187,8 +187,8 @@ __device__ __forceinline__ void ln_fwd_tile(const T* x, const RunStrides& xs, T*
 {
     const T* px = x + (offset_of(at.cell, xs) + me.cg * xs.sc) + at.lane;
     const long long x_step = geo.g * xs.sc;
-    // mean and centred squares of eight channels at a time, joined with those before (Chan et al.): no cancellation,
-    // whatever the mean
+    // mean and centred squares of eight channels at a time, joined with those before (Chan et al.): off by roundings of
+    // |mean| / deviation, as x - mean is by the rounding of the mean, not by their squares
     float mean[V], m2[V];
 #pragma unroll
     for (int e = 0; e < V; ++e)
