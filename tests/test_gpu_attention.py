@@ -242,6 +242,42 @@ def test_the_same_bits_every_run_on_streams_and_in_graphs(dtype):
         assert all(torch.equal(a, b) for a, b in zip(out, want))
 
 
+@pytest.mark.parametrize("dtype", TYPES, ids=["f32", "bf16"])
+@pytest.mark.parametrize("masked", [False, True])
+def test_a_captured_query_replayed_with_other_inputs(masked, dtype):
+    """Two graphs of one layer replayed at once on two streams, then again: what they read is what is there now."""
+    be, g = backend(), torch.Generator().manual_seed(16)
+    layer, graphs = dc.Attention(be, 4, 4, 2), []
+    for keys in (5000, 777):
+        q, k, v = (torch.zeros(2, h * 64, 1, c, dtype=dtype, device="cuda") for h, c in ((4, 1), (2, keys), (2, keys)))
+        o, lse = torch.zeros_like(q), torch.zeros(2, 4, 1, device="cuda")
+        mask = torch.ones(2, keys, dtype=torch.uint8, device="cuda") if masked else None
+        args = (*(tensor(t, be) for t in (q, k, v, o)), lse)
+        layer.forward(*args, kv_mask=mask)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            layer.forward(*args, kv_mask=mask)
+        graphs.append((graph, torch.cuda.Stream(), q, k, v, o, lse, mask))
+    for _ in range(3):
+        want = []
+        for _, _, q, k, v, _, _, mask in graphs:
+            for t in (q, k, v):
+                t.copy_(torch.randn(t.shape, generator=g))
+            if masked:
+                mask.copy_(torch.rand(mask.shape, generator=g) < 0.7)
+            host = [t.cpu() for t in (q, k, v)]
+            want.append(R.attention(heads(host[0], 4), heads(host[1], 2), heads(host[2], 2), 0.125,
+                                    kv_mask=mask.cpu() if masked else None, dtype=dtype))
+        torch.cuda.synchronize()
+        for graph, stream, *_ in graphs:
+            with torch.cuda.stream(stream):
+                graph.replay()
+        torch.cuda.synchronize()
+        for (_, _, _, _, _, o, lse, _), w in zip(graphs, want):
+            R.close(lse, w["lse"], "lse")
+            R.close(heads(o, 4), w["o"], "o")
+
+
 def test_masks_of_many_cells():
     """A mask is counted in parts of 8192 cells and more, from any address; any byte that is not zero counts."""
     g = torch.Generator().manual_seed(15)
