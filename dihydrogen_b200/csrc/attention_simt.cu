@@ -19,10 +19,6 @@ namespace
 constexpr int AS_TILE = 64;
 constexpr int AS_PITCH = 68; // floats: rows 16-byte aligned, four rows on different banks
 constexpr int AS_THREADS = 256;
-#ifndef SLOTV
-#define SLOTV 2
-#endif
-constexpr int AS_LEAST = 1;  // tiles a part of a split axis walks at least
 
 // One head's cells, 64 from the r0-th on of those that are there, to shared memory as [channel][cell]; cells that are not,
 // and channels up to D, as zeros.
