@@ -45,7 +45,7 @@ struct AfShape
 template <int D, bool APART>
 constexpr bool af_fits = AfShape<D, APART>::O_AT + 2 * D <= AfShape<D, APART>::COLUMNS
                          && AfShape<D, APART>::BLOCKS * (AfShape<D, APART>::SMEM + 1024) <= 228 * 1024;
-static_assert(af_fits<64, false> && af_fits<64, true> && af_fits<128, false> && af_fits<128, true>,
+static_assert(af_fits<64, false> && af_fits<64, true> && af_fits<128, false>,
               "tensor memory of a block, shared memory of an SM's blocks");
 static_assert(2 * AfShape<64, false>::TEAM_REGS + AfShape<64, false>::OTHER_REGS <= 3 * 80, "registers of two blocks");
 
@@ -493,7 +493,7 @@ int32_t af_launch(const AttnProblem& p, const AtMaps& maps, cudaStream_t stream)
 int32_t attn_tc_fwd_launch(const AttnProblem& p, const AtMaps& maps, cudaStream_t stream)
 {
     if (attn_tc_apart(p))
-        return p.d <= 64 ? af_launch<64, true>(p, maps, stream) : af_launch<128, true>(p, maps, stream);
+        return af_launch<64, true>(p, maps, stream);
     return p.d <= 64 ? af_launch<64, false>(p, maps, stream) : af_launch<128, false>(p, maps, stream);
 }
 

@@ -37,14 +37,12 @@ struct LnGeom
     long long tiles;  // of all groups of a block
 };
 
-// How a warp's cells lie.  FLAT: units of V neighbours packed over short runs.  ROWS: 32 V cells of one run, a lane has
-// V neighbours.  SPLIT: the same cells where a run starts off the alignment of such accesses, a lane's are 32 apart.
-// In the last two everything but the lane is the same for a warp, so that a channel's address costs no instruction
-// of the lanes.
+// How a warp's cells lie.  FLAT: units of V neighbours packed over short runs.  SPLIT: 32 V cells of one run that starts
+// off the alignment of accesses of V, a lane's are 32 apart; everything but the lane is the same for a warp then, so that a
+// channel's address costs no instruction of the lanes.
 enum LnMode
 {
     LN_FLAT,
-    LN_ROWS,
     LN_SPLIT
 };
 
@@ -73,13 +71,8 @@ struct LnAt
         cell = cell_at<32 * V>(g.units, g.per_run, g.rows, g.rows_inner, live ? chunk : 0);
         const long long left = live ? g.units.len - cell.pos : 0;
         full = left >= 32 * V;
-        lane = MODE == LN_ROWS ? l * V : l;
-        if (full)
-            have = V;
-        else if (MODE == LN_ROWS)
-            have = l * V < left ? V : 0; // runs are multiples of V
-        else
-            have = l < left ? (int) (left - l + 31) / 32 : 0;
+        lane = l;
+        have = full ? V : l < left ? (int) (left - l + 31) / 32 : 0;
     }
     __device__ __forceinline__ long long stat(const LnGeom& g) const { return cell.n * g.units.cells + cell.cell; }
 };
@@ -522,17 +515,19 @@ struct LnChoice
 LnChoice ln_choose(int c, int vmax, long long len, long long cells)
 {
     LnChoice h;
-    // Four cells a thread where that leaves every SM a block of tiles; else one.  A run's last tile wastes up to a
-    // quarter of the lanes; shorter runs are packed.
+    // Four cells a thread where that leaves every SM a block of tiles (64 x 96^3 fp32, forward and backward, 82 + 112 us,
+    // 133 + 161 with one; 32 x 2 x 64^2, 4.5 + 4.5 and 3.9 + 4.5 with one), 32 apart where accesses of four are not aligned
+    // (200 x 2 x 19 x 37 x 53 bf16 23 + 36 us, with one 32 + 54) and runs are so long that their last tiles waste a quarter
+    // of the lanes at most.
     const bool four = cells >= 4ll * 32 * num_sms();
-    h.mode = four && len >= 512 ? (vmax == 4 ? LN_ROWS : LN_SPLIT) : LN_FLAT;
-    h.v = h.mode != LN_FLAT || (four && vmax == 4) ? 4 : 1;
+    h.mode = four && vmax < 4 && len >= 512 ? LN_SPLIT : LN_FLAT;
+    h.v = h.mode == LN_SPLIT || (four && vmax == 4) ? 4 : 1;
     // as many warps a group as have eight channels each, more where there are few tiles
     const long long tiles = (cells + 32 * h.v - 1) / (32 * h.v);
     h.g = 1;
     while (h.g < LN_WARPS && (c > LN_STEP * h.g || (c >= 2 * h.g && tiles * h.g < 8ll * num_sms())))
         h.g *= 2;
-    h.keep = c == LN_STEP * h.g;
+    h.keep = c == LN_STEP * h.g; // (64 x 96^3 fp32 101 + 131 us without)
     return h;
 }
 
@@ -620,8 +615,6 @@ int32_t ln_with_shape(const LnChoice& h, F f)
 {
     using std::integral_constant;
     const auto shape = [&](auto keep) -> int32_t {
-        if (h.mode == LN_ROWS)
-            return f(integral_constant<int, 4>(), integral_constant<int, LN_ROWS>(), keep);
         if (h.mode == LN_SPLIT)
             return f(integral_constant<int, 4>(), integral_constant<int, LN_SPLIT>(), keep);
         return h.v == 4 ? f(integral_constant<int, 4>(), integral_constant<int, LN_FLAT>(), keep)
