@@ -13,7 +13,7 @@
 // slots, 56 % of the exponentials' unit, hand-overs between.  128 channels, 8 heads on 12288 cells: 611 us (1010 TFLOP/s),
 // causal 309 us; the tensor pipe and the exponentials at half each.
 //
-// Few queries (APART): both teams have the same 128 of them and a part of the keys each.
+// Few queries of such heads, many keys (APART): both teams have the same 128 queries and a part of the keys each.
 #include "attention_tc.cuh"
 
 namespace dcb
