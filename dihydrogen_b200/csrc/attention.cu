@@ -429,8 +429,10 @@ int64_t attn_carve(AttnProblem* p, int32_t dtype, bool backward, void* workspace
 {
     Carve w{static_cast<char*>(workspace)};
     const bool tc = dtype == DCB_BF16;
-    const bool thin = !backward && attn_thin(*p, dtype);
-    if (thin)
+    const bool thin = backward ? attn_thin_backward(*p, dtype) : attn_thin(*p, dtype);
+    if (thin && backward)
+        attn_thin_bwd_splits(p);
+    else if (thin)
         attn_thin_splits(p, dtype);
     else
         (tc ? attn_tc_splits : attn_simt_splits)(p, backward);
@@ -670,7 +672,10 @@ int32_t dcb_attention_bwd(const dcb_attention_desc* ad, const dcb_nd_desc* qd, c
     });
     if (e)
         return e;
-    if (int32_t err = ad->dtype == DCB_BF16 ? attn_tc_bwd(p, s) : attn_simt_bwd(p, s))
+    const int32_t err = attn_thin_backward(p, ad->dtype) ? attn_thin_bwd(p, s)
+                        : ad->dtype == DCB_BF16   ? attn_tc_bwd(p, s)
+                                                  : attn_simt_bwd(p, s);
+    if (err)
         return err;
     if (p.q_splits > 1)
     {

@@ -99,6 +99,9 @@ inline int attn_splits(long long work, int steps, long long slots)
 constexpr int ATTN_THIN_BF16 = 1, ATTN_THIN_F32 = 8; // cells of q
 bool attn_thin(const AttnProblem& p, int32_t dtype);
 void attn_thin_splits(AttnProblem* p, int32_t dtype);
+bool attn_thin_backward(const AttnProblem& p, int32_t dtype);
+void attn_thin_bwd_splits(AttnProblem* p);
+int32_t attn_thin_bwd(const AttnProblem& p, cudaStream_t stream);
 int32_t attn_thin_fwd(const AttnProblem& p, int32_t dtype, cudaStream_t stream);
 
 // Kernels of attention_tc.cu (bf16) and attention_simt.cu (fp32), both behind attn_index, which fills the sides.
