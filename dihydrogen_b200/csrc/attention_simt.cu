@@ -9,7 +9,7 @@
 //
 // Bound by the fp32 pipes and shared memory: 2 x 8 heads of 64 on 32^2 cells take 155 us forward (28 TFLOP/s), 368 and
 // 221 us backward.  From 65 channels on the backward kernels' tiles leave room for one block an SM, and wait more: 8 heads of
-// 128, 2 key heads, 40 x 55 cells, a training step 3.1 ms (15 TFLOP/s).
+// 128, 2 key heads, 40 x 55 cells, a training step 3.1 ms (22 TFLOP/s).
 #include "attention.cuh"
 
 namespace dcb
