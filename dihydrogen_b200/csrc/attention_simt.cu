@@ -439,18 +439,35 @@ int32_t as_with(int d, F f)
 
 } // namespace
 
+// Parts of a walk over `steps` tiles, for `work` walks of which `slots` go at a time: how many rounds there are, and how
+// long one takes, start and end of a block counted as a tile.
+static int as_parts(long long work, int steps, long long slots)
+{
+    int best = 1;
+    long long least = 0;
+    for (int s = 1; s <= std::min(steps, 64); ++s)
+    {
+        const long long cost = (work * s + slots - 1) / slots * (attn_tiles(steps, s) + 1);
+        if (s == 1 || 100 * cost < 97 * least)
+            best = s, least = cost;
+    }
+    return best;
+}
+
 void attn_simt_splits(AttnProblem* p, bool backward)
 {
-    // Parts of one tile and more: a training step of 4 heads of 32 on 9 x 11 x 13 cells, some missing, 163 us with four
-    // tiles at least and 115 so.  Four blocks an SM: dkv 30 -> 34 us there, 368 -> 378 for 2 x 8 heads of 64 on 32^2.
-    const long long slots = 2ll * num_sms(); // two blocks an SM
+    const long long slots = (p->d <= 64 ? 2ll : 1ll) * num_sms(); // blocks an SM has room for
     const int left = p->q_mask || p->kv_mask ? 2 : 1; // masks are taken to leave half of either side
     const int q_tiles = attn_tiles(p->sq, AS_TILE), k_tiles = attn_tiles(p->sk, AS_TILE);
-    const auto walks = [&](long long n) { return (n + left - 1) / left; };
-    p->kv_splits = attn_splits(walks((long long) p->n * p->q_heads * q_tiles), k_tiles / left, slots);
-    p->q_splits = !backward ? 1
-                            : attn_splits(walks((long long) p->n * p->kv_heads * k_tiles), q_tiles * p->group / left,
-                                          slots);
+    // Causal walks differ in length: parts enough for three blocks an SM (two of 64 channels) even them out.  4 heads of
+    // 96, 40 x 55 cells, causal, forward 266 us, by rounds 379; 4 heads of 128, 2 key heads, 40 x 41, 242 by rounds, 292
+    // with parts for two blocks an SM.
+    const auto parts = [&](long long work, int steps) {
+        work = (work + left - 1) / left, steps /= left;
+        return p->causal ? attn_splits(work, steps, (p->d <= 64 ? 2ll : 3ll) * num_sms()) : as_parts(work, steps, slots);
+    };
+    p->kv_splits = parts((long long) p->n * p->q_heads * q_tiles, k_tiles);
+    p->q_splits = backward ? parts((long long) p->n * p->kv_heads * k_tiles, q_tiles * p->group) : 1;
 }
 
 int32_t attn_simt_fwd(const AttnProblem& p, cudaStream_t stream)
