@@ -46,6 +46,14 @@ struct AthKeys
         for (int l = 0; l < LOADS; ++l)
             v.r[l].load(row + at[l]);
     }
+    // What was fetched in place of keys from `end` on becomes 0: a weight of 0 times an infinity would not be.
+    __device__ __forceinline__ void clear_behind(Values& v, int end) const
+    {
+#pragma unroll
+        for (int l = 0; l < LOADS; ++l)
+            if (key(l * WIDE) >= end)
+                v.r[l].clear();
+    }
     // keys up to `end`, which WIDE divides or which is the last
     __device__ __forceinline__ void store(T* row, const float (&v)[KEYS], int end) const
     {
@@ -146,6 +154,10 @@ __global__ void __launch_bounds__(32 * WARPS, 16 / WARPS) attn_thin_fwd_kernel(c
         for (int c = 0; c < CHANNELS; ++c)
             mine.load(v[c], values + min(c0 + c, p.d - 1) * p.v.sc);
         __syncthreads(); // the next tile's shares
+        if (j0 + 32 * V > hi)
+#pragma unroll
+            for (int c = 0; c < CHANNELS; ++c)
+                mine.clear_behind(v[c], hi);
         float most = -INFINITY;
 #pragma unroll
         for (int e = 0; e < V; ++e)
