@@ -17,6 +17,10 @@ namespace
 {
 
 constexpr int ATH_KEYS = 8; // of a lane, in a tile
+// Keys of a part, at most, forward: a lane adds up a 32nd of them one after the other, and after 2^15 terms of like size
+// such a sum was off by 2.6e-4 (2^10: 4e-6 at most).  More than so many parts would be a long sum themselves.  40 x 8
+// queries on 4 key heads of 64, 2^18 keys, fp32: 4.1 ms, in whole walks 7.0.
+constexpr int ATH_PART_KEYS = 1 << 15, ATH_MOST_PARTS = 4096;
 constexpr float ATH_GROWTH = 8.f; // a lane's base is renewed where a score is more than 2^8 above it
 
 template <class T, int KEYS, bool GATHER>
@@ -425,11 +429,12 @@ bool attn_thin(const AttnProblem& p, int32_t dtype)
 
 void attn_thin_splits(AttnProblem* p, int32_t dtype)
 {
-    // the blocks that run at a time, 16 warps an SM; a part has a tile at least
+    // the blocks that run at a time, 16 warps an SM; a part has a tile at least, ATH_PART_KEYS at most
     const int channels = dtype == DCB_BF16 && !p->kv_mask && p->sk % 8 == 0 ? ath_channels<bf16>() : 8;
     const int warps = (p->d <= 32 ? 32 : p->d <= 64 ? 64 : 128) / channels;
-    p->kv_splits = attn_splits((long long) p->n * p->q_heads * p->sq, attn_tiles(p->sk, 32 * ATH_KEYS),
-                               (16ll / warps) * num_sms());
+    p->kv_splits = std::max(attn_splits((long long) p->n * p->q_heads * p->sq, attn_tiles(p->sk, 32 * ATH_KEYS),
+                                        (16ll / warps) * num_sms()),
+                            std::min(attn_tiles(p->sk, ATH_PART_KEYS), ATH_MOST_PARTS));
     p->q_splits = 1;
 }
 

@@ -35,3 +35,32 @@ def test_infinite_values_of_the_first_keys(masked, queries, dtype):
         dc.Attention(be, 4, hq, hk).forward(*ts, o, lse, kv_mask=mask.cuda() if masked else None)
         R.close(lse, want["lse"], "lse")
         R.close(heads(o.buffer, hq), want["o"], "o")
+
+
+@pytest.mark.parametrize("queries,causal", [(8, False), (1, False), (8, True)])
+def test_sums_over_a_million_keys(queries, causal):
+    """Weights within 2^-10 of one another and equal values: roundings of one long running sum would all go one way
+    (2.6e-4 of the result after 2^15 terms of a lane).  Heads enough that no key axis has to be cut for the SMs' sake."""
+    keys, d, rows = 1 << 20, 64, 160
+    heads_q = rows // queries
+    g = torch.Generator(device="cuda").manual_seed(22)
+    be = backend()
+    q = torch.zeros(1, heads_q * d, 1, queries, device="cuda")
+    q[:, ::d] = 1.0
+    k = torch.zeros(1, d, 1, keys, device="cuda")
+    k[:, 0] = torch.rand(1, keys, generator=g, device="cuda") * (2.0 ** -10 * math.log(2.0) * math.sqrt(d))
+    v = (torch.arange(d, device="cuda", dtype=torch.float32)[:, None] * 0.1 + 0.1).expand(1, d, keys)[:, :, None].contiguous()
+    o, lse = torch.full_like(q, math.nan), torch.full((1, heads_q, queries), math.nan, device="cuda")
+    dc.Attention(be, 4, heads_q, 1, causal=causal).forward(*(tensor(t, be) for t in (q, k, v, o)), lse)
+    s = k[0, 0, 0].double() / math.sqrt(d)
+    sees = torch.arange(keys - queries + 1, keys + 1) if causal else torch.full((queries,), keys)
+    want = torch.stack([torch.logsumexp(s[:int(c)], 0) for c in sees])
+    # an output is a quotient of sums of the same weights: runs of at most 2^10 terms of a lane, the lanes (5), the
+    # parts (2^5) and the joins' and the quotient's products, either sum
+    u = 2.0 ** -24
+    bound = 2 * (2 ** 10 + 5 + 2 ** 5 + 8) * u
+    off = (o.reshape(heads_q, d, queries).double() / v[0, :, 0, 0].double()[:, None] - 1).abs().max()
+    assert float(off) <= bound, (float(off), bound)
+    # lse: its sum's roundings, those of a score (a product, scale) and its own in powers of two
+    off = (lse[0].double() - want).abs().max()
+    assert float(off) <= bound / 2 + 4 * u * 14, float(off)
