@@ -19,7 +19,7 @@ namespace
 {
 
 constexpr int LN_STEP = 8;    // channels at a time
-constexpr int LN_WARPS = 8;   // of a block
+constexpr int LN_WARPS = 8;   // of a block; a group has 1, 2, 4 or all of them
 constexpr int LN_MAX_CHANNELS = 16384; // the backward kernel's sums of a channel fill 128 KB of shared memory
 
 // Blocks of the backward kernel that an SM's registers hold.
@@ -140,6 +140,13 @@ struct LnSelf
     }
 };
 
+// The warps of a group wait for one another only: how many cells a group has, and so which code its barriers stand in, is
+// its own.  Barrier 0 is the block's.
+__device__ __forceinline__ void ln_group_sync(const LnGeom& g, const LnSelf& me)
+{
+    asm volatile("bar.sync %0, %1;" ::"r"(1 + me.group), "r"(32 * g.g) : "memory");
+}
+
 template <int M>
 struct LnSome
 {
@@ -257,7 +264,7 @@ __device__ __forceinline__ void ln_fwd_tile(const T* x, const RunStrides& xs, T*
         for (int e = 0; e < V; ++e)
             all[e] = mean[e] * me.count;
         store_elems<V>(sums + (me.cg * 32 + me.lane) * V, all);
-        __syncthreads();
+        ln_group_sync(geo, me);
         ln_gather<V>(sums, geo.g, me.lane, all);
 #pragma unroll
         for (int e = 0; e < V; ++e)
@@ -267,7 +274,7 @@ __device__ __forceinline__ void ln_fwd_tile(const T* x, const RunStrides& xs, T*
             mean[e] = all[e] * geo.inv_c;
         }
         store_elems<V>(squares + (me.cg * 32 + me.lane) * V, m2);
-        __syncthreads(); // behind it nobody reads `sums`, and behind the next tile's first nobody `squares`
+        ln_group_sync(geo, me); // behind it nobody reads `sums`, and behind the next tile's first nobody `squares`
         ln_gather<V>(squares, geo.g, me.lane, m2);
     }
     float inv[V];
@@ -328,12 +335,6 @@ __global__ void __launch_bounds__(32 * LN_WARPS, 4)
     wait_for_previous_kernel(x, scale, bias);
     for (long long tile = blockIdx.x; tile < geo.tiles; tile += gridDim.x)
     {
-        if (me.group == me.groups) // more warps than groups take
-        {
-            if (geo.g > 1)
-                __syncthreads(), __syncthreads();
-            continue;
-        }
         const LnAt<V, MODE> at(geo, (tile * me.groups + me.group) * 32, me.lane);
         if (at.full)
             ln_fwd_tile<T, V, MODE, true, KEEP>(x, xs, y, ys, scale, bias, eps, mean_out, inv_std_out, geo, me, at, sums,
@@ -418,7 +419,7 @@ __device__ __forceinline__ void ln_bwd_tile(const T* x, const RunStrides& xs, co
     {
         store_elems<V>(mine + (me.cg * 32 + me.lane) * V, a);
         store_elems<V>(mine + (LN_WARPS * 32 + me.cg * 32 + me.lane) * V, b);
-        __syncthreads(); // the other half of the sums' room is free again behind the next tile's barrier
+        ln_group_sync(geo, me); // the other half of the sums' room is free again behind the next tile's barrier
         ln_gather<V>(mine, geo.g, me.lane, a);
         ln_gather<V>(mine + LN_WARPS * 32 * V, geo.g, me.lane, b);
     }
@@ -475,12 +476,6 @@ __global__ void __launch_bounds__(32 * LN_WARPS, ln_bwd_blocks(V))
     int turn = 0;
     for (long long tile = blockIdx.x; tile < geo.tiles; tile += gridDim.x, turn ^= 1)
     {
-        if (me.group == me.groups) // more warps than groups take
-        {
-            if (geo.g > 1)
-                __syncthreads();
-            continue;
-        }
         const LnAt<V, MODE> at(geo, (tile * me.groups + me.group) * 32, me.lane);
         float* mine = reinterpret_cast<float*>(room[turn]) + me.group * geo.g * 32 * V;
         float* sums = acc + me.group * 2 * geo.c;
