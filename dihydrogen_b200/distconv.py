@@ -64,8 +64,9 @@ class _Geometry:
         self.base = t.dtype.itemsize * t.get_local_offset([0] * t.nd)
         self.split_root = t.is_split_root()
         self.owned = tuple(slice(o, o + l) for o, l in reversed(list(zip(self.overlap, self.local))))
-        # all cells and channels of a sample are here
-        self.whole = not any(t.dist.is_distributed(d) and t.dist.locale_shape[d] > 1 for d in range(t.nd - 1))
+        # all cells and channels of a sample are here; all channels of a cell are
+        cut = [t.dist.is_distributed(d) and t.dist.locale_shape[d] > 1 for d in range(t.nd - 1)]
+        self.whole, self.whole_cells = not any(cut), not cut[-1]
         self.operand = None  # descriptor of the owned cells, by reference
         self.descs = {}    # widths -> NdDesc
         self.offsets = {}  # widths -> byte offset of the window
@@ -1564,12 +1565,19 @@ def _check_alike(what, first, *others):
     return device
 
 
+def _check_whole_cells(what, *tensors):
+    for t in tensors:
+        if not t._geo().whole_cells:
+            raise ValueError(f"{what} needs all channels of a cell on one rank: re-distribute the tensor "
+                             "(TensorShuffler)")
+
+
 class LayerNormalization:
     """Layer normalisation over the channels of every cell.  No counterpart in
     the reference; beside ``BatchNormalization``.  Takes tensors of
-    torch.float32 and torch.bfloat16, partitioned or not: a cell needs its own
-    channels only, and the gradients of scale and bias are all-reduced like
-    batch-norm's.  ``scale``, ``bias`` and their gradients are contiguous torch
+    torch.float32 and torch.bfloat16, partitioned along samples and space or not:
+    a cell needs its own channels only, all of which have to be on its rank, and
+    the gradients of scale and bias are all-reduced like batch-norm's.  ``scale``, ``bias`` and their gradients are contiguous torch
     tensors of C floats, ``mean`` and ``inv_std`` of one float per sample and
     owned cell."""
 
@@ -1588,6 +1596,7 @@ class LayerNormalization:
     def forward(self, input: Tensor, scale, bias, output: Tensor, mean=None, inv_std=None):
         """``scale`` and ``bias`` may be None (1 and 0); so may ``mean`` and
         ``inv_std`` where no backward pass follows.  ``output`` may be ``input``."""
+        _check_whole_cells("layer normalisation", input, output)
         dev = _check_alike("layer normalisation", input, output)
         C, size = input.local_shape[-2], input._geo().size
         if size == 0:
@@ -1603,6 +1612,7 @@ class LayerNormalization:
                         d_input: Tensor):
         """``d_input`` and this rank's sums of the gradients of scale and bias
         (None: not wanted).  ``d_input`` may be ``d_output`` or ``input``."""
+        _check_whole_cells("layer normalisation", input, d_output, d_input)
         dev = _check_alike("layer normalisation", input, d_output, d_input)
         C, s, geo = input.local_shape[-2], self.be.stream, input._geo()
         if (scale_gradient is None) != (bias_gradient is None):

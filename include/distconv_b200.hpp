@@ -2475,9 +2475,18 @@ private:
     std::vector<void*> m_all;
     int64_t m_bytes = 0;
 };
+
+inline void require_whole_cells(std::initializer_list<TensorF*> ts, const char* what)
+{
+    for (const TensorF* t : ts)
+    {
+        const int c = t->get_num_dims() - 2;
+        util::require(!t->get_distribution().is_distributed(c) || t->get_distribution().get_locale_shape()[c] == 1, what);
+    }
+}
 } // namespace internal
 
-// Layer normalisation over the channels of every cell, partitioned tensors or not.  mean and inv_std: a float per sample
+// Layer normalisation over the channels of every cell, tensors partitioned along samples and space or not.  mean and inv_std: a float per sample
 // and owned cell; scale and bias may be null.
 class LayerNormalization
 {
@@ -2488,6 +2497,7 @@ public:
     int forward(TensorF& input, const float* scale, const float* bias, TensorF& output, float* mean = nullptr,
                 float* inv_std = nullptr)
     {
+        internal::require_whole_cells({&input, &output}, "LayerNormalization: a cell's channels have to be on one rank");
         if (input.get_local_size() == 0)
             return 0;
         const dcb_nd_desc xd = input.nd_desc(), yd = output.nd_desc();
@@ -2500,6 +2510,8 @@ public:
     int backward_stage1(TensorF& input, TensorF& d_output, const float* mean, const float* inv_std, const float* scale,
                         float* scale_gradient, float* bias_gradient, TensorF& d_input)
     {
+        internal::require_whole_cells({&input, &d_output, &d_input},
+                                      "LayerNormalization: a cell's channels have to be on one rank");
         const size_t bytes = (size_t) input.get_local_shape()[-2] * sizeof(float);
         const bool counts = input.get_local_size() != 0 && input.is_split_root();
         if (input.get_local_size() != 0)

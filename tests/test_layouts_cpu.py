@@ -1,0 +1,31 @@
+"""Layouts that the operators of attention between cells refuse because a rank would work out something else than the
+whole tensor's result: no GPU."""
+import pytest
+import torch
+
+import dihydrogen_b200 as dc
+
+
+class Backend:
+    stream = None
+
+
+def shard(shape, grid, rank=0, dtype=torch.float32):
+    size = 1
+    for e in grid:
+        size *= e
+    t = dc.Tensor(shape, dc.Locale(rank, size), dc.Distribution.make_distribution(grid), dtype=dtype)
+    t.allocate("cpu")
+    return t
+
+
+def test_layer_norm_needs_all_channels_of_a_cell():
+    ln = dc.LayerNormalization(Backend(), 4, 1e-5)
+    x, whole = shard([6, 4, 8, 2], [1, 1, 2, 1]), shard([6, 4, 4, 2], [1, 1, 1, 1])
+    assert x.local_shape == whole.local_shape
+    for a, b in ((x, x), (whole, x), (x, whole)):
+        with pytest.raises(ValueError, match="channels of a cell"):
+            ln.forward(a, None, None, b)
+    for args in ((x, whole, whole), (whole, x, whole), (whole, whole, x)):
+        with pytest.raises(ValueError, match="channels of a cell"):
+            ln.backward(*args[:2], None, None, None, None, None, args[2])
