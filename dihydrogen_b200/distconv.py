@@ -524,6 +524,11 @@ class ChannelSlice:
         return s[:-2] + [self.count, s[-1]]
 
     @property
+    def offset(self):
+        o = self.tensor.offset
+        return o[:-2] + [o[-2] + self.first, o[-1]]
+
+    @property
     def buffer(self):
         """The whole tensor's."""
         return self.tensor.buffer
@@ -1661,8 +1666,9 @@ class RotaryPositions:
     channels are turned by the position along D (or time), the next ones by the
     position along H, then W, the rest is copied, as are the heads from
     ``rotated_heads`` on (the values of a packed projection).  Positions are
-    global: a shard of a partitioned tensor gets the angles of the whole one.
-    Input and output are of torch.float32 or torch.bfloat16 each; a
+    global: a shard of a partitioned tensor gets the angles of the whole one, and
+    a layer that was set up for one shard refuses others.  All channels of a cell
+    have to be on one rank.  Input and output are of torch.float32 or torch.bfloat16 each; a
     single-precision projection is rounded on its way to ``Attention``."""
 
     def __init__(self, backend: BackendDNNLib, num_dims: int):
@@ -1685,6 +1691,7 @@ class RotaryPositions:
         nsd = self.nsd
         if input.nd != self.num_dims or len(axis_channels) != nsd or (step is not None and len(step) != nsd):
             raise ValueError(f"axis_channels and step have {nsd} entries, W first")
+        _check_whole_cells("rotary positions", input)
         if self._plan:
             _abi.lib().dcb_rotary_plan_destroy(self._plan)
             self._plan = ctypes.c_void_p()
@@ -1695,12 +1702,15 @@ class RotaryPositions:
         for i in range(nsd):
             rd.axis_channels[2 - i], rd.origin[2 - i] = axis_channels[i], input.offset[i]
             rd.step[2 - i] = 1.0 if step is None else float(step[i])
-        self._local = list(input.local_shape)
+        self._local, self._at = list(input.local_shape), list(input.offset[:-2])
         call("dcb_rotary_plan_create", ctypes.byref(rd), ctypes.byref(input._make_nd_desc()), ctypes.byref(self._plan))
 
     def _apply(self, x: Tensor, y: Tensor, inverse):
         if x.local_shape[:-1] != self._local[:-1] or y.local_shape != x.local_shape:
             raise ValueError(f"local shapes {x.local_shape} and {y.local_shape}, set up for {self._local}")
+        if x.offset[:-2] != self._at or y.offset[:-2] != self._at:
+            raise ValueError(f"cells from {x.offset[:-2]} and {y.offset[:-2]} on, set up for those from {self._at} on")
+        _check_whole_cells("rotary positions", x, y)
         if _device(x) != _device(y):
             raise ValueError("rotary positions: tensors on two devices")
         if x._geo().size == 0:

@@ -2549,7 +2549,7 @@ private:
 };
 
 // Rotary positions on the grid of a tensor's cells; positions are global, so that a shard gets the angles of the whole
-// tensor.  axis_channels (even) in reference order, W first.
+// tensor; a layer set up for one shard refuses others.  All channels of a cell are on one rank.  axis_channels (even) in reference order, W first.
 class RotaryPositions
 {
 public:
@@ -2563,6 +2563,7 @@ public:
         const int nsd = m_num_dims - 2;
         util::require((int) axis_channels.size() == nsd && input.get_num_dims() == m_num_dims && head_dim > 0,
                       "RotaryPositions::setup: one entry per spatial dimension");
+        internal::require_whole_cells({&input}, "RotaryPositions: a cell's channels have to be on one rank");
         dcb_rotary_desc rd{};
         rd.nsd = nsd;
         rd.head_dim = head_dim;
@@ -2576,6 +2577,7 @@ public:
             rd.axis_channels[2 - i] = axis_channels[i];
             rd.origin[2 - i] = input.get_global_index()[i];
         }
+        m_at = input.get_global_index();
         const dcb_nd_desc xd = input.nd_desc();
         dcb_rotary_plan_destroy(m_plan);
         m_plan = nullptr;
@@ -2587,6 +2589,11 @@ public:
 private:
     int apply(TensorF& x, TensorF& y, int inverse)
     {
+        for (const TensorF* t : {&x, &y})
+            for (int i = 0; i < m_num_dims - 2; ++i)
+                util::require(t->get_num_dims() == m_num_dims && (m_at.empty() || t->get_global_index()[i] == m_at[i]),
+                              "RotaryPositions: cells at other positions than those it was set up for");
+        internal::require_whole_cells({&x, &y}, "RotaryPositions: a cell's channels have to be on one rank");
         if (x.get_local_size() == 0)
             return 0;
         const dcb_nd_desc xd = x.nd_desc(), yd = y.nd_desc();
@@ -2597,6 +2604,7 @@ private:
     }
     BackendDNNLib& m_be;
     int m_num_dims;
+    tensor::IndexVector m_at; // the first cell's global index
     dcb_rotary_plan* m_plan = nullptr;
 };
 

@@ -51,6 +51,16 @@ int main()
         refused("layer norm backward",
                 [&] { ln.backward(whole, cut, nullptr, nullptr, nullptr, nullptr, nullptr, whole); });
     }
+    { // cells at other positions than the layer was set up for
+        TensorF first = shard({12, 6, 8, 2}, {2, 1, 1, 1}, 0, 2), second = shard({12, 6, 8, 2}, {2, 1, 1, 1}, 1, 2),
+                cut = shard({6, 6, 16, 2}, {1, 1, 2, 1}, 0, 2);
+        RotaryPositions rot(be, 4);
+        refused("rotary positions, channels", [&] { rot.setup(cut, 4, {2, 2}); });
+        rot.setup(first, 4, {2, 2});
+        refused("rotary positions, place", [&] { rot.forward(second, second); });
+        refused("rotary positions, output", [&] { rot.backward(first, second); });
+        refused("rotary positions, channels", [&] { rot.forward(cut, cut); });
+    }
     if (failures)
         return 1;
     std::printf("shim_layouts_check OK\n");

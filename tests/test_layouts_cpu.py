@@ -29,3 +29,14 @@ def test_layer_norm_needs_all_channels_of_a_cell():
     for args in ((x, whole, whole), (whole, x, whole), (whole, whole, x)):
         with pytest.raises(ValueError, match="channels of a cell"):
             ln.backward(*args[:2], None, None, None, None, None, args[2])
+
+
+def test_rotary_positions_need_all_channels_of_a_cell():
+    rot = dc.RotaryPositions(Backend(), 4)
+    with pytest.raises(ValueError, match="channels of a cell"):
+        rot.setup(shard([6, 4, 8, 2], [1, 1, 2, 1]), 4, [2, 2])
+
+
+def test_channel_slices_lie_where_their_tensor_does():
+    t = shard([6, 4, 8, 2], [2, 1, 1, 1], rank=1)
+    assert t.offset == [3, 0, 0, 0] and t.channel_slice(5, 2).offset == [3, 0, 5, 0]
