@@ -1673,12 +1673,13 @@ class RotaryPositions:
 
     def __init__(self, backend: BackendDNNLib, num_dims: int):
         self.be, self.num_dims, self.nsd = backend, num_dims, num_dims - 2
-        self._plan = ctypes.c_void_p()
+        self._plans = {}  # geometry -> plan, as long as the layer lives: captured graphs read their tables
+        self._plan = None
 
     def __del__(self):
         try:
-            if getattr(self, "_plan", None):
-                _abi.lib().dcb_rotary_plan_destroy(self._plan)
+            for p in getattr(self, "_plans", {}).values():
+                _abi.lib().dcb_rotary_plan_destroy(p)
         except Exception:
             pass
 
@@ -1687,14 +1688,13 @@ class RotaryPositions:
         """``axis_channels`` (even; how many of a head's channels belong to an
         axis) and ``step`` (what a position counts, 1 by default) in reference
         order (W first).  ``interleaved``: pairs are neighbours, not the two
-        halves of an axis' channels."""
+        halves of an axis' channels.  The tables of every geometry that a layer
+        was set up for stay until the layer goes (a few hundred kilobytes each):
+        graphs captured before another set-up can be replayed after it."""
         nsd = self.nsd
         if input.nd != self.num_dims or len(axis_channels) != nsd or (step is not None and len(step) != nsd):
             raise ValueError(f"axis_channels and step have {nsd} entries, W first")
         _check_whole_cells("rotary positions", input)
-        if self._plan:
-            _abi.lib().dcb_rotary_plan_destroy(self._plan)
-            self._plan = ctypes.c_void_p()
         rd = _abi.RotaryDesc()
         rd.nsd, rd.head_dim, rd.interleaved, rd.base = nsd, head_dim, bool(interleaved), float(base)
         heads = input.local_shape[-2] // head_dim if head_dim > 0 else 0
@@ -1703,7 +1703,12 @@ class RotaryPositions:
             rd.axis_channels[2 - i], rd.origin[2 - i] = axis_channels[i], input.offset[i]
             rd.step[2 - i] = 1.0 if step is None else float(step[i])
         self._local, self._at = list(input.local_shape), list(input.offset[:-2])
-        call("dcb_rotary_plan_create", ctypes.byref(rd), ctypes.byref(input._make_nd_desc()), ctypes.byref(self._plan))
+        key = (bytes(rd), tuple(input.local_shape[:-1]), torch.cuda.current_device() if torch.cuda.is_available() else -1)
+        self._plan = self._plans.get(key)
+        if self._plan is None:
+            plan = ctypes.c_void_p()
+            call("dcb_rotary_plan_create", ctypes.byref(rd), ctypes.byref(input._make_nd_desc()), ctypes.byref(plan))
+            self._plan = self._plans[key] = plan
 
     def _apply(self, x: Tensor, y: Tensor, inverse):
         if x.local_shape[:-1] != self._local[:-1] or y.local_shape != x.local_shape:

@@ -2549,13 +2549,19 @@ private:
 };
 
 // Rotary positions on the grid of a tensor's cells; positions are global, so that a shard gets the angles of the whole
-// tensor; a layer set up for one shard refuses others.  All channels of a cell are on one rank.  axis_channels (even) in reference order, W first.
+// tensor; a layer set up for one shard refuses others.  All channels of a cell are on one rank.  axis_channels (even) in
+// reference order, W first.  The tables of every geometry that a layer was set up for stay until the layer goes: graphs
+// captured before another set-up can be replayed after it.
 class RotaryPositions
 {
 public:
     RotaryPositions(BackendDNNLib& backend, int num_dims) : m_be(backend), m_num_dims(num_dims) {}
     RotaryPositions(const RotaryPositions&) = delete;
-    ~RotaryPositions() { dcb_rotary_plan_destroy(m_plan); }
+    ~RotaryPositions()
+    {
+        for (const Known& k : m_known)
+            dcb_rotary_plan_destroy(k.plan);
+    }
     // rotated_heads < 0: all
     void setup(TensorF& input, int head_dim, const std::vector<int>& axis_channels, int rotated_heads = -1,
                double base = 10000.0, bool interleaved = false)
@@ -2579,9 +2585,19 @@ public:
         }
         m_at = input.get_global_index();
         const dcb_nd_desc xd = input.nd_desc();
-        dcb_rotary_plan_destroy(m_plan);
         m_plan = nullptr;
-        util::check(dcb_rotary_plan_create(&rd, &xd, &m_plan), "rotary plan");
+        Known now{{rd.head_dim, rd.rotated_heads, rd.interleaved, xd.c}, base, 0, nullptr};
+        util::require(cudaGetDevice(&now.device) == cudaSuccess, "RotaryPositions::setup: no device");
+        for (int i = 0; i < 3; ++i)
+            now.key.insert(now.key.end(), {rd.axis_channels[i], rd.origin[i], xd.dims[i]});
+        for (const Known& k : m_known)
+            if (k.key == now.key && k.base == now.base && k.device == now.device)
+                m_plan = k.plan;
+        if (m_plan != nullptr)
+            return;
+        util::check(dcb_rotary_plan_create(&rd, &xd, &now.plan), "rotary plan");
+        m_known.push_back(now);
+        m_plan = now.plan;
     }
     int forward(TensorF& input, TensorF& output) { return apply(input, output, 0); }
     int backward(TensorF& d_output, TensorF& d_input) { return apply(d_output, d_input, 1); }
@@ -2604,8 +2620,16 @@ private:
     }
     BackendDNNLib& m_be;
     int m_num_dims;
+    struct Known
+    {
+        std::vector<int64_t> key; // the geometry
+        double base;
+        int device;
+        dcb_rotary_plan* plan;
+    };
     tensor::IndexVector m_at; // the first cell's global index
-    dcb_rotary_plan* m_plan = nullptr;
+    std::vector<Known> m_known;
+    dcb_rotary_plan* m_plan = nullptr; // one of those
 };
 
 // Scaled dot-product attention from the cells of one tensor to those of another, or its own.  A sample's cells and

@@ -61,6 +61,45 @@ int main()
         refused("rotary positions, output", [&] { rot.backward(first, second); });
         refused("rotary positions, channels", [&] { rot.forward(cut, cut); });
     }
+    { // a graph captured before another set-up
+        cudaStream_t stream;
+        cudaStreamCreateWithFlags(&stream, cudaStreamNonBlocking);
+        {
+            BackendDNNLib on_stream(loc, stream);
+            TensorF x = shard({9, 7, 8, 1}, {1, 1, 1, 1}, 0, 1), y = shard({9, 7, 8, 1}, {1, 1, 1, 1}, 0, 1),
+                    z = shard({5, 3, 8, 1}, {1, 1, 1, 1}, 0, 1);
+            for (TensorF* t : {&x, &y, &z})
+                t->allocate();
+            std::vector<float> in((size_t) x.get_local_size()), before(in.size()), after(in.size());
+            for (size_t i = 0; i < in.size(); ++i)
+                in[i] = (float) (i % 23) - 11.f;
+            cudaMemcpy(x.get_buffer(), in.data(), in.size() * sizeof(float), cudaMemcpyHostToDevice);
+            RotaryPositions rot(on_stream, 4);
+            rot.setup(x, 8, {4, 4});
+            rot.forward(x, y);
+            on_stream.wait();
+            cudaMemcpy(before.data(), y.get_buffer(), in.size() * sizeof(float), cudaMemcpyDeviceToHost);
+            cudaGraph_t graph;
+            cudaGraphExec_t exec;
+            cudaStreamBeginCapture(stream, cudaStreamCaptureModeThreadLocal);
+            rot.forward(x, y);
+            cudaStreamEndCapture(stream, &graph);
+            cudaGraphInstantiate(&exec, graph, 0);
+            rot.setup(z, 8, {2, 6}, -1, 10.0);
+            rot.forward(z, z);
+            on_stream.wait();
+            cudaMemset(y.get_buffer(), 0, in.size() * sizeof(float));
+            cudaDeviceSynchronize();
+            cudaGraphLaunch(exec, stream);
+            on_stream.wait();
+            cudaMemcpy(after.data(), y.get_buffer(), in.size() * sizeof(float), cudaMemcpyDeviceToHost);
+            if (cudaGetLastError() != cudaSuccess || after != before)
+                std::printf("rotary positions: a graph lost its tables\n"), ++failures;
+            cudaGraphExecDestroy(exec);
+            cudaGraphDestroy(graph);
+        }
+        cudaStreamDestroy(stream);
+    }
     if (failures)
         return 1;
     std::printf("shim_layouts_check OK\n");

@@ -47,3 +47,30 @@ def test_channel_slices_are_turned_in_place():
     want = R.rotary(x[:, 4:16], 6, (4, 2), 2, 10000.0, False, [0, 0], [1.0, 1.0], False)
     R.close(t.buffer[:, 4:16], want, "turned")
     assert torch.equal(t.buffer[:, :4].cpu(), x[:, :4]) and torch.equal(t.buffer[:, 16:].cpu(), x[:, 16:])
+
+
+def test_a_graph_outlives_another_setup():
+    """The tables that a captured graph reads stay while the layer does; the same geometry again gets the same ones."""
+    be = backend()
+    x = torch.randn(1, 16, 12, 20)
+    t, y = tensor(x.cuda(), be), tensor(torch.empty(x.shape, device="cuda"), be)
+    other = tensor(torch.randn(1, 16, 40, 30).cuda(), be)
+    rot = dc.RotaryPositions(be, 4)
+    rot.setup(t, 16, [8, 8])
+    rot.forward(t, y)
+    want = y.buffer.clone()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        rot.forward(t, y)
+    for base in (10.0, 100.0, 1000.0):
+        rot.setup(other, 16, [4, 12], base=base)
+        rot.forward(other, other)
+    assert len(rot._plans) == 4
+    rot.setup(t, 16, [8, 8])
+    assert len(rot._plans) == 4
+    y.buffer.zero_()
+    graph.replay()
+    assert torch.equal(y.buffer, want)
+    y.buffer.zero_()
+    rot.forward(t, y)
+    assert torch.equal(y.buffer, want)
