@@ -282,6 +282,9 @@ int32_t dcb_rotary_plan_create(const dcb_rotary_desc* rd, const dcb_nd_desc* xd,
         err = cudaMalloc(&p->tables, floats * sizeof(float));
         if (err == cudaSuccess)
             err = cudaMemcpy(p->tables, host.data(), floats * sizeof(float), cudaMemcpyHostToDevice);
+        // a copy from pageable memory returns when its source may go; kernels on other streams need it arrived
+        if (err == cudaSuccess)
+            err = cudaStreamSynchronize(nullptr);
     }
     if (err != cudaSuccess)
     {

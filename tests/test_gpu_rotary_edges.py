@@ -74,3 +74,19 @@ def test_a_graph_outlives_another_setup():
     y.buffer.zero_()
     rot.forward(t, y)
     assert torch.equal(y.buffer, want)
+
+
+def test_tables_are_there_for_every_stream():
+    """A kernel on a stream that waits for no other, straight behind the set-up."""
+    s = torch.cuda.Stream()
+    be = backend(s)
+    x = torch.randn(1, 64, 1, 20001)
+    t, y = tensor(x.cuda(), be), tensor(torch.empty(x.shape, device="cuda"), be)
+    want = R.rotary(x, 64, (0, 64), 1, 10000.0, False, [0, 0], [1.0, 1.0], False)
+    torch.cuda.synchronize()
+    for _ in range(3):
+        rot = dc.RotaryPositions(be, 4)
+        rot.setup(t, 64, [64, 0])
+        rot.forward(t, y)
+        s.synchronize()
+        R.close(y.buffer, want, "turned")
