@@ -347,9 +347,14 @@ int32_t attn_fill(int32_t dtype, const AttnTensor& t, int n, long long channels,
     });
 }
 
+// Of a sample; 2^40 stands for all numbers from there on, whatever their product wraps to.
 int64_t cells_of(const dcb_nd_desc& d)
 {
-    return d.dims[0] * d.dims[1] * d.dims[2];
+    constexpr int64_t MANY = 1ll << 40;
+    int64_t cells = 1;
+    for (int i = 0; i < 3; ++i)
+        cells = cells == 0 || d.dims[i] == 0 ? 0 : d.dims[i] >= MANY / cells ? MANY : cells * d.dims[i];
+    return cells;
 }
 
 // What follows from the shapes alone.

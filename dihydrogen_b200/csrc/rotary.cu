@@ -221,6 +221,12 @@ int32_t dcb_rotary_plan_create(const dcb_rotary_desc* rd, const dcb_nd_desc* xd,
     DCB_REQUIRE(rd->nsd == xd->nsd, "nsd differs from the tensor's");
     DCB_REQUIRE(rd->head_dim >= 1 && xd->c >= 1 && xd->c % rd->head_dim == 0 && xd->c < (1 << 30),
                 "channels must be heads of head_dim");
+    for (int i = 0; i < 3; ++i)
+        if (xd->dims[i] >= (1ll << 31))
+        {
+            set_last_error("unsupported: 2^31 cells along an axis");
+            return DCB_UNSUPPORTED;
+        }
     const int64_t heads = xd->c / rd->head_dim;
     DCB_REQUIRE(rd->rotated_heads >= 0 && rd->rotated_heads <= heads, "rotated_heads out of range");
     int64_t turned = 0;

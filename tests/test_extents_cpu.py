@@ -1,0 +1,27 @@
+"""Extents and positions that the operators of attention between cells refuse before they work anything out: no GPU."""
+import ctypes
+
+import pytest
+
+from dihydrogen_b200 import _abi
+from test_attention_cpu import attention, desc, nd, rotary, status
+
+
+@pytest.mark.parametrize("dims", [(1 << 32, 1 << 32), (1 << 16, 1 << 31, 1 << 31), (1 << 62, 4), (3, 1 << 62, 1 << 62),
+                                  (1 << 15, 1 << 15)])
+def test_cells_whose_number_wraps(dims):
+    few = nd(1, 8, 4, 7)
+    assert attention(desc(), nd(1, 16, *dims), few) == _abi.UNSUPPORTED
+    assert attention(desc(), nd(1, 16, 4, 7), nd(1, 8, *dims)) == _abi.UNSUPPORTED
+    assert status("dcb_attention_workspace_bytes", desc(), nd(1, 16, *dims), few, 0) == -1
+
+
+@pytest.mark.parametrize("dims", [(0, 1 << 62, 1), (1 << 62, 0, 1), (0, 1 << 31, 4), (0, 1 << 61, 0)])
+def test_rotary_tables_of_an_empty_tensor_with_a_long_axis(dims):
+    assert rotary(xd=nd(1, 24, *dims), nsd=3, axis=(2, 4, 2)) == _abi.UNSUPPORTED
+
+
+def test_rotary_tables_that_no_memory_holds():
+    assert rotary(xd=nd(1, 1 << 16, 0, (1 << 31) - 1, 0), nsd=3, head_dim=1 << 16, rotated_heads=1,
+                  axis=(0, 1 << 16, 0)) == _abi.BAD_ARG
+    assert b"memory" in _abi.lib().dcb_last_error()
