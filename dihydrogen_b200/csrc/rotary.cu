@@ -14,7 +14,7 @@
 struct dcb_rotary_plan
 {
     dcb_rotary_desc rd;
-    int64_t n, c, dims[3];
+    int64_t c, dims[3];
     float* tables;        // per axis: cosines [pair][position], then sines
     long long table_at[3]; // in floats
     int device;
@@ -261,7 +261,6 @@ int32_t dcb_rotary_plan_create(const dcb_rotary_desc* rd, const dcb_nd_desc* xd,
         return DCB_BAD_ARG;
     }
     p->rd = *rd;
-    p->n = xd->n;
     p->c = xd->c;
     p->tables = nullptr;
     long long at = 0;
@@ -270,6 +269,15 @@ int32_t dcb_rotary_plan_create(const dcb_rotary_desc* rd, const dcb_nd_desc* xd,
         p->dims[i] = xd->dims[i];
         p->table_at[i] = at;
         const int pairs = rd->axis_channels[i] / 2;
+        // the largest angle is one end's, of the first or the last pair
+        for (int j : {0, pairs - 1})
+            for (double end : {(double) rd->origin[i], (double) rd->origin[i] + xd->dims[i]})
+                if (pairs > 0 && !std::isfinite(rd->step[i] * end * std::pow(rd->base, -2.0 * j / rd->axis_channels[i])))
+                {
+                    delete p;
+                    set_last_error("bad argument: positions whose angles are not finite");
+                    return DCB_BAD_ARG;
+                }
         for (int j = 0; j < pairs; ++j)
         {
             const double per = std::pow(rd->base, -2.0 * j / rd->axis_channels[i]);

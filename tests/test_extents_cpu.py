@@ -25,3 +25,15 @@ def test_rotary_tables_that_no_memory_holds():
     assert rotary(xd=nd(1, 1 << 16, 0, (1 << 31) - 1, 0), nsd=3, head_dim=1 << 16, rotated_heads=1,
                   axis=(0, 1 << 16, 0)) == _abi.BAD_ARG
     assert b"memory" in _abi.lib().dcb_last_error()
+
+
+@pytest.mark.parametrize("kw", [dict(base=1e-320), dict(step=1e308), dict(step=-1e308), dict(base=1e-300, step=1e100)])
+def test_rotary_angles_that_are_not_finite(kw):
+    """base^(-2j / a) or step times a position passes what a double holds: the table would be NaN."""
+    rd = _abi.RotaryDesc()
+    rd.nsd, rd.head_dim, rd.rotated_heads, rd.base = 2, 256, 1, kw.get("base", 100.0)
+    rd.axis_channels[1], rd.axis_channels[2] = 0, 256
+    for i in range(3):
+        rd.step[i] = kw.get("step", 1.0)
+    assert status("dcb_rotary_plan_create", rd, nd(1, 256, 3, 500), ctypes.byref(ctypes.c_void_p())) == _abi.BAD_ARG
+    assert b"finite" in _abi.lib().dcb_last_error()
