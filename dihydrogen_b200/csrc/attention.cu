@@ -1,6 +1,9 @@
 // Attention between cells: argument checks, workspace, the kernels beside the products.
 #include "attention.cuh"
 
+#include <initializer_list>
+#include <utility>
+
 namespace dcb
 {
 namespace
@@ -417,6 +420,88 @@ int32_t attn_tensor(const dcb_nd_desc* d, const dcb_nd_desc* like, const void* p
     return DCB_OK;
 }
 
+// The memory of an operand or a result, in bytes: n x c rows.
+struct AttnRows
+{
+    const char* p;
+    int64_t n, c, sn, sc, row;
+    int64_t first() const { return std::min<int64_t>(0, (n - 1) * sn) + std::min<int64_t>(0, (c - 1) * sc); }
+    int64_t last() const { return std::max<int64_t>(0, (n - 1) * sn) + std::max<int64_t>(0, (c - 1) * sc) + row; }
+};
+
+AttnRows attn_rows(const AttnTensor& t, int32_t dtype, const dcb_nd_desc& d)
+{
+    const int64_t es = elem_bytes(dtype);
+    return AttnRows{static_cast<const char*>(t.p), d.n, d.c, t.sn * es, t.sc * es, cells_of(d) * es};
+}
+
+AttnRows attn_rows(const void* p, int64_t bytes)
+{
+    return AttnRows{static_cast<const char*>(p), 1, 1, 0, 0, bytes};
+}
+
+// Whether they share a byte.  Rows with the same strides (slices of one packed tensor) are compared one by one, others by
+// their extent.
+bool attn_overlap(AttnRows a, AttnRows b)
+{
+    for (const AttnRows* r : {&a, &b})
+        if (!r->p || r->n == 0 || r->c == 0 || r->row == 0)
+            return false;
+    // how far b's first row lies behind a's: addresses may be anything
+    const int64_t apart = (int64_t) (reinterpret_cast<uintptr_t>(b.p) - reinterpret_cast<uintptr_t>(a.p));
+    if (apart + b.first() >= a.last() || apart + b.last() <= a.first())
+        return false;
+    // a stride that nothing steps over is the other's
+    if (a.n == 1)
+        a.sn = b.n == 1 ? 0 : b.sn;
+    if (b.n == 1)
+        b.sn = a.sn;
+    if (a.c == 1)
+        a.sc = b.c == 1 ? 0 : b.sc;
+    if (b.c == 1)
+        b.sc = a.sc;
+    if (a.sc > a.sn) // the longer steps first
+        for (AttnRows* r : {&a, &b})
+            std::swap(r->n, r->c), std::swap(r->sn, r->sc);
+    if (a.sn != b.sn || a.sc != b.sc || a.sn < 0 || a.sc < 0)
+        return true;
+    // rows i, j of a and i + k, j + l of b share a byte if apart + k sn + l sc lies in (-b.row, a.row)
+    const auto near = [](int64_t at, int64_t step, int64_t lo, int64_t hi, int64_t below, int64_t above, auto f) {
+        // every k in [lo, hi] with at + k step in (below, above)
+        if (step > 0)
+        {
+            const auto floor_div = [](int64_t x, int64_t d) { return x >= 0 ? x / d : -((-x + d - 1) / d); };
+            lo = std::max(lo, floor_div(below - at, step) + 1);
+            hi = std::min(hi, -floor_div(at - above, step) - 1);
+        }
+        else if (at <= below || at >= above)
+            return false;
+        else
+            hi = std::min(hi, lo);
+        for (int64_t k = lo; k <= hi; ++k)
+            if (f(at + k * step))
+                return true;
+        return false;
+    };
+    const int64_t reach = a.sc * std::max(a.c, b.c);
+    return near(apart, a.sn, 1 - a.n, b.n - 1, -b.row - reach, a.row + reach, [&](int64_t at) {
+        return near(at, a.sc, 1 - a.c, b.c - 1, -b.row, a.row, [](int64_t) { return true; });
+    });
+}
+
+// No result shares memory with an operand or another result.
+int32_t attn_places(std::initializer_list<AttnRows> results, std::initializer_list<AttnRows> operands)
+{
+    for (auto r = results.begin(); r != results.end(); ++r)
+    {
+        for (const AttnRows& x : operands)
+            DCB_REQUIRE(!attn_overlap(*r, x), "a result in an operand's place");
+        for (auto other = r + 1; other != results.end(); ++other)
+            DCB_REQUIRE(!attn_overlap(*r, *other), "two results in one place");
+    }
+    return DCB_OK;
+}
+
 // The workspace, piece by piece; a null base only counts.
 struct Carve
 {
@@ -589,7 +674,11 @@ int32_t dcb_attention_fwd(const dcb_attention_desc* ad, const dcb_nd_desc* qd, c
     if (p.n == 0 || p.sq == 0)
         return DCB_OK;
     DCB_REQUIRE(lse, "null lse");
-    DCB_REQUIRE(o != q && (p.sk == 0 || (o != k && o != v)), "a result in an operand's place");
+    const int64_t cells_q = (int64_t) p.n * p.sq, cells_k = (int64_t) p.n * p.sk;
+    if (int32_t e = attn_places({attn_rows(p.o, ad->dtype, *qd), attn_rows(lse, 4 * p.q_heads * cells_q)},
+                                {attn_rows(p.q, ad->dtype, *qd), attn_rows(p.k, ad->dtype, *kd),
+                                 attn_rows(p.v, ad->dtype, *kd), attn_rows(q_mask, cells_q), attn_rows(kv_mask, cells_k)}))
+        return e;
     cudaStream_t s = as_stream(stream);
     p.lse = static_cast<float*>(lse);
     p.q_mask = static_cast<const uint8_t*>(q_mask);
@@ -640,13 +729,14 @@ int32_t dcb_attention_bwd(const dcb_attention_desc* ad, const dcb_nd_desc* qd, c
             return e;
     if (p.n == 0)
         return DCB_OK;
-    const void* const results[] = {dq, dk, dv};
-    for (int r = 0; r < 3; ++r)
-    {
-        for (const void* x : {q, k, v, o, d_o, lse})
-            DCB_REQUIRE(!results[r] || results[r] != x, "a result in an operand's place");
-        DCB_REQUIRE(!results[r] || results[r] != results[(r + 1) % 3], "two results in one place");
-    }
+    const int64_t cells_q = (int64_t) p.n * p.sq, cells_k = (int64_t) p.n * p.sk;
+    if (int32_t e = attn_places({attn_rows(p.dq, ad->dtype, *qd), attn_rows(p.dk, ad->dtype, *kd),
+                                 attn_rows(p.dv, ad->dtype, *kd)},
+                                {attn_rows(p.q, ad->dtype, *qd), attn_rows(p.k, ad->dtype, *kd),
+                                 attn_rows(p.v, ad->dtype, *kd), attn_rows(p.o, ad->dtype, *qd),
+                                 attn_rows(p.d_o, ad->dtype, *qd), attn_rows(lse, 4 * p.q_heads * cells_q),
+                                 attn_rows(q_mask, cells_q), attn_rows(kv_mask, cells_k)}))
+        return e;
     cudaStream_t s = as_stream(stream);
     if (p.sq == 0 || p.sk == 0) // one side is empty: the other's gradients are zero
     {
