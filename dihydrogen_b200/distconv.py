@@ -1590,7 +1590,7 @@ class LayerNormalization:
         if not epsilon >= 0:
             raise ValueError("epsilon must not be negative")
         self.be, self.num_dims, self.epsilon = backend, num_dims, float(epsilon)
-        self._last = (None, 0)
+        self._last = (None, None, 0)  # geometry, device, workspace bytes
 
     def new_statistics(self, input: Tensor):
         """Memory for ``mean`` and ``inv_std`` of a tensor like ``input``."""
@@ -1635,9 +1635,9 @@ class LayerNormalization:
         dtype = _DTYPES[input.dtype]
         keep, ws, nbytes = None, 0, 0
         if gw:
-            if self._last[0] is not geo:
-                self._last = (geo, _abi.lib().dcb_ln_bwd_workspace_bytes(xd, dtype))
-            nbytes = self._last[1]
+            if self._last[0] is not geo or self._last[1] != dev:
+                self._last = (geo, dev, _abi.lib().dcb_ln_bwd_workspace_bytes(xd, dtype))
+            nbytes = self._last[2]
             keep, ws = _workspace(nbytes, s, dev)
         call("dcb_ln_bwd", xd, dtype, x, dyd, dy, pm, pi, _vector("scale", scale, C, dev), dxd, dx, gw, gb, ws,
              nbytes, _stream_ptr(s))
@@ -1762,14 +1762,16 @@ class Attention:
         if self.q_heads < 1 or self.kv_heads < 1 or self.q_heads % self.kv_heads:
             raise ValueError("q_heads must be a multiple of kv_heads")
         self.scale, self.causal = scale, bool(causal)
-        self._known = {}  # shapes and type -> (descriptor, workspace bytes forward, backward)
-        self._recent = (None, None, None, None)  # the latest of them
+        self._known = {}  # shapes, type and device -> (descriptor, workspace bytes forward, backward)
+        self._recent = (None, None, None, None, None)  # the latest of them
 
-    def _desc(self, q, k, shape_q, shape_k):
+    KNOWN = 64  # geometries that are kept, the latest
+
+    def _desc(self, q, k, shape_q, shape_k, device):
         recent = self._recent
-        if shape_q == recent[0] and shape_k == recent[1] and q.dtype is recent[2]:
-            return recent[3]
-        key = (tuple(shape_q), tuple(shape_k), q.dtype)
+        if shape_q == recent[0] and shape_k == recent[1] and q.dtype is recent[2] and device == recent[3]:
+            return recent[4]
+        key = (tuple(shape_q), tuple(shape_k), q.dtype, device)
         got = self._known.get(key)
         if got is None:
             if shape_q[-2] % self.q_heads or shape_q[-2] == 0:
@@ -1783,8 +1785,10 @@ class Attention:
                 if n < 0:
                     raise ValueError("attention: " + _abi.lib().dcb_last_error().decode())
                 size.append(n)
+            if len(self._known) >= self.KNOWN:
+                del self._known[next(iter(self._known))]
             got = self._known[key] = (ctypes.byref(ad), size)
-        self._recent = (list(shape_q), list(shape_k), q.dtype, got)
+        self._recent = (list(shape_q), list(shape_k), q.dtype, device, got)
         return got
 
     def _checked(self, q, k, q_like, kv_like, lse, q_mask, kv_mask):
@@ -1810,9 +1814,10 @@ class Attention:
         shape_q, shape_k, pl, pq, pk = self._checked(q, k, (output,), (v,), lse, q_mask, kv_mask)
         if 0 in shape_q:
             return 0
-        ad, size = self._desc(q, k, shape_q, shape_k)
+        device = lse.get_device()
+        ad, size = self._desc(q, k, shape_q, shape_k, device)
         s = self.be.stream
-        keep, ws = _workspace(size[0], s, lse.get_device())
+        keep, ws = _workspace(size[0], s, device)
         call("dcb_attention_fwd", ad, *q._operand(), *k._operand(), *v._operand(), pq, pk, *output._operand(), pl, ws,
              size[0], _stream_ptr(s))
         return 0
@@ -1822,9 +1827,10 @@ class Attention:
         shape_q, shape_k, pl, pq, pk = self._checked(q, k, (output, d_output, d_q), (v, d_k, d_v), lse, q_mask, kv_mask)
         if shape_q[-1] == 0:
             return 0
-        ad, size = self._desc(q, k, shape_q, shape_k)
+        device = lse.get_device()
+        ad, size = self._desc(q, k, shape_q, shape_k, device)
         s = self.be.stream
-        keep, ws = _workspace(size[1], s, lse.get_device())
+        keep, ws = _workspace(size[1], s, device)
         call("dcb_attention_bwd", ad, *q._operand(), *k._operand(), *v._operand(), pq, pk, *output._operand(), pl,
              *d_output._operand(), *d_q._operand(), *d_k._operand(), *d_v._operand(), ws, size[1], _stream_ptr(s))
         return 0
