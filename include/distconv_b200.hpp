@@ -2446,8 +2446,8 @@ private:
 // ---- attention between cells, and what goes with it (no counterpart in the reference) ----
 namespace internal
 {
-// Device memory that a layer keeps for its calls, which have to follow one another (one stream, or ordered streams).
-// What it has grown out of stays until the layer goes: a captured graph may still use it.
+// Device memory that a layer keeps for its calls, on each device that it is used on; the calls have to follow one another
+// (one stream, or ordered streams).  What it has grown out of stays until the layer goes: a captured graph may still use it.
 class Workspace
 {
 public:
@@ -2455,25 +2455,39 @@ public:
     Workspace(const Workspace&) = delete;
     ~Workspace()
     {
-        for (void* p : m_all)
-            cudaFree(p);
+        for (const Block& b : m_all)
+            cudaFree(b.p);
     }
+    // The newest block of the current device, null if there is none and no bytes are asked for.
     void* get(int64_t bytes)
     {
-        if (bytes > m_bytes)
+        int device = 0;
+        if (cudaGetDevice(&device) != cudaSuccess)
+            throw std::runtime_error("no device for a layer's workspace");
+        const Block* have = nullptr;
+        for (const Block& b : m_all)
+            if (b.device == device)
+                have = &b;
+        if (bytes <= (have ? have->bytes : 0))
+            return have ? have->p : nullptr;
+        void* p = nullptr;
+        if (cudaMalloc(&p, (size_t) bytes) != cudaSuccess)
         {
-            void* p = nullptr;
-            if (cudaMalloc(&p, (size_t) bytes) != cudaSuccess)
-                throw std::runtime_error("cudaMalloc of a layer's workspace failed");
-            m_all.push_back(p);
-            m_bytes = bytes;
+            (void) cudaGetLastError();
+            throw std::runtime_error("cudaMalloc of a layer's workspace failed");
         }
-        return m_all.empty() ? nullptr : m_all.back();
+        m_all.push_back(Block{p, bytes, device});
+        return p;
     }
 
 private:
-    std::vector<void*> m_all;
-    int64_t m_bytes = 0;
+    struct Block
+    {
+        void* p;
+        int64_t bytes;
+        int device;
+    };
+    std::vector<Block> m_all;
 };
 
 inline void require_whole_cells(std::initializer_list<TensorF*> ts, const char* what)

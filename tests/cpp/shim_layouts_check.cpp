@@ -100,6 +100,13 @@ int main()
         }
         cudaStreamDestroy(stream);
     }
+    { // a layer's workspace: what it has grown out of stays
+        internal::Workspace ws;
+        void *none = ws.get(0), *small = ws.get(1000), *again = ws.get(500), *large = ws.get(1 << 20), *back = ws.get(1000);
+        if (none != nullptr || again != small || large == small || back != large || cudaMemset(small, 1, 1000) != cudaSuccess
+            || cudaMemset(large, 1, 1 << 20) != cudaSuccess)
+            std::printf("workspace: other blocks than asked for\n"), ++failures;
+    }
     if (failures)
         return 1;
     std::printf("shim_layouts_check OK\n");
