@@ -825,10 +825,15 @@ def owned_box(t: Tensor, rank: int):
 class TensorShuffler:
     """tensor::TensorMPICUDAShuffler (shuffle_mpi_cuda.hpp:14-512): moves a
     tensor between two distributions of the same global shape.  Cells travel
-    as peer stores into the owner's receive window; see csrc/shuffle.cu."""
+    as peer stores into the owner's receive window; see csrc/shuffle.cu.  Takes
+    torch.float32: what is to be torch.bfloat16 is re-distributed before it is
+    rounded (``RotaryPositions`` rounds on its way, also with no head turned)."""
 
     def __init__(self, src: Tensor, dst: Tensor, connect=True):
         assert list(src.shape) == list(dst.shape) and src.locale.size == dst.locale.size
+        for t in (src, dst):
+            if t.dtype is not torch.float32:
+                raise TypeError(f"TensorShuffler takes torch.float32, not {t.dtype}: re-distribute before the rounding")
         self.src, self.dst = src, dst
         self.locale = src.locale
         self._plans = {}
@@ -1574,7 +1579,7 @@ def _check_whole_cells(what, *tensors):
     for t in tensors:
         if not t._geo().whole_cells:
             raise ValueError(f"{what} needs all channels of a cell on one rank: re-distribute the tensor "
-                             "(TensorShuffler)")
+                             "(TensorShuffler, in torch.float32)")
 
 
 class LayerNormalization:
@@ -1745,8 +1750,9 @@ class Attention:
     torch.float32 (multiplied in fp32) or torch.bfloat16 (tensor cores); query
     head h reads key head h // (q_heads // kv_heads).  Cells are in memory order
     (D, H, W); ``causal`` lets cell i of the queries see the keys up to
-    i + (keys - queries).  A sample's cells have to be on one rank: re-distribute
-    a spatially partitioned tensor to sample-parallel first (``TensorShuffler``).
+    i + (keys - queries).  A sample's cells have to be on one rank: a spatially
+    partitioned projection is re-distributed to sample-parallel in torch.float32
+    (``TensorShuffler``) and rounded behind that (``RotaryPositions``).
     ``num_dims`` is the queries'; an image's cells may read a volume's.
 
     ``q_mask`` / ``kv_mask``: arrays of bool or uint8, one per sample and cell, 0
@@ -1798,7 +1804,7 @@ class Attention:
         for t in (q, k, *q_like, *kv_like):
             if not t._geo().whole:
                 raise ValueError("attention needs all cells and channels of a sample on one rank: re-distribute the "
-                                 "tensor (TensorShuffler)")
+                                 "tensor (TensorShuffler, in torch.float32)")
         device = _check_alike("attention", q, *q_like)
         _check_alike("attention", k, *kv_like)
         shape_q, shape_k = q.local_shape, k.local_shape

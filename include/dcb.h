@@ -495,8 +495,8 @@ int32_t dcb_rotary_apply(const dcb_rotary_plan* plan, const dcb_nd_desc* xd,
  * that a mask takes out hold is never interpreted, and their results are 0;
  * `causal` only sets the weight of a later cell to 0, its values have to be finite.
  * A sample's cells lie contiguous (a shard without halo; re-distribute a spatially
- * partitioned tensor to sample-parallel first); sample and channel strides are
- * free.  All tensors are of desc->dtype; lse is n x q_heads x cells of q floats.
+ * partitioned tensor to sample-parallel first, in fp32); sample and channel strides
+ * are free.  All tensors are of desc->dtype; lse is n x q_heads x cells of q floats.
  * No result overlaps an operand or another result.  fp32 tensors are multiplied in
  * fp32; bf16 tensors on the tensor cores with fp32 accumulation, and their weights
  * exp(s) and the gradients of s are rounded to bf16 as operands (a single query's

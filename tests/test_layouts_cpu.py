@@ -40,3 +40,12 @@ def test_rotary_positions_need_all_channels_of_a_cell():
 def test_channel_slices_lie_where_their_tensor_does():
     t = shard([6, 4, 8, 2], [2, 1, 1, 1], rank=1)
     assert t.offset == [3, 0, 0, 0] and t.channel_slice(5, 2).offset == [3, 0, 5, 0]
+
+
+def test_redistribution_of_16_bits_is_refused_with_the_way_round():
+    a, b = shard([6, 4, 8, 2], [2, 1, 1, 1], dtype=torch.bfloat16), shard([6, 4, 8, 2], [1, 1, 1, 2], dtype=torch.bfloat16)
+    with pytest.raises(TypeError, match="before the rounding"):
+        dc.TensorShuffler(a, b, connect=False)
+    part = shard([6, 4, 8, 2], [2, 1, 1, 1])
+    with pytest.raises(ValueError, match="in torch.float32"):
+        dc.Attention(Backend(), 4, 2).forward(part, part, part, part, None)
