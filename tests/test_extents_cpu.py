@@ -37,3 +37,11 @@ def test_rotary_angles_that_are_not_finite(kw):
         rd.step[i] = kw.get("step", 1.0)
     assert status("dcb_rotary_plan_create", rd, nd(1, 256, 3, 500), ctypes.byref(ctypes.c_void_p())) == _abi.BAD_ARG
     assert b"finite" in _abi.lib().dcb_last_error()
+
+
+@pytest.mark.parametrize("scale", [2.4e38, 2.9e38, 3.4e38])
+def test_attention_scales_that_overflow_in_powers_of_two(scale):
+    few = nd(1, 8, 4, 7)
+    assert attention(desc(scale=scale), nd(1, 16, 4, 7), few) == _abi.BAD_ARG
+    assert b"scale" in _abi.lib().dcb_last_error()
+    assert status("dcb_attention_workspace_bytes", desc(scale=2.3e38), nd(1, 16, 4, 7), few, 0) >= 0
