@@ -50,7 +50,16 @@ struct AthKeys
         for (int l = 0; l < LOADS; ++l)
             v.r[l].load(row + at[l]);
     }
-    // What was fetched in place of keys from `end` on becomes 0: a weight of 0 times an infinity would not be.
+    // Values of keys from `end` on are 0: a weight of 0 times an infinity that was fetched in their place would not be.
+    // Where a lane's keys are one access its condition costs nothing (2 x 8 heads x 64 over 32^3 bf16 keys: 38.8 us, 40.2
+    // with a look behind the loads); with eight of them it does (31 x 33 x 31 keys: 98 us and 75).
+    __device__ __forceinline__ void load_until(Values& v, const T* row, int end) const
+    {
+        if (LOADS > 1 || first < end)
+            load(v, row);
+        else
+            v.r[0].clear();
+    }
     __device__ __forceinline__ void clear_behind(Values& v, int end) const
     {
 #pragma unroll
@@ -156,9 +165,9 @@ __global__ void __launch_bounds__(32 * WARPS, 16 / WARPS) attn_thin_fwd_kernel(c
         }
 #pragma unroll
         for (int c = 0; c < CHANNELS; ++c)
-            mine.load(v[c], values + min(c0 + c, p.d - 1) * p.v.sc);
+            mine.load_until(v[c], values + min(c0 + c, p.d - 1) * p.v.sc, hi);
         __syncthreads(); // the next tile's shares
-        if (j0 + 32 * V > hi)
+        if (Keys::LOADS > 1 && j0 + 32 * V > hi)
 #pragma unroll
             for (int c = 0; c < CHANNELS; ++c)
                 mine.clear_behind(v[c], hi);
