@@ -376,7 +376,8 @@ int32_t attn_shapes(const dcb_attention_desc* ad, const dcb_nd_desc* qd, const d
     const int64_t d = qd->c / ad->q_heads;
     DCB_REQUIRE(kd->c == d * ad->kv_heads, "channels of k must be kv_heads heads of q's size");
     DCB_REQUIRE(qd->n == kd->n, "q and k differ in samples");
-    DCB_REQUIRE(ad->scale > 0.f && std::isfinite(ad->scale * ATTN_LOG2E), "scale must be positive, and finite times log2(e)");
+    DCB_REQUIRE(ad->scale > 0.f && std::isfinite(ad->scale * ATTN_LOG2E),
+                "scale must be positive, and finite times log2(e)");
     if (d > ATTN_MAX_HEAD)
     {
         set_last_error("unsupported: heads of more than 128 channels");

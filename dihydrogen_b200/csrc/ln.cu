@@ -9,8 +9,8 @@
 // thread's channels in registers instead, addresses and predicates of the unrolled accesses took 50
 // instructions an element and 15 million bf16 values in rows of odd length 40 us.)
 //
-// Bound by HBM: 64 x 96^3 fp32 79 us forward, 112 backward (5.9 TB/s).  Rows of odd length by instruction issue: 2 x 200 x
-// 19 x 37 x 53 bf16 forward 22 us (2.7 TB/s).
+// Bound by HBM: 64 x 96^3 fp32 81 us forward, 112 backward (5.6 and 6.1 TB/s).  Rows of odd length by instruction issue:
+// 2 x 200 x 19 x 37 x 53 bf16 forward 21 us (2.9 TB/s).
 #include "elem.cuh"
 
 namespace dcb
@@ -190,7 +190,8 @@ __device__ __forceinline__ void ln_fwd_tile(const T* x, const RunStrides& xs, T*
     // Mean and centred squares of eight channels at a time, joined with those before (Chan et al.).  Every mean goes with
     // what its rounding left, `rest`: a difference of rounded means would put an error of first order in |mean| /
     // deviation into the squares (64 channels, mean 1000, deviation 1: 2.6e-5 of inv_std, so 1.7e-7).  Steps are powers
-    // of two, and bf16 values whose sum is rounded at all differ by as much as they are large: only fp32 steps leave a rest.
+    // of two, and bf16 values whose sum is rounded at all differ by as much as they are large: only fp32 steps leave a
+    // rest.
     constexpr bool ROUNDED = sizeof(T) == 4;
     float mean[V], rest[V], m2[V];
 #pragma unroll
@@ -537,9 +538,9 @@ struct LnChoice
 LnChoice ln_choose(int c, int vmax, long long len, long long cells)
 {
     LnChoice h;
-    // Four cells a thread where that leaves every SM a block of tiles (64 x 96^3 fp32, forward and backward, 82 + 112 us,
-    // 133 + 161 with one; 32 x 2 x 64^2, 4.5 + 4.5 and 3.9 + 4.5 with one), 32 apart where accesses of four are not aligned
-    // (200 x 2 x 19 x 37 x 53 bf16 23 + 36 us, with one 32 + 54) and runs are so long that their last tiles waste a quarter
+    // Four cells a thread where that leaves every SM a block of tiles (64 x 96^3 fp32, forward and backward, 81 + 112 us,
+    // 136 + 160 with one; 32 x 2 x 64^2, 4.5 + 4.5 and 3.9 + 4.5 with one), 32 apart where accesses of four are not aligned
+    // (200 x 2 x 19 x 37 x 53 bf16 17 + 31 us, with one 29 + 55) and runs are so long that their last tiles waste a quarter
     // of the lanes at most.
     const bool four = cells >= 4ll * 32 * num_sms();
     h.mode = four && vmax < 4 && len >= 512 ? LN_SPLIT : LN_FLAT;
@@ -549,7 +550,7 @@ LnChoice ln_choose(int c, int vmax, long long len, long long cells)
     h.g = 1;
     while (h.g < LN_WARPS && (c > LN_STEP * h.g || (c >= 2 * h.g && tiles * h.g < 8ll * num_sms())))
         h.g *= 2;
-    h.keep = c == LN_STEP * h.g; // (64 x 96^3 fp32 101 + 131 us without)
+    h.keep = c == LN_STEP * h.g; // (64 x 96^3 fp32 87 + 131 us without)
     return h;
 }
 

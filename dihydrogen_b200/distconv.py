@@ -1758,8 +1758,8 @@ class Attention:
     ``q_mask`` / ``kv_mask``: arrays of bool or uint8, one per sample and cell, 0
     where a cell is not there; whatever such a cell holds is never read into a
     result.  A cell that sees nothing gets 0 (``lse``: -infinity) and takes no
-    part in any gradient.  ``lse`` has one float per sample, query head and
-    cell."""
+    part in any gradient (its query and gradient have to be finite where no mask
+    takes it out).  ``lse`` has one float per sample, query head and cell."""
 
     def __init__(self, backend: BackendDNNLib, num_dims: int, q_heads: int, kv_heads: Optional[int] = None,
                  scale: Optional[float] = None, causal: bool = False):

@@ -415,7 +415,8 @@ int64_t dcb_pool_bwd_workspace_bytes(const dcb_pool_desc* pd,
  * x, y, dy, dx are of `dtype` (DCB_F32 or DCB_BF16; W has unit stride; no other
  * stride is restricted and the descriptors may differ in strides); scale, bias and
  * their gradients are C floats; mean and inv_std are one float per sample and
- * cell, dense in the order N, D, H, W.  All sums are fp32 or wider.
+ * cell, dense in the order N, D, H, W.  All sums are fp32 or wider.  More than 16384
+ * channels: DCB_UNSUPPORTED.
  * ------------------------------------------------------------------------ */
 /* scale and bias may be null (1 and 0), mean and inv_std too (not wanted).  y may
  * be x, with its strides. */
@@ -466,13 +467,16 @@ typedef struct dcb_rotary_desc
 
 typedef struct dcb_rotary_plan dcb_rotary_plan;
 /* Checks the geometry and lays down the cosines and sines of the window's
- * positions (worked out in fp64, held as fp32).  xd: extents only. */
+ * positions (worked out in fp64, held as fp32; an angle that is not finite is a bad
+ * argument), which have arrived when the call returns.  xd: extents only.  A plan
+ * lives for as long as a captured graph may apply it. */
 int32_t dcb_rotary_plan_create(const dcb_rotary_desc* rd,
                                const dcb_nd_desc* xd, dcb_rotary_plan** plan);
 int32_t dcb_rotary_plan_destroy(dcb_rotary_plan* plan);
 /* y = turned x; inverse != 0 turns back, which is also the gradient.  The types
  * may differ (x is rounded once, as it is written).  xd and yd have the plan's
- * extents; W has unit stride; y may be x where type and strides are the same.
+ * extents; W has unit stride; y may be x where type and strides are the same.  2^31
+ * cells of a sample, 2^17 channels of a head, 2^16 samples: DCB_UNSUPPORTED.
  * Reads the plan only: calls may overlap.  The plan and the tensors live on the
  * current device. */
 int32_t dcb_rotary_apply(const dcb_rotary_plan* plan, const dcb_nd_desc* xd,
@@ -491,13 +495,13 @@ int32_t dcb_rotary_apply(const dcb_rotary_plan* plan, const dcb_nd_desc* xd,
  * i may see j if q_mask (n x cells of q bytes, may be null) is not 0 at i, kv_mask
  * (n x cells of k) not at j, and, where `causal`, j <= i + (cells of k - cells of
  * q).  A cell that sees nothing gets o = 0, lse = -infinity and takes no part in
- * any gradient (its d_o has to be finite where no mask takes it out).  What cells
+ * any gradient (its q and d_o have to be finite where no mask takes it out).  What cells
  * that a mask takes out hold is never interpreted, and their results are 0;
  * `causal` only sets the weight of a later cell to 0, its values have to be finite.
  * A sample's cells lie contiguous (a shard without halo; re-distribute a spatially
  * partitioned tensor to sample-parallel first, in fp32); sample and channel strides
  * are free.  All tensors are of desc->dtype; lse is n x q_heads x cells of q floats.
- * No result overlaps an operand or another result.  fp32 tensors are multiplied in
+ * A result that shares memory with an operand or another result is refused.  fp32 tensors are multiplied in
  * fp32; bf16 tensors on the tensor cores with fp32 accumulation, and their weights
  * exp(s) and the gradients of s are rounded to bf16 as operands (a single query's
  * weights stay fp32).  The same bits every run.
