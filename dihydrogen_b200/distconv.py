@@ -1679,7 +1679,7 @@ class RotaryPositions:
     def __init__(self, backend: BackendDNNLib, num_dims: int):
         self.be, self.num_dims, self.nsd = backend, num_dims, num_dims - 2
         self._plans = {}  # geometry -> plan, as long as the layer lives: captured graphs read their tables
-        self._plan = None
+        self._plan = self._local = self._at = None
 
     def __del__(self):
         try:
@@ -1707,6 +1707,7 @@ class RotaryPositions:
         for i in range(nsd):
             rd.axis_channels[2 - i], rd.origin[2 - i] = axis_channels[i], input.offset[i]
             rd.step[2 - i] = 1.0 if step is None else float(step[i])
+        self._plan = None  # stays so if the geometry is refused
         self._local, self._at = list(input.local_shape), list(input.offset[:-2])
         key = (bytes(rd), tuple(input.local_shape[:-1]), torch.cuda.current_device() if torch.cuda.is_available() else -1)
         self._plan = self._plans.get(key)
@@ -1716,6 +1717,8 @@ class RotaryPositions:
             self._plan = self._plans[key] = plan
 
     def _apply(self, x: Tensor, y: Tensor, inverse):
+        if self._plan is None:
+            raise ValueError("rotary positions: no setup, or one that was refused")
         if x.local_shape[:-1] != self._local[:-1] or y.local_shape != x.local_shape:
             raise ValueError(f"local shapes {x.local_shape} and {y.local_shape}, set up for {self._local}")
         if x.offset[:-2] != self._at or y.offset[:-2] != self._at:

@@ -49,3 +49,13 @@ def test_redistribution_of_16_bits_is_refused_with_the_way_round():
     part = shard([6, 4, 8, 2], [2, 1, 1, 1])
     with pytest.raises(ValueError, match="in torch.float32"):
         dc.Attention(Backend(), 4, 2).forward(part, part, part, part, None)
+
+
+def test_rotary_positions_without_a_setup():
+    rot, x = dc.RotaryPositions(Backend(), 4), shard([6, 4, 8, 2], [1, 1, 1, 1])
+    with pytest.raises(ValueError, match="setup"):
+        rot.forward(x, x)
+    with pytest.raises(dc._abi.DcbError):
+        rot.setup(x, 4, [3, 1])  # axes have pairs of channels
+    with pytest.raises(ValueError, match="setup"):
+        rot.backward(x, x)
