@@ -64,3 +64,41 @@ def test_sums_over_a_million_keys(queries, causal):
     # lse: its sum's roundings, those of a score (a product, scale) and its own in powers of two
     off = (lse[0].double() - want).abs().max()
     assert float(off) <= bound / 2 + 4 * u * 14, float(off)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=["f32", "bf16"])
+def test_gradients_whose_offsets_pass_32_bits(dtype):
+    """Keys, values and their gradients of 2^31 elements and more: equal weights, values that depend on the channel and the
+    half; layer norm backward over the same memory."""
+    cells, d = (1 << 25) + 40, 64
+    be = backend()
+    k = torch.zeros(1, d, 1, cells, dtype=dtype, device="cuda")
+    v, dk, dv = (torch.empty_like(k) for _ in range(3))
+    channel = torch.arange(d, device="cuda", dtype=torch.float32).to(dtype)
+    v[0, :, 0, : cells // 2], v[0, :, 0, cells // 2:] = channel[:, None], -3 * channel[:, None]
+    q, d_o = (torch.ones(1, d, 1, 2, dtype=dtype, device="cuda") for _ in range(2))
+    o, dq, lse = torch.empty_like(q), torch.full_like(q, math.nan), torch.empty(1, 1, 2, device="cuda")
+    tq, tk, tv, to, tdo, tdq, tdk, tdv = (tensor(t, be) for t in (q, k, v, o, d_o, dq, dk, dv))
+    at = dc.Attention(be, 4, 1)
+    at.forward(tq, tk, tv, to, lse)
+    at.backward(tq, tk, tv, to, lse, tdo, tdq, tdk, tdv)
+    assert at.status() == dc._abi.OK and not dq.any()
+    # weights 2^-lse with lse of 25 in powers of two: three roundings of that size; of the sums 64 products each; bf16 two
+    # roundings as an operand and one as a result
+    rel = 3 * 25 * 2.0 ** -24 + 200 * 2.0 ** -24 + (3 * R.U16 if dtype == torch.bfloat16 else 0.0)
+    for j, sign in ((0, 1), (cells // 2 - 1, 1), (cells // 2, -1), (cells - 1, -1)):
+        assert float((dv[0, :, 0, j].double() * cells / 2 - 1).abs().max()) <= rel
+        # two queries: scale p (d_o v - d_o o) q = (2016 + 2016) / 8 of either
+        assert float((dk[0, :, 0, j].double() * cells / (sign * 1008) - 1).abs().max()) <= 2 * rel
+    ln = dc.LayerNormalization(be, 4, 1e-5)
+    mean, inv = ln.new_statistics(tv)
+    ln.forward(tv, None, None, tdk, mean, inv)
+    k[:] = (channel * channel / 64)[None, :, None, None]
+    ln.backward(tv, tk, mean, inv, None, None, None, tdv)
+    for j in (0, cells // 2 - 1, cells // 2, cells - 1):
+        x = v[:, :, :, j].double().requires_grad_()
+        y = (x - x.mean(1, keepdim=True)) / (x.var(1, keepdim=True, correction=0) + 1e-5).sqrt()
+        want, = torch.autograd.grad(y, x, k[:, :, :, j].double())
+        off = (dv[:, :, :, j].double() - want).abs()
+        # sums of 64 terms of at most 64, an operand of inv * that
+        assert bool((off <= R.stored(dtype) * want.abs() + 100 * 2.0 ** -24 * 64 * float(inv.flatten()[j])).all())
