@@ -64,9 +64,8 @@ class _Geometry:
         self.base = t.dtype.itemsize * t.get_local_offset([0] * t.nd)
         self.split_root = t.is_split_root()
         self.owned = tuple(slice(o, o + l) for o, l in reversed(list(zip(self.overlap, self.local))))
-        # all cells and channels of a sample are here; all channels of a cell are
-        cut = [t.dist.is_distributed(d) and t.dist.locale_shape[d] > 1 for d in range(t.nd - 1)]
-        self.whole, self.whole_cells = not any(cut), not cut[-1]
+        # all cells and channels of a sample are here
+        self.whole = not any(t.dist.is_distributed(d) and t.dist.locale_shape[d] > 1 for d in range(t.nd - 1))
         self.operand = None  # descriptor of the owned cells, by reference
         self.descs = {}    # widths -> NdDesc
         self.offsets = {}  # widths -> byte offset of the window
@@ -241,6 +240,8 @@ class Tensor:
         self.dist = dist.copy()
         self.nd = len(self.shape)
         self._local_shape_of = local_shape_of
+        # all channels of a cell are here
+        self.whole_cells = self.nd < 2 or not (self.dist.is_distributed(-2) and self.dist.locale_shape[-2] > 1)
         self.proc_idx = locale.get_rank_idx(self.dist)
         self.split_idx = [p // self.dist.get_num_ranks_per_split(i) for i, p in enumerate(self.proc_idx)]
         self.local_shape = self._local_of(self.proc_idx)
@@ -515,7 +516,7 @@ class ChannelSlice:
         if not 0 <= first <= first + count <= tensor.local_shape[-2]:
             raise ValueError(f"channels {first} to {first + count} of {tensor.local_shape[-2]}")
         self.tensor, self.first, self.count = tensor, first, count
-        self.dtype, self.dist, self.nd = tensor.dtype, tensor.dist, tensor.nd
+        self.dtype, self.dist, self.nd, self.whole_cells = tensor.dtype, tensor.dist, tensor.nd, tensor.whole_cells
         self._of = None
 
     @property
@@ -1577,7 +1578,7 @@ def _check_alike(what, first, *others):
 
 def _check_whole_cells(what, *tensors):
     for t in tensors:
-        if not t._geo().whole_cells:
+        if not t.whole_cells:
             raise ValueError(f"{what} needs all channels of a cell on one rank: re-distribute the tensor "
                              "(TensorShuffler, in torch.float32)")
 
