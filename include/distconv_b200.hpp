@@ -2500,8 +2500,8 @@ inline void require_whole_cells(std::initializer_list<TensorF*> ts, const char* 
 }
 } // namespace internal
 
-// Layer normalisation over the channels of every cell, tensors partitioned along samples and space or not.  mean and inv_std: a float per sample
-// and owned cell; scale and bias may be null.
+// Layer normalisation over the channels of every cell, tensors partitioned along samples and space or not.  mean and
+// inv_std: a float per sample and owned cell; scale and bias may be null.
 class LayerNormalization
 {
 public:
